@@ -231,9 +231,9 @@ def _run_plain_rotary(s):
 
 
 def _held(amax):
-    """The smallest power of two of which 448 hold the largest magnitude of a block."""
+    """The smallest power of two, from 2^-40 to 2^60, of which 448 hold the largest magnitude of a block."""
     m, e = torch.frexp(amax)
-    return torch.ldexp(torch.ones_like(amax), torch.where(m <= 0.875, e - 9, e - 8).clamp(-60, 119))
+    return torch.ldexp(torch.ones_like(amax), torch.where(m <= 0.875, e - 9, e - 8).clamp(-40, 60))
 
 
 def _run_plain_append(s):
@@ -377,7 +377,7 @@ def _exact_append(s):
             for n in ("k", "v"):
                 x = new[n][:, lo - start:hi - start]
                 most = x.abs().amax((-1, -2))
-                step = torch.exp2(torch.ceil(torch.log2(most.clamp_min(1e-300) / 448.0)).clamp(-59, 119))
+                step = torch.exp2(torch.ceil(torch.log2(most.clamp_min(1e-300) / 448.0)).clamp(-39, 60))
                 step = torch.where(most <= 224.0 * step, step / 2, step)   # where the logarithm of a power of two came out above it
                 older = lo - block * BLOCK
                 if older:
