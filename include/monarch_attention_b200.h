@@ -46,7 +46,8 @@ enum {
   MA_B200_UNSUPPORTED = 2,      /* valid problem that the requested kernel cannot run         */
   MA_B200_CUDA_ERROR = 3,       /* a CUDA runtime / driver call failed (see last_error)       */
   MA_B200_DEVICE_WAIT_EXPIRED = 4, /* a bounded on-device wait gave up; output is undefined   */
-  MA_B200_WORKSPACE_TOO_SMALL = 5
+  MA_B200_WORKSPACE_TOO_SMALL = 5,
+  MA_B200_DEVICE_BAD_SEQUENCE = 6 /* a kernel met a length, count or page outside its range (see ma_b200_poll_cache_status) */
 };
 
 /* Element types.  q and k share qk_dtype; v and out share v_dtype. */
@@ -292,6 +293,103 @@ MA_B200_API int ma_b200_forward_host_grouped(const ma_b200_problem* p, int heads
 MA_B200_API int ma_b200_host_chunk_plan(int E, int H, int heads_per_chunk, int elements_per_chunk, int least_heads, int32_t* chunks,
                                         int capacity);
 MA_B200_API const char* ma_b200_host_last_error(void);
+
+/*
+ * What a decoder needs beside the attention above (no counterpart in the reference, whose models encode): rotary
+ * positions, a paged key/value cache in 8 bits, and softmax attention of new tokens over it.
+ */
+
+/* Rotary positions: pair i of a head (features (i, dim/2 + i) for HALF, (2i, 2i + 1) for INTERLEAVED, i < dim/2) at position
+ * p is turned by p * f_i and multiplied by `magnitude`; features from dim on stay as they are.  turns[i] (HOST memory, dim/2
+ * entries, read during the call) is f_i / (2 pi) in units of 2^-64 turns, so that angles are exact at any position. */
+enum { MA_B200_PAIRS_HALF = 0, MA_B200_PAIRS_INTERLEAVED = 1 };
+typedef struct ma_b200_rotary {
+  int32_t dim;   /* even, at most 256 and the head width */
+  int32_t pairs; /* MA_B200_PAIRS_* */
+  float magnitude;
+  const uint64_t* turns;
+} ma_b200_rotary;
+
+/* Rotates q (E, H, N, D) into q_out and k (E, Hk, N, D) into k_out (H or Hk may be 0: that tensor is not looked at); an output
+ * may be its input (same pointer and strides).  positions: int32 or int64 by (batch, token) with any strides, or NULL: 0 .. N-1.
+ * inverse != 0 applies the transpose, which is the gradient: it turns back (and multiplies by magnitude again). */
+typedef struct ma_b200_rotation {
+  int32_t abi_version;
+  int32_t E, H, Hk, N, D;
+  int32_t dtype; /* of q and k */
+  int32_t inverse;
+  ma_b200_tensor q, q_out, k, k_out;
+  const void* positions;
+  int32_t positions_i64;
+  int64_t pos_stride_e, pos_stride_n;
+  ma_b200_rotary rotary;
+} ma_b200_rotation;
+MA_B200_API int ma_b200_rotary_apply(const ma_b200_rotation* p, void* stream);
+
+/* A paged cache: k and v are (pages, heads, page_size, width) in e4m3, k_scale and v_scale (pages, heads, page_size / 16) in f32:
+ * the 16 tokens of a block of a head stand for code * scale.  Strides count elements; rows of k and v lie on 16-byte boundaries, the
+ * scales of a page and head next to one another.  width is 64 or 128, page_size a power of two from 16 on. */
+typedef struct ma_b200_cache {
+  void *k, *v;
+  float *k_scale, *v_scale;
+  int32_t pages, heads, page_size, width;
+  int64_t k_stride_page, k_stride_head, k_stride_token;
+  int64_t v_stride_page, v_stride_head, v_stride_token;
+  int64_t ks_stride_page, ks_stride_head;
+  int64_t vs_stride_page, vs_stride_head;
+} ma_b200_cache;
+
+/* Which tokens of which sequence a call is about.  page_table (E, table_pages) int32: the page of each run of page_size tokens of
+ * a sequence.  lengths (E) int32: tokens of each sequence, those of the call among them.  counts (E) int32: how many of the
+ * call's N tokens a sequence brings (the rest is padding behind them), or NULL: N.  Token n of the call is at position
+ * lengths[e] - counts[e] + n.  All three are read on the device.  A length that the table has no room for, a count above N (or, when
+ * appending, above the length) or a page outside the cache is never followed out of bounds: what it concerns is left out (appending)
+ * or has an undefined result (attention), and ma_b200_poll_cache_status reports it. */
+typedef struct ma_b200_sequences {
+  const int32_t* page_table;
+  int64_t table_stride;
+  int32_t table_pages;
+  const int32_t* lengths;
+  const int32_t* counts;
+} ma_b200_sequences;
+
+/* Writes k and v (E, cache heads, N, width; bf16 or f16) into the cache at the call's positions, k rotated there if `rotary` is given
+ * (dim a multiple of 8).  A block's scale is the smallest power of two from 2^-40 to 2^60 with which 448 holds its largest magnitude, and never
+ * falls while the block has older tokens; those are re-expressed when it rises.  Values are rounded to nearest even; magnitudes
+ * above 448 * 2^60 are stored as that, NaN as NaN.  If H > 0, q (E, H, N, width) is rotated into q_out (which may be q) in the same
+ * launch, rows of padding as zeros.  The pages that a call writes must belong to one sequence each. */
+typedef struct ma_b200_append {
+  int32_t abi_version;
+  int32_t E, H, N;
+  int32_t dtype;
+  ma_b200_tensor k, v, q, q_out;
+  ma_b200_cache cache;
+  ma_b200_sequences sequences;
+  const ma_b200_rotary* rotary; /* or NULL */
+} ma_b200_append;
+MA_B200_API int ma_b200_cache_append(const ma_b200_append* p, void* stream);
+
+/* Softmax attention of q (E, H, N, width; bf16 or f16; query head h reads cache head h / (H / heads)) over the sequences' cached tokens
+ * into out.  causal: token n sees positions up to its own, else all `lengths`.  window > 0 (causal only): the last `window`
+ * of those.  softcap > 0: scores s become softcap * tanh(s / softcap).  Rows without a key, and rows of padding, are zero. */
+typedef struct ma_b200_attend {
+  int32_t abi_version;
+  int32_t E, H, N;
+  int32_t dtype;
+  int32_t causal, window;
+  float scale, softcap;
+  ma_b200_tensor q, out;
+  ma_b200_cache cache;
+  ma_b200_sequences sequences;
+} ma_b200_attend;
+/* Scratch bytes of the call (0 on an invalid problem); the workspace is 256-byte aligned and needs no initialisation.  Calls that may
+ * overlap in time need one each. */
+MA_B200_API size_t ma_b200_cache_attend_workspace_bytes(const ma_b200_attend* p);
+MA_B200_API int ma_b200_cache_attend(const ma_b200_attend* p, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Without synchronising anything: has a kernel of the cache on `device` met a length, count or page outside its range since the last
+ * poll?  MA_B200_OK, or MA_B200_DEVICE_BAD_SEQUENCE once per incident; trails the GPU by at most the kernels in flight. */
+MA_B200_API int ma_b200_poll_cache_status(int device);
 
 MA_B200_API int32_t ma_b200_abi_version(void);
 

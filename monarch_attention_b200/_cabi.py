@@ -17,7 +17,7 @@ KERNEL_NAMES = {KERNEL_AUTO: "auto", KERNEL_GENERIC: "generic", KERNEL_TCGEN05: 
                 KERNEL_WARP_MMA: "warp-mma", KERNEL_HEAD_FUSED: "head-fused",
                 KERNEL_TF32X3: "tf32x3", KERNEL_HEAD_RESIDENT: "head-resident",
                 KERNEL_TILE: "tile"}
-OK, INVALID_ARGUMENT, UNSUPPORTED, CUDA_ERROR, DEVICE_WAIT_EXPIRED, WORKSPACE_TOO_SMALL = range(6)
+OK, INVALID_ARGUMENT, UNSUPPORTED, CUDA_ERROR, DEVICE_WAIT_EXPIRED, WORKSPACE_TOO_SMALL, DEVICE_BAD_SEQUENCE = range(7)
 
 LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "lib", "libmonarch_attention_b200.so")
 
@@ -29,6 +29,8 @@ EXPORTS = (
     "ma_b200_host_scratch_bytes_grouped", "ma_b200_forward_host_grouped", "ma_b200_host_chunk_plan",
     "ma_b200_poll_device_status", "ma_b200_selftest_wait_expiry", "ma_b200_selftest_generic_general_form",
     "ma_b200_backward_workspace_bytes", "ma_b200_backward", "ma_b200_forward_typed_mask", "ma_b200_backward_typed_mask",
+    "ma_b200_rotary_apply", "ma_b200_cache_append", "ma_b200_cache_attend_workspace_bytes", "ma_b200_cache_attend",
+    "ma_b200_poll_cache_status",
 )
 
 
@@ -49,6 +51,42 @@ class Problem(C.Structure):
 
 class Gradients(C.Structure):
     _fields_ = [(n, Tensor4) for n in ("grad_out", "dq", "dk", "dv")]
+
+
+PAIRS_HALF, PAIRS_INTERLEAVED = 0, 1
+
+
+class Rotary(C.Structure):
+    _fields_ = [("dim", C.c_int32), ("pairs", C.c_int32), ("magnitude", C.c_float), ("turns", C.POINTER(C.c_uint64))]
+
+
+class Rotation(C.Structure):
+    _fields_ = [(n, C.c_int32) for n in ("abi_version", "E", "H", "Hk", "N", "D", "dtype", "inverse")] + \
+               [(n, Tensor4) for n in ("q", "q_out", "k", "k_out")] + \
+               [("positions", C.c_void_p), ("positions_i64", C.c_int32), ("pos_stride_e", C.c_int64), ("pos_stride_n", C.c_int64),
+                ("rotary", Rotary)]
+
+
+class Cache(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("k", "v", "k_scale", "v_scale")] + \
+               [(n, C.c_int32) for n in ("pages", "heads", "page_size", "width")] + \
+               [(n, C.c_int64) for n in ("k_stride_page", "k_stride_head", "k_stride_token", "v_stride_page", "v_stride_head", "v_stride_token",
+                                         "ks_stride_page", "ks_stride_head", "vs_stride_page", "vs_stride_head")]
+
+
+class Sequences(C.Structure):
+    _fields_ = [("page_table", C.c_void_p), ("table_stride", C.c_int64), ("table_pages", C.c_int32), ("lengths", C.c_void_p), ("counts", C.c_void_p)]
+
+
+class Append(C.Structure):
+    _fields_ = [(n, C.c_int32) for n in ("abi_version", "E", "H", "N", "dtype")] + [(n, Tensor4) for n in ("k", "v", "q", "q_out")] + \
+               [("cache", Cache), ("sequences", Sequences), ("rotary", C.POINTER(Rotary))]
+
+
+class Attend(C.Structure):
+    _fields_ = [(n, C.c_int32) for n in ("abi_version", "E", "H", "N", "dtype", "causal", "window")] + \
+               [("scale", C.c_float), ("softcap", C.c_float)] + [(n, Tensor4) for n in ("q", "out")] + \
+               [("cache", Cache), ("sequences", Sequences)]
 
 
 class WorkspaceLayout(C.Structure):
@@ -120,6 +158,16 @@ def load() -> C.CDLL:
     lib.ma_b200_forward_host_grouped.restype = C.c_int
     lib.ma_b200_host_chunk_plan.argtypes = [C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, C.POINTER(C.c_int32), C.c_int]
     lib.ma_b200_host_chunk_plan.restype = C.c_int
+    lib.ma_b200_rotary_apply.argtypes = [C.POINTER(Rotation), C.c_void_p]
+    lib.ma_b200_rotary_apply.restype = C.c_int
+    lib.ma_b200_cache_append.argtypes = [C.POINTER(Append), C.c_void_p]
+    lib.ma_b200_cache_append.restype = C.c_int
+    lib.ma_b200_cache_attend_workspace_bytes.argtypes = [C.POINTER(Attend)]
+    lib.ma_b200_cache_attend_workspace_bytes.restype = C.c_size_t
+    lib.ma_b200_cache_attend.argtypes = [C.POINTER(Attend), C.c_void_p, C.c_size_t, C.c_void_p]
+    lib.ma_b200_cache_attend.restype = C.c_int
+    lib.ma_b200_poll_cache_status.argtypes = [C.c_int]
+    lib.ma_b200_poll_cache_status.restype = C.c_int
     lib.ma_b200_host_last_error.argtypes = []
     lib.ma_b200_host_last_error.restype = C.c_char_p
     if lib.ma_b200_abi_version() != ABI_VERSION:

@@ -18,9 +18,9 @@ CSRC = os.path.join(PKG, "csrc")
 LIB_DIR = os.path.join(PKG, "lib")
 LIB_PATH = os.path.join(LIB_DIR, "libmonarch_attention_b200.so")
 NATIVE_PATH = os.path.join(PKG, "_native.so")
-NATIVE_SOURCE = "ma_torch.cpp"
-SOURCES = ["ma_api.cu", "ma_generic.cu", "ma_tc.cu", "ma_fused.cu", "ma_warp.cu", "ma_warp_f32.cu", "ma_head.cu", "ma_head_f16.cu", "ma_head_states.cu", "ma_head_states_f16.cu", "ma_tile.cu", "ma_flow.cu", "ma_flow_f16.cu", "ma_backward.cu", "ma_backward_f16.cu", "ma_backward_f32.cu", "ma_noalloc.cu", "ma_host.cu"]
-HEADERS = ["ma_common.cuh", "ma_tile_common.cuh", "ma_flow.inc", "ma_head.inc", "ma_backward.inc", "ma_warp_common.cuh", "ma_warp_kernels.inc", "ma_warp_head.inc", "ma_warp_wide.inc", "ma_sm100.cuh", "ma_tc_plan.cuh", os.path.join("..", "..", "include", "monarch_attention_b200.h")]
+NATIVE_SOURCES = ["ma_torch.cpp", "ma_torch_cache.cpp"]
+SOURCES = ["ma_api.cu", "ma_generic.cu", "ma_tc.cu", "ma_fused.cu", "ma_warp.cu", "ma_warp_f32.cu", "ma_head.cu", "ma_head_f16.cu", "ma_head_states.cu", "ma_head_states_f16.cu", "ma_tile.cu", "ma_flow.cu", "ma_flow_f16.cu", "ma_backward.cu", "ma_backward_f16.cu", "ma_backward_f32.cu", "ma_noalloc.cu", "ma_host.cu", "ma_rotary.cu", "ma_cache_append.cu", "ma_cache_attend.cu", "ma_cache_api.cu"]
+HEADERS = ["ma_common.cuh", "ma_tile_common.cuh", "ma_flow.inc", "ma_head.inc", "ma_backward.inc", "ma_warp_common.cuh", "ma_warp_kernels.inc", "ma_warp_head.inc", "ma_warp_wide.inc", "ma_sm100.cuh", "ma_tc_plan.cuh", "ma_rotary.cuh", "ma_cache.cuh", "ma_torch.h", os.path.join("..", "..", "include", "monarch_attention_b200.h")]
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
@@ -45,26 +45,25 @@ def _older(path: str, than: float) -> bool:
     return not os.path.exists(path) or os.path.getmtime(path) < than
 
 
-def _native_command(obj: str) -> list[str]:
+def _native_command(src: str, obj: str) -> list[str]:
     from torch.utils.cpp_extension import include_paths
     inc = [f"-I{p}" for p in include_paths() + ["/usr/local/cuda/include", sysconfig.get_paths()["include"]]]
     return ["g++", "-O2", "-std=c++17", "-fPIC", "-fvisibility=hidden", "-DTORCH_API_INCLUDE_EXTENSION_H",
-            "-DTORCH_EXTENSION_NAME=_native", *inc, "-c", os.path.join(CSRC, NATIVE_SOURCE), "-o", obj]
+            "-DTORCH_EXTENSION_NAME=_native", *inc, "-c", os.path.join(CSRC, src), "-o", obj]
 
 
 def build(force: bool = False, verbose: bool = False) -> str:
     """Compiles what is older than its sources: the headers count for every source."""
     os.makedirs(LIB_DIR, exist_ok=True)
     common = max(_newest(HEADERS), os.path.getmtime(os.path.abspath(__file__)))
-    jobs, objs = [], []
-    for src in [NATIVE_SOURCE] + SOURCES:
+    jobs, objs, native_objs = [], [], []
+    for src in NATIVE_SOURCES + SOURCES:
         obj = os.path.join(LIB_DIR, os.path.splitext(src)[0] + ".o")
-        if src != NATIVE_SOURCE:
-            objs.append(obj)
+        (native_objs if src in NATIVE_SOURCES else objs).append(obj)
         if not force and not _older(obj, max(common, _newest([src]))):
             continue
-        if src == NATIVE_SOURCE:
-            cmd = _native_command(obj)
+        if src in NATIVE_SOURCES:
+            cmd = _native_command(src, obj)
         else:
             cmd = [find_nvcc(), *(["-Xptxas", "-v"] if verbose else []), *NVCC_FLAGS, "-c", os.path.join(CSRC, src), "-o", obj]
         jobs.append((src, subprocess.Popen(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)))
@@ -80,10 +79,9 @@ def build(force: bool = False, verbose: bool = False) -> str:
     if _older(LIB_PATH, newest):
         subprocess.check_call([find_nvcc(), "-shared", "-gencode", "arch=compute_100a,code=sm_100a", "-Xcompiler", "-fPIC",
                                "-o", LIB_PATH, *objs, "-cudart", "static"])
-    native_obj = os.path.join(LIB_DIR, os.path.splitext(NATIVE_SOURCE)[0] + ".o")
-    if _older(NATIVE_PATH, os.path.getmtime(native_obj)):
+    if _older(NATIVE_PATH, max(os.path.getmtime(o) for o in native_objs)):
         from torch.utils.cpp_extension import library_paths
-        subprocess.check_call(["g++", "-shared", "-o", NATIVE_PATH, native_obj, f"-L{LIB_DIR}", "-l:" + os.path.basename(LIB_PATH),
+        subprocess.check_call(["g++", "-shared", "-o", NATIVE_PATH, *native_objs, f"-L{LIB_DIR}", "-l:" + os.path.basename(LIB_PATH),
                                "-Wl,-rpath,$ORIGIN/lib", *(f"-L{p}" for p in library_paths()), "-lc10", "-lc10_cuda",
                                "-ltorch_cpu", "-ltorch_cuda", "-ltorch", "-ltorch_python"])
     return LIB_PATH

@@ -19,6 +19,14 @@ int fail(int code, const std::string& msg) {
   return code;
 }
 
+}  // namespace
+
+namespace ma {
+int fail_with(int code, const std::string& msg) { return fail(code, msg); }
+}  // namespace ma
+
+namespace {
+
 size_t dtype_size(int dt) {
   switch (dt) {
     case MA_B200_F32: return 4;
@@ -490,6 +498,7 @@ const char* ma_b200_status_string(int status) {
     case MA_B200_CUDA_ERROR: return "CUDA error";
     case MA_B200_DEVICE_WAIT_EXPIRED: return "device-side bounded wait expired";
     case MA_B200_WORKSPACE_TOO_SMALL: return "workspace too small";
+    case MA_B200_DEVICE_BAD_SEQUENCE: return "length, count or page out of range";
     default: return "unknown status";
   }
 }

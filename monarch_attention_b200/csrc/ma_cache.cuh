@@ -1,0 +1,70 @@
+// A paged cache of keys and values in 8 bits (e4m3), with a scale for each block of 16 tokens of a head, and what its kernels share.
+#pragma once
+
+#include "ma_rotary.cuh"
+
+namespace ma {
+
+constexpr int kScaleBlock = 16;  // tokens that share a scale
+
+// Strides in elements of each tensor; the features of a row lie next to one another.
+struct CacheArgs {
+  uint8_t *k, *v;         // (pages, heads, page size, D) e4m3
+  float *k_scale, *v_scale;  // (pages, heads, page size / 16)
+  long long k_sp, k_sh, k_st, v_sp, v_sh, v_st;
+  long long ks_sp, ks_sh, vs_sp, vs_sh;
+  int pages, heads, page_shift;  // page size = 1 << page_shift
+  const int* table;  // (E, table_pages) page of each run of page-size tokens
+  long long table_se;
+  int table_pages;
+  const int* lengths;  // (E) tokens of a sequence, those of the call among them
+  const int* counts;   // (E) tokens of a sequence in the call, or nullptr: N
+  int* status;         // mapped host word: what was wrong with a table, length or count
+};
+
+enum CacheFault { kBadLength = 1, kBadPage = 2 };
+
+__device__ __forceinline__ void report(int* status, int code) {
+  if (status != nullptr) *reinterpret_cast<volatile int*>(status) = code;
+}
+
+// Tokens of sequence e and how many of them the call brings, held to what the table and the call have room for; false if they had to be.
+__device__ __forceinline__ bool sequence_of(const CacheArgs& c, int e, int N, int* len, int* count) {
+  const int room = (int)min((long long)c.table_pages << c.page_shift, 0x7fffff00LL);
+  const int l = c.lengths[e], n = c.counts != nullptr ? c.counts[e] : N;
+  *len = min(max(l, 0), room);
+  *count = min(max(n, 0), N);
+  return l == *len && n == *count;
+}
+
+// Page of the tokens from `position` on, or -1.
+__device__ __forceinline__ int page_of(const CacheArgs& c, int e, int position) {
+  const int i = position >> c.page_shift;
+  if (i >= c.table_pages) return -1;
+  const int page = c.table[e * c.table_se + i];
+  return page >= 0 && page < c.pages ? page : -1;
+}
+
+struct AppendArgs {
+  CacheArgs cache;
+  View4 k, v, q, q_out;
+  int E, N, H;  // H: query heads, 0 = none
+  RotaryArgs rotary;
+};
+cudaError_t launch_append(const AppendArgs& a, int dtype, int width, cudaStream_t stream);
+
+struct AttendArgs {
+  CacheArgs cache;
+  View4 q, out;
+  int E, N, H, group;   // group: query heads of a key head
+  int causal, window;   // window 0: none
+  float scale, softcap;  // softcap 0: none
+  int row_blocks;       // blocks of 8 * kernel tiles rows; row = token * group + head of the group
+  float *part_o, *part_ml;  // of the pieces of split heads: two a CTA
+  int4* split;              // one a CTA: the head whose pieces begin there
+};
+// Bytes of scratch, and how many row tiles and CTAs the call takes.
+size_t attend_workspace(int E, int N, int H, int kv_heads, int width, long long longest);
+cudaError_t launch_attend(AttendArgs a, int dtype, int width, void* workspace, long long longest, cudaStream_t stream);
+
+}  // namespace ma

@@ -1,0 +1,618 @@
+// Softmax attention of a few query rows over a paged cache in 8 bits.
+//
+// Bound by memory: a key/value pair of a head is 2 D bytes and takes part in 4 D operations a row, so that up to some 30 rows the cache's
+// bytes are all that counts.  The kernel is built around them:
+//  * The keys of all sequences and heads are one list of steps of 128 tokens, shared out evenly: CTA c takes steps [c S / G, (c + 1) S / G)
+//    whatever the lengths are, so that a ragged batch and a single long sequence both fill the GPU.  Lengths are read on the device; a
+//    head whose steps lie in several CTAs has its pieces joined by a second small kernel.
+//  * A warp takes 32 of a step's tokens, through a ring of its own in shared memory that is filled asynchronously, steps ahead and
+//    across the ends of heads; nothing in the loop waits for another warp.
+//  * Scores are taken as (keys x rows): the keys are the 16-row operand of the 16 x 8 x 16 matrix instruction and up to 8 query rows (the heads
+//    of a group, times tokens) its 8 columns, so that no part of it is padding when 8 rows share a key head.  Bytes go from shared memory
+//    straight into operand registers: the order of features in a contraction is free, and a lane's 16 bytes of a row are taken
+//    as they lie.  The weighted values are (features x rows) in the same way, two tokens' bytes interleaved by byte permutation; the
+//    weights change sides by an 8 x 8 transpose between lanes.
+//  * e4m3 is exact in f16, so the products are f16 with 32-bit sums whatever the queries' type; a bf16 row is scaled by a power of two to
+//    magnitudes of 1 to 2 first (exact but for elements 2^-23 below the row's largest).  A block's key scale multiplies its scores; its value
+//    scale goes into the weights, and the running maximum is taken over weight times scale, so that f16 weights are at most 1.
+#include <math_constants.h>
+
+#include <type_traits>
+
+#include "ma_cache.cuh"
+#include "ma_sm100.cuh"
+
+namespace ma {
+namespace {
+
+using sm100::ex2;
+using sm100::kLog2e;
+using sm100::smem_u32;
+
+constexpr int kWarps = 4, kSlice = 32, kStep = kWarps * kSlice;  // tokens of a warp and of a CTA at a time
+
+template <int D, int NT>
+struct Shape {
+  static constexpr int kStages = D == 128 ? 3 : 4;
+  static constexpr int kStageBytes = 2 * kSlice * D + 16;
+  static constexpr int kRows = 8 * NT;
+  static constexpr int kJoinFloats = kRows * D + 2 * NT * 2 * 32;  // of one warp: sums, maxima and denominators
+  static constexpr size_t kSmem = (size_t)kWarps * kStages * kStageBytes + 2 * kJoinFloats * sizeof(float);
+};
+
+// Byte offset of 16-byte piece `piece` of token t in a slice: pieces are permuted so that neither the reads of the keys (8 rows x 4 pieces)
+// nor those of the values (tokens 0, 2, 4, 6 x 8 pieces) meet in a bank.
+template <int D>
+__device__ __forceinline__ uint32_t piece_at(uint32_t t, uint32_t piece) {
+  if constexpr (D == 128) return t * 128 + ((piece ^ ((t & 2) ^ ((((t >> 2) ^ t) & 1) << 2))) << 4);
+  return (t >> 1) * 128 + (((((t & 1) << 2) | piece) ^ (((t >> 1) & 3) << 1)) << 4);
+}
+
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool real) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(real ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void copy4(uint32_t dst, const void* src, bool real) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(real ? 4 : 0) : "memory");
+}
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copies_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+// Two e4m3 values as two f16, exactly.
+__device__ __forceinline__ uint32_t widen(uint32_t two) {
+  uint32_t r;
+  asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, lo;\n\t}" : "=r"(r) : "r"(two));
+  return r;
+}
+__device__ __forceinline__ uint32_t widen_upper(uint32_t two) {
+  uint32_t r;
+  asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, hi;\n\t}" : "=r"(r) : "r"(two));
+  return r;
+}
+__device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t transpose8(uint32_t x) {
+  uint32_t r;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
+  return r;
+}
+__device__ __forceinline__ uint4 lds128(uint32_t at) {
+  uint4 v;
+  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at));
+  return v;
+}
+__device__ __forceinline__ uint2 lds64(uint32_t at) {
+  uint2 v;
+  asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(at));
+  return v;
+}
+__device__ __forceinline__ float lds32(uint32_t at) {
+  float v;
+  asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(at));
+  return v;
+}
+
+// What a sequence's keys look like to the call.
+struct Sequence {
+  int len, count, lo, steps;  // keys [lo, len) are looked at, in `steps` steps (one at least)
+};
+__device__ __forceinline__ Sequence sequence(const AttendArgs& a, int e) {
+  Sequence s;
+  sequence_of(a.cache, e, a.N, &s.len, &s.count);
+  s.lo = a.window > 0 ? max(s.len - s.count - a.window + 1, 0) & ~(kScaleBlock - 1) : 0;
+  s.steps = max((s.len - s.lo + kStep - 1) / kStep, 1);
+  return s;
+}
+
+// A place in the list of steps.
+struct Place {
+  int e, unit, step;  // unit: key head * row blocks + row block
+  Sequence s;
+};
+__device__ __forceinline__ void advance(const AttendArgs& a, int units, Place* p) {
+  if (++p->step < p->s.steps) return;
+  p->step = 0;
+  if (++p->unit < units) return;
+  p->unit = 0;
+  if (++p->e < a.E) p->s = sequence(a, p->e);
+}
+
+template <typename T, int D, int NT>
+__global__ void __launch_bounds__(kWarps * 32) attend_kernel(const __grid_constant__ AttendArgs a) {
+  using S = Shape<D, NT>;
+  constexpr int kWords = D / 16;   // 32-bit words of a key row that a lane holds; also products of 16 features, and feature tiles of 16
+  constexpr int kValueWords = D / 32;
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ long long warp_sum[kWarps];
+  __shared__ int where_e;
+  __shared__ long long where_at;
+  const CacheArgs& c = a.cache;
+  const int tid = threadIdx.x, w = tid >> 5, lane = tid & 31, g = lane >> 2, q4 = lane & 3;
+  const int units = c.heads * a.row_blocks;
+  grid_wait();
+
+  // --- this CTA's share of the steps: prefix sums over the sequences, a run of them per thread
+  const int run = (a.E + kWarps * 32 - 1) / (kWarps * 32);
+  long long mine = 0;
+  for (int e = tid * run; e < min(a.E, (tid + 1) * run); ++e) {
+    const Sequence s = sequence(a, e);
+    mine += s.steps;
+    int x, y;
+    if (blockIdx.x == 0 && !sequence_of(c, e, a.N, &x, &y)) report(c.status, kBadLength);
+  }
+  long long upto = mine;
+#pragma unroll
+  for (int m = 1; m < 32; m <<= 1) {
+    const long long o = __shfl_up_sync(0xffffffffu, upto, m);
+    if (lane >= m) upto += o;
+  }
+  if (lane == 31) warp_sum[w] = upto;
+  __syncthreads();
+  for (int i = 0; i < w; ++i) upto += warp_sum[i];
+  long long total = 0;
+  for (int i = 0; i < kWarps; ++i) total += warp_sum[i];
+  total *= units;
+  const long long ctas = min((long long)gridDim.x, total);
+  if (blockIdx.x >= ctas) {
+    if (tid == 0) a.split[blockIdx.x] = make_int4(-1, 0, 0, 0);
+    return;
+  }
+  const long long begin = blockIdx.x * total / ctas, end = (blockIdx.x + 1) * total / ctas;
+  if ((upto - mine) * units <= begin && begin < upto * units) {
+    long long at = (upto - mine) * units;
+    int e = tid * run;
+    for (;; ++e) {
+      const long long n = (long long)sequence(a, e).steps * units;
+      if (begin < at + n) break;
+      at += n;
+    }
+    where_e = e;
+    where_at = begin - at;
+  }
+  __syncthreads();
+  Place now;
+  now.e = where_e;
+  now.s = sequence(a, now.e);
+  now.unit = (int)(where_at / now.s.steps);
+  now.step = (int)(where_at % now.s.steps);
+  Place ahead = now;
+
+  // --- the warp's ring of slices
+  const uint32_t ring = smem_u32(smem) + w * S::kStages * S::kStageBytes;
+  float* const join = reinterpret_cast<float*>(smem + kWarps * S::kStages * S::kStageBytes);
+  constexpr int kLanesPerRow = D / 16, kRowsPerPass = 32 / kLanesPerRow;
+  auto fetch = [&](int stage) {
+    const int head = ahead.unit / a.row_blocks;
+    const int t0 = ahead.s.lo + ahead.step * kStep + w * kSlice;
+    const int left = ahead.s.len - t0;
+    if (left > 0) {
+      const uint32_t at = ring + stage * S::kStageBytes;
+      const int page_a = page_of(c, ahead.e, t0), page_b = left > kScaleBlock ? page_of(c, ahead.e, t0 + kScaleBlock) : -1;
+      if ((page_a < 0 || (left > kScaleBlock && page_b < 0)) && lane == 0) report(c.status, kBadPage);
+      const int in_a = t0 & ((1 << c.page_shift) - 1), in_b = (t0 + kScaleBlock) & ((1 << c.page_shift) - 1);
+      const int piece = lane % kLanesPerRow;
+#pragma unroll
+      for (int i = 0; i < kSlice / kRowsPerPass; ++i) {
+        const int t = i * kRowsPerPass + lane / kLanesPerRow;
+        const bool upper = i * kRowsPerPass >= kScaleBlock;
+        const int page = upper ? page_b : page_a, row = (upper ? in_b - kScaleBlock : in_a) + t;
+        const bool real = t < left && page >= 0;
+        const long long p = real ? page : 0, r = real ? row : 0;
+        copy16(at + piece_at<D>(t, piece), c.k + p * c.k_sp + head * c.k_sh + r * c.k_st + piece * 16, real);
+        copy16(at + kSlice * D + piece_at<D>(t, piece), c.v + p * c.v_sp + head * c.v_sh + r * c.v_st + piece * 16, real);
+      }
+      if (lane < 4) {
+        const int page = lane & 1 ? page_b : page_a, row = lane & 1 ? in_b : in_a;
+        const long long p = page >= 0 ? page : 0;
+        const float* src = lane < 2 ? c.k_scale + p * c.ks_sp + head * c.ks_sh : c.v_scale + p * c.vs_sp + head * c.vs_sh;
+        copy4(at + 2 * kSlice * D + lane * 4, src + (page >= 0 ? row / kScaleBlock : 0), page >= 0);
+      }
+    }
+  };
+  const int steps = (int)(end - begin);
+#pragma unroll
+  for (int i = 0; i < S::kStages - 1; ++i) {
+    if (i < steps) {
+      fetch(i);
+      advance(a, units, &ahead);
+    }
+    copies_commit();
+  }
+
+  uint32_t qf[NT][kWords][2];   // query rows as the second operand
+  float row_scale[NT][2];       // of rows 2 q4, 2 q4 + 1: score units of log2 e
+  int low[NT][2], high[NT][2];  // keys [low, high) that these rows see
+  int full_low = 0, full_high = 0;  // keys that all rows see
+  float o[NT][kWords][4], top[NT][2], sum[NT][2];
+  bool fresh = true;
+  int stage = 0;
+  bool later = false;  // the CTA has finished a piece of a head
+  for (int i = 0; i < steps; ++i) {
+    copies_wait<S::kStages - 2>();
+    __syncwarp();
+    if (i + S::kStages - 1 < steps) {
+      fetch(stage == 0 ? S::kStages - 1 : stage - 1);
+      advance(a, units, &ahead);
+    }
+    copies_commit();
+    const int head = now.unit / a.row_blocks, row0 = (now.unit % a.row_blocks) * S::kRows;
+    if (fresh) {
+      fresh = false;
+      full_low = 0;
+      full_high = now.s.len;
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        const int r = row0 + n * 8 + g, token = r / a.group, h = head * a.group + r % a.group;
+        const bool real = token < now.s.count;
+        const T* src = reinterpret_cast<const T*>(a.q.ptr) + (real ? now.e * a.q.se + h * a.q.sh + token * a.q.sn : 0);
+        float factor = a.scale * kLog2e;
+        uint2 raw[kWords];
+#pragma unroll
+        for (int s = 0; s < kWords; ++s)
+          raw[s] = real ? *reinterpret_cast<const uint2*>(src + (s >> 2) * 64 + q4 * 16 + (s & 3) * 4) : make_uint2(0, 0);
+        if constexpr (sizeof(T) == 2 && !std::is_same<T, __half>::value) {
+          float amax = 0.0f;
+#pragma unroll
+          for (int s = 0; s < kWords; ++s) {
+            const float2 x = sm100::unpack2<T>(raw[s].x), y = sm100::unpack2<T>(raw[s].y);
+            amax = fmaxf(fmaxf(amax, fmaxf(fabsf(x.x), fabsf(x.y))), fmaxf(fabsf(y.x), fabsf(y.y)));
+          }
+          amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+          amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+          const int exponent = min(max((int)(__float_as_uint(amax) >> 23), 27), 227);  // biased
+          const float down = __uint_as_float((uint32_t)(254 - exponent) << 23);
+          factor *= __uint_as_float((uint32_t)exponent << 23);
+#pragma unroll
+          for (int s = 0; s < kWords; ++s) {
+            const float2 x = sm100::unpack2<T>(raw[s].x), y = sm100::unpack2<T>(raw[s].y);
+            qf[n][s][0] = sm100::pack2<__half>(x.x * down, x.y * down);
+            qf[n][s][1] = sm100::pack2<__half>(y.x * down, y.y * down);
+          }
+        } else {
+#pragma unroll
+          for (int s = 0; s < kWords; ++s) {
+            qf[n][s][0] = raw[s].x;
+            qf[n][s][1] = raw[s].y;
+          }
+        }
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          row_scale[n][j] = __shfl_sync(0xffffffffu, factor, (2 * q4 + j) * 4);
+          const int t = (row0 + n * 8 + 2 * q4 + j) / a.group;  // token of the call
+          const int place = now.s.len - now.s.count + t;
+          high[n][j] = t >= now.s.count ? 0 : a.causal ? place + 1 : now.s.len;
+          low[n][j] = a.window > 0 ? place - a.window + 1 : 0;
+          if (t < now.s.count) {
+            full_high = min(full_high, high[n][j]);
+            full_low = max(full_low, low[n][j]);
+          }
+          top[n][j] = -CUDART_INF_F;
+          sum[n][j] = 0.0f;
+        }
+#pragma unroll
+        for (int m = 0; m < kWords; ++m)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) o[n][m][j] = 0.0f;
+      }
+#pragma unroll
+      for (int m = 1; m < 4; m <<= 1) {
+        full_high = min(full_high, __shfl_xor_sync(0xffffffffu, full_high, m));
+        full_low = max(full_low, __shfl_xor_sync(0xffffffffu, full_low, m));
+      }
+    }
+
+    const int t0 = now.s.lo + now.step * kStep + w * kSlice;
+    if (t0 < now.s.len) {
+      const uint32_t at = ring + stage * S::kStageBytes;
+      float s[2][NT][4];
+#pragma unroll
+      for (int mt = 0; mt < 2; ++mt) {
+        uint32_t kw[2][kWords];
+#pragma unroll
+        for (int r = 0; r < 2; ++r)
+#pragma unroll
+          for (int h = 0; h < kWords / 4; ++h) {
+            const uint4 v = lds128(at + piece_at<D>(mt * 16 + r * 8 + g, q4 + 4 * h));
+            kw[r][4 * h] = v.x; kw[r][4 * h + 1] = v.y; kw[r][4 * h + 2] = v.z; kw[r][4 * h + 3] = v.w;
+          }
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) s[mt][n][j] = 0.0f;
+#pragma unroll
+        for (int k = 0; k < kWords; ++k) {
+          const uint32_t a0 = widen(kw[0][k]), a1 = widen(kw[1][k]), a2 = widen_upper(kw[0][k]), a3 = widen_upper(kw[1][k]);
+#pragma unroll
+          for (int n = 0; n < NT; ++n) mma(s[mt][n], a0, a1, a2, a3, qf[n][k][0], qf[n][k][1]);
+        }
+      }
+      const uint32_t scales = at + 2 * kSlice * D;
+      const float ks[2] = {lds32(scales), lds32(scales + 4)}, vs[2] = {lds32(scales + 8), lds32(scales + 12)};
+      const float vl[2] = {__log2f(vs[0]), __log2f(vs[1])};
+      const bool whole = t0 >= full_low && t0 + kSlice <= full_high;
+      uint32_t weights[2][NT][2];
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        float most[2] = {-CUDART_INF_F, -CUDART_INF_F};
+#pragma unroll
+        for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            float x = s[mt][n][j] * (ks[mt] * row_scale[n][j & 1]);
+            if (a.softcap > 0.0f)  // softcap * tanh(x / softcap): tanh y = 1 - 2 / (exp(2 y) + 1), off by 2^-23 of the cap at most
+              x = a.softcap * kLog2e * (1.0f - __fdividef(2.0f, ex2(x * (2.0f / a.softcap)) + 1.0f));
+            const int t = t0 + mt * 16 + g + (j >> 1) * 8;
+            if (!whole && (t < low[n][j & 1] || t >= high[n][j & 1])) x = -CUDART_INF_F;
+            s[mt][n][j] = x;
+            most[j & 1] = fmaxf(most[j & 1], x + vl[mt]);
+          }
+        float base[2];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+#pragma unroll
+          for (int m = 4; m < 32; m <<= 1) most[j] = fmaxf(most[j], __shfl_xor_sync(0xffffffffu, most[j], m));
+          const float before = top[n][j];
+          top[n][j] = fmaxf(before, most[j]);
+          base[j] = top[n][j] == -CUDART_INF_F ? 0.0f : top[n][j];
+          const float shrink = ex2(before - base[j]);
+          sum[n][j] *= shrink;
+#pragma unroll
+          for (int m = 0; m < kWords; ++m) {
+            o[n][m][j] *= shrink;
+            o[n][m][2 + j] *= shrink;
+          }
+        }
+#pragma unroll
+        for (int mt = 0; mt < 2; ++mt) {
+          float p[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            p[j] = ex2(s[mt][n][j] - base[j & 1]);
+            sum[n][j & 1] += p[j];
+            p[j] *= vs[mt];
+          }
+          weights[mt][n][0] = transpose8(sm100::pack2<__half>(p[0], p[1]));
+          weights[mt][n][1] = transpose8(sm100::pack2<__half>(p[2], p[3]));
+        }
+      }
+#pragma unroll
+      for (int mt = 0; mt < 2; ++mt) {
+        uint32_t vw[4][kValueWords];  // tokens 2 q4, 2 q4 + 1, 2 q4 + 8, 2 q4 + 9
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int t = mt * 16 + 2 * q4 + (j & 1) + (j >> 1) * 8;
+          if constexpr (D == 128) {
+            const uint4 v = lds128(at + kSlice * D + piece_at<D>(t, g));
+            vw[j][0] = v.x; vw[j][1] = v.y; vw[j][2] = v.z; vw[j][3] = v.w;
+          } else {
+            const uint2 v = lds64(at + kSlice * D + piece_at<D>(t, g >> 1) + (g & 1) * 8);
+            vw[j][0] = v.x; vw[j][1] = v.y;
+          }
+        }
+#pragma unroll
+        for (int k = 0; k < kValueWords; ++k) {
+          const uint32_t x0 = __byte_perm(vw[0][k], vw[1][k], 0x5140), x1 = __byte_perm(vw[0][k], vw[1][k], 0x7362);
+          const uint32_t y0 = __byte_perm(vw[2][k], vw[3][k], 0x5140), y1 = __byte_perm(vw[2][k], vw[3][k], 0x7362);
+          const uint32_t a0 = widen(x0), a1 = widen_upper(x0), a2 = widen(y0), a3 = widen_upper(y0);
+          const uint32_t b0 = widen(x1), b1 = widen_upper(x1), b2 = widen(y1), b3 = widen_upper(y1);
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+            mma(o[n][2 * k], a0, a1, a2, a3, weights[mt][n][0], weights[mt][n][1]);
+            mma(o[n][2 * k + 1], b0, b1, b2, b3, weights[mt][n][0], weights[mt][n][1]);
+          }
+        }
+      }
+    }
+    stage = stage + 1 == S::kStages ? 0 : stage + 1;
+
+    const bool last_of_head = now.step + 1 == now.s.steps;
+    if (last_of_head || i + 1 == steps) {
+      fresh = true;
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+          for (int m = 4; m < 32; m <<= 1) sum[n][j] += __shfl_xor_sync(0xffffffffu, sum[n][j], m);
+      // warps 2, 3 into 0, 1, then 1 into 0, lane by lane
+      auto put = [&](float* to) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+#pragma unroll
+          for (int m = 0; m < kWords; ++m)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) to[((n * kWords + m) * 4 + j) * 32 + lane] = o[n][m][j];
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            to[S::kRows * D + (n * 2 + j) * 64 + lane] = top[n][j];
+            to[S::kRows * D + (n * 2 + j) * 64 + 32 + lane] = sum[n][j];
+          }
+        }
+      };
+      auto take = [&](const float* from) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const float theirs = from[S::kRows * D + (n * 2 + j) * 64 + lane], more = from[S::kRows * D + (n * 2 + j) * 64 + 32 + lane];
+            const float both = fmaxf(top[n][j], theirs), base = both == -CUDART_INF_F ? 0.0f : both;
+            const float x = ex2(top[n][j] - base), y = ex2(theirs - base);
+            top[n][j] = both;
+            sum[n][j] = sum[n][j] * x + more * y;
+#pragma unroll
+            for (int m = 0; m < kWords; ++m) {
+              o[n][m][j] = o[n][m][j] * x + from[((n * kWords + m) * 4 + j) * 32 + lane] * y;
+              o[n][m][2 + j] = o[n][m][2 + j] * x + from[((n * kWords + m) * 4 + 2 + j) * 32 + lane] * y;
+            }
+          }
+      };
+      if (w >= 2) put(join + (w - 2) * S::kJoinFloats);
+      __syncthreads();
+      if (w < 2) take(join + w * S::kJoinFloats);
+      __syncthreads();
+      if (w == 1) put(join);
+      __syncthreads();
+      if (w == 0) {
+        take(join);
+        const bool alone = last_of_head && i >= now.step;  // all of the head's steps were this CTA's
+        const int slot = 2 * blockIdx.x + (later ? 1 : 0);
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const int r = n * 8 + 2 * q4 + j, token = (row0 + r) / a.group, h = head * a.group + (row0 + r) % a.group;
+            constexpr int kRun = D / 8;  // neighbouring features of a lane
+            float x[kRun];
+#pragma unroll
+            for (int m = 0; m < kWords; ++m) {
+              x[2 * m] = o[n][m][j];
+              x[2 * m + 1] = o[n][m][2 + j];
+            }
+            if (alone) {
+              if (token >= a.N) continue;
+              const float inverse = token < now.s.count && sum[n][j] > 0.0f ? 1.0f / sum[n][j] : 0.0f;
+              T* dst = reinterpret_cast<T*>(const_cast<void*>(a.out.ptr)) + now.e * a.out.se + h * a.out.sh + token * a.out.sn + g * kRun;
+#pragma unroll
+              for (int v = 0; v < kRun / 8; ++v) {
+                uint4 y;
+                const float* z = x + 8 * v;
+                y.x = sm100::pack2<T>(z[0] * inverse, z[1] * inverse);
+                y.y = sm100::pack2<T>(z[2] * inverse, z[3] * inverse);
+                y.z = sm100::pack2<T>(z[4] * inverse, z[5] * inverse);
+                y.w = sm100::pack2<T>(z[6] * inverse, z[7] * inverse);
+                reinterpret_cast<uint4*>(dst)[v] = y;
+              }
+            } else {
+              float* dst = a.part_o + ((size_t)slot * S::kRows + r) * D + g * kRun;
+#pragma unroll
+              for (int v = 0; v < kRun / 4; ++v) reinterpret_cast<float4*>(dst)[v] = make_float4(x[4 * v], x[4 * v + 1], x[4 * v + 2], x[4 * v + 3]);
+              if (g == 0) {
+                a.part_ml[((size_t)slot * S::kRows + r) * 2] = top[n][j];
+                a.part_ml[((size_t)slot * S::kRows + r) * 2 + 1] = sum[n][j];
+              }
+            }
+          }
+      }
+      __syncthreads();
+      if (tid == 0 && i + 1 == steps) {
+        // a head that goes on in the next CTA and began here: this CTA's entry names it and the CTA of its last step
+        int4 entry = make_int4(-1, 0, 0, 0);
+        const bool began = i >= now.step;
+        if (!last_of_head && began) {
+          const long long last = end - 1 + (now.s.steps - 1 - now.step);
+          entry = make_int4(now.e, now.unit, (int)(((last + 1) * ctas - 1) / total), later ? 1 : 0);
+        }
+        a.split[blockIdx.x] = entry;
+      }
+      later = true;
+    }
+    advance(a, units, &now);
+  }
+}
+
+// Joins the pieces of the heads that were split: a CTA for each CTA of the kernel above (most have nothing to do) and row.
+template <typename T, int D, int NT>
+__global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ AttendArgs a) {
+  constexpr int kLanes = D / 4, kGroups = 256 / kLanes, kRows = 8 * NT;
+  __shared__ float4 sums[256];
+  __shared__ float reduced[8];
+  grid_wait();
+  const int4 entry = a.split[blockIdx.x];
+  if (entry.x < 0) return;
+  const int e = entry.x, head = entry.y / a.row_blocks, r = blockIdx.y, row = (entry.y % a.row_blocks) * kRows + r;
+  const int token = row / a.group, h = head * a.group + row % a.group;
+  if (token >= a.N) return;
+  int len, count;
+  sequence_of(a.cache, e, a.N, &len, &count);
+  const int pieces = entry.z - (int)blockIdx.x + 1;
+  auto slot = [&](int i) { return (size_t)(2 * (blockIdx.x + i) + (i == 0 ? entry.w : 0)) * kRows + r; };
+  const int tid = threadIdx.x;
+  float top = -CUDART_INF_F;
+  for (int i = tid; i < pieces; i += 256) top = fmaxf(top, a.part_ml[2 * slot(i)]);
+#pragma unroll
+  for (int m = 16; m > 0; m >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, m));
+  if ((tid & 31) == 0) reduced[tid >> 5] = top;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < 8; ++i) top = fmaxf(top, reduced[i]);
+  const float base = top == -CUDART_INF_F ? 0.0f : top;
+  const int lane = tid % kLanes, group = tid / kLanes;
+  float4 acc = make_float4(0, 0, 0, 0);
+  float total = 0.0f;
+  for (int i = group; i < pieces; i += kGroups) {
+    const float weight = ex2(a.part_ml[2 * slot(i)] - base);
+    const float4 x = reinterpret_cast<const float4*>(a.part_o + slot(i) * D)[lane];
+    total += weight * a.part_ml[2 * slot(i) + 1];
+    acc.x += weight * x.x; acc.y += weight * x.y; acc.z += weight * x.z; acc.w += weight * x.w;
+  }
+  __shared__ float totals[kGroups];
+  sums[tid] = acc;
+  if (lane == 0) totals[group] = total;
+  __syncthreads();
+  if (group != 0) return;
+  for (int i = 1; i < kGroups; ++i) {
+    const float4 x = sums[i * kLanes + lane];
+    acc.x += x.x; acc.y += x.y; acc.z += x.z; acc.w += x.w;
+    total += totals[i];
+  }
+  const float inverse = token < count && total > 0.0f ? 1.0f / total : 0.0f;
+  T* dst = reinterpret_cast<T*>(const_cast<void*>(a.out.ptr)) + e * a.out.se + h * a.out.sh + token * a.out.sn + lane * 4;
+  *reinterpret_cast<uint2*>(dst) = make_uint2(sm100::pack2<T>(acc.x * inverse, acc.y * inverse), sm100::pack2<T>(acc.z * inverse, acc.w * inverse));
+}
+
+int row_tiles(int rows) { return rows <= 8 ? 1 : rows <= 16 ? 2 : 4; }
+int ctas_per_sm(int width) { return width == 128 ? 2 : 3; }
+
+// CTAs of a call: what the GPU holds at once, and no more than the steps that the lengths can have.
+long long grid_of(int E, int N, int H, int kv_heads, int width, long long longest) {
+  const int rows = H / kv_heads * N, nt = row_tiles(rows);
+  const long long units = (long long)E * kv_heads * ((rows + 8 * nt - 1) / (8 * nt));
+  const long long steps = units * ((longest + kStep - 1) / kStep > 1 ? (longest + kStep - 1) / kStep : 1);
+  const long long most = (long long)ctas_per_sm(width) * sm_count();
+  return steps < most ? steps : most;
+}
+
+template <typename T, int D, int NT>
+cudaError_t launch(AttendArgs& a, long long grid, bool split, cudaStream_t stream) {
+  const void* fn = (const void*)attend_kernel<T, D, NT>;
+  constexpr size_t smem = Shape<D, NT>::kSmem;
+  cudaError_t err = allow_dynamic_smem(fn, smem);
+  if (err != cudaSuccess) return err;
+  void* args[] = {(void*)&a};
+  err = launch_kernel(fn, dim3((unsigned)grid), dim3(kWarps * 32), args, smem, stream);
+  if (err != cudaSuccess || !split) return err;
+  return launch_kernel((const void*)join_kernel<T, D, NT>, dim3((unsigned)grid, 8 * NT), dim3(256), args, 0, stream);
+}
+
+}  // namespace
+
+size_t attend_workspace(int E, int N, int H, int kv_heads, int width, long long longest) {
+  const long long grid = grid_of(E, N, H, kv_heads, width, longest), rows = 8 * row_tiles(H / kv_heads * N);
+  const size_t entries = ((size_t)grid * sizeof(int4) + 255) / 256 * 256;
+  return entries + (size_t)grid * 2 * rows * (width + 2) * sizeof(float);
+}
+
+cudaError_t launch_attend(AttendArgs a, int dtype, int width, void* workspace, long long longest, cudaStream_t stream) {
+  const int rows = a.group * a.N, nt = row_tiles(rows);
+  const long long grid = grid_of(a.E, a.N, a.H, a.cache.heads, width, longest);
+  a.row_blocks = (rows + 8 * nt - 1) / (8 * nt);
+  char* at = reinterpret_cast<char*>(workspace);
+  a.split = reinterpret_cast<int4*>(at);
+  at += ((size_t)grid * sizeof(int4) + 255) / 256 * 256;
+  a.part_o = reinterpret_cast<float*>(at);
+  a.part_ml = a.part_o + (size_t)grid * 2 * 8 * nt * width;
+  const bool split = longest > kStep;  // (a head of one step is never split)
+  const bool bf = dtype == MA_B200_BF16;
+#define MA_ATTEND(T, D) \
+  (nt == 1 ? launch<T, D, 1>(a, grid, split, stream) : nt == 2 ? launch<T, D, 2>(a, grid, split, stream) : launch<T, D, 4>(a, grid, split, stream))
+  if (width == 128) return bf ? MA_ATTEND(__nv_bfloat16, 128) : MA_ATTEND(__half, 128);
+  return bf ? MA_ATTEND(__nv_bfloat16, 64) : MA_ATTEND(__half, 64);
+#undef MA_ATTEND
+}
+
+}  // namespace ma

@@ -223,7 +223,8 @@ size_t fused_counter_bytes(const Geometry& g);
 cudaError_t launch_fused(const TcPlan* plan, const Geometry& g, int* counters, int stage_begin, int stage_end,
                          int wait_deps, int spin_limit, cudaStream_t stream);
 // Device address of the mapped host word that a kernel whose bounded wait gave up stores its code in (nullptr: none).
-int* host_status_word(int device);
+// (word 0: an expired wait; word 1: the cache kernels, ma_cache.cuh).
+int* host_status_word(int device, int word = 0);
 // tcgen05 stage kernels, one 128-row tile per CTA: block size and count up to 256, D <= 64, masks and padding (ma_tile.cu).
 bool tile_supported(const Geometry& g, int qk_dtype, int v_dtype, const char** why);
 // wait_expiry (self-test): a wait of every CTA runs out.
@@ -236,6 +237,6 @@ cudaError_t launch_clear(void* p, size_t bytes, cudaStream_t stream);
 cudaError_t launch_flow(const Geometry& g, int dtype, int* counters, int* host_status, bool wait_expiry, cudaStream_t stream);
 // Code of a bounded device-side wait that gave up on `device` since the last poll (0 = none); reads a mapped
 // host word, so it needs no synchronisation.
-int fused_poll_status(int device);
+int fused_poll_status(int device, int word = 0);
 
 }  // namespace ma

@@ -47,6 +47,7 @@
 //   warp 22    MMA issuer 2: the second contraction of item n, O written over the item's S
 // All hand-offs are mbarriers; every wait is bounded and abortable (see ma_sm100.cuh).
 #include <cuda.h>
+#include <string.h>
 
 #include <mutex>
 #include <type_traits>
@@ -865,17 +866,18 @@ int g_sm_count[64];
 
 size_t fused_counter_bytes(const Geometry& g) { return (size_t)g.E * g.H * 2 * g.T * sizeof(int); }
 
-int fused_poll_status(int device) {
+int fused_poll_status(int device, int word) {
   if (device < 0 || device >= 64) return 0;
   std::lock_guard<std::mutex> lock(g_host_status_mutex);
   HostStatus& hs = g_host_status[device];
   if (hs.host == nullptr) return 0;
-  const int code = *reinterpret_cast<volatile int*>(hs.host);
-  if (code != 0) *reinterpret_cast<volatile int*>(hs.host) = 0;
+  volatile int* const at = hs.host + word;
+  const int code = *at;
+  if (code != 0) *at = 0;
   return code;
 }
 
-int* host_status_word(int device) {
+int* host_status_word(int device, int word) {
   if (device < 0 || device >= 64) return nullptr;
   std::lock_guard<std::mutex> lock(g_host_status_mutex);
   HostStatus& hs = g_host_status[device];
@@ -887,7 +889,7 @@ int* host_status_word(int device) {
     (void)cudaThreadExchangeStreamCaptureMode(&mode);
     void* hp = nullptr;
     if (cudaHostAlloc(&hp, 64, cudaHostAllocMapped) == cudaSuccess) {
-      *reinterpret_cast<int*>(hp) = 0;
+      memset(hp, 0, 64);
       void* dp = nullptr;
       if (cudaHostGetDevicePointer(&dp, hp, 0) == cudaSuccess) {
         hs.host = reinterpret_cast<int*>(hp);
@@ -899,7 +901,7 @@ int* host_status_word(int device) {
     (void)cudaThreadExchangeStreamCaptureMode(&mode);
     (void)cudaGetLastError();
   }
-  return hs.dev;
+  return hs.dev != nullptr ? hs.dev + word : nullptr;
 }
 
 // Runs stages [stage_begin, stage_end) in one cooperative launch.

@@ -6,44 +6,14 @@
 // 25 us per call.  The workspace is allocated per call and released as soon as the kernels are queued: the allocator
 // is stream-ordered, so the memory is reused by the next call on the stream, nothing is held between calls, and calls
 // from several threads or streams cannot meet in one workspace.
-#include <ATen/cuda/EmptyTensor.h>
-#include <c10/cuda/CUDACachingAllocator.h>
-#include <c10/cuda/CUDAGuard.h>
-#include <c10/cuda/CUDAStream.h>
-#include <torch/csrc/autograd/custom_function.h>
-#include <torch/csrc/autograd/python_variable.h>
-#include <torch/csrc/Exceptions.h>
-#include <torch/extension.h>
-
-#include "../../include/monarch_attention_b200.h"
+#include "ma_torch.h"
 
 namespace {
 
 using at::Tensor;
 using std::optional;
 
-int dtype_code(at::ScalarType t) {
-  switch (t) {
-    case at::kFloat: return MA_B200_F32;
-    case at::kBFloat16: return MA_B200_BF16;
-    case at::kHalf: return MA_B200_F16;
-    default: return -1;
-  }
-}
-
-void raise_for_status(int code) {
-  if (code == MA_B200_OK) return;
-  const std::string msg = std::string("monarch_attention_b200: ") + ma_b200_status_string(code) + ": " + ma_b200_last_error();
-  TORCH_CHECK_VALUE(code != MA_B200_INVALID_ARGUMENT && code != MA_B200_UNSUPPORTED && code != MA_B200_WORKSPACE_TOO_SMALL, msg);
-  TORCH_CHECK(false, msg);
-}
-
-ma_b200_tensor view4(const Tensor& t) {
-  const auto s = t.strides();
-  return {t.data_ptr(), s[0], s[1], s[2]};
-}
-
-Tensor unit_inner(const Tensor& t) { return t.stride(-1) == 1 || t.size(-1) == 1 ? t : t.contiguous(); }
+using namespace ma_torch;
 
 void check_inputs(const Tensor& q, const Tensor& k, const Tensor& v, const optional<Tensor>& mask) {
   TORCH_CHECK_VALUE(q.dim() == 4 && k.dim() == 4 && v.dim() == 4, "query, key and value must have shape (batch, heads, tokens, width)");
@@ -228,6 +198,14 @@ PyObject* py_forward(PyObject*, PyObject* const* args, Py_ssize_t n) {
 
 PyMethodDef methods[] = {{"forward", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(py_forward)), METH_FASTCALL,
                           "forward(q, k, v, mask, T, B, pre_pad, kernel, out, token_major) -> Tensor | None"},
+                         {"rotary", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(py_rotary)), METH_FASTCALL,
+                          "rotary(q, k | None, turns, dim, pairs, magnitude, positions | None, inverse) -> (Tensor, Tensor | None)"},
+                         {"append", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(py_append)), METH_FASTCALL,
+                          "append(k_cache, v_cache, k_scale, v_scale, k, v, page_table, lengths, counts | None, query | None, turns | None, dim, "
+                          "pairs, magnitude) -> Tensor | None"},
+                         {"attend", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(py_attend)), METH_FASTCALL,
+                          "attend(q, k_cache, v_cache, k_scale, v_scale, page_table, lengths, counts | None, causal, scale, softcap, window, "
+                          "out | None, token_major) -> Tensor"},
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_native", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

@@ -20,6 +20,7 @@ import torch
 import torch.nn as nn
 
 from . import _cabi
+from .rotary import rotary_b200
 
 Tensor = torch.Tensor
 MonarchAttentionFn = Callable[[Tensor, Tensor, Tensor, "Tensor | None", int, int, bool], Tensor]
@@ -75,16 +76,20 @@ def _check_device_free_inputs(q: Tensor, k: Tensor, v: Tensor, attn_mask: Tensor
 _native_forward = None
 
 
-def _load_native():
-    """The native entry point (monarch_attention_b200/_native.so); raises RuntimeError when it has not been built."""
-    global _native_forward
+def native_module():
+    """The native entry points (monarch_attention_b200/_native.so); raises RuntimeError when they have not been built."""
     _cabi.load()
     try:
         from . import _native
     except ImportError as err:
         raise RuntimeError("monarch_attention_b200/_native.so is missing or does not match this PyTorch: build it with "
                            "`python -m monarch_attention_b200.build`. There is no fallback implementation.") from err
-    _native_forward = _native.forward
+    return _native
+
+
+def _load_native():
+    global _native_forward
+    _native_forward = native_module().forward
     return _native_forward
 
 
@@ -166,8 +171,12 @@ class MonarchAttention(nn.Module):
         # Set to True to get the result as a view of a (batch, tokens, heads, width) buffer (see
         # monarch_attention_b200); only the default implementation honours it.
         self.token_major_output = False
+        # Set to a RotaryPositions to have queries and keys rotated at positions 0 .. N-1 before the attention.
+        self.rotary = None
 
     def forward(self, query, key, value, attention_mask=None):
+        if self.rotary is not None:
+            query, key = rotary_b200(query, key, self.rotary)
         if self.token_major_output and self._impl_fn is monarch_attention_b200:
             return monarch_attention_b200(query, key, value, attention_mask, self.num_steps, self.block_size,
                                           self.pad_type == PadType.pre, token_major_output=True)
