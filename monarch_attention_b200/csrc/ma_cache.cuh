@@ -60,6 +60,7 @@ struct AttendArgs {
   int causal, window;   // window 0: none
   float scale, softcap;  // softcap 0: none
   int row_blocks;       // blocks of 8 * kernel tiles rows; row = token * group + head of the group
+  uint32_t k16[3], v16[3];  // strides of a page, head and token in units of 16 bytes: products with them are one instruction
   float *part_o, *part_ml;  // of the pieces of split heads: two a CTA
   int4* split;              // one a CTA: the head whose pieces begin there
 };

@@ -38,7 +38,7 @@ int check_cache(const ma_b200_cache& c, const ma_b200_sequences& s, int E, int H
       reinterpret_cast<uintptr_t>(c.v_scale) % 4 != 0)
     return invalid("cache: k and v must be 16-byte, the scales 4-byte aligned");
   for (int64_t st : {c.k_stride_page, c.k_stride_head, c.k_stride_token, c.v_stride_page, c.v_stride_head, c.v_stride_token})
-    if (st < 0 || st % 16 != 0) return invalid("cache: strides of k and v must be multiples of 16 and not negative");
+    if (st < 0 || st % 16 != 0 || st / 16 > 0xffffffffLL) return invalid("cache: strides of k and v must be multiples of 16, below 2^36 and not negative");
   for (int64_t st : {c.ks_stride_page, c.ks_stride_head, c.vs_stride_page, c.vs_stride_head})
     if (st < 0) return invalid("cache: negative stride of the scales");
   if (s.page_table == nullptr || s.lengths == nullptr) return invalid("page_table and lengths must not be NULL");
@@ -92,7 +92,7 @@ int ma_b200_rotary_apply(const ma_b200_rotation* p, void* stream) {
   ma::RotaryArgs rotary;
   if (const char* why = ma::rotary_args(&p->rotary, p->D, &rotary)) return invalid(why);
   if (p->inverse) rotary.sign = -1.0f;
-  if ((long long)p->E * ((p->N + 15) / 16) > 0x7fffffffLL || p->H + p->Hk > 65535 || p->D > 1 << 16) return invalid("too many tokens, heads or features");
+  if ((long long)p->E * p->N > 0x7fffffffLL || p->H + p->Hk > 65535 || p->D > 1 << 16) return invalid("too many tokens, heads or features");
   return launched(ma::launch_rotary(p, rotary, reinterpret_cast<cudaStream_t>(stream)), "rotary");
 }
 
@@ -102,11 +102,11 @@ int ma_b200_cache_append(const ma_b200_append* p, void* stream) {
   ma::AppendArgs a{};
   int rc = check_cache(p->cache, p->sequences, p->E, p->H, p->N, p->dtype, &a.cache);
   if (rc != MA_B200_OK) return rc;
-  const size_t lane = p->cache.width / 32 * 2;  // bytes that a lane reads at once
+  const size_t lane = 16;  // bytes that a lane reads at once
   if ((rc = check_tensor(p->k, "k", 2, lane)) != MA_B200_OK || (rc = check_tensor(p->v, "v", 2, lane)) != MA_B200_OK) return rc;
   if (p->H > 0 && ((rc = check_tensor(p->q, "q", 2, lane)) != MA_B200_OK || (rc = check_tensor(p->q_out, "q_out", 2, lane)) != MA_B200_OK)) return rc;
   if (const char* why = ma::rotary_args(p->rotary, p->cache.width, &a.rotary)) return invalid(why);
-  if (p->rotary != nullptr && p->rotary->dim % 8 != 0) return fail_with(MA_B200_UNSUPPORTED, "rotary: dim must be a multiple of 8 here");
+  if (p->rotary != nullptr && p->rotary->dim % 16 != 0) return fail_with(MA_B200_UNSUPPORTED, "rotary: dim must be a multiple of 16 here");
   if ((long long)p->E * ((p->N + 14) / 16 + 1) > 0x7fffffffLL || (long long)2 * p->cache.heads + p->H > (1 << 18)) return invalid("too many tokens or heads");
   a.k = view(p->k); a.v = view(p->v); a.q = view(p->q); a.q_out = view(p->q_out);
   a.E = p->E; a.N = p->N; a.H = p->H;

@@ -5,31 +5,23 @@
 // raise its scale without a second rounding: older codes move by whole exponents, exact but for subnormal ones.  n is held to [-40, 60]: the
 // attention's sums are in units of the largest weight times scale, and scales further apart than 2^100 would leave 32 bits.
 //
-// A warp takes one head of one block, for the keys, the values or the queries: lane l holds features [l D/32, (l+1) D/32) of the 16 tokens in
-// registers, so that a row is one coalesced access, the partner of a rotated feature is in the same lane (interleaved pairs) or a
-// shuffle away (half), and the block's magnitude is a reduction over the warp.  The sines of the block's positions are computed once for
-// the CTA's warps.  Bound by memory for prompts (16-bit rows in, 8-bit rows out), by latency for single tokens.
+// A lane holds 8 neighbouring features of a row (16 bytes), so that the partner of a rotated feature is in the same lane (interleaved
+// pairs) or a shuffle away (half); the sines of a CTA's tokens are computed once into shared memory.
+//  * Prompts: a CTA takes a block of 16 tokens and some heads, a lane one of the tokens, whose sines it keeps in registers while it
+//    walks over the heads, several rows in flight.  A block's largest magnitude is a reduction over each warp and a maximum in shared
+//    memory; rows stay in registers in 16 bits until the scale is known.  Bound by memory.
+//  * Single tokens: a row is all there is of a block, so rows of different heads are spread over the warps, and nothing is exchanged
+//    between them.  Bound by latency: the row's load does not wait for the length and the page.
 #include <cuda_fp8.h>
 
 #include "ma_cache.cuh"
+#include "ma_sm100.cuh"
 
 namespace ma {
 namespace {
 
-constexpr int kWarps = 8;
-
-template <int F>
-struct Word;
-template <>
-struct Word<4> {
-  using Half = uint2;
-  using Code = uint32_t;
-};
-template <>
-struct Word<2> {
-  using Half = uint32_t;
-  using Code = uint16_t;
-};
+constexpr int kWarps = 8, kThreads = 32 * kWarps;
+constexpr int F = 8;  // features of a lane
 
 // The smallest n in [-40, 60] with amax <= 448 * 2^n, as 2^n: 448 = 1.75 * 2^8, so a mantissa above 1.75 takes one more.
 __device__ __forceinline__ float scale_for(float amax) {
@@ -37,155 +29,262 @@ __device__ __forceinline__ float scale_for(float amax) {
   return __uint_as_float((uint32_t)(min(max(n, -40), 60) + 127) << 23);
 }
 
-template <int F>
-__device__ __forceinline__ typename Word<F>::Code to_codes(const float (&x)[F]) {
-  uint32_t w = 0;
-#pragma unroll
-  for (int i = 0; i < F; i += 2) w |= (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(x[i], x[i + 1]), __NV_SATFINITE, __NV_E4M3) << (8 * i);
-  return (typename Word<F>::Code)w;
+__device__ __forceinline__ uint32_t four_codes(float a, float b, float c, float d) {
+  return (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3) |
+         (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(c, d), __NV_SATFINITE, __NV_E4M3) << 16;
 }
-template <int F>
-__device__ __forceinline__ void from_codes(typename Word<F>::Code w, float (&x)[F]) {
+__device__ __forceinline__ uint2 to_codes(const float (&x)[F]) { return make_uint2(four_codes(x[0], x[1], x[2], x[3]), four_codes(x[4], x[5], x[6], x[7])); }
+// Codes of a block whose scale has risen by 1 / ratio.
+__device__ __forceinline__ uint32_t moved(uint32_t codes, float ratio) {
+  const float2 lo = __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)codes, __NV_E4M3)));
+  const float2 hi = __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(codes >> 16), __NV_E4M3)));
+  return four_codes(lo.x * ratio, lo.y * ratio, hi.x * ratio, hi.y * ratio);
+}
+
+template <typename T>
+__device__ __forceinline__ void widen(const uint4& raw, float (&x)[F]) {
+  const uint32_t words[4] = {raw.x, raw.y, raw.z, raw.w};
 #pragma unroll
-  for (int i = 0; i < F; i += 2) {
-    const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)((uint32_t)w >> (8 * i)), __NV_E4M3);
-    const float2 f = __half22float2(__half2(h));
-    x[i] = f.x;
-    x[i + 1] = f.y;
+  for (int i = 0; i < 4; ++i) {
+    const float2 f = sm100::unpack2<T>(words[i]);
+    x[2 * i] = f.x;
+    x[2 * i + 1] = f.y;
+  }
+}
+template <typename T>
+__device__ __forceinline__ uint4 narrow(const float (&x)[F]) {
+  return make_uint4(sm100::pack2<T>(x[0], x[1]), sm100::pack2<T>(x[2], x[3]), sm100::pack2<T>(x[4], x[5]), sm100::pack2<T>(x[6], x[7]));
+}
+__device__ __forceinline__ float largest(const float (&x)[F]) {
+  float m = fabsf(x[0]);
+#pragma unroll
+  for (int i = 1; i < F; ++i) m = fmaxf(m, fabsf(x[i]));
+  return m;
+}
+
+// How the lane's features f0 .. f0 + 7 are rotated at one position.
+struct Turn {
+  float2 cs[F];  // half: of each feature, the sine with its sign; interleaved: of its four pairs
+  int partner;   // lane that holds the other half
+  bool turned;
+};
+// `sines`: those of the position, by pair; not looked at where `real` is false.
+template <int D>
+__device__ __forceinline__ Turn turn_of(const RotaryArgs& r, const float2* sines, bool real, int lane, int f0) {
+  Turn t;
+  t.turned = f0 < 2 * r.pairs;
+  const bool upper = f0 >= r.pairs;
+  constexpr int kLanes = D / F;  // of a row
+  t.partner = !t.turned || r.interleaved ? lane : (lane & ~(kLanes - 1)) | ((lane & (kLanes - 1)) + (upper ? -r.pairs / F : r.pairs / F));
+#pragma unroll
+  for (int i = 0; i < F; ++i) {
+    t.cs[i] = make_float2(1.0f, 0.0f);
+    if (!t.turned || !real) continue;
+    if (!r.interleaved) {
+      t.cs[i] = sines[f0 + i - (upper ? r.pairs : 0)];
+      if (!upper) t.cs[i].y = -t.cs[i].y;
+    } else if (i < F / 2) {
+      t.cs[i] = sines[f0 / 2 + i];
+    }
+  }
+  return t;
+}
+// Features of a row turned in place (the whole warp takes part).
+__device__ __forceinline__ void apply(const RotaryArgs& r, const Turn& t, float (&x)[F]) {
+  if (r.interleaved) {
+#pragma unroll
+    for (int i = 0; i < F; i += 2) {
+      const float u = x[i], w = x[i + 1];
+      x[i] = u * t.cs[i / 2].x - w * t.cs[i / 2].y;
+      x[i + 1] = u * t.cs[i / 2].y + w * t.cs[i / 2].x;
+    }
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < F; ++i) {
+    const float w = __shfl_sync(0xffffffffu, x[i], t.partner);
+    x[i] = x[i] * t.cs[i].x + w * t.cs[i].y;
   }
 }
 
+// What a call has to know of sequence e; counts that cannot be are taken as none.
+__device__ __forceinline__ void span_of(const CacheArgs& c, int e, int N, bool reports, int* len, int* count) {
+  bool fine = sequence_of(c, e, N, len, count);
+  if (*count > *len) fine = false;
+  if (fine) return;
+  if (reports) report(c.status, kBadLength);
+  *count = 0;
+}
+
 template <typename T, int D>
-__global__ void __launch_bounds__(kWarps * 32) append_kernel(const __grid_constant__ AppendArgs a) {
-  constexpr int F = D / 32;
-  using Half = typename Word<F>::Half;
-  using Code = typename Word<F>::Code;
+__global__ void __launch_bounds__(kThreads, 2) append_kernel(const __grid_constant__ AppendArgs a) {
+  constexpr int kLanes = D / F, kRows = 32 / kLanes;               // rows of a warp at once
+  constexpr int kTeam = kScaleBlock / kRows, kTeams = kWarps / kTeam;  // warps that hold the 16 tokens of a head between them
+  constexpr int kHeads = 4;                                        // of keys, and of values, that a team has in flight
   __shared__ float2 table[kScaleBlock * D / 2];
+  __shared__ unsigned int most[3][kTeams][2][kHeads];
   const CacheArgs& c = a.cache;
+  const int tid = threadIdx.x, lane = tid & 31, f0 = (lane & (kLanes - 1)) * F;
+  const int team = (tid >> 5) / kTeam, slot = ((tid >> 5) % kTeam) * kRows + lane / kLanes;  // the lane's token of the block
   grid_wait();
   const int blocks = (a.N + kScaleBlock - 2) / kScaleBlock + 1;  // that N tokens can touch
   const int e = blockIdx.x / blocks;
   int len, count;
-  bool fine = sequence_of(c, e, a.N, &len, &count);
-  if (count > len) fine = false;
-  if (!fine) {  // nothing is appended
-    if (threadIdx.x == 0 && blockIdx.y == 0) report(c.status, kBadLength);
-    count = 0;
-  }
+  span_of(c, e, a.N, tid == 0 && blockIdx.y == 0, &len, &count);
   const int start = len - count;
   const int base = (start / kScaleBlock + blockIdx.x % blocks) * kScaleBlock;  // position of the block's first token
   const int pairs = a.rotary.pairs;
   // slots [first, last) of the block take new tokens
   const int first = max(start - base, 0), last = min(max(len - base, 0), kScaleBlock);
-  if (first < last)
-    for (int i = threadIdx.x; i < (last - first) * pairs; i += kWarps * 32) {
-      const int t = first + i / pairs, j = i % pairs;
-      table[t * pairs + j] = rotary_turn(a.rotary, j, base + t);
-    }
-  __syncthreads();
-  const int page = first < last ? page_of(c, e, base) : -1;
-  if (first < last && page < 0 && threadIdx.x == 0 && blockIdx.y == 0) report(c.status, kBadPage);
+  const bool any = first < last;
+  if (any)
+    for (int i = first * pairs + tid; i < last * pairs; i += kThreads) table[i] = rotary_turn(a.rotary, i % pairs, base + i / pairs);
+  if (tid < 3 * kTeams * 2 * kHeads) (&most[0][0][0][0])[tid] = 0;
+  const int page = any ? page_of(c, e, base) : -1;
+  if (any && page < 0 && tid == 0 && blockIdx.y == 0) report(c.status, kBadPage);
   const int in_page = base & ((1 << c.page_shift) - 1);
-  const int lane = threadIdx.x & 31, f0 = lane * F;
-  const int tasks = 2 * c.heads + a.H;
-  for (int task = blockIdx.y * kWarps + (threadIdx.x >> 5); task < tasks; task += gridDim.y * kWarps) {
-    const int kind = task < c.heads ? 0 : task < 2 * c.heads ? 1 : 2;  // keys, values, queries
-    const int h = task - kind * c.heads;
+  __syncthreads();
+  const bool fresh = slot >= first && slot < last;  // the lane's token is new
+  const int n = base + slot - start;                // the call's number of it
+  const Turn turn = turn_of<D>(a.rotary, table + slot * pairs, fresh, lane, f0);
+
+  // --- keys and values, kHeads at a time
+  const int stride = gridDim.y * kTeams * kHeads;
+  if (page >= 0) {
+    int round = 0;
+    for (int g0 = blockIdx.y * kTeams * kHeads; g0 < c.heads; g0 += stride, round = round == 2 ? 0 : round + 1) {  // (the same for all teams)
+      const int h0 = g0 + team * kHeads;
+      uint4 raw[2][kHeads];
+      float before[2][kHeads];
+#pragma unroll
+      for (int kind = 0; kind < 2; ++kind)
+#pragma unroll
+        for (int h = 0; h < kHeads; ++h) {
+          const View4& view = kind == 0 ? a.k : a.v;
+          raw[kind][h] = make_uint4(0, 0, 0, 0);
+          before[kind][h] = 0.0f;
+          if (h0 + h >= c.heads) continue;
+          if (fresh) raw[kind][h] = *reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(view.ptr) + e * view.se + (h0 + h) * view.sh + n * view.sn + f0);
+          if (first > 0)  // the block has older tokens, and a scale
+            before[kind][h] = (kind == 0 ? c.k_scale + page * c.ks_sp + (h0 + h) * c.ks_sh : c.v_scale + page * c.vs_sp + (h0 + h) * c.vs_sh)[in_page / kScaleBlock];
+        }
+#pragma unroll
+      for (int kind = 0; kind < 2; ++kind)
+#pragma unroll
+        for (int h = 0; h < kHeads; ++h) {
+          float x[F];
+          widen<T>(raw[kind][h], x);
+          if (kind == 0 && pairs > 0) apply(a.rotary, turn, x);
+          const unsigned int bits = __reduce_max_sync(0xffffffffu, __float_as_uint(largest(x)));  // (slots without a new token are zero)
+          if (lane == 0) atomicMax(&most[round][team][kind][h], bits);
+        }
+      // the maxima of the round after next are zero again for all behind this barrier: their last readers were before the one before it
+      if (tid < kTeams * 2 * kHeads) (&most[round == 2 ? 0 : round + 1][0][0][0])[tid] = 0;
+      __syncthreads();
+#pragma unroll
+      for (int kind = 0; kind < 2; ++kind)
+#pragma unroll
+        for (int h = 0; h < kHeads; ++h) {
+          const float scale = fmaxf(scale_for(__uint_as_float(most[round][team][kind][h])), before[kind][h]);
+          float x[F];
+          widen<T>(raw[kind][h], x);
+          if (kind == 0 && pairs > 0) apply(a.rotary, turn, x);
+          if (h0 + h >= c.heads) continue;
+          uint2* const row = reinterpret_cast<uint2*>((kind == 0 ? c.k + page * c.k_sp + (h0 + h) * c.k_sh + (in_page + slot) * c.k_st
+                                                                 : c.v + page * c.v_sp + (h0 + h) * c.v_sh + (in_page + slot) * c.v_st) + f0);
+          if (fresh) {
+            const float inverse = 1.0f / scale;
+#pragma unroll
+            for (int i = 0; i < F; ++i) x[i] *= inverse;
+            *row = to_codes(x);
+          } else if (slot < first && scale != before[kind][h]) {
+            const uint2 codes = *row;
+            const float ratio = before[kind][h] / scale;
+            *row = make_uint2(moved(codes.x, ratio), moved(codes.y, ratio));
+          }
+          if (slot == first && f0 == 0)
+            (kind == 0 ? c.k_scale + page * c.ks_sp + (h0 + h) * c.ks_sh : c.v_scale + page * c.vs_sp + (h0 + h) * c.vs_sh)[in_page / kScaleBlock] = scale;
+        }
+    }
+  }
+
+  // --- queries; rows behind the sequence's tokens become zeros
+  const bool mine = n >= 0 && n < a.N;
+  const T* src = reinterpret_cast<const T*>(a.q.ptr) + e * a.q.se + n * a.q.sn + f0;
+  T* dst = reinterpret_cast<T*>(const_cast<void*>(a.q_out.ptr)) + e * a.q_out.se + n * a.q_out.sn + f0;
+  constexpr int kInFlight = 8;
+  for (int h0 = (blockIdx.y * kTeams + team) * kInFlight; h0 < a.H; h0 += gridDim.y * kTeams * kInFlight) {
+    uint4 raw[kInFlight];
+#pragma unroll
+    for (int i = 0; i < kInFlight; ++i) {
+      raw[i] = make_uint4(0, 0, 0, 0);
+      if (fresh && h0 + i < a.H) raw[i] = *reinterpret_cast<const uint4*>(src + (h0 + i) * a.q.sh);
+    }
+#pragma unroll
+    for (int i = 0; i < kInFlight; ++i) {
+      float x[F];
+      widen<T>(raw[i], x);
+      if (pairs > 0) apply(a.rotary, turn, x);
+      if (mine && h0 + i < a.H) *reinterpret_cast<uint4*>(dst + (h0 + i) * a.q_out.sh) = narrow<T>(x);
+    }
+  }
+}
+
+// One token of each sequence: a row of 128 features, two to a warp, or of 64, four.
+template <typename T, int D>
+__global__ void __launch_bounds__(kThreads) append_token_kernel(const __grid_constant__ AppendArgs a) {
+  constexpr int kLanes = D / F, kRows = 32 / kLanes;
+  __shared__ float2 table[D / 2];
+  const CacheArgs& c = a.cache;
+  const int lane = threadIdx.x & 31, f0 = (lane & (kLanes - 1)) * F, e = blockIdx.x;
+  const int task = (blockIdx.y * kWarps + (threadIdx.x >> 5)) * kRows + lane / kLanes, tasks = 2 * c.heads + a.H;
+  const int kind = task < c.heads ? 0 : task < 2 * c.heads ? 1 : 2;  // keys, values, queries
+  const int h = task - kind * c.heads;
+  grid_wait();
+  uint4 raw = make_uint4(0, 0, 0, 0);
+  if (task < tasks) {
     const View4& view = kind == 0 ? a.k : kind == 1 ? a.v : a.q;
-    const T* src = reinterpret_cast<const T*>(view.ptr) + e * view.se + h * view.sh + f0;
-    Half raw[kScaleBlock];
+    raw = *reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(view.ptr) + e * view.se + h * view.sh + f0);
+  }
+  int len, count;
+  span_of(c, e, 1, threadIdx.x == 0 && blockIdx.y == 0, &len, &count);
+  const int position = max(len - 1, 0), first = position & (kScaleBlock - 1), pairs = a.rotary.pairs;
+  const int page = count > 0 ? page_of(c, e, position) : -1;
+  if (threadIdx.x < pairs) table[threadIdx.x] = rotary_turn(a.rotary, threadIdx.x, position);
+  if (count > 0 && page < 0 && threadIdx.x == 0 && blockIdx.y == 0) report(c.status, kBadPage);
+  const bool cached = task < 2 * c.heads && page >= 0;
+  const int in_page = position & ((1 << c.page_shift) - 1);
+  float* at = nullptr;
+  float before = 0.0f;
+  if (cached) {
+    at = (kind == 0 ? c.k_scale + page * c.ks_sp + h * c.ks_sh : c.v_scale + page * c.vs_sp + h * c.vs_sh) + in_page / kScaleBlock;
+    if (first > 0) before = *at;
+  }
+  __syncthreads();  // (also: the row's lanes have read the older scale)
+  float x[F];
+  widen<T>(raw, x);
+  if (pairs > 0) apply(a.rotary, turn_of<D>(a.rotary, table, kind != 1, lane, f0), x);  // (values, next to keys in a warp, keep theirs)
+  float amax = largest(x);
 #pragma unroll
-    for (int t = 0; t < kScaleBlock; ++t)
-      raw[t] = t >= first && t < last ? *reinterpret_cast<const Half*>(src + (base + t - start) * view.sn) : Half{};
-    float x[kScaleBlock][F];
+  for (int m = kLanes / 2; m > 0; m >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, m));
+  if (task < tasks && kind == 2) {
+    T* const dst = reinterpret_cast<T*>(const_cast<void*>(a.q_out.ptr)) + e * a.q_out.se + h * a.q_out.sh + f0;
+    *reinterpret_cast<uint4*>(dst) = count > 0 ? narrow<T>(x) : make_uint4(0, 0, 0, 0);
+  }
+  if (!cached) return;
+  const float scale = fmaxf(scale_for(amax), before);
+  const long long st = kind == 0 ? c.k_st : c.v_st;
+  uint8_t* const block = (kind == 0 ? c.k + page * c.k_sp + h * c.k_sh : c.v + page * c.v_sp + h * c.v_sh) + (in_page - first) * st + f0;
+  if (f0 == 0) *at = scale;
+  const float inverse = 1.0f / scale;
 #pragma unroll
-    for (int t = 0; t < kScaleBlock; ++t) {
-      const T* r = reinterpret_cast<const T*>(&raw[t]);
-#pragma unroll
-      for (int i = 0; i < F; ++i) x[t][i] = Cvt<T>::to_f(r[i]);
-    }
-    if (kind != 1 && pairs > 0) {
-      const bool turned = f0 < 2 * pairs;
-      if (a.rotary.interleaved) {
-#pragma unroll
-        for (int t = 0; t < kScaleBlock; ++t) {
-          if (t < first || t >= last || !turned) continue;
-#pragma unroll
-          for (int i = 0; i < F; i += 2) {
-            const float2 cs = table[t * pairs + (f0 + i) / 2];
-            const float u = x[t][i], w = x[t][i + 1];
-            x[t][i] = u * cs.x - w * cs.y;
-            x[t][i + 1] = u * cs.y + w * cs.x;
-          }
-        }
-      } else {
-        const bool upper = f0 >= pairs;
-        const int other = (lane + (upper ? -pairs / F : pairs / F)) & 31, j = upper ? f0 - pairs : f0;
-#pragma unroll
-        for (int t = 0; t < kScaleBlock; ++t) {
-          if (t < first || t >= last) continue;  // (the same for the whole warp)
-#pragma unroll
-          for (int i = 0; i < F; ++i) {
-            const float w = __shfl_sync(0xffffffffu, x[t][i], other);
-            if (turned) {
-              const float2 cs = table[t * pairs + j + i];
-              x[t][i] = upper ? w * cs.y + x[t][i] * cs.x : x[t][i] * cs.x - w * cs.y;
-            }
-          }
-        }
-      }
-    }
-    if (kind == 2) {
-      T* dst = reinterpret_cast<T*>(const_cast<void*>(a.q_out.ptr)) + e * a.q_out.se + h * a.q_out.sh + f0;
-#pragma unroll
-      for (int t = 0; t < kScaleBlock; ++t) {
-        const int n = base + t - start;  // rows behind the sequence's tokens become zeros
-        if (n < 0 || n >= a.N) continue;
-        Half out;
-        T* r = reinterpret_cast<T*>(&out);
-#pragma unroll
-        for (int i = 0; i < F; ++i) r[i] = Cvt<T>::from_f(t < last ? x[t][i] : 0.0f);
-        *reinterpret_cast<Half*>(dst + n * a.q_out.sn) = out;
-      }
-      continue;
-    }
-    if (page < 0) continue;
-    float amax = 0.0f;
-#pragma unroll
-    for (int t = 0; t < kScaleBlock; ++t)
-#pragma unroll
-      for (int i = 0; i < F; ++i) amax = fmaxf(amax, fabsf(x[t][i]));  // (slots without a new token are zero)
-#pragma unroll
-    for (int m = 16; m > 0; m >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, m));
-    float* at = kind == 0 ? c.k_scale + page * c.ks_sp + h * c.ks_sh : c.v_scale + page * c.vs_sp + h * c.vs_sh;
-    at += in_page / kScaleBlock;
-    float scale = scale_for(amax), before = scale;
-    if (first > 0) {  // the block has older tokens
-      before = *at;
-      scale = fmaxf(scale, before);
-    }
-    __syncwarp();
-    if (lane == 0) *at = scale;
-    uint8_t* rows = kind == 0 ? c.k + page * c.k_sp + h * c.k_sh : c.v + page * c.v_sp + h * c.v_sh;
-    const long long pitch = kind == 0 ? c.k_st : c.v_st;
-    rows += in_page * pitch + f0;
-    if (scale != before) {
-      const float ratio = before / scale;
-      for (int t = 0; t < first; ++t) {
-        float y[F];
-        from_codes<F>(*reinterpret_cast<const Code*>(rows + t * pitch), y);
-#pragma unroll
-        for (int i = 0; i < F; ++i) y[i] *= ratio;
-        *reinterpret_cast<Code*>(rows + t * pitch) = to_codes<F>(y);
-      }
-    }
-    const float inverse = 1.0f / scale;
-#pragma unroll
-    for (int t = 0; t < kScaleBlock; ++t) {
-      if (t < first || t >= last) continue;
-#pragma unroll
-      for (int i = 0; i < F; ++i) x[t][i] *= inverse;
-      *reinterpret_cast<Code*>(rows + t * pitch) = to_codes<F>(x[t]);
+  for (int i = 0; i < F; ++i) x[i] *= inverse;
+  *reinterpret_cast<uint2*>(block + first * st) = to_codes(x);
+  if (first > 0 && scale != before) {
+    const float ratio = before / scale;
+    for (int t = 0; t < first; ++t) {
+      uint2* const row = reinterpret_cast<uint2*>(block + t * st);
+      *row = make_uint2(moved(row->x, ratio), moved(row->y, ratio));
     }
   }
 }
@@ -193,15 +292,22 @@ __global__ void __launch_bounds__(kWarps * 32) append_kernel(const __grid_consta
 }  // namespace
 
 cudaError_t launch_append(const AppendArgs& a, int dtype, int width, cudaStream_t stream) {
-  const long long blocks = (a.N + kScaleBlock - 2) / kScaleBlock + 1;
-  const int rounds = (2 * a.cache.heads + a.H + kWarps - 1) / kWarps;
-  // few blocks: a round of tasks for each CTA, so that no warp takes a second
-  const long long wanted = 4LL * sm_count() / (a.E * blocks) + 1;
-  const unsigned y = (unsigned)(wanted < rounds ? wanted : rounds);
-  const void* fn = dtype == MA_B200_BF16 ? (width == 128 ? (const void*)append_kernel<__nv_bfloat16, 128> : (const void*)append_kernel<__nv_bfloat16, 64>)
-                                         : (width == 128 ? (const void*)append_kernel<__half, 128> : (const void*)append_kernel<__half, 64>);
   void* args[] = {(void*)&a};
-  return launch_kernel(fn, dim3((unsigned)(a.E * blocks), y), dim3(kWarps * 32), args, 0, stream);
+  const bool bf = dtype == MA_B200_BF16;
+  if (a.N == 1) {
+    const int rows = kWarps * 32 * F / width;  // of a CTA
+    const void* fn = bf ? (width == 128 ? (const void*)append_token_kernel<__nv_bfloat16, 128> : (const void*)append_token_kernel<__nv_bfloat16, 64>)
+                        : (width == 128 ? (const void*)append_token_kernel<__half, 128> : (const void*)append_token_kernel<__half, 64>);
+    return launch_kernel(fn, dim3(a.E, (2 * a.cache.heads + a.H + rows - 1) / rows), dim3(kThreads), args, 0, stream);
+  }
+  const void* fn = bf ? (width == 128 ? (const void*)append_kernel<__nv_bfloat16, 128> : (const void*)append_kernel<__nv_bfloat16, 64>)
+                      : (width == 128 ? (const void*)append_kernel<__half, 128> : (const void*)append_kernel<__half, 64>);
+  const long long blocks = (long long)a.E * ((a.N + kScaleBlock - 2) / kScaleBlock + 1);
+  // few blocks: their heads are spread over more CTAs, each of which computes the sines again
+  const int per = width == 128 ? 4 : 8;
+  const int groups = (a.cache.heads + per - 1) / per;
+  const long long wanted = 4LL * sm_count() / blocks + 1;
+  return launch_kernel(fn, dim3((unsigned)blocks, (unsigned)(wanted < groups ? wanted : groups)), dim3(kThreads), args, 0, stream);
 }
 
 }  // namespace ma

@@ -29,15 +29,19 @@ using sm100::ex2;
 using sm100::kLog2e;
 using sm100::smem_u32;
 
+constexpr float kSlack = 8.0f;  // weights are at most 2^8 of the reference: f16 holds them as exactly as those up to 1
 constexpr int kWarps = 4, kSlice = 32, kStep = kWarps * kSlice;  // tokens of a warp and of a CTA at a time
 
 template <int D, int NT>
 struct Shape {
-  static constexpr int kStages = D == 128 ? 3 : 4;
+  static constexpr int kStages = D == 128 ? 2 : 3;
   static constexpr int kStageBytes = 2 * kSlice * D + 16;
   static constexpr int kRows = 8 * NT;
-  static constexpr int kJoinFloats = kRows * D + 2 * NT * 2 * 32;  // of one warp: sums, maxima and denominators
-  static constexpr size_t kSmem = (size_t)kWarps * kStages * kStageBytes + 2 * kJoinFloats * sizeof(float);
+  static constexpr bool kSharedRows = NT > 1;  // the query rows' operands are in shared memory: there are no registers for them
+  static constexpr int kRing = kWarps * kStages * kStageBytes;
+  static constexpr int kOperandBytes = kSharedRows ? kRows * D * 2 : 0;
+  static constexpr int kSmem = kRing + kOperandBytes;
+  static constexpr int kCtas = NT == 4 ? 2 : 3;  // of an SM: what registers and shared memory allow
 };
 
 // Byte offset of 16-byte piece `piece` of token t in a slice: pieces are permuted so that neither the reads of the keys (8 rows x 4 pieces)
@@ -48,7 +52,10 @@ __device__ __forceinline__ uint32_t piece_at(uint32_t t, uint32_t piece) {
   return (t >> 1) * 128 + (((((t & 1) << 2) | piece) ^ (((t >> 1) & 3) << 1)) << 4);
 }
 
-__device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool real) {
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool real) {  // else zeros
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(real ? 16 : 0) : "memory");
 }
 __device__ __forceinline__ void copy4(uint32_t dst, const void* src, bool real) {
@@ -72,7 +79,7 @@ __device__ __forceinline__ uint32_t widen_upper(uint32_t two) {
   return r;
 }
 __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
@@ -81,22 +88,6 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
   asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
   return r;
 }
-__device__ __forceinline__ uint4 lds128(uint32_t at) {
-  uint4 v;
-  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at));
-  return v;
-}
-__device__ __forceinline__ uint2 lds64(uint32_t at) {
-  uint2 v;
-  asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(at));
-  return v;
-}
-__device__ __forceinline__ float lds32(uint32_t at) {
-  float v;
-  asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(at));
-  return v;
-}
-
 // What a sequence's keys look like to the call.
 struct Sequence {
   int len, count, lo, steps;  // keys [lo, len) are looked at, in `steps` steps (one at least)
@@ -111,30 +102,35 @@ __device__ __forceinline__ Sequence sequence(const AttendArgs& a, int e) {
 
 // A place in the list of steps.
 struct Place {
-  int e, unit, step;  // unit: key head * row blocks + row block
+  int e, head, block, step;  // block: of rows
   Sequence s;
 };
-__device__ __forceinline__ void advance(const AttendArgs& a, int units, Place* p) {
+__device__ __forceinline__ void advance(const AttendArgs& a, Place* p) {
   if (++p->step < p->s.steps) return;
   p->step = 0;
-  if (++p->unit < units) return;
-  p->unit = 0;
+  if (++p->block < a.row_blocks) return;
+  p->block = 0;
+  if (++p->head < a.cache.heads) return;
+  p->head = 0;
   if (++p->e < a.E) p->s = sequence(a, p->e);
 }
 
 template <typename T, int D, int NT>
-__global__ void __launch_bounds__(kWarps * 32) attend_kernel(const __grid_constant__ AttendArgs a) {
+__global__ void __launch_bounds__(kWarps * 32, Shape<D, NT>::kCtas) attend_kernel(const __grid_constant__ AttendArgs a) {
   using S = Shape<D, NT>;
   constexpr int kWords = D / 16;   // 32-bit words of a key row that a lane holds; also products of 16 features, and feature tiles of 16
   constexpr int kValueWords = D / 32;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ long long warp_sum[kWarps];
+  __shared__ __align__(16) float row_scale[S::kRows];
+  __shared__ __align__(16) int2 row_keys[S::kRows];  // keys [x, y) that a row sees
+  __shared__ float2 tops[kWarps][S::kRows];           // running maximum and sum of each warp
   __shared__ int where_e;
   __shared__ long long where_at;
   const CacheArgs& c = a.cache;
   const int tid = threadIdx.x, w = tid >> 5, lane = tid & 31, g = lane >> 2, q4 = lane & 3;
   const int units = c.heads * a.row_blocks;
-  grid_wait();
+  stage_begin();  // (the joining kernel may come up where there is room)
 
   // --- this CTA's share of the steps: prefix sums over the sequences, a run of them per thread
   const int run = (a.E + kWarps * 32 - 1) / (kWarps * 32);
@@ -178,88 +174,105 @@ __global__ void __launch_bounds__(kWarps * 32) attend_kernel(const __grid_consta
   Place now;
   now.e = where_e;
   now.s = sequence(a, now.e);
-  now.unit = (int)(where_at / now.s.steps);
-  now.step = (int)(where_at % now.s.steps);
+  const int unit = (int)(where_at / now.s.steps);
+  now.step = (int)(where_at - (long long)unit * now.s.steps);
+  now.head = unit / a.row_blocks;
+  now.block = unit - now.head * a.row_blocks;
   Place ahead = now;
 
   // --- the warp's ring of slices
   const uint32_t ring = smem_u32(smem) + w * S::kStages * S::kStageBytes;
-  float* const join = reinterpret_cast<float*>(smem + kWarps * S::kStages * S::kStageBytes);
-  constexpr int kLanesPerRow = D / 16, kRowsPerPass = 32 / kLanesPerRow;
+  uint2* const shared_rows = reinterpret_cast<uint2*>(smem + S::kRing);
+  constexpr int kLanesPerRow = D / 16, kRowsPerPass = 32 / kLanesPerRow, kPasses = kScaleBlock / kRowsPerPass;  // passes of 16 tokens
+  const int lane_row = lane / kLanesPerRow, piece = lane % kLanesPerRow;
+  const int page_mask = (1 << c.page_shift) - 1;
+  // Pages of the slice that is fetched next: looked up a slice earlier, so that the copies do not wait for the table.
+  int pages[2] = {-1, -1};
+  auto look_up = [&]() {
+    const int t0 = ahead.s.lo + ahead.step * kStep + w * kSlice;
+#pragma unroll
+    for (int b = 0; b < 2; ++b) pages[b] = t0 + b * kScaleBlock < ahead.s.len ? page_of(c, ahead.e, t0 + b * kScaleBlock) : -1;
+  };
   auto fetch = [&](int stage) {
-    const int head = ahead.unit / a.row_blocks;
     const int t0 = ahead.s.lo + ahead.step * kStep + w * kSlice;
     const int left = ahead.s.len - t0;
-    if (left > 0) {
-      const uint32_t at = ring + stage * S::kStageBytes;
-      const int page_a = page_of(c, ahead.e, t0), page_b = left > kScaleBlock ? page_of(c, ahead.e, t0 + kScaleBlock) : -1;
-      if ((page_a < 0 || (left > kScaleBlock && page_b < 0)) && lane == 0) report(c.status, kBadPage);
-      const int in_a = t0 & ((1 << c.page_shift) - 1), in_b = (t0 + kScaleBlock) & ((1 << c.page_shift) - 1);
-      const int piece = lane % kLanesPerRow;
+    if (left <= 0) return;
+    const uint32_t at = ring + stage * S::kStageBytes;
+    const bool whole = left >= kSlice && pages[0] >= 0 && pages[1] >= 0;
+    if (!whole && lane == 0 && (pages[0] < 0 || (left > kScaleBlock && pages[1] < 0))) report(c.status, kBadPage);
 #pragma unroll
-      for (int i = 0; i < kSlice / kRowsPerPass; ++i) {
-        const int t = i * kRowsPerPass + lane / kLanesPerRow;
-        const bool upper = i * kRowsPerPass >= kScaleBlock;
-        const int page = upper ? page_b : page_a, row = (upper ? in_b - kScaleBlock : in_a) + t;
-        const bool real = t < left && page >= 0;
-        const long long p = real ? page : 0, r = real ? row : 0;
-        copy16(at + piece_at<D>(t, piece), c.k + p * c.k_sp + head * c.k_sh + r * c.k_st + piece * 16, real);
-        copy16(at + kSlice * D + piece_at<D>(t, piece), c.v + p * c.v_sp + head * c.v_sh + r * c.v_st + piece * 16, real);
+    for (int b = 0; b < 2; ++b) {
+      const uint32_t page = max(pages[b], 0), row = ((t0 + b * kScaleBlock) & page_mask) + lane_row;
+      const uint8_t* k = c.k + 16 * (page * (uint64_t)a.k16[0] + ahead.head * (uint64_t)a.k16[1] + row * (uint64_t)a.k16[2] + piece);
+      const uint8_t* v = c.v + 16 * (page * (uint64_t)a.v16[0] + ahead.head * (uint64_t)a.v16[1] + row * (uint64_t)a.v16[2] + piece);
+      if (whole) {
+#pragma unroll
+        for (int i = 0; i < kPasses; ++i, k += a.k16[2] * (16ull * kRowsPerPass), v += a.v16[2] * (16ull * kRowsPerPass)) {
+          const uint32_t to = at + piece_at<D>(b * kScaleBlock + i * kRowsPerPass + lane_row, piece);
+          copy16(to, k);
+          copy16(to + kSlice * D, v);
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < kPasses; ++i, k += a.k16[2] * (16ull * kRowsPerPass), v += a.v16[2] * (16ull * kRowsPerPass)) {
+          const int t = b * kScaleBlock + i * kRowsPerPass + lane_row;
+          const bool real = t < left && pages[b] >= 0;
+          copy16(at + piece_at<D>(t, piece), real ? k : c.k, real);
+          copy16(at + kSlice * D + piece_at<D>(t, piece), real ? v : c.v, real);
+        }
       }
-      if (lane < 4) {
-        const int page = lane & 1 ? page_b : page_a, row = lane & 1 ? in_b : in_a;
-        const long long p = page >= 0 ? page : 0;
-        const float* src = lane < 2 ? c.k_scale + p * c.ks_sp + head * c.ks_sh : c.v_scale + p * c.vs_sp + head * c.vs_sh;
-        copy4(at + 2 * kSlice * D + lane * 4, src + (page >= 0 ? row / kScaleBlock : 0), page >= 0);
-      }
+    }
+    if (lane < 4) {  // scales: keys of both blocks, values of both
+      const int page = lane & 1 ? pages[1] : pages[0], row = (t0 + (lane & 1) * kScaleBlock) & page_mask;
+      const long long p = max(page, 0);
+      const float* src = lane < 2 ? c.k_scale + p * c.ks_sp + ahead.head * c.ks_sh : c.v_scale + p * c.vs_sp + ahead.head * c.vs_sh;
+      copy4(at + 2 * kSlice * D + lane * 4, src + (page >= 0 ? row / kScaleBlock : 0), page >= 0);
     }
   };
   const int steps = (int)(end - begin);
+  look_up();
 #pragma unroll
   for (int i = 0; i < S::kStages - 1; ++i) {
     if (i < steps) {
       fetch(i);
-      advance(a, units, &ahead);
+      advance(a, &ahead);
+      if (i + 1 < steps) look_up();
     }
     copies_commit();
   }
 
-  uint32_t qf[NT][kWords][2];   // query rows as the second operand
-  float row_scale[NT][2];       // of rows 2 q4, 2 q4 + 1: score units of log2 e
-  int low[NT][2], high[NT][2];  // keys [low, high) that these rows see
-  int full_low = 0, full_high = 0;  // keys that all rows see
-  float o[NT][kWords][4], top[NT][2], sum[NT][2];
-  bool fresh = true;
+  uint32_t qf[S::kSharedRows ? 1 : NT][kWords][2];  // query rows as the second operand
+  float o[NT][kWords][4], top[NT][2], sum[NT][2];   // of rows 2 q4, 2 q4 + 1 of each tile
+  int full_low = 0, full_high = 0;                  // keys that all rows see
+  bool fresh = true, later = false;                 // a head begins; the CTA has finished (a piece of) one
   int stage = 0;
-  bool later = false;  // the CTA has finished a piece of a head
   for (int i = 0; i < steps; ++i) {
     copies_wait<S::kStages - 2>();
     __syncwarp();
     if (i + S::kStages - 1 < steps) {
       fetch(stage == 0 ? S::kStages - 1 : stage - 1);
-      advance(a, units, &ahead);
+      advance(a, &ahead);
+      if (i + S::kStages < steps) look_up();
     }
     copies_commit();
-    const int head = now.unit / a.row_blocks, row0 = (now.unit % a.row_blocks) * S::kRows;
+    const int row0 = now.block * S::kRows;
     if (fresh) {
       fresh = false;
-      full_low = 0;
-      full_high = now.s.len;
-#pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        const int r = row0 + n * 8 + g, token = r / a.group, h = head * a.group + r % a.group;
+      // Rows 8 n + g as operands, and what their scores are multiplied by (units of log2 e).
+      auto load_rows = [&](int n, uint32_t (&to)[kWords][2]) {
+        const int r = row0 + n * 8 + g, token = r / a.group, h = now.head * a.group + r - token * a.group;
         const bool real = token < now.s.count;
         const T* src = reinterpret_cast<const T*>(a.q.ptr) + (real ? now.e * a.q.se + h * a.q.sh + token * a.q.sn : 0);
         float factor = a.scale * kLog2e;
         uint2 raw[kWords];
 #pragma unroll
-        for (int s = 0; s < kWords; ++s)
-          raw[s] = real ? *reinterpret_cast<const uint2*>(src + (s >> 2) * 64 + q4 * 16 + (s & 3) * 4) : make_uint2(0, 0);
-        if constexpr (sizeof(T) == 2 && !std::is_same<T, __half>::value) {
+        for (int k = 0; k < kWords; ++k)
+          raw[k] = real ? *reinterpret_cast<const uint2*>(src + (k >> 2) * 64 + q4 * 16 + (k & 3) * 4) : make_uint2(0, 0);
+        if constexpr (!std::is_same<T, __half>::value) {
           float amax = 0.0f;
 #pragma unroll
-          for (int s = 0; s < kWords; ++s) {
-            const float2 x = sm100::unpack2<T>(raw[s].x), y = sm100::unpack2<T>(raw[s].y);
+          for (int k = 0; k < kWords; ++k) {
+            const float2 x = sm100::unpack2<T>(raw[k].x), y = sm100::unpack2<T>(raw[k].y);
             amax = fmaxf(fmaxf(amax, fmaxf(fabsf(x.x), fabsf(x.y))), fmaxf(fabsf(y.x), fabsf(y.y)));
           }
           amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
@@ -268,105 +281,145 @@ __global__ void __launch_bounds__(kWarps * 32) attend_kernel(const __grid_consta
           const float down = __uint_as_float((uint32_t)(254 - exponent) << 23);
           factor *= __uint_as_float((uint32_t)exponent << 23);
 #pragma unroll
-          for (int s = 0; s < kWords; ++s) {
-            const float2 x = sm100::unpack2<T>(raw[s].x), y = sm100::unpack2<T>(raw[s].y);
-            qf[n][s][0] = sm100::pack2<__half>(x.x * down, x.y * down);
-            qf[n][s][1] = sm100::pack2<__half>(y.x * down, y.y * down);
+          for (int k = 0; k < kWords; ++k) {
+            const float2 x = sm100::unpack2<T>(raw[k].x), y = sm100::unpack2<T>(raw[k].y);
+            to[k][0] = sm100::pack2<__half>(x.x * down, x.y * down);
+            to[k][1] = sm100::pack2<__half>(y.x * down, y.y * down);
           }
         } else {
 #pragma unroll
-          for (int s = 0; s < kWords; ++s) {
-            qf[n][s][0] = raw[s].x;
-            qf[n][s][1] = raw[s].y;
+          for (int k = 0; k < kWords; ++k) {
+            to[k][0] = raw[k].x;
+            to[k][1] = raw[k].y;
           }
         }
+        return factor;
+      };
+      if constexpr (S::kSharedRows) {  // a tile of rows a warp
+        if (w < NT) {
+          const float factor = load_rows(w, qf[0]);
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          row_scale[n][j] = __shfl_sync(0xffffffffu, factor, (2 * q4 + j) * 4);
-          const int t = (row0 + n * 8 + 2 * q4 + j) / a.group;  // token of the call
-          const int place = now.s.len - now.s.count + t;
-          high[n][j] = t >= now.s.count ? 0 : a.causal ? place + 1 : now.s.len;
-          low[n][j] = a.window > 0 ? place - a.window + 1 : 0;
-          if (t < now.s.count) {
-            full_high = min(full_high, high[n][j]);
-            full_low = max(full_low, low[n][j]);
-          }
-          top[n][j] = -CUDART_INF_F;
-          sum[n][j] = 0.0f;
+          for (int k = 0; k < kWords; ++k) shared_rows[(w * kWords + k) * 32 + lane] = make_uint2(qf[0][k][0], qf[0][k][1]);
+          if (q4 == 0) row_scale[w * 8 + g] = factor;
         }
+      } else {
+        const float factor = load_rows(0, qf[0]);
+        if (w == 0 && q4 == 0) row_scale[g] = factor;
+      }
+      if (tid < S::kRows) {
+        const int token = (row0 + tid) / a.group, place = now.s.len - now.s.count + token;
+        row_keys[tid] = make_int2(a.window > 0 ? place - a.window + 1 : 0, token >= now.s.count ? 0 : a.causal ? place + 1 : now.s.len);
+      }
+      __syncthreads();
+      // rows are in the order of their tokens; those of padding have results of zero whatever they see
+      full_low = 0;
+      full_high = now.s.len;
+      if (a.causal && row0 / a.group < now.s.count) {
+        const int last = min((row0 + S::kRows - 1) / a.group, now.s.count - 1);
+        full_high = row_keys[0].y;
+        if (a.window > 0) full_low = now.s.len - now.s.count + last - a.window + 1;
+      }
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        top[n][0] = top[n][1] = -CUDART_INF_F;
+        sum[n][0] = sum[n][1] = 0.0f;
 #pragma unroll
         for (int m = 0; m < kWords; ++m)
 #pragma unroll
           for (int j = 0; j < 4; ++j) o[n][m][j] = 0.0f;
       }
-#pragma unroll
-      for (int m = 1; m < 4; m <<= 1) {
-        full_high = min(full_high, __shfl_xor_sync(0xffffffffu, full_high, m));
-        full_low = max(full_low, __shfl_xor_sync(0xffffffffu, full_low, m));
-      }
     }
 
     const int t0 = now.s.lo + now.step * kStep + w * kSlice;
     if (t0 < now.s.len) {
-      const uint32_t at = ring + stage * S::kStageBytes;
+      const uint8_t* const keys = smem + (w * S::kStages + stage) * S::kStageBytes;
+      const uint8_t* const values = keys + kSlice * D;
       float s[2][NT][4];
+      uint32_t kw[2][2][kWords];
 #pragma unroll
-      for (int mt = 0; mt < 2; ++mt) {
-        uint32_t kw[2][kWords];
+      for (int mt = 0; mt < 2; ++mt)
 #pragma unroll
         for (int r = 0; r < 2; ++r)
 #pragma unroll
           for (int h = 0; h < kWords / 4; ++h) {
-            const uint4 v = lds128(at + piece_at<D>(mt * 16 + r * 8 + g, q4 + 4 * h));
-            kw[r][4 * h] = v.x; kw[r][4 * h + 1] = v.y; kw[r][4 * h + 2] = v.z; kw[r][4 * h + 3] = v.w;
+            const uint4 v = *reinterpret_cast<const uint4*>(keys + piece_at<D>(mt * 16 + r * 8 + g, q4 + 4 * h));
+            kw[mt][r][4 * h] = v.x; kw[mt][r][4 * h + 1] = v.y; kw[mt][r][4 * h + 2] = v.z; kw[mt][r][4 * h + 3] = v.w;
           }
+#pragma unroll
+      for (int mt = 0; mt < 2; ++mt)
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
           for (int j = 0; j < 4; ++j) s[mt][n][j] = 0.0f;
+      // (the two blocks' products take turns: a product waits for the one before it in its sum)
 #pragma unroll
-        for (int k = 0; k < kWords; ++k) {
-          const uint32_t a0 = widen(kw[0][k]), a1 = widen(kw[1][k]), a2 = widen_upper(kw[0][k]), a3 = widen_upper(kw[1][k]);
+      for (int k = 0; k < kWords; ++k)
 #pragma unroll
-          for (int n = 0; n < NT; ++n) mma(s[mt][n], a0, a1, a2, a3, qf[n][k][0], qf[n][k][1]);
+        for (int mt = 0; mt < 2; ++mt) {
+          const uint32_t a0 = widen(kw[mt][0][k]), a1 = widen(kw[mt][1][k]), a2 = widen_upper(kw[mt][0][k]), a3 = widen_upper(kw[mt][1][k]);
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+            if constexpr (S::kSharedRows) {
+              const uint2 b = shared_rows[(n * kWords + k) * 32 + lane];
+              mma(s[mt][n], a0, a1, a2, a3, b.x, b.y);
+            } else {
+              mma(s[mt][n], a0, a1, a2, a3, qf[n][k][0], qf[n][k][1]);
+            }
+          }
         }
-      }
-      const uint32_t scales = at + 2 * kSlice * D;
-      const float ks[2] = {lds32(scales), lds32(scales + 4)}, vs[2] = {lds32(scales + 8), lds32(scales + 12)};
+      const float4 scales = *reinterpret_cast<const float4*>(keys + 2 * kSlice * D);
+      const float ks[2] = {scales.x, scales.y}, vs[2] = {scales.z, scales.w};
       const float vl[2] = {__log2f(vs[0]), __log2f(vs[1])};
       const bool whole = t0 >= full_low && t0 + kSlice <= full_high;
       uint32_t weights[2][NT][2];
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
+        const float2 rs = *reinterpret_cast<const float2*>(row_scale + n * 8 + 2 * q4);
         float most[2] = {-CUDART_INF_F, -CUDART_INF_F};
 #pragma unroll
         for (int mt = 0; mt < 2; ++mt)
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
-            float x = s[mt][n][j] * (ks[mt] * row_scale[n][j & 1]);
+            float x = s[mt][n][j] * (ks[mt] * (j & 1 ? rs.y : rs.x));
             if (a.softcap > 0.0f)  // softcap * tanh(x / softcap): tanh y = 1 - 2 / (exp(2 y) + 1), off by 2^-23 of the cap at most
               x = a.softcap * kLog2e * (1.0f - __fdividef(2.0f, ex2(x * (2.0f / a.softcap)) + 1.0f));
-            const int t = t0 + mt * 16 + g + (j >> 1) * 8;
-            if (!whole && (t < low[n][j & 1] || t >= high[n][j & 1])) x = -CUDART_INF_F;
             s[mt][n][j] = x;
-            most[j & 1] = fmaxf(most[j & 1], x + vl[mt]);
           }
-        float base[2];
+        if (!whole) {
+          const int4 seen = *reinterpret_cast<const int4*>(row_keys + n * 8 + 2 * q4);
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
+          for (int mt = 0; mt < 2; ++mt)
 #pragma unroll
-          for (int m = 4; m < 32; m <<= 1) most[j] = fmaxf(most[j], __shfl_xor_sync(0xffffffffu, most[j], m));
-          const float before = top[n][j];
-          top[n][j] = fmaxf(before, most[j]);
-          base[j] = top[n][j] == -CUDART_INF_F ? 0.0f : top[n][j];
-          const float shrink = ex2(before - base[j]);
-          sum[n][j] *= shrink;
+            for (int j = 0; j < 4; ++j) {
+              const int t = t0 + mt * 16 + g + (j >> 1) * 8;
+              if (t < (j & 1 ? seen.z : seen.x) || t >= (j & 1 ? seen.w : seen.y)) s[mt][n][j] = -CUDART_INF_F;
+            }
+        }
 #pragma unroll
-          for (int m = 0; m < kWords; ++m) {
-            o[n][m][j] *= shrink;
-            o[n][m][2 + j] *= shrink;
+        for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) most[j & 1] = fmaxf(most[j & 1], s[mt][n][j] + vl[mt]);
+        // The rows' reference is raised only when a weight would pass 2^kSlack: seldom once a head's first keys have been seen, and until then
+        // no lane has to know the others' scores.
+        if (__any_sync(0xffffffffu, most[0] > top[n][0] + kSlack || most[1] > top[n][1] + kSlack)) {
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+#pragma unroll
+            for (int m = 4; m < 32; m <<= 1) most[j] = fmaxf(most[j], __shfl_xor_sync(0xffffffffu, most[j], m));
+            const float before = top[n][j];
+            top[n][j] = fmaxf(before, most[j]);
+            const float shrink = ex2(before - (top[n][j] == -CUDART_INF_F ? 0.0f : top[n][j]));
+            sum[n][j] *= shrink;
+#pragma unroll
+            for (int m = 0; m < kWords; ++m) {
+              o[n][m][j] *= shrink;
+              o[n][m][2 + j] *= shrink;
+            }
           }
         }
+        float base[2];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) base[j] = top[n][j] == -CUDART_INF_F ? 0.0f : top[n][j];
 #pragma unroll
         for (int mt = 0; mt < 2; ++mt) {
           float p[4];
@@ -387,10 +440,10 @@ __global__ void __launch_bounds__(kWarps * 32) attend_kernel(const __grid_consta
         for (int j = 0; j < 4; ++j) {
           const int t = mt * 16 + 2 * q4 + (j & 1) + (j >> 1) * 8;
           if constexpr (D == 128) {
-            const uint4 v = lds128(at + kSlice * D + piece_at<D>(t, g));
+            const uint4 v = *reinterpret_cast<const uint4*>(values + piece_at<D>(t, g));
             vw[j][0] = v.x; vw[j][1] = v.y; vw[j][2] = v.z; vw[j][3] = v.w;
           } else {
-            const uint2 v = lds64(at + kSlice * D + piece_at<D>(t, g >> 1) + (g & 1) * 8);
+            const uint2 v = *reinterpret_cast<const uint2*>(values + piece_at<D>(t, g >> 1) + (g & 1) * 8);
             vw[j][0] = v.x; vw[j][1] = v.y;
           }
         }
@@ -408,130 +461,115 @@ __global__ void __launch_bounds__(kWarps * 32) attend_kernel(const __grid_consta
         }
       }
     }
-    stage = stage + 1 == S::kStages ? 0 : stage + 1;
 
     const bool last_of_head = now.step + 1 == now.s.steps;
     if (last_of_head || i + 1 == steps) {
+      // --- the four warps' sums into one: each brings its own to the common maximum and leaves it in its ring, in the stage that it has
+      // just used up, two tiles of rows at a time; warp w then adds up rows 2 w and 2 w + 1 of each tile
       fresh = true;
 #pragma unroll
       for (int n = 0; n < NT; ++n)
 #pragma unroll
-        for (int j = 0; j < 2; ++j)
+        for (int j = 0; j < 2; ++j) {
 #pragma unroll
           for (int m = 4; m < 32; m <<= 1) sum[n][j] += __shfl_xor_sync(0xffffffffu, sum[n][j], m);
-      // warps 2, 3 into 0, 1, then 1 into 0, lane by lane
-      auto put = [&](float* to) {
+          if (g == 0) tops[w][n * 8 + 2 * q4 + j] = make_float2(top[n][j], sum[n][j]);
+        }
+      __syncthreads();
+      const bool alone = last_of_head && i >= now.step;  // all of the head's steps were this CTA's
+      const int slot = 2 * blockIdx.x + (later ? 1 : 0);
+      constexpr int kTiles = NT < 2 ? NT : 2;
+      float* const mine = reinterpret_cast<float*>(smem + (w * S::kStages + stage) * S::kStageBytes);
 #pragma unroll
-        for (int n = 0; n < NT; ++n) {
+      for (int n0 = 0; n0 < NT; n0 += kTiles) {
 #pragma unroll
-          for (int m = 0; m < kWords; ++m)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) to[((n * kWords + m) * 4 + j) * 32 + lane] = o[n][m][j];
+        for (int n = n0; n < n0 + kTiles; ++n)
 #pragma unroll
           for (int j = 0; j < 2; ++j) {
-            to[S::kRows * D + (n * 2 + j) * 64 + lane] = top[n][j];
-            to[S::kRows * D + (n * 2 + j) * 64 + 32 + lane] = sum[n][j];
+            float most = -CUDART_INF_F;
+#pragma unroll
+            for (int v = 0; v < kWarps; ++v) most = fmaxf(most, tops[v][n * 8 + 2 * q4 + j].x);
+            const float x = ex2(top[n][j] - (most == -CUDART_INF_F ? 0.0f : most));
+#pragma unroll
+            for (int m = 0; m < kWords; ++m) {
+              mine[(((n - n0) * kWords + m) * 4 + j) * 32 + lane] = o[n][m][j] * x;
+              mine[(((n - n0) * kWords + m) * 4 + 2 + j) * 32 + lane] = o[n][m][2 + j] * x;
+            }
+          }
+        __syncthreads();
+        // 8 neighbouring features of a row a lane (64 features: 4), in the places where the lanes of the product had them
+        constexpr int kRun = D / 16;
+        const int j = lane >> 4, u = lane & 15, from_g = u >> 1, m0 = (u & 1) * (kWords / 2);
+#pragma unroll
+        for (int n = n0; n < n0 + kTiles; ++n) {
+          const int r = n * 8 + 2 * w + j;
+          float x[kRun];
+#pragma unroll
+          for (int f = 0; f < kRun; ++f) x[f] = 0.0f;
+#pragma unroll
+          for (int v = 0; v < kWarps; ++v) {
+            const float* theirs = reinterpret_cast<const float*>(smem + (v * S::kStages + stage) * S::kStageBytes);
+#pragma unroll
+            for (int f = 0; f < kRun; ++f) x[f] += theirs[(((n - n0) * kWords + m0 + f / 2) * 4 + j + 2 * (f & 1)) * 32 + from_g * 4 + w];
+          }
+          float most = -CUDART_INF_F, total = 0.0f;
+#pragma unroll
+          for (int v = 0; v < kWarps; ++v) most = fmaxf(most, tops[v][r].x);
+          const float base = most == -CUDART_INF_F ? 0.0f : most;
+#pragma unroll
+          for (int v = 0; v < kWarps; ++v) total += tops[v][r].y * ex2(tops[v][r].x - base);
+          if (alone) {
+            const int token = (row0 + r) / a.group, h = now.head * a.group + row0 + r - token * a.group;
+            if (token >= a.N) continue;
+            const float inverse = token < now.s.count && total > 0.0f ? 1.0f / total : 0.0f;
+            T* dst = reinterpret_cast<T*>(const_cast<void*>(a.out.ptr)) + now.e * a.out.se + h * a.out.sh + token * a.out.sn + u * kRun;
+            if constexpr (D == 128)
+              *reinterpret_cast<uint4*>(dst) = make_uint4(sm100::pack2<T>(x[0] * inverse, x[1] * inverse), sm100::pack2<T>(x[2] * inverse, x[3] * inverse),
+                                                          sm100::pack2<T>(x[4] * inverse, x[5] * inverse), sm100::pack2<T>(x[6] * inverse, x[7] * inverse));
+            else
+              *reinterpret_cast<uint2*>(dst) = make_uint2(sm100::pack2<T>(x[0] * inverse, x[1] * inverse), sm100::pack2<T>(x[2] * inverse, x[3] * inverse));
+          } else {
+            float* dst = a.part_o + ((size_t)slot * S::kRows + r) * D + u * kRun;
+#pragma unroll
+            for (int f = 0; f < kRun; f += 4) *reinterpret_cast<float4*>(dst + f) = make_float4(x[f], x[f + 1], x[f + 2], x[f + 3]);
+            if (u == 0) *reinterpret_cast<float2*>(a.part_ml + ((size_t)slot * S::kRows + r) * 2) = make_float2(most, total);
           }
         }
-      };
-      auto take = [&](const float* from) {
-#pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            const float theirs = from[S::kRows * D + (n * 2 + j) * 64 + lane], more = from[S::kRows * D + (n * 2 + j) * 64 + 32 + lane];
-            const float both = fmaxf(top[n][j], theirs), base = both == -CUDART_INF_F ? 0.0f : both;
-            const float x = ex2(top[n][j] - base), y = ex2(theirs - base);
-            top[n][j] = both;
-            sum[n][j] = sum[n][j] * x + more * y;
-#pragma unroll
-            for (int m = 0; m < kWords; ++m) {
-              o[n][m][j] = o[n][m][j] * x + from[((n * kWords + m) * 4 + j) * 32 + lane] * y;
-              o[n][m][2 + j] = o[n][m][2 + j] * x + from[((n * kWords + m) * 4 + 2 + j) * 32 + lane] * y;
-            }
-          }
-      };
-      if (w >= 2) put(join + (w - 2) * S::kJoinFloats);
-      __syncthreads();
-      if (w < 2) take(join + w * S::kJoinFloats);
-      __syncthreads();
-      if (w == 1) put(join);
-      __syncthreads();
-      if (w == 0) {
-        take(join);
-        const bool alone = last_of_head && i >= now.step;  // all of the head's steps were this CTA's
-        const int slot = 2 * blockIdx.x + (later ? 1 : 0);
-#pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            const int r = n * 8 + 2 * q4 + j, token = (row0 + r) / a.group, h = head * a.group + (row0 + r) % a.group;
-            constexpr int kRun = D / 8;  // neighbouring features of a lane
-            float x[kRun];
-#pragma unroll
-            for (int m = 0; m < kWords; ++m) {
-              x[2 * m] = o[n][m][j];
-              x[2 * m + 1] = o[n][m][2 + j];
-            }
-            if (alone) {
-              if (token >= a.N) continue;
-              const float inverse = token < now.s.count && sum[n][j] > 0.0f ? 1.0f / sum[n][j] : 0.0f;
-              T* dst = reinterpret_cast<T*>(const_cast<void*>(a.out.ptr)) + now.e * a.out.se + h * a.out.sh + token * a.out.sn + g * kRun;
-#pragma unroll
-              for (int v = 0; v < kRun / 8; ++v) {
-                uint4 y;
-                const float* z = x + 8 * v;
-                y.x = sm100::pack2<T>(z[0] * inverse, z[1] * inverse);
-                y.y = sm100::pack2<T>(z[2] * inverse, z[3] * inverse);
-                y.z = sm100::pack2<T>(z[4] * inverse, z[5] * inverse);
-                y.w = sm100::pack2<T>(z[6] * inverse, z[7] * inverse);
-                reinterpret_cast<uint4*>(dst)[v] = y;
-              }
-            } else {
-              float* dst = a.part_o + ((size_t)slot * S::kRows + r) * D + g * kRun;
-#pragma unroll
-              for (int v = 0; v < kRun / 4; ++v) reinterpret_cast<float4*>(dst)[v] = make_float4(x[4 * v], x[4 * v + 1], x[4 * v + 2], x[4 * v + 3]);
-              if (g == 0) {
-                a.part_ml[((size_t)slot * S::kRows + r) * 2] = top[n][j];
-                a.part_ml[((size_t)slot * S::kRows + r) * 2 + 1] = sum[n][j];
-              }
-            }
-          }
+        __syncthreads();
       }
-      __syncthreads();
       if (tid == 0 && i + 1 == steps) {
         // a head that goes on in the next CTA and began here: this CTA's entry names it and the CTA of its last step
         int4 entry = make_int4(-1, 0, 0, 0);
-        const bool began = i >= now.step;
-        if (!last_of_head && began) {
+        if (!last_of_head && i >= now.step) {
           const long long last = end - 1 + (now.s.steps - 1 - now.step);
-          entry = make_int4(now.e, now.unit, (int)(((last + 1) * ctas - 1) / total), later ? 1 : 0);
+          entry = make_int4(now.e, now.head * a.row_blocks + now.block, (int)(((last + 1) * ctas - 1) / total), later ? 1 : 0);
         }
         a.split[blockIdx.x] = entry;
       }
       later = true;
     }
-    advance(a, units, &now);
+    stage = stage + 1 == S::kStages ? 0 : stage + 1;
+    advance(a, &now);
   }
 }
 
-// Joins the pieces of the heads that were split: a CTA for each CTA of the kernel above (most have nothing to do) and row.
-template <typename T, int D, int NT>
-__global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ AttendArgs a) {
-  constexpr int kLanes = D / 4, kGroups = 256 / kLanes, kRows = 8 * NT;
+// Joins the pieces of the heads that were split: a CTA for each CTA of the kernel above (many have nothing to do) and row.  The pieces' weights
+// come first, for all at once; then every 16 bytes of a row is the sum over the pieces of one of several groups of threads, with many
+// loads in flight: 222 pieces of 128 features take 3 us, one piece after the other took 17.
+template <typename T, int D>
+__global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ AttendArgs a, int tile_rows) {
+  constexpr int kLanes = D / 4, kGroups = 256 / kLanes, kMost = 1024, kInFlight = 8;
+  __shared__ float weights[kMost], reduced[8], totals[8];
   __shared__ float4 sums[256];
-  __shared__ float reduced[8];
   grid_wait();
   const int4 entry = a.split[blockIdx.x];
   if (entry.x < 0) return;
-  const int e = entry.x, head = entry.y / a.row_blocks, r = blockIdx.y, row = (entry.y % a.row_blocks) * kRows + r;
-  const int token = row / a.group, h = head * a.group + row % a.group;
+  const int e = entry.x, head = entry.y / a.row_blocks, r = blockIdx.y, row = (entry.y - head * a.row_blocks) * tile_rows + r;
+  const int token = row / a.group, h = head * a.group + row - token * a.group;
   if (token >= a.N) return;
-  int len, count;
-  sequence_of(a.cache, e, a.N, &len, &count);
   const int pieces = entry.z - (int)blockIdx.x + 1;
-  auto slot = [&](int i) { return (size_t)(2 * (blockIdx.x + i) + (i == 0 ? entry.w : 0)) * kRows + r; };
-  const int tid = threadIdx.x;
+  auto slot = [&](int i) { return (size_t)(2 * (blockIdx.x + i) + (i == 0 ? entry.w : 0)) * tile_rows + r; };
+  const int tid = threadIdx.x, lane = tid % kLanes, group = tid / kLanes;
   float top = -CUDART_INF_F;
   for (int i = tid; i < pieces; i += 256) top = fmaxf(top, a.part_ml[2 * slot(i)]);
 #pragma unroll
@@ -541,39 +579,59 @@ __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ Atten
 #pragma unroll
   for (int i = 0; i < 8; ++i) top = fmaxf(top, reduced[i]);
   const float base = top == -CUDART_INF_F ? 0.0f : top;
-  const int lane = tid % kLanes, group = tid / kLanes;
   float4 acc = make_float4(0, 0, 0, 0);
   float total = 0.0f;
-  for (int i = group; i < pieces; i += kGroups) {
-    const float weight = ex2(a.part_ml[2 * slot(i)] - base);
-    const float4 x = reinterpret_cast<const float4*>(a.part_o + slot(i) * D)[lane];
-    total += weight * a.part_ml[2 * slot(i) + 1];
-    acc.x += weight * x.x; acc.y += weight * x.y; acc.z += weight * x.z; acc.w += weight * x.w;
+  for (int i0 = 0; i0 < pieces; i0 += kMost) {
+    const int n = min(kMost, pieces - i0);
+    for (int i = tid; i < n; i += 256) {
+      const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + 2 * slot(i0 + i));
+      weights[i] = ex2(ml.x - base);
+      total += weights[i] * ml.y;
+    }
+    __syncthreads();
+    for (int i = group; i < n; i += kGroups * kInFlight) {
+      float4 x[kInFlight];
+#pragma unroll
+      for (int j = 0; j < kInFlight; ++j)
+        x[j] = i + j * kGroups < n ? reinterpret_cast<const float4*>(a.part_o + slot(i0 + i + j * kGroups) * D)[lane] : make_float4(0, 0, 0, 0);
+#pragma unroll
+      for (int j = 0; j < kInFlight; ++j) {
+        const float weight = i + j * kGroups < n ? weights[i + j * kGroups] : 0.0f;
+        acc.x += weight * x[j].x; acc.y += weight * x[j].y; acc.z += weight * x[j].z; acc.w += weight * x[j].w;
+      }
+    }
+    __syncthreads();
   }
-  __shared__ float totals[kGroups];
+#pragma unroll
+  for (int m = 16; m > 0; m >>= 1) total += __shfl_xor_sync(0xffffffffu, total, m);
+  if ((tid & 31) == 0) totals[tid >> 5] = total;
   sums[tid] = acc;
-  if (lane == 0) totals[group] = total;
   __syncthreads();
   if (group != 0) return;
+#pragma unroll
   for (int i = 1; i < kGroups; ++i) {
     const float4 x = sums[i * kLanes + lane];
     acc.x += x.x; acc.y += x.y; acc.z += x.z; acc.w += x.w;
-    total += totals[i];
   }
+  total = 0.0f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) total += totals[i];
+  int len, count;
+  sequence_of(a.cache, e, a.N, &len, &count);
   const float inverse = token < count && total > 0.0f ? 1.0f / total : 0.0f;
   T* dst = reinterpret_cast<T*>(const_cast<void*>(a.out.ptr)) + e * a.out.se + h * a.out.sh + token * a.out.sn + lane * 4;
   *reinterpret_cast<uint2*>(dst) = make_uint2(sm100::pack2<T>(acc.x * inverse, acc.y * inverse), sm100::pack2<T>(acc.z * inverse, acc.w * inverse));
 }
 
 int row_tiles(int rows) { return rows <= 8 ? 1 : rows <= 16 ? 2 : 4; }
-int ctas_per_sm(int width) { return width == 128 ? 2 : 3; }
+int ctas_per_sm(int nt) { return nt == 4 ? Shape<128, 4>::kCtas : Shape<128, 1>::kCtas; }
 
 // CTAs of a call: what the GPU holds at once, and no more than the steps that the lengths can have.
 long long grid_of(int E, int N, int H, int kv_heads, int width, long long longest) {
   const int rows = H / kv_heads * N, nt = row_tiles(rows);
   const long long units = (long long)E * kv_heads * ((rows + 8 * nt - 1) / (8 * nt));
   const long long steps = units * ((longest + kStep - 1) / kStep > 1 ? (longest + kStep - 1) / kStep : 1);
-  const long long most = (long long)ctas_per_sm(width) * sm_count();
+  const long long most = (long long)ctas_per_sm(nt) * sm_count();
   return steps < most ? steps : most;
 }
 
@@ -586,7 +644,10 @@ cudaError_t launch(AttendArgs& a, long long grid, bool split, cudaStream_t strea
   void* args[] = {(void*)&a};
   err = launch_kernel(fn, dim3((unsigned)grid), dim3(kWarps * 32), args, smem, stream);
   if (err != cudaSuccess || !split) return err;
-  return launch_kernel((const void*)join_kernel<T, D, NT>, dim3((unsigned)grid, 8 * NT), dim3(256), args, 0, stream);
+  int tile_rows = 8 * NT;
+  void* join_args[] = {(void*)&a, (void*)&tile_rows};
+  const int rows = a.group * a.N < tile_rows ? a.group * a.N : tile_rows;
+  return launch_kernel((const void*)join_kernel<T, D>, dim3((unsigned)grid, rows), dim3(256), join_args, 0, stream);
 }
 
 }  // namespace
@@ -601,6 +662,9 @@ cudaError_t launch_attend(AttendArgs a, int dtype, int width, void* workspace, l
   const int rows = a.group * a.N, nt = row_tiles(rows);
   const long long grid = grid_of(a.E, a.N, a.H, a.cache.heads, width, longest);
   a.row_blocks = (rows + 8 * nt - 1) / (8 * nt);
+  const CacheArgs& c = a.cache;
+  const long long strides[6] = {c.k_sp, c.k_sh, c.k_st, c.v_sp, c.v_sh, c.v_st};
+  for (int i = 0; i < 6; ++i) (i < 3 ? a.k16[i] : a.v16[i - 3]) = (uint32_t)(strides[i] / 16);
   char* at = reinterpret_cast<char*>(workspace);
   a.split = reinterpret_cast<int4*>(at);
   at += ((size_t)grid * sizeof(int4) + 255) / 256 * 256;

@@ -1,5 +1,10 @@
 // Native halves of the rotary positions, the paged cache and the attention over it: input checks, results and
 // workspaces from PyTorch's caching allocator, and the launches through the C ABI.
+#include <ATen/ExpandUtils.h>
+#include <torch/csrc/autograd/function.h>
+#include <torch/csrc/autograd/functions/utils.h>
+#include <torch/csrc/autograd/saved_variable.h>
+
 #include "ma_torch.h"
 
 namespace ma_torch {
@@ -59,14 +64,19 @@ void check_rotated(const Tensor& q, const optional<Tensor>& k, const optional<Te
   }
 }
 
+// An uninitialised tensor of t's shape and order of strides (at::empty_like without its way through the dispatcher).
+Tensor new_like(const Tensor& t) {
+  const at::TensorOptions o = at::TensorOptions().dtype(t.scalar_type()).device(t.device());
+  if (t.is_non_overlapping_and_dense()) return at::detail::empty_strided_cuda(t.sizes(), t.strides(), o);
+  return at::detail::empty_strided_cuda(t.sizes(), at::infer_dense_strides(t.sizes(), t.strides()), o);
+}
+
 // Rotated copies of q and k (undefined ones are left out).
 std::pair<Tensor, Tensor> rotate(const Tensor& q_in, const Tensor& k_in, const Rotary& r, const optional<Tensor>& positions, bool inverse) {
   const Tensor& any = q_in.defined() ? q_in : k_in;
   const c10::cuda::CUDAGuard guard(any.device());
   const Tensor q = q_in.defined() ? unit_inner(q_in) : q_in, k = k_in.defined() ? unit_inner(k_in) : k_in;
-  Tensor q_out = q.defined() ? at::empty_like(q) : q, k_out = k.defined() ? at::empty_like(k) : k;
-  if (q_out.defined()) q_out = unit_inner(q_out);
-  if (k_out.defined()) k_out = unit_inner(k_out);
+  const Tensor q_out = q.defined() ? new_like(q) : q, k_out = k.defined() ? new_like(k) : k;
   const int64_t E = any.size(0), N = any.size(2), D = any.size(3);
   TORCH_CHECK_VALUE(r.dim <= D, "rotary dim ", r.dim, " exceeds the head width ", D);
   ma_b200_rotation p{};
@@ -93,49 +103,48 @@ std::pair<Tensor, Tensor> rotate(const Tensor& q_in, const Tensor& k_in, const R
 
 std::pair<Tensor, Tensor> rotate_any(const Tensor& q, const Tensor& k, const Rotary& r, const optional<Tensor>& positions, bool inverse);
 
-// The rotation is linear: its gradient is the inverse rotation (times the magnitude again), itself differentiable.
-struct RotaryFunction : torch::autograd::Function<RotaryFunction> {
-  static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, const Tensor& x, const optional<Tensor>& y, const Tensor& turns,
-                                                int64_t dim, int64_t pairs, double magnitude, const optional<Tensor>& positions, bool inverse) {
-    at::AutoDispatchBelowADInplaceOrView below;
-    ctx->set_materialize_grads(false);
-    ctx->saved_data["turns"] = turns;
-    ctx->saved_data["dim"] = dim;
-    ctx->saved_data["pairs"] = pairs;
-    ctx->saved_data["magnitude"] = magnitude;
-    ctx->saved_data["inverse"] = inverse;
-    if (positions.has_value()) ctx->save_for_backward({*positions});
-    const auto out = rotate(x, y.value_or(Tensor()), Rotary{turns, dim, pairs, magnitude}, positions, inverse);
-    if (!y.has_value()) return {out.first};
-    return {out.first, out.second};
-  }
-  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
-    const Rotary r{ctx->saved_data["turns"].toTensor(), ctx->saved_data["dim"].toInt(), ctx->saved_data["pairs"].toInt(),
-                   ctx->saved_data["magnitude"].toDouble()};
-    const auto saved = ctx->get_saved_variables();
+// The rotation is linear: its gradient is the inverse rotation (times the magnitude again), itself differentiable.  A node of its own:
+// a training step of a small layer is bound by the host, and the general function object with its dictionary costs it 20 us.
+struct RotaryBackward : torch::autograd::Node {
+  Rotary rotary;
+  torch::autograd::SavedVariable positions;
+  bool has_positions, inverse;
+
+  torch::autograd::variable_list apply(torch::autograd::variable_list&& grads) override {
     std::pair<Tensor, Tensor> d;
     const Tensor dx = grads[0], dy = grads.size() > 1 ? grads[1] : Tensor();
     if (dx.defined() || dy.defined())
-      d = rotate_any(dx, dy, r, saved.empty() ? std::nullopt : optional<Tensor>(saved[0]), !ctx->saved_data["inverse"].toBool());
-    return {d.first, d.second, Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
+      d = rotate_any(dx, dy, rotary, has_positions ? optional<Tensor>(positions.unpack()) : std::nullopt, !inverse);
+    if (grads.size() > 1) return {d.first, d.second};
+    return {d.first};
   }
+  void release_variables() override { positions.reset_data(); }
+  std::string name() const override { return "RotaryBackward"; }
 };
+
+// Rotated copies of x and (where defined) y, both of which need a gradient.
+std::pair<Tensor, Tensor> rotate_with_history(const Tensor& x, const Tensor& y, const Rotary& r, const optional<Tensor>& positions, bool inverse) {
+  const auto out = rotate(x.detach(), y.defined() ? y.detach() : y, r, positions, inverse);
+  const std::shared_ptr<RotaryBackward> node(new RotaryBackward, torch::autograd::deleteNode);
+  node->rotary = r;
+  node->has_positions = positions.has_value();
+  if (positions.has_value()) node->positions = torch::autograd::SavedVariable(*positions, false);
+  node->inverse = inverse;
+  node->set_next_edges(y.defined() ? torch::autograd::collect_next_edges(x, y) : torch::autograd::collect_next_edges(x));
+  torch::autograd::set_history(out.first, node);
+  if (y.defined()) torch::autograd::set_history(out.second, node);
+  return out;
+}
 
 // (Either of q and k may be undefined.)
 std::pair<Tensor, Tensor> rotate_any(const Tensor& q, const Tensor& k, const Rotary& r, const optional<Tensor>& positions, bool inverse) {
   const bool grad = at::GradMode::is_enabled();
   const bool gq = grad && q.defined() && q.requires_grad(), gk = grad && k.defined() && k.requires_grad();
   if (!gq && !gk) return rotate(q, k, r, positions, inverse);
-  auto apply = [&](const Tensor& x, const optional<Tensor>& y) {
-    return RotaryFunction::apply(x, y, r.turns, r.dim, r.pairs, r.magnitude, positions, inverse);
-  };
-  if (gq && gk) {
-    const auto out = apply(q, k);
-    return {out[0], out[1]};
-  }
+  if (gq && gk) return rotate_with_history(q, k, r, positions, inverse);
   // one of the two has no gradient: its result is not to hang on the other's graph
-  if (gq) return {apply(q, std::nullopt)[0], k.defined() ? rotate(Tensor(), k, r, positions, inverse).second : k};
-  return {q.defined() ? rotate(q, Tensor(), r, positions, inverse).first : q, apply(k, std::nullopt)[0]};
+  if (gq) return {rotate_with_history(q, Tensor(), r, positions, inverse).first, k.defined() ? rotate(Tensor(), k, r, positions, inverse).second : k};
+  return {q.defined() ? rotate(q, Tensor(), r, positions, inverse).first : q, rotate_with_history(k, Tensor(), r, positions, inverse).first};
 }
 
 // ---------------------------------------------------------------------------------------------- paged cache
@@ -206,7 +215,7 @@ Tensor append(const Cache& cache, const Tensor& k_in, const Tensor& v_in, const 
   TORCH_CHECK_VALUE(k_in.size(1) == p.cache.heads && k_in.size(3) == p.cache.width, "key shape ", k_in.sizes(), " does not match the cache's ",
                     p.cache.heads, " heads of ", p.cache.width);
   p.sequences = sequences_struct(table, lengths, counts, k_in.size(0), k_in.device());
-  const size_t lane = p.cache.width / 16;
+  const size_t lane = 16;
   Tensor q, q_out;
   if (query.has_value()) {
     check_16bit(*query, "query");
@@ -214,7 +223,7 @@ Tensor append(const Cache& cache, const Tensor& k_in, const Tensor& v_in, const 
                           query->scalar_type() == k_in.scalar_type() && query->device() == k_in.device(),
                       "query must match the key in batch, tokens, width, dtype and device");
     q = aligned(*query, lane);
-    q_out = at::empty_like(q);
+    q_out = new_like(q);
     p.H = (int32_t)q.size(1);
     p.q = view4(q);
     p.q_out = view4(q_out);

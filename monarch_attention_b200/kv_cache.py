@@ -67,7 +67,7 @@ def append_kv_b200(cache: PagedKV, key: Tensor, value: Tensor, page_table: Tenso
                    query: Tensor | None = None, rotary: RotaryPositions | None = None) -> Tensor | None:
     """Writes ``key`` and ``value`` (E, heads, N, width; bfloat16 or float16) into the cache at the call's positions.
 
-    With ``rotary`` (``dim`` a multiple of 8) keys are rotated at their positions on the way, and so is ``query`` (E, H, N, width), whose
+    With ``rotary`` (``dim`` a multiple of 16) keys are rotated at their positions on the way, and so is ``query`` (E, H, N, width), whose
     rotated copy is returned, with rows of padding as zeros.  A block's scale is the smallest power of two from 2^-40 to 2^60 with which 448 holds the
     block's largest magnitude.  It never falls while the block has older tokens; when it rises they are re-expressed, which is exact but for
     values that become subnormal.  Magnitudes above 448 * 2^60 (infinities) are stored as that, NaN as NaN.  The pages that a call writes to

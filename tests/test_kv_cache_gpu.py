@@ -38,7 +38,7 @@ STEPS = [  # tokens of each call
 @pytest.mark.parametrize("E,H,Hk,D,page,dim,pairs,dtype,layout", [
     (1, 1, 1, 64, 16, 64, "half", torch.bfloat16, "heads"), (3, 6, 2, 128, 64, 128, "interleaved", torch.bfloat16, "tokens"),
     (2, 12, 12, 64, 32, 32, "half", torch.float16, "tokens"), (2, 5, 5, 128, 16, 0, "half", torch.float16, "heads"),
-    (4, 8, 1, 128, 128, 64, "half", torch.bfloat16, "tokens"), (2, 3, 3, 64, 64, 8, "interleaved", torch.float16, "tokens")])
+    (4, 8, 1, 128, 128, 64, "half", torch.bfloat16, "tokens"), (2, 3, 3, 64, 64, 16, "interleaved", torch.float16, "tokens"), (1, 4, 9, 128, 32, 16, "half", torch.bfloat16, "heads")])
 def test_append_matches_the_definition(E, H, Hk, D, page, dim, pairs, dtype, layout, steps):
     import monarch_attention_b200 as ma
     total = sum(steps)
