@@ -62,7 +62,9 @@ struct AttendArgs {
   int row_blocks;       // blocks of 8 * kernel tiles rows; row = token * group + head of the group
   uint32_t k16[3], v16[3];  // strides of a page, head and token in units of 16 bytes: products with them are one instruction
   float *part_o, *part_ml;  // of the pieces of split heads: two a CTA
-  int4* split;              // one a CTA: the head whose pieces begin there
+  int4* split;              // where heads have been split: an entry a CTA or
+  int split_by_head;        // (1) a head and block of rows
+  int whole_heads;          // 1: no head is split
 };
 // Bytes of scratch, and how many row tiles and CTAs the call takes.
 size_t attend_workspace(int E, int N, int H, int kv_heads, int width, long long longest);

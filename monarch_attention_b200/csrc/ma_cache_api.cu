@@ -67,7 +67,8 @@ int check_attend_shape(const ma_b200_attend* p) {
   if (p->E <= 0 || p->H <= 0 || p->N <= 0 || p->cache.heads <= 0 || p->cache.page_size <= 0 || p->sequences.table_pages <= 0)
     return invalid("E, H, N, the cache's heads and page size and the table's columns must be positive");
   if (p->H % p->cache.heads != 0) return invalid("H must be a multiple of the cache's heads");
-  if ((long long)p->H / p->cache.heads * p->N > (1 << 28)) return invalid("too many query rows of a head");
+  const long long rows = (long long)p->H / p->cache.heads * p->N;
+  if (rows > (1 << 28) || (rows + 7) / 8 * p->cache.heads * p->E > 0x7fffffffLL) return invalid("too many query rows");
   return MA_B200_OK;
 }
 

@@ -35,13 +35,13 @@ constexpr int kWarps = 4, kSlice = 32, kStep = kWarps * kSlice;  // tokens of a 
 template <int D, int NT>
 struct Shape {
   static constexpr int kStages = D == 128 ? 2 : 3;
-  static constexpr int kStageBytes = 2 * kSlice * D + 16;
+  static constexpr int kStageBytes = 2 * kSlice * D + 16;  // keys, values and their two scales each
   static constexpr int kRows = 8 * NT;
   static constexpr bool kSharedRows = NT > 1;  // the query rows' operands are in shared memory: there are no registers for them
   static constexpr int kRing = kWarps * kStages * kStageBytes;
   static constexpr int kOperandBytes = kSharedRows ? kRows * D * 2 : 0;
   static constexpr int kSmem = kRing + kOperandBytes;
-  static constexpr int kCtas = NT == 4 ? 2 : 3;  // of an SM: what registers and shared memory allow
+  static constexpr int kCtas = NT > 2 ? 2 : 3;  // of an SM: what registers and shared memory allow
 };
 
 // Byte offset of 16-byte piece `piece` of token t in a slice: pieces are permuted so that neither the reads of the keys (8 rows x 4 pieces)
@@ -100,6 +100,24 @@ __device__ __forceinline__ Sequence sequence(const AttendArgs& a, int e) {
   return s;
 }
 
+// The steps of a call in `parts` shares that differ by one at most, the longer ones spread evenly: share i begins at i * whole + i * rest / parts.
+// (Divisions of 64 bits take longer than all else in front of the first load.)
+struct Share {
+  long long whole;
+  int rest, parts;
+  __device__ Share(long long total, int n) : parts(n) {
+    whole = total < 0x7fffffff ? (int)total / n : total / n;
+    rest = (int)(total - whole * n);
+  }
+  __device__ long long first(int i) const { return i * whole + (int)((long long)i * rest < 0x7fffffff ? i * rest / parts : (long long)i * rest / parts); }
+  __device__ int of(long long step) const {  // the share that a step is in
+    int i = min((int)((float)step / ((float)whole + (float)rest / (float)parts)) + 1, parts - 1);  // (within a share or two)
+    while (first(i) > step) --i;
+    while (i + 1 < parts && first(i + 1) <= step) ++i;
+    return i;
+  }
+};
+
 // A place in the list of steps.
 struct Place {
   int e, head, block, step;  // block: of rows
@@ -132,50 +150,71 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<D, NT>::kCtas) attend_kerne
   const int units = c.heads * a.row_blocks;
   stage_begin();  // (the joining kernel may come up where there is room)
 
-  // --- this CTA's share of the steps: prefix sums over the sequences, a run of them per thread
-  const int run = (a.E + kWarps * 32 - 1) / (kWarps * 32);
-  long long mine = 0;
-  for (int e = tid * run; e < min(a.E, (tid + 1) * run); ++e) {
-    const Sequence s = sequence(a, e);
-    mine += s.steps;
-    int x, y;
-    if (blockIdx.x == 0 && !sequence_of(c, e, a.N, &x, &y)) report(c.status, kBadLength);
-  }
-  long long upto = mine;
-#pragma unroll
-  for (int m = 1; m < 32; m <<= 1) {
-    const long long o = __shfl_up_sync(0xffffffffu, upto, m);
-    if (lane >= m) upto += o;
-  }
-  if (lane == 31) warp_sum[w] = upto;
-  __syncthreads();
-  for (int i = 0; i < w; ++i) upto += warp_sum[i];
-  long long total = 0;
-  for (int i = 0; i < kWarps; ++i) total += warp_sum[i];
-  total *= units;
-  const long long ctas = min((long long)gridDim.x, total);
-  if (blockIdx.x >= ctas) {
-    if (tid == 0) a.split[blockIdx.x] = make_int4(-1, 0, 0, 0);
-    return;
-  }
-  const long long begin = blockIdx.x * total / ctas, end = (blockIdx.x + 1) * total / ctas;
-  if ((upto - mine) * units <= begin && begin < upto * units) {
-    long long at = (upto - mine) * units;
-    int e = tid * run;
-    for (;; ++e) {
-      const long long n = (long long)sequence(a, e).steps * units;
-      if (begin < at + n) break;
-      at += n;
-    }
-    where_e = e;
-    where_at = begin - at;
-  }
-  __syncthreads();
+  // --- this CTA's share of the steps
   Place now;
-  now.e = where_e;
-  now.s = sequence(a, now.e);
-  const int unit = (int)(where_at / now.s.steps);
-  now.step = (int)(where_at - (long long)unit * now.s.steps);
+  long long total = 0, ctas = gridDim.x, end = 0;  // steps of the call, CTAs that have some, and the end of this one's
+  Share share(0, 1);
+  int steps = 0, unit;
+  if (a.whole_heads) {  // as many heads (and blocks of rows) as another CTA
+    const long long heads = (long long)a.E * units, u0 = blockIdx.x * heads / ctas, u1 = (blockIdx.x + 1) * heads / ctas;
+    now.e = (int)(u0 / units);
+    unit = (int)(u0 - (long long)now.e * units);
+    now.s = sequence(a, now.e);
+    now.step = 0;
+    for (long long u = u0; u < u1;) {
+      const int e = (int)(u / units);
+      const long long next = min(u1, (long long)(e + 1) * units);
+      steps += (int)(next - u) * sequence(a, e).steps;
+      u = next;
+    }
+    int x, y;
+    for (int e = blockIdx.x * kWarps * 32 + tid; e < a.E; e += gridDim.x * kWarps * 32)
+      if (!sequence_of(c, e, a.N, &x, &y)) report(c.status, kBadLength);
+  } else {  // prefix sums over the sequences, a run of them per thread
+    const int run = (a.E + kWarps * 32 - 1) / (kWarps * 32);
+    long long mine = 0;
+    for (int e = tid * run; e < min(a.E, (tid + 1) * run); ++e) {
+      mine += sequence(a, e).steps;
+      int x, y;
+      if (blockIdx.x == 0 && !sequence_of(c, e, a.N, &x, &y)) report(c.status, kBadLength);
+    }
+    long long upto = mine;
+#pragma unroll
+    for (int m = 1; m < 32; m <<= 1) {
+      const long long o = __shfl_up_sync(0xffffffffu, upto, m);
+      if (lane >= m) upto += o;
+    }
+    if (lane == 31) warp_sum[w] = upto;
+    __syncthreads();
+    for (int i = 0; i < w; ++i) upto += warp_sum[i];
+    for (int i = 0; i < kWarps; ++i) total += warp_sum[i];
+    total *= units;
+    ctas = min(ctas, total);
+    if (blockIdx.x >= ctas) {
+      if (tid == 0 && !a.split_by_head) a.split[blockIdx.x] = make_int4(-1, 0, 0, 0);
+      return;
+    }
+    share = Share(total, (int)ctas);
+    const long long begin = share.first(blockIdx.x);
+    end = share.first(blockIdx.x + 1);
+    steps = (int)(end - begin);
+    if ((upto - mine) * units <= begin && begin < upto * units) {
+      long long at = (upto - mine) * units;
+      int e = tid * run;
+      for (;; ++e) {
+        const long long n = (long long)sequence(a, e).steps * units;
+        if (begin < at + n) break;
+        at += n;
+      }
+      where_e = e;
+      where_at = begin - at;
+    }
+    __syncthreads();
+    now.e = where_e;
+    now.s = sequence(a, now.e);
+    unit = where_at < 0x7fffffff ? (int)where_at / now.s.steps : (int)(where_at / now.s.steps);
+    now.step = (int)(where_at - (long long)unit * now.s.steps);
+  }
   now.head = unit / a.row_blocks;
   now.block = unit - now.head * a.row_blocks;
   Place ahead = now;
@@ -205,20 +244,17 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<D, NT>::kCtas) attend_kerne
       const uint32_t page = max(pages[b], 0), row = ((t0 + b * kScaleBlock) & page_mask) + lane_row;
       const uint8_t* k = c.k + 16 * (page * (uint64_t)a.k16[0] + ahead.head * (uint64_t)a.k16[1] + row * (uint64_t)a.k16[2] + piece);
       const uint8_t* v = c.v + 16 * (page * (uint64_t)a.v16[0] + ahead.head * (uint64_t)a.v16[1] + row * (uint64_t)a.v16[2] + piece);
-      if (whole) {
 #pragma unroll
-        for (int i = 0; i < kPasses; ++i, k += a.k16[2] * (16ull * kRowsPerPass), v += a.v16[2] * (16ull * kRowsPerPass)) {
-          const uint32_t to = at + piece_at<D>(b * kScaleBlock + i * kRowsPerPass + lane_row, piece);
+      for (int i = 0; i < kPasses; ++i, k += a.k16[2] * (16ull * kRowsPerPass), v += a.v16[2] * (16ull * kRowsPerPass)) {
+        const int t = b * kScaleBlock + i * kRowsPerPass + lane_row;
+        const uint32_t to = at + piece_at<D>(t, piece);
+        if (whole) {
           copy16(to, k);
           copy16(to + kSlice * D, v);
-        }
-      } else {
-#pragma unroll
-        for (int i = 0; i < kPasses; ++i, k += a.k16[2] * (16ull * kRowsPerPass), v += a.v16[2] * (16ull * kRowsPerPass)) {
-          const int t = b * kScaleBlock + i * kRowsPerPass + lane_row;
+        } else {
           const bool real = t < left && pages[b] >= 0;
-          copy16(at + piece_at<D>(t, piece), real ? k : c.k, real);
-          copy16(at + kSlice * D + piece_at<D>(t, piece), real ? v : c.v, real);
+          copy16(to, real ? k : c.k, real);
+          copy16(to + kSlice * D, real ? v : c.v, real);
         }
       }
     }
@@ -229,7 +265,6 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<D, NT>::kCtas) attend_kerne
       copy4(at + 2 * kSlice * D + lane * 4, src + (page >= 0 ? row / kScaleBlock : 0), page >= 0);
     }
   };
-  const int steps = (int)(end - begin);
   look_up();
 #pragma unroll
   for (int i = 0; i < S::kStages - 1; ++i) {
@@ -247,14 +282,6 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<D, NT>::kCtas) attend_kerne
   bool fresh = true, later = false;                 // a head begins; the CTA has finished (a piece of) one
   int stage = 0;
   for (int i = 0; i < steps; ++i) {
-    copies_wait<S::kStages - 2>();
-    __syncwarp();
-    if (i + S::kStages - 1 < steps) {
-      fetch(stage == 0 ? S::kStages - 1 : stage - 1);
-      advance(a, &ahead);
-      if (i + S::kStages < steps) look_up();
-    }
-    copies_commit();
     const int row0 = now.block * S::kRows;
     if (fresh) {
       fresh = false;
@@ -329,7 +356,14 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<D, NT>::kCtas) attend_kerne
           for (int j = 0; j < 4; ++j) o[n][m][j] = 0.0f;
       }
     }
-
+    copies_wait<S::kStages - 2>();
+    __syncwarp();
+    if (i + S::kStages - 1 < steps) {
+      fetch(stage == 0 ? S::kStages - 1 : stage - 1);
+      advance(a, &ahead);
+      if (i + S::kStages < steps) look_up();
+    }
+    copies_commit();
     const int t0 = now.s.lo + now.step * kStep + w * kSlice;
     if (t0 < now.s.len) {
       const uint8_t* const keys = smem + (w * S::kStages + stage) * S::kStageBytes;
@@ -368,10 +402,9 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<D, NT>::kCtas) attend_kerne
           }
         }
       const float4 scales = *reinterpret_cast<const float4*>(keys + 2 * kSlice * D);
-      const float ks[2] = {scales.x, scales.y}, vs[2] = {scales.z, scales.w};
-      const float vl[2] = {__log2f(vs[0]), __log2f(vs[1])};
-      const bool whole = t0 >= full_low && t0 + kSlice <= full_high;
+      const float ks[2] = {scales.x, scales.y}, vs[2] = {scales.z, scales.w}, vl[2] = {__log2f(scales.z), __log2f(scales.w)};
       uint32_t weights[2][NT][2];
+      const bool whole = t0 >= full_low && t0 + kSlice <= full_high;
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
         const float2 rs = *reinterpret_cast<const float2*>(row_scale + n * 8 + 2 * q4);
@@ -464,8 +497,8 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<D, NT>::kCtas) attend_kerne
 
     const bool last_of_head = now.step + 1 == now.s.steps;
     if (last_of_head || i + 1 == steps) {
-      // --- the four warps' sums into one: each brings its own to the common maximum and leaves it in its ring, in the stage that it has
-      // just used up, two tiles of rows at a time; warp w then adds up rows 2 w and 2 w + 1 of each tile
+      // --- the four warps' sums into one: each brings its own to the common maximum and leaves it in its ring, in the stage that it has just
+      // used up, a tile of rows at a time (by turns in its two halves); warp w then adds up rows 2 w and 2 w + 1
       fresh = true;
 #pragma unroll
       for (int n = 0; n < NT; ++n)
@@ -478,31 +511,26 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<D, NT>::kCtas) attend_kerne
       __syncthreads();
       const bool alone = last_of_head && i >= now.step;  // all of the head's steps were this CTA's
       const int slot = 2 * blockIdx.x + (later ? 1 : 0);
-      constexpr int kTiles = NT < 2 ? NT : 2;
       float* const mine = reinterpret_cast<float*>(smem + (w * S::kStages + stage) * S::kStageBytes);
 #pragma unroll
-      for (int n0 = 0; n0 < NT; n0 += kTiles) {
+      for (int n = 0; n < NT; ++n) {
 #pragma unroll
-        for (int n = n0; n < n0 + kTiles; ++n)
+        for (int j = 0; j < 2; ++j) {
+          float most = -CUDART_INF_F;
 #pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            float most = -CUDART_INF_F;
+          for (int v = 0; v < kWarps; ++v) most = fmaxf(most, tops[v][n * 8 + 2 * q4 + j].x);
+          const float x = ex2(top[n][j] - (most == -CUDART_INF_F ? 0.0f : most));
 #pragma unroll
-            for (int v = 0; v < kWarps; ++v) most = fmaxf(most, tops[v][n * 8 + 2 * q4 + j].x);
-            const float x = ex2(top[n][j] - (most == -CUDART_INF_F ? 0.0f : most));
-#pragma unroll
-            for (int m = 0; m < kWords; ++m) {
-              mine[(((n - n0) * kWords + m) * 4 + j) * 32 + lane] = o[n][m][j] * x;
-              mine[(((n - n0) * kWords + m) * 4 + 2 + j) * 32 + lane] = o[n][m][2 + j] * x;
-            }
+          for (int m = 0; m < kWords; ++m) {
+            mine[(n & 1) * 8 * D + (m * 4 + j) * 32 + lane] = o[n][m][j] * x;
+            mine[(n & 1) * 8 * D + (m * 4 + 2 + j) * 32 + lane] = o[n][m][2 + j] * x;
           }
+        }
         __syncthreads();
         // 8 neighbouring features of a row a lane (64 features: 4), in the places where the lanes of the product had them
         constexpr int kRun = D / 16;
-        const int j = lane >> 4, u = lane & 15, from_g = u >> 1, m0 = (u & 1) * (kWords / 2);
-#pragma unroll
-        for (int n = n0; n < n0 + kTiles; ++n) {
-          const int r = n * 8 + 2 * w + j;
+        const int j = lane >> 4, u = lane & 15, r = n * 8 + 2 * w + j;
+        if (row0 + r < a.N * a.group) {
           float x[kRun];
 #pragma unroll
           for (int f = 0; f < kRun; ++f) x[f] = 0.0f;
@@ -510,18 +538,17 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<D, NT>::kCtas) attend_kerne
           for (int v = 0; v < kWarps; ++v) {
             const float* theirs = reinterpret_cast<const float*>(smem + (v * S::kStages + stage) * S::kStageBytes);
 #pragma unroll
-            for (int f = 0; f < kRun; ++f) x[f] += theirs[(((n - n0) * kWords + m0 + f / 2) * 4 + j + 2 * (f & 1)) * 32 + from_g * 4 + w];
+            for (int f = 0; f < kRun; ++f) x[f] += theirs[(n & 1) * 8 * D + (((u & 1) * (kWords / 2) + f / 2) * 4 + j + 2 * (f & 1)) * 32 + (u >> 1) * 4 + w];
           }
-          float most = -CUDART_INF_F, total = 0.0f;
+          float most = -CUDART_INF_F, all = 0.0f;
 #pragma unroll
           for (int v = 0; v < kWarps; ++v) most = fmaxf(most, tops[v][r].x);
           const float base = most == -CUDART_INF_F ? 0.0f : most;
 #pragma unroll
-          for (int v = 0; v < kWarps; ++v) total += tops[v][r].y * ex2(tops[v][r].x - base);
+          for (int v = 0; v < kWarps; ++v) all += tops[v][r].y * ex2(tops[v][r].x - base);
           if (alone) {
             const int token = (row0 + r) / a.group, h = now.head * a.group + row0 + r - token * a.group;
-            if (token >= a.N) continue;
-            const float inverse = token < now.s.count && total > 0.0f ? 1.0f / total : 0.0f;
+            const float inverse = token < now.s.count && all > 0.0f ? 1.0f / all : 0.0f;
             T* dst = reinterpret_cast<T*>(const_cast<void*>(a.out.ptr)) + now.e * a.out.se + h * a.out.sh + token * a.out.sn + u * kRun;
             if constexpr (D == 128)
               *reinterpret_cast<uint4*>(dst) = make_uint4(sm100::pack2<T>(x[0] * inverse, x[1] * inverse), sm100::pack2<T>(x[2] * inverse, x[3] * inverse),
@@ -532,19 +559,20 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<D, NT>::kCtas) attend_kerne
             float* dst = a.part_o + ((size_t)slot * S::kRows + r) * D + u * kRun;
 #pragma unroll
             for (int f = 0; f < kRun; f += 4) *reinterpret_cast<float4*>(dst + f) = make_float4(x[f], x[f + 1], x[f + 2], x[f + 3]);
-            if (u == 0) *reinterpret_cast<float2*>(a.part_ml + ((size_t)slot * S::kRows + r) * 2) = make_float2(most, total);
+            if (u == 0) *reinterpret_cast<float2*>(a.part_ml + ((size_t)slot * S::kRows + r) * 2) = make_float2(most, all);
           }
         }
-        __syncthreads();
       }
-      if (tid == 0 && i + 1 == steps) {
-        // a head that goes on in the next CTA and began here: this CTA's entry names it and the CTA of its last step
+      __syncthreads();
+      if (tid == 0 && !a.whole_heads && (a.split_by_head ? i >= now.step : i + 1 == steps)) {
+        // a head that began here and goes on in the next CTA: the entry names it, this CTA, and the CTA of its last step
+        const int which = (now.e * c.heads + now.head) * a.row_blocks + now.block;
         int4 entry = make_int4(-1, 0, 0, 0);
         if (!last_of_head && i >= now.step) {
           const long long last = end - 1 + (now.s.steps - 1 - now.step);
-          entry = make_int4(now.e, now.head * a.row_blocks + now.block, (int)(((last + 1) * ctas - 1) / total), later ? 1 : 0);
+          entry = make_int4(which, blockIdx.x, share.of(last), later ? 1 : 0);
         }
-        a.split[blockIdx.x] = entry;
+        a.split[a.split_by_head ? which : (int)blockIdx.x] = entry;
       }
       later = true;
     }
@@ -553,25 +581,37 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<D, NT>::kCtas) attend_kerne
   }
 }
 
-// Joins the pieces of the heads that were split: a CTA for each CTA of the kernel above (many have nothing to do) and row.  The pieces' weights
-// come first, for all at once; then every 16 bytes of a row is the sum over the pieces of one of several groups of threads, with many
-// loads in flight: 222 pieces of 128 features take 3 us, one piece after the other took 17.
+// Joins the pieces of the heads that were split: a CTA for each entry of the table of the kernel above, row, and 32 features.  Every 16 bytes
+// of a row are summed over the pieces by several threads, each with many loads in flight, on their way before the weights are known.  The table has an entry for each head where there are fewer heads than CTAs, else one for each CTA.
 template <typename T, int D>
 __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ AttendArgs a, int tile_rows) {
-  constexpr int kLanes = D / 4, kGroups = 256 / kLanes, kMost = 1024, kInFlight = 8;
-  __shared__ float weights[kMost], reduced[8], totals[8];
+  constexpr int W = 32, kLanes = W / 4, kGroups = 256 / kLanes, kMost = 1024, kInFlight = 8;
+  __shared__ float2 weights[kMost];  // of the first pieces: maximum and sum
   __shared__ float4 sums[256];
+  __shared__ float totals[256], reduced[8];
   grid_wait();
   const int4 entry = a.split[blockIdx.x];
   if (entry.x < 0) return;
-  const int e = entry.x, head = entry.y / a.row_blocks, r = blockIdx.y, row = (entry.y - head * a.row_blocks) * tile_rows + r;
-  const int token = row / a.group, h = head * a.group + row - token * a.group;
+  const int block = entry.x % a.row_blocks, head = entry.x / a.row_blocks % a.cache.heads, e = entry.x / a.row_blocks / a.cache.heads;
+  const int r = blockIdx.y, row = block * tile_rows + r, token = row / a.group, h = head * a.group + row - token * a.group;
   if (token >= a.N) return;
-  const int pieces = entry.z - (int)blockIdx.x + 1;
-  auto slot = [&](int i) { return (size_t)(2 * (blockIdx.x + i) + (i == 0 ? entry.w : 0)) * tile_rows + r; };
+  const int pieces = entry.z - entry.y + 1;
+  auto slot = [&](int i) { return (size_t)(2 * (entry.y + i) + (i == 0 ? entry.w : 0)) * tile_rows + r; };
   const int tid = threadIdx.x, lane = tid % kLanes, group = tid / kLanes;
+  const float4* const rows = reinterpret_cast<const float4*>(a.part_o) + blockIdx.z * kLanes + lane;
+  float4 x[kInFlight];
+  auto load = [&](int i) {
+#pragma unroll
+    for (int j = 0; j < kInFlight; ++j)
+      if (i + j * kGroups < pieces) x[j] = rows[slot(i + j * kGroups) * (D / 4)];
+  };
+  load(group);  // (on the way while the weights are found)
   float top = -CUDART_INF_F;
-  for (int i = tid; i < pieces; i += 256) top = fmaxf(top, a.part_ml[2 * slot(i)]);
+  for (int i = tid; i < pieces; i += 256) {
+    const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + 2 * slot(i));
+    if (i < kMost) weights[i] = ml;
+    top = fmaxf(top, ml.x);
+  }
 #pragma unroll
   for (int m = 16; m > 0; m >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, m));
   if ((tid & 31) == 0) reduced[tid >> 5] = top;
@@ -581,73 +621,119 @@ __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ Atten
   const float base = top == -CUDART_INF_F ? 0.0f : top;
   float4 acc = make_float4(0, 0, 0, 0);
   float total = 0.0f;
-  for (int i0 = 0; i0 < pieces; i0 += kMost) {
-    const int n = min(kMost, pieces - i0);
-    for (int i = tid; i < n; i += 256) {
-      const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + 2 * slot(i0 + i));
-      weights[i] = ex2(ml.x - base);
-      total += weights[i] * ml.y;
-    }
-    __syncthreads();
-    for (int i = group; i < n; i += kGroups * kInFlight) {
-      float4 x[kInFlight];
+  for (int i = group; i < pieces; i += kGroups * kInFlight) {
 #pragma unroll
-      for (int j = 0; j < kInFlight; ++j)
-        x[j] = i + j * kGroups < n ? reinterpret_cast<const float4*>(a.part_o + slot(i0 + i + j * kGroups) * D)[lane] : make_float4(0, 0, 0, 0);
-#pragma unroll
-      for (int j = 0; j < kInFlight; ++j) {
-        const float weight = i + j * kGroups < n ? weights[i + j * kGroups] : 0.0f;
-        acc.x += weight * x[j].x; acc.y += weight * x[j].y; acc.z += weight * x[j].z; acc.w += weight * x[j].w;
-      }
+    for (int j = 0; j < kInFlight; ++j) {
+      const int n = i + j * kGroups;
+      if (n >= pieces) break;
+      const float2 ml = n < kMost ? weights[n] : *reinterpret_cast<const float2*>(a.part_ml + 2 * slot(n));
+      const float weight = ex2(ml.x - base);
+      total += weight * ml.y;
+      acc.x += weight * x[j].x; acc.y += weight * x[j].y; acc.z += weight * x[j].z; acc.w += weight * x[j].w;
     }
-    __syncthreads();
+    load(i + kGroups * kInFlight);
   }
-#pragma unroll
-  for (int m = 16; m > 0; m >>= 1) total += __shfl_xor_sync(0xffffffffu, total, m);
-  if ((tid & 31) == 0) totals[tid >> 5] = total;
   sums[tid] = acc;
+  totals[tid] = total;
   __syncthreads();
   if (group != 0) return;
-#pragma unroll
-  for (int i = 1; i < kGroups; ++i) {
-    const float4 x = sums[i * kLanes + lane];
-    acc.x += x.x; acc.y += x.y; acc.z += x.z; acc.w += x.w;
+  for (int i = 1; i < min(kGroups, pieces); ++i) {
+    const float4 y = sums[i * kLanes + lane];
+    acc.x += y.x; acc.y += y.y; acc.z += y.z; acc.w += y.w;
+    total += totals[i * kLanes + lane];
   }
-  total = 0.0f;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) total += totals[i];
   int len, count;
   sequence_of(a.cache, e, a.N, &len, &count);
   const float inverse = token < count && total > 0.0f ? 1.0f / total : 0.0f;
-  T* dst = reinterpret_cast<T*>(const_cast<void*>(a.out.ptr)) + e * a.out.se + h * a.out.sh + token * a.out.sn + lane * 4;
+  T* dst = reinterpret_cast<T*>(const_cast<void*>(a.out.ptr)) + e * a.out.se + h * a.out.sh + token * a.out.sn + blockIdx.z * W + lane * 4;
   *reinterpret_cast<uint2*>(dst) = make_uint2(sm100::pack2<T>(acc.x * inverse, acc.y * inverse), sm100::pack2<T>(acc.z * inverse, acc.w * inverse));
 }
 
-int row_tiles(int rows) { return rows <= 8 ? 1 : rows <= 16 ? 2 : 4; }
-int ctas_per_sm(int nt) { return nt == 4 ? Shape<128, 4>::kCtas : Shape<128, 1>::kCtas; }
+// The same where there are many rows: a warp for each row, without a word to the others.
+template <typename T, int D>
+__global__ void __launch_bounds__(256) join_rows_kernel(const __grid_constant__ AttendArgs a, int tile_rows, int rows, int entries) {
+  constexpr int kRun = D / 32, kInFlight = 4;
+  using Run = std::conditional_t<kRun == 4, float4, float2>;
+  grid_wait();
+  const int lane = threadIdx.x & 31, task = blockIdx.x * 8 + (threadIdx.x >> 5), at = task / rows, r = task - at * rows;
+  if (at >= entries) return;
+  const int4 entry = a.split[at];
+  if (entry.x < 0) return;
+  const int block = entry.x % a.row_blocks, unit = entry.x / a.row_blocks, e = unit / a.cache.heads, head = unit - e * a.cache.heads;
+  const int row = block * tile_rows + r, token = row / a.group, h = head * a.group + row - token * a.group;
+  if (token >= a.N) return;
+  const int pieces = entry.z - entry.y + 1;
+  auto slot = [&](int i) { return (size_t)(2 * (entry.y + i) + (i == 0 ? entry.w : 0)) * tile_rows + r; };
+  float acc[kRun] = {}, total = 0.0f, top = -CUDART_INF_F;
+  for (int i0 = 0; i0 < pieces; i0 += kInFlight) {
+    float2 ml[kInFlight];
+    Run x[kInFlight];
+#pragma unroll
+    for (int j = 0; j < kInFlight; ++j) {
+      ml[j] = make_float2(-CUDART_INF_F, 0.0f);
+      x[j] = Run{};
+      if (i0 + j >= pieces) continue;
+      ml[j] = *reinterpret_cast<const float2*>(a.part_ml + 2 * slot(i0 + j));
+      x[j] = reinterpret_cast<const Run*>(a.part_o + slot(i0 + j) * D)[lane];
+    }
+    const float before = top;
+#pragma unroll
+    for (int j = 0; j < kInFlight; ++j) top = fmaxf(top, ml[j].x);
+    const float base = top == -CUDART_INF_F ? 0.0f : top, shrink = ex2(before - base);
+    total *= shrink;
+#pragma unroll
+    for (int f = 0; f < kRun; ++f) acc[f] *= shrink;
+#pragma unroll
+    for (int j = 0; j < kInFlight; ++j) {
+      const float weight = ex2(ml[j].x - base);
+      total += weight * ml[j].y;
+      const float* y = reinterpret_cast<const float*>(&x[j]);
+#pragma unroll
+      for (int f = 0; f < kRun; ++f) acc[f] += weight * y[f];
+    }
+  }
+  int len, count;
+  sequence_of(a.cache, e, a.N, &len, &count);
+  const float inverse = token < count && total > 0.0f ? 1.0f / total : 0.0f;
+  T* dst = reinterpret_cast<T*>(const_cast<void*>(a.out.ptr)) + e * a.out.se + h * a.out.sh + token * a.out.sn + lane * kRun;
+  if constexpr (kRun == 4)
+    *reinterpret_cast<uint2*>(dst) = make_uint2(sm100::pack2<T>(acc[0] * inverse, acc[1] * inverse), sm100::pack2<T>(acc[2] * inverse, acc[3] * inverse));
+  else
+    *reinterpret_cast<uint32_t*>(dst) = sm100::pack2<T>(acc[0] * inverse, acc[1] * inverse);
+}
+
+int row_tiles(int rows) { return rows <= 32 ? (rows + 7) / 8 : 4; }
+int ctas_per_sm(int nt) { return nt > 2 ? Shape<128, 4>::kCtas : Shape<128, 1>::kCtas; }
+
+constexpr int kWholeSteps = 4;  // heads of up to as many steps are not split
 
 // CTAs of a call: what the GPU holds at once, and no more than the steps that the lengths can have.
 long long grid_of(int E, int N, int H, int kv_heads, int width, long long longest) {
   const int rows = H / kv_heads * N, nt = row_tiles(rows);
   const long long units = (long long)E * kv_heads * ((rows + 8 * nt - 1) / (8 * nt));
-  const long long steps = units * ((longest + kStep - 1) / kStep > 1 ? (longest + kStep - 1) / kStep : 1);
+  const long long steps = longest <= kWholeSteps * kStep ? units : units * ((longest + kStep - 1) / kStep);
   const long long most = (long long)ctas_per_sm(nt) * sm_count();
   return steps < most ? steps : most;
 }
 
 template <typename T, int D, int NT>
-cudaError_t launch(AttendArgs& a, long long grid, bool split, cudaStream_t stream) {
+cudaError_t launch(AttendArgs& a, long long grid, cudaStream_t stream) {
   const void* fn = (const void*)attend_kernel<T, D, NT>;
   constexpr size_t smem = Shape<D, NT>::kSmem;
   cudaError_t err = allow_dynamic_smem(fn, smem);
   if (err != cudaSuccess) return err;
   void* args[] = {(void*)&a};
   err = launch_kernel(fn, dim3((unsigned)grid), dim3(kWarps * 32), args, smem, stream);
-  if (err != cudaSuccess || !split) return err;
+  if (err != cudaSuccess || a.whole_heads) return err;
   int tile_rows = 8 * NT;
   void* join_args[] = {(void*)&a, (void*)&tile_rows};
-  const int rows = a.group * a.N < tile_rows ? a.group * a.N : tile_rows;
-  return launch_kernel((const void*)join_kernel<T, D>, dim3((unsigned)grid, rows), dim3(256), join_args, 0, stream);
+  const unsigned rows = a.group * a.N < tile_rows ? a.group * a.N : tile_rows;
+  const long long entries = a.split_by_head ? (long long)a.E * a.cache.heads * a.row_blocks : grid;
+  // few heads have many pieces each: their rows are cut into parts of 32 features
+  if (entries * rows < 2 * sm_count()) return launch_kernel((const void*)join_kernel<T, D>, dim3((unsigned)entries, rows, D / 32), dim3(256), join_args, 0, stream);
+  int n_rows = (int)rows, n_entries = (int)entries;
+  void* rows_args[] = {(void*)&a, (void*)&tile_rows, (void*)&n_rows, (void*)&n_entries};
+  return launch_kernel((const void*)join_rows_kernel<T, D>, dim3((unsigned)((entries * rows + 7) / 8)), dim3(256), rows_args, 0, stream);
 }
 
 }  // namespace
@@ -670,10 +756,13 @@ cudaError_t launch_attend(AttendArgs a, int dtype, int width, void* workspace, l
   at += ((size_t)grid * sizeof(int4) + 255) / 256 * 256;
   a.part_o = reinterpret_cast<float*>(at);
   a.part_ml = a.part_o + (size_t)grid * 2 * 8 * nt * width;
-  const bool split = longest > kStep;  // (a head of one step is never split)
+  a.split_by_head = (long long)a.E * a.cache.heads * a.row_blocks <= grid;
+  // A head of a few steps stays with one CTA: a second kernel costs 3 us, a step 0.7.
+  a.whole_heads = longest <= kWholeSteps * kStep;
   const bool bf = dtype == MA_B200_BF16;
 #define MA_ATTEND(T, D) \
-  (nt == 1 ? launch<T, D, 1>(a, grid, split, stream) : nt == 2 ? launch<T, D, 2>(a, grid, split, stream) : launch<T, D, 4>(a, grid, split, stream))
+  (nt == 1 ? launch<T, D, 1>(a, grid, stream) : nt == 2 ? launch<T, D, 2>(a, grid, stream) : \
+   nt == 3 ? launch<T, D, 3>(a, grid, stream) : launch<T, D, 4>(a, grid, stream))
   if (width == 128) return bf ? MA_ATTEND(__nv_bfloat16, 128) : MA_ATTEND(__half, 128);
   return bf ? MA_ATTEND(__nv_bfloat16, 64) : MA_ATTEND(__half, 64);
 #undef MA_ATTEND
