@@ -68,6 +68,11 @@ struct AttendArgs {
 };
 // Bytes of scratch, and how many row tiles and CTAs the call takes.
 size_t attend_workspace(int E, int N, int H, int kv_heads, int width, long long longest);
-cudaError_t launch_attend(AttendArgs a, int dtype, int width, void* workspace, long long longest, cudaStream_t stream);
+cudaError_t launch_attend(AttendArgs a, int dtype, int width, void* workspace, long long longest, int* wait_status, cudaStream_t stream);
+// The pieces of `entries` heads and blocks of tile_rows rows (a.split, a.part_o, a.part_ml; a head's pieces `stride` slots apart) into a.out.
+cudaError_t launch_join(const AttendArgs& a, int dtype, int width, int tile_rows, int entries, int stride, cudaStream_t stream);
+// The kernel for many rows (ma_cache_prompt.cu).
+size_t prompt_workspace(int E, int N, int H, int kv_heads, int width, long long longest);
+cudaError_t launch_prompt(AttendArgs a, int dtype, int width, void* workspace, long long longest, int* wait_status, cudaStream_t stream);
 
 }  // namespace ma

@@ -132,10 +132,13 @@ int ma_b200_cache_attend(const ma_b200_attend* p, void* workspace, size_t worksp
   if (workspace == nullptr || reinterpret_cast<uintptr_t>(workspace) % 256 != 0) return invalid("workspace is NULL or not 256-byte aligned");
   if (workspace_bytes < need)
     return fail_with(MA_B200_WORKSPACE_TOO_SMALL, "workspace has " + std::to_string(workspace_bytes) + " bytes, need " + std::to_string(need));
+  int dev = 0;
+  (void)cudaGetDevice(&dev);
+  int* const wait_status = ma::host_status_word(dev, 0);
   a.q = view(p->q); a.out = view(p->out);
   a.E = p->E; a.N = p->N; a.H = p->H; a.group = p->H / p->cache.heads;
   a.causal = p->causal != 0; a.window = p->window; a.scale = p->scale; a.softcap = p->softcap;
-  return launched(ma::launch_attend(a, p->dtype, p->cache.width, workspace, most, reinterpret_cast<cudaStream_t>(stream)), "attention over the cache");
+  return launched(ma::launch_attend(a, p->dtype, p->cache.width, workspace, most, wait_status, reinterpret_cast<cudaStream_t>(stream)), "attention over the cache");
 }
 
 int ma_b200_poll_cache_status(int device) {

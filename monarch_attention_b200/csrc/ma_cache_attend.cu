@@ -651,7 +651,7 @@ __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ Atten
 
 // The same where there are many rows: a warp for each row, without a word to the others.
 template <typename T, int D>
-__global__ void __launch_bounds__(256) join_rows_kernel(const __grid_constant__ AttendArgs a, int tile_rows, int rows, int entries) {
+__global__ void __launch_bounds__(256) join_rows_kernel(const __grid_constant__ AttendArgs a, int tile_rows, int rows, int entries, int stride) {
   constexpr int kRun = D / 32, kInFlight = 4;
   using Run = std::conditional_t<kRun == 4, float4, float2>;
   grid_wait();
@@ -663,7 +663,7 @@ __global__ void __launch_bounds__(256) join_rows_kernel(const __grid_constant__ 
   const int row = block * tile_rows + r, token = row / a.group, h = head * a.group + row - token * a.group;
   if (token >= a.N) return;
   const int pieces = entry.z - entry.y + 1;
-  auto slot = [&](int i) { return (size_t)(2 * (entry.y + i) + (i == 0 ? entry.w : 0)) * tile_rows + r; };
+  auto slot = [&](int i) { return (size_t)(stride * (entry.y + i) + (i == 0 ? entry.w : 0)) * tile_rows + r; };
   float acc[kRun] = {}, total = 0.0f, top = -CUDART_INF_F;
   for (int i0 = 0; i0 < pieces; i0 += kInFlight) {
     float2 ml[kInFlight];
@@ -705,6 +705,8 @@ __global__ void __launch_bounds__(256) join_rows_kernel(const __grid_constant__ 
 int row_tiles(int rows) { return rows <= 32 ? (rows + 7) / 8 : 4; }
 int ctas_per_sm(int nt) { return nt > 2 ? Shape<128, 4>::kCtas : Shape<128, 1>::kCtas; }
 
+constexpr long long kPromptRows = 65;  // from as many rows on, the tcgen05 kernel
+
 constexpr int kWholeSteps = 4;  // heads of up to as many steps are not split
 
 // CTAs of a call: what the GPU holds at once, and no more than the steps that the lengths can have.
@@ -731,26 +733,34 @@ cudaError_t launch(AttendArgs& a, long long grid, cudaStream_t stream) {
   const long long entries = a.split_by_head ? (long long)a.E * a.cache.heads * a.row_blocks : grid;
   // few heads have many pieces each: their rows are cut into parts of 32 features
   if (entries * rows < 2 * sm_count()) return launch_kernel((const void*)join_kernel<T, D>, dim3((unsigned)entries, rows, D / 32), dim3(256), join_args, 0, stream);
-  int n_rows = (int)rows, n_entries = (int)entries;
-  void* rows_args[] = {(void*)&a, (void*)&tile_rows, (void*)&n_rows, (void*)&n_entries};
-  return launch_kernel((const void*)join_rows_kernel<T, D>, dim3((unsigned)((entries * rows + 7) / 8)), dim3(256), rows_args, 0, stream);
+  return launch_join(a, std::is_same<T, __half>::value ? MA_B200_F16 : MA_B200_BF16, D, tile_rows, (int)entries, 2, stream);
 }
 
 }  // namespace
 
+cudaError_t launch_join(const AttendArgs& a, int dtype, int width, int tile_rows, int entries, int stride, cudaStream_t stream) {
+  int rows = a.group * a.N < tile_rows ? a.group * a.N : tile_rows;
+  void* args[] = {(void*)&a, (void*)&tile_rows, (void*)&rows, (void*)&entries, (void*)&stride};
+  const bool bf = dtype == MA_B200_BF16;
+  const void* fn = width == 128 ? (bf ? (const void*)join_rows_kernel<__nv_bfloat16, 128> : (const void*)join_rows_kernel<__half, 128>)
+                                : (bf ? (const void*)join_rows_kernel<__nv_bfloat16, 64> : (const void*)join_rows_kernel<__half, 64>);
+  return launch_kernel(fn, dim3((unsigned)(((long long)entries * rows + 7) / 8)), dim3(256), args, 0, stream);
+}
+
 size_t attend_workspace(int E, int N, int H, int kv_heads, int width, long long longest) {
+  if (H / kv_heads * (long long)N >= kPromptRows) return prompt_workspace(E, N, H, kv_heads, width, longest);
   const long long grid = grid_of(E, N, H, kv_heads, width, longest), rows = 8 * row_tiles(H / kv_heads * N);
   const size_t entries = ((size_t)grid * sizeof(int4) + 255) / 256 * 256;
   return entries + (size_t)grid * 2 * rows * (width + 2) * sizeof(float);
 }
 
-cudaError_t launch_attend(AttendArgs a, int dtype, int width, void* workspace, long long longest, cudaStream_t stream) {
+cudaError_t launch_attend(AttendArgs a, int dtype, int width, void* workspace, long long longest, int* wait_status, cudaStream_t stream) {
+  const long long strides[6] = {a.cache.k_sp, a.cache.k_sh, a.cache.k_st, a.cache.v_sp, a.cache.v_sh, a.cache.v_st};
+  for (int i = 0; i < 6; ++i) (i < 3 ? a.k16[i] : a.v16[i - 3]) = (uint32_t)(strides[i] / 16);
+  if (a.group * (long long)a.N >= kPromptRows) return launch_prompt(a, dtype, width, workspace, longest, wait_status, stream);
   const int rows = a.group * a.N, nt = row_tiles(rows);
   const long long grid = grid_of(a.E, a.N, a.H, a.cache.heads, width, longest);
   a.row_blocks = (rows + 8 * nt - 1) / (8 * nt);
-  const CacheArgs& c = a.cache;
-  const long long strides[6] = {c.k_sp, c.k_sh, c.k_st, c.v_sp, c.v_sh, c.v_st};
-  for (int i = 0; i < 6; ++i) (i < 3 ? a.k16[i] : a.v16[i - 3]) = (uint32_t)(strides[i] / 16);
   char* at = reinterpret_cast<char*>(workspace);
   a.split = reinterpret_cast<int4*>(at);
   at += ((size_t)grid * sizeof(int4) + 255) / 256 * 256;

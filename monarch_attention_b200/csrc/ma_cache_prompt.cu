@@ -1,0 +1,501 @@
+// Softmax attention of many query rows (a prompt, or a piece of one) over a paged cache in 8 bits, on the tcgen05 tensor cores.
+//
+// Bound by the tensor cores and by the exponentials (as many cycles at 128 features: 2 x 256 x 128 x 128 x 2 operations of a step are 2048 cycles,
+// its 256 x 128 exponentials 2048 of the special function units).  A CTA takes 256 rows (tokens times heads of a group) of a key head and
+// walks over its keys, 128 at a step:
+//  * Seven warps bring keys and values: bytes from global memory into registers, half a step ahead, and from there, widened to f16 (exact),
+//    into swizzled tiles in shared memory.  Two tiles of rows share them, so that the conversion and the shared memory's traffic, which a
+//    single tile would be bound by, count half.
+//  * One warp issues the products: scores S = Q K^T into tensor memory, and O += P V with the weights P read from tensor memory, where they
+//    take the place of their scores.  While the rows of one tile are exponentiated, the products of the other run.
+//  * Two warpgroups have a row a thread: the row's 128 scores go to registers in one go, and the maximum, the weights and their sum need no
+//    other thread.  Scales of blocks are applied as in the kernel for few rows (ma_cache_attend.cu): the keys' to the scores, the
+//    values' to the weights, with a reference that is raised (and O multiplied) only when a weight would pass 2^8.
+// Every wait is bounded; one that gives up ends the CTA's others, and the next call on the device reports it.
+#include <math_constants.h>
+
+#include <type_traits>
+
+#include "ma_cache.cuh"
+#include "ma_sm100.cuh"
+
+namespace ma {
+namespace {
+
+using namespace sm100;
+
+constexpr int kKeys = 128, kTileRows = 128, kRows = 2 * kTileRows;
+constexpr int kThreads = 512, kBringers = 224;  // warps 0-3, 4-7: rows; 8-14: keys and values; 15: products
+constexpr int kRowRegs = 176, kHelperRegs = 80;
+static_assert(256 * (kRowRegs + kHelperRegs) <= kThreads * 128, "setmaxnreg draws on the launch's registers");
+constexpr int kRing = 8;  // steps whose pages and scales are kept
+constexpr float kSlack = 8.0f;
+
+enum Bar { kQ0, kQ1, kKFull, kKEmpty = kKFull + 2, kVFull = kKEmpty + 2, kVEmpty = kVFull + 2, kS0 = kVEmpty + 2, kS1, kP0, kP1, kO, kBars };
+
+// What the rows need of a step's 8 blocks.
+struct alignas(16) Blocks {
+  float k_scale[8], v_scale[8], v_log[8];
+  int page[8];
+};
+
+template <int D>
+struct Layout {
+  static constexpr int kTileBytes = 128 * D * 2;  // 128 rows in f16: panels of 64 features
+  static constexpr int kQ = 0, kK = 2 * kTileBytes, kV = kK + 2 * kTileBytes, kBlocks = kV + 2 * kTileBytes;
+  static constexpr int kBarriers = kBlocks + kRing * (int)sizeof(Blocks), kFlags = kBarriers + 8 * kBars, kBytes = kFlags + 16;
+  static constexpr int kSmem = kBytes + 1024;  // (tiles start on 1024-byte boundaries)
+};
+
+struct PromptArgs {
+  AttendArgs a;
+  int pieces;        // that the keys of a CTA's rows are cut into
+  int* wait_status;  // mapped host word: a wait that gave up
+};
+
+template <int N>
+__device__ __forceinline__ void regs_inc() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N>
+__device__ __forceinline__ void regs_dec() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
+
+__device__ __forceinline__ uint32_t widen2(uint32_t codes, bool upper) {
+  uint32_t r;
+  asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, lo;\n\t}" : "=r"(r) : "r"(upper ? codes >> 16 : codes));
+  return r;
+}
+// 16 codes as two 16-byte chunks of a row: `chunk` and the one after it, in either order (lanes on different panels start with different ones,
+// so that they do not meet in a bank).
+__device__ __forceinline__ void put_codes(uint32_t panel, uint32_t row, uint32_t chunk, bool second_first, const uint4& c) {
+  uint32_t w[8] = {widen2(c.x, false), widen2(c.x, true), widen2(c.y, false), widen2(c.y, true),
+                   widen2(c.z, false), widen2(c.z, true), widen2(c.w, false), widen2(c.w, true)};
+  const uint32_t a = panel + swz(row, chunk), b = panel + swz(row, chunk + 1);
+  st_shared_v4(second_first ? b : a, second_first ? w[4] : w[0], second_first ? w[5] : w[1], second_first ? w[6] : w[2], second_first ? w[7] : w[3]);
+  st_shared_v4(second_first ? a : b, second_first ? w[0] : w[4], second_first ? w[1] : w[5], second_first ? w[2] : w[6], second_first ? w[3] : w[7]);
+}
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_constant__ PromptArgs args) {
+  using L = Layout<D>;
+  constexpr int kPanel = 128 * 128, kPieces = kKeys * D / 16, kPer = (kPieces + kBringers - 1) / kBringers, kPiecesPerRow = D / 16;
+  constexpr uint32_t kTmemS = 0, kTmemO = 256;  // columns: S (and P) of both tiles, then O of both
+  extern __shared__ uint8_t smem_raw[];
+  const AttendArgs& a = args.a;
+  const CacheArgs& c = a.cache;
+  const uint32_t base = (smem_u32(smem_raw) + 1023) & ~1023u;
+  uint8_t* const smem = smem_raw + (base - smem_u32(smem_raw));
+  Blocks* const blocks = reinterpret_cast<Blocks*>(smem + L::kBlocks);
+  volatile int* const abort_flag = reinterpret_cast<volatile int*>(smem + L::kFlags);
+  const int tid = threadIdx.x, warp = tid >> 5;
+  auto bar = [&](int i) { return base + L::kBarriers + 8 * i; };
+  // (the vote brings the lanes of a warp back together, and of one mind)
+  auto wait = [&](int b, uint32_t phase) {
+    const bool r = __all_sync(0xffffffffu, mbar_wait_abortable(bar(b), phase & 1u, abort_flag));
+    if (!r) *abort_flag = 1;
+    return r;
+  };
+
+  grid_wait();
+  // --- the CTA's rows and keys; row blocks with more keys come first
+  const int piece = blockIdx.x % args.pieces, unit = blockIdx.x / args.pieces;  // unit: (block from the last on, sequence, head)
+  const int e_head = unit % (a.E * c.heads), block = a.row_blocks - 1 - unit / (a.E * c.heads);
+  const int e = e_head / c.heads, head = e_head % c.heads, row0 = block * kRows;
+  int len, count;
+  const bool fine = sequence_of(c, e, a.N, &len, &count);
+  if (!fine && tid == 0) report(c.status, kBadLength);
+  const int first_token = row0 / a.group, last_token = min((row0 + kRows - 1) / a.group, count - 1);
+  const bool two = row0 + kTileRows < count * a.group;  // the second tile has rows
+  int lo = 0, hi = len;
+  if (a.causal) hi = min(len, len - count + last_token + 1);
+  if (a.window > 0) lo = max(len - count + first_token - a.window + 1, 0) & ~(kScaleBlock - 1);
+  if (first_token >= count) hi = lo;
+  const int all_steps = max((hi - lo + kKeys - 1) / kKeys, 0);
+  const int step0 = (int)((long long)piece * all_steps / args.pieces), steps = (int)((long long)(piece + 1) * all_steps / args.pieces) - step0;
+  lo += step0 * kKeys;
+
+  if (tid == 0) {
+    mbar_init(bar(kQ0), 128);
+    mbar_init(bar(kQ1), 128);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(bar(kKFull + i), kBringers);
+      mbar_init(bar(kVFull + i), kBringers);
+      mbar_init(bar(kKEmpty + i), 1);
+      mbar_init(bar(kVEmpty + i), 1);
+      mbar_init(bar(kS0 + i), 1);
+      mbar_init(bar(kP0 + i), 128);
+    }
+    mbar_init(bar(kO), 1);
+    *abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 15) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(base + L::kFlags + 4), "r"(512) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(smem + L::kFlags + 4);
+
+  if (warp < 8) {
+    // =========================== a row a thread ======================================================================
+    regs_inc<kRowRegs>();
+    const int tile = warp >> 2, r = tid & 127, row = row0 + tile * kTileRows + r;
+    const int token = row / a.group, h = head * a.group + row - token * a.group;
+    const bool exists = token < a.N, real = token < count;
+    const uint32_t lanes = (uint32_t)(warp & 3) << 21;  // the warp's 32 lanes of tensor memory
+    const uint32_t t_s = tmem + kTmemS + tile * 128 + lanes, t_o = tmem + kTmemO + tile * 128 + lanes;
+    const bool works = steps > 0 && (tile == 0 || two);
+    float factor = fabsf(a.scale) * kLog2e, top = -CUDART_INF_F, sum = 0.0f;
+    bool ok = true;
+    if (works) {
+      // the query row in f16, brought to magnitudes of 1 to 2 by a power of two (bf16), with the sign of the scale
+      const uint4* src = reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(a.q.ptr) + (real ? e * a.q.se + h * a.q.sh + token * a.q.sn : 0));
+      uint4 raw[D / 8];
+#pragma unroll
+      for (int i = 0; i < D / 8; ++i) raw[i] = real ? src[i] : make_uint4(0, 0, 0, 0);
+      float down = 1.0f;
+      if constexpr (!std::is_same<T, __half>::value) {
+        float amax = 0.0f;
+#pragma unroll
+        for (int i = 0; i < D / 8; ++i) {
+          const uint32_t w[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const float2 x = unpack2<T>(w[j]);
+            amax = fmaxf(amax, fmaxf(fabsf(x.x), fabsf(x.y)));
+          }
+        }
+        const int exponent = min(max((int)(__float_as_uint(amax) >> 23), 27), 227);  // biased
+        down = __uint_as_float((uint32_t)(254 - exponent) << 23);
+        factor *= __uint_as_float((uint32_t)exponent << 23);
+      }
+      if (a.scale < 0.0f) down = -down;
+      const uint32_t to = base + L::kQ + tile * L::kTileBytes;
+#pragma unroll
+      for (int i = 0; i < D / 8; ++i) {
+        const uint32_t w[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+        uint32_t y[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float2 x = unpack2<T>(w[j]);
+          y[j] = pack2<__half>(x.x * down, x.y * down);
+        }
+        st_shared_v4(to + (i >> 3) * kPanel + swz(r, i & 7), y[0], y[1], y[2], y[3]);
+      }
+      fence_async_smem();
+      mbar_arrive(bar(kQ0 + tile));
+      const int place = len - count + token;
+      const int high = !real ? 0 : a.causal ? place + 1 : len, low = a.window > 0 ? place - a.window + 1 : 0;
+      for (int i = 0; i < steps; ++i) {
+        ok = wait(kS0 + tile, i);
+        if (!ok) break;
+        tc_fence_after();
+        float v[4][32];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) tmem_ld32_nowait(t_s + 32 * q, v[q]);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) tmem_wait_ld(v[q]);
+        const Blocks& b = blocks[i & (kRing - 1)];
+        const int t0 = lo + i * kKeys;
+        auto f = [&](int j) { return a.softcap > 0.0f ? 1.0f : factor * b.k_scale[j]; };  // (scores in units of log2 e) = f * S
+        if (a.softcap > 0.0f) {
+#pragma unroll
+          for (int q = 0; q < 4; ++q)
+#pragma unroll
+            for (int j = 0; j < 32; ++j)
+              v[q][j] = a.softcap * kLog2e * (1.0f - __fdividef(2.0f, ex2(v[q][j] * factor * b.k_scale[2 * q + j / 16] * (2.0f / a.softcap)) + 1.0f));
+        }
+        if (t0 < low || t0 + kKeys > high) {
+#pragma unroll
+          for (int q = 0; q < 4; ++q)
+#pragma unroll
+            for (int j = 0; j < 32; ++j)
+              if (t0 + 32 * q + j < low || t0 + 32 * q + j >= high) v[q][j] = -CUDART_INF_F;
+        }
+        float most = -CUDART_INF_F;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const float* x = &v[j / 2][(j & 1) * 16];
+          float m0 = max3(x[0], x[1], x[2]), m1 = max3(x[3], x[4], x[5]);
+          m0 = max3(m0, x[6], x[7]);
+          m1 = max3(m1, x[8], x[9]);
+          m0 = max3(m0, x[10], x[11]);
+          m1 = max3(m1, x[12], x[13]);
+          m0 = max3(m0, x[14], x[15]);
+          most = fmaxf(most, fmaxf(m0, m1) * f(j) + b.v_log[j]);
+        }
+        if (__any_sync(0xffffffffu, most > top + kSlack)) {
+          const float before = top;
+          top = fmaxf(top, most);
+          const float shrink = ex2(before - (top == -CUDART_INF_F ? 0.0f : top));
+          sum *= shrink;
+          if (i > 0) {  // (the scores of this step are there, so the products of the one before are done)
+#pragma unroll 1
+            for (int q = 0; q < D / 16; ++q) {  // (few at a time: the scores are in registers)
+              float o[16];
+              uint32_t y[16];
+              tmem_ld16_nowait(t_o + 16 * q, o);
+              tmem_wait_ld16(o);
+#pragma unroll
+              for (int j = 0; j < 16; ++j) y[j] = __float_as_uint(o[j] * shrink);
+              tmem_st16(t_o + 16 * q, y);
+            }
+          }
+        }
+        const float ref = top == -CUDART_INF_F ? 0.0f : top;
+        const float2 minus = make_float2(-ref, -ref);
+        float2 part[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          uint32_t y[16];
+#pragma unroll
+          for (int j = 0; j < 32; j += 2) {
+            const float fj = f(2 * q + j / 16), vj = b.v_scale[2 * q + j / 16];
+            float2 p = fma2(make_float2(v[q][j], v[q][j + 1]), make_float2(fj, fj), minus);
+            p = make_float2(ex2(p.x), ex2(p.y));
+            part[(j >> 1) & 1] = add2(part[(j >> 1) & 1], p);
+            p = mul2(p, make_float2(vj, vj));
+            y[j / 2] = pack2<__half>(p.x, p.y);
+          }
+          tmem_st16(t_s + 16 * q, y);
+        }
+        sum += (part[0].x + part[0].y) + (part[1].x + part[1].y);
+        tmem_wait_st();
+        tc_fence_before();
+        mbar_arrive(bar(kP0 + tile));
+      }
+      if (ok) {
+        ok = wait(kO, 0);
+        tc_fence_after();
+      }
+    }
+    // --- result: rows without a key, and of padding, are zero
+    if (ok) {
+      const float inverse = real && sum > 0.0f ? 1.0f / sum : 0.0f;
+      const size_t slot = ((size_t)unit * args.pieces + piece) * kRows + tile * kTileRows + r;
+      T* const dst = reinterpret_cast<T*>(const_cast<void*>(a.out.ptr)) + e * a.out.se + h * a.out.sh + token * a.out.sn;
+#pragma unroll
+      for (int q = 0; q < D / 32; ++q) {
+        float o[32];
+        if (works) {
+          tmem_ld32(t_o + 32 * q, o);
+        } else {
+#pragma unroll
+          for (int j = 0; j < 32; ++j) o[j] = 0.0f;
+        }
+        if (!exists) continue;
+        if (args.pieces == 1) {
+#pragma unroll
+          for (int j = 0; j < 32; j += 8)
+            *reinterpret_cast<uint4*>(dst + 32 * q + j) =
+                make_uint4(pack2<T>(o[j] * inverse, o[j + 1] * inverse), pack2<T>(o[j + 2] * inverse, o[j + 3] * inverse),
+                           pack2<T>(o[j + 4] * inverse, o[j + 5] * inverse), pack2<T>(o[j + 6] * inverse, o[j + 7] * inverse));
+        } else {
+#pragma unroll
+          for (int j = 0; j < 32; j += 4) *reinterpret_cast<float4*>(a.part_o + slot * D + 32 * q + j) = make_float4(o[j], o[j + 1], o[j + 2], o[j + 3]);
+        }
+      }
+      if (args.pieces > 1 && exists) *reinterpret_cast<float2*>(a.part_ml + 2 * slot) = make_float2(top, sum);
+    }
+    if (args.pieces > 1 && tid == 0 && piece == 0)
+      a.split[unit] = make_int4((e * c.heads + head) * a.row_blocks + block, unit * args.pieces, (unit + 1) * args.pieces - 1, 0);
+  } else {
+    regs_dec<kHelperRegs>();
+  }
+  if (warp >= 8 && warp < 15) {
+    // =========================== keys and values =====================================================================
+    const int t = tid - 256, page_mask = (1 << c.page_shift) - 1;
+    // Threads 0-7 look after a block each: its page two steps ahead of its scales, those a step ahead of the bytes.
+    auto page_at = [&](int i) {
+      const int at = lo + i * kKeys + t * kScaleBlock;
+      if (i >= steps || at >= len) return -1;
+      const int page = page_of(c, e, at);
+      if (page < 0) report(c.status, kBadPage);
+      return page;
+    };
+    auto scale_at = [&](const float* scales, long long sp, long long sh, int i, int page) {
+      return page < 0 ? 1.0f : scales[page * sp + head * sh + ((lo + i * kKeys + t * kScaleBlock) & page_mask) / kScaleBlock];
+    };
+    auto put_blocks = [&](int i, int page, float ks, float vs) {
+      Blocks& b = blocks[i & (kRing - 1)];
+      b.page[t] = page;
+      b.k_scale[t] = ks;
+      b.v_scale[t] = vs;
+      b.v_log[t] = __log2f(vs);
+    };
+    auto meet = [&]() { asm volatile("bar.sync 1, %0;" ::"n"(kBringers) : "memory"); };
+    int page_next = -1;
+    if (t < 8) {
+      for (int i = 0; i < 2; ++i) {
+        const int page = page_at(i);
+        put_blocks(i, page, scale_at(c.k_scale, c.ks_sp, c.ks_sh, i, page), scale_at(c.v_scale, c.vs_sp, c.vs_sh, i, page));
+      }
+      page_next = page_at(2);
+    }
+    meet();
+    uint4 raw[2][kPer];  // keys and values on their way
+    auto load = [&](int which, int i) {
+      const uint8_t* const all = which ? c.v : c.k;
+      const uint32_t sp = which ? a.v16[0] : a.k16[0], sh = which ? a.v16[1] : a.k16[1], st = which ? a.v16[2] : a.k16[2];
+      const Blocks& b = blocks[i & (kRing - 1)];
+#pragma unroll
+      for (int j = 0; j < kPer; ++j) {
+        const int at = t + j * kBringers, row = at / kPiecesPerRow, token = lo + i * kKeys + row;
+        raw[which][j] = make_uint4(0, 0, 0, 0);
+        if (at >= kPieces || token >= len) continue;
+        const int page = b.page[row / kScaleBlock];
+        if (page >= 0)
+          raw[which][j] = *reinterpret_cast<const uint4*>(
+              all + 16 * ((uint32_t)page * (uint64_t)sp + (uint32_t)head * (uint64_t)sh + (uint32_t)(token & page_mask) * (uint64_t)st + at % kPiecesPerRow));
+      }
+    };
+    auto put = [&](int which, uint32_t to) {
+#pragma unroll
+      for (int j = 0; j < kPer; ++j) {
+        const int at = t + j * kBringers, row = at / kPiecesPerRow, p = at % kPiecesPerRow;
+        if (at < kPieces) put_codes(to + (p >> 2) * kPanel, row, 2 * (p & 3), p >> 2 & 1, raw[which][j]);
+      }
+      fence_async_smem();
+    };
+    if (steps > 0) {
+      load(0, 0);
+      load(1, 0);
+    }
+    bool ok = true;  // (whatever happens, all meet at each step)
+    for (int i = 0; i < steps; ++i) {
+      float ks = 1.0f, vs = 1.0f;
+      int page_after = -1;
+      if (t < 8) {
+        ks = scale_at(c.k_scale, c.ks_sp, c.ks_sh, i + 2, page_next);
+        vs = scale_at(c.v_scale, c.vs_sp, c.vs_sh, i + 2, page_next);
+        page_after = page_at(i + 3);
+      }
+      const int stage = i & 1;
+      ok = ok && (i < 2 || wait(kKEmpty + stage, (i >> 1) - 1));
+      if (ok) {
+        put(0, base + L::kK + stage * L::kTileBytes);
+        mbar_arrive(bar(kKFull + stage));
+      }
+      if (i + 1 < steps) load(0, i + 1);
+      ok = ok && (i < 2 || wait(kVEmpty + stage, (i >> 1) - 1));
+      if (ok) {
+        put(1, base + L::kV + stage * L::kTileBytes);
+        mbar_arrive(bar(kVFull + stage));
+      }
+      if (i + 1 < steps) load(1, i + 1);
+      if (t < 8) {
+        put_blocks(i + 2, page_next, ks, vs);
+        page_next = page_after;
+      }
+      meet();
+    }
+  } else if (warp == 15) {
+    // =========================== products ============================================================================
+    constexpr uint32_t kScores = instr_desc(0, 0, 0, kKeys, kTileRows), kSums = instr_desc(0, 0, 1, D, kTileRows);
+    const uint32_t q0 = smem_desc_lo(base + L::kQ, 16), k0 = smem_desc_lo(base + L::kK, 16), v0 = smem_desc_lo(base + L::kV, kPanel);
+    constexpr uint32_t kTileUnits = L::kTileBytes >> 4;
+    auto scores = [&](int tile, int i) {
+      const uint32_t da = q0 + tile * kTileUnits, db = k0 + (i & 1) * kTileUnits;
+#pragma unroll
+      for (int kk = 0; kk < D / 16; ++kk)
+        mma_f16_lo(tmem + kTmemS + tile * 128, da + (kk >> 2) * (kPanel >> 4) + (kk & 3) * 2, db + (kk >> 2) * (kPanel >> 4) + (kk & 3) * 2, kScores, kk > 0);
+      mma_commit(bar(kS0 + tile));
+    };
+    auto sums = [&](int tile, int i) {
+      const uint32_t db = v0 + (i & 1) * kTileUnits;
+#pragma unroll
+      for (int kk = 0; kk < kKeys / 16; ++kk)
+        mma_f16_ts(tmem + kTmemO + tile * 128, tmem + kTmemS + tile * 128 + kk * 8, db + kk * 128, kSums, i > 0 || kk > 0);
+    };
+    const int tiles = two ? 2 : 1;
+    bool ok = steps > 0;
+    for (int tile = 0; tile < tiles && ok; ++tile) ok = wait(kQ0 + tile, 0);
+    ok = ok && wait(kKFull, 0);
+    if (ok) {
+      tc_fence_after();
+      if (elect_one()) {
+        for (int tile = 0; tile < tiles; ++tile) scores(tile, 0);
+        mma_commit(bar(kKEmpty));
+      }
+      __syncwarp();
+    }
+    for (int i = 0; i < steps && ok; ++i) {
+      ok = wait(kVFull + (i & 1), i >> 1);
+      if (i + 1 < steps) ok = ok && wait(kKFull + (i + 1 & 1), (i + 1) >> 1);
+      for (int tile = 0; tile < tiles && ok; ++tile) {
+        ok = wait(kP0 + tile, i);
+        if (!ok) break;
+        tc_fence_after();
+        if (elect_one()) {
+          sums(tile, i);
+          if (tile == tiles - 1) mma_commit(bar(kVEmpty + (i & 1)));
+          if (i + 1 < steps) {
+            scores(tile, i + 1);
+            if (tile == tiles - 1) mma_commit(bar(kKEmpty + (i + 1 & 1)));
+          } else if (tile == tiles - 1) {
+            mma_commit(bar(kO));
+          }
+        }
+        __syncwarp();
+      }
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (tid == 0 && *abort_flag != 0 && args.wait_status != nullptr) *reinterpret_cast<volatile int*>(args.wait_status) = 800;
+  if (warp == 15) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+}
+
+}  // namespace
+
+// Pieces that the keys of 256 rows are cut into: with fewer blocks of rows than SMs, what brings them to all SMs, as long as a piece has
+// four steps at least.
+int prompt_pieces(int E, int N, int H, int kv_heads, long long longest) {
+  const long long units = (long long)E * kv_heads * (((long long)H / kv_heads * N + kRows - 1) / kRows);
+  const long long fill = sm_count() / units, most = longest / (4 * kKeys);
+  return (int)(fill < 2 || most < 2 ? 1 : fill < most ? fill : most);
+}
+
+size_t prompt_workspace(int E, int N, int H, int kv_heads, int width, long long longest) {
+  const long long pieces = prompt_pieces(E, N, H, kv_heads, longest);
+  if (pieces == 1) return 256;
+  const size_t units = (size_t)E * kv_heads * (((size_t)H / kv_heads * N + kRows - 1) / kRows);
+  return (units * sizeof(int4) + 255) / 256 * 256 + units * pieces * kRows * (width + 2) * sizeof(float);
+}
+
+cudaError_t launch_prompt(AttendArgs a, int dtype, int width, void* workspace, long long longest, int* wait_status, cudaStream_t stream) {
+  a.row_blocks = (a.group * a.N + kRows - 1) / kRows;
+  const long long units = (long long)a.E * a.cache.heads * a.row_blocks;
+  PromptArgs args{a, prompt_pieces(a.E, a.N, a.H, a.cache.heads, longest), wait_status};
+  if (a.scale == 0.0f) args.a.scale = 1e-30f;  // (a mask is minus infinity times the factor)
+  char* at = reinterpret_cast<char*>(workspace);
+  args.a.split = reinterpret_cast<int4*>(at);
+  args.a.part_o = reinterpret_cast<float*>(at + ((size_t)units * sizeof(int4) + 255) / 256 * 256);
+  args.a.part_ml = args.a.part_o + (size_t)units * args.pieces * kRows * width;
+  const bool bf = dtype == MA_B200_BF16;
+  const void* fn = width == 128 ? (bf ? (const void*)prompt_kernel<__nv_bfloat16, 128> : (const void*)prompt_kernel<__half, 128>)
+                                : (bf ? (const void*)prompt_kernel<__nv_bfloat16, 64> : (const void*)prompt_kernel<__half, 64>);
+  const size_t smem = width == 128 ? Layout<128>::kSmem : Layout<64>::kSmem;
+  // a build whose launch does not cover the roles' registers must not start: setmaxnreg would wait for them without end
+  static std::atomic<unsigned long long> checked[4];
+  int dev = 0;
+  cudaError_t err = cudaGetDevice(&dev);
+  if (err != cudaSuccess) return err;
+  std::atomic<unsigned long long>& done = checked[(width == 128) * 2 + bf];
+  if (dev >= 64 || !(done.load(std::memory_order_relaxed) >> dev & 1)) {
+    cudaFuncAttributes fa;
+    err = cudaFuncGetAttributes(&fa, fn);
+    if (err != cudaSuccess) return err;
+    if (fa.numRegs * kThreads < 256 * (kRowRegs + kHelperRegs) || fa.numRegs > kRowRegs || fa.numRegs < kHelperRegs) return cudaErrorLaunchOutOfResources;
+    if (dev < 64) done.fetch_or(1ull << dev, std::memory_order_relaxed);
+  }
+  err = allow_dynamic_smem(fn, smem);
+  if (err != cudaSuccess) return err;
+  void* params[] = {(void*)&args};
+  err = launch_kernel(fn, dim3((unsigned)(units * args.pieces)), dim3(kThreads), params, smem, stream);
+  if (err != cudaSuccess || args.pieces == 1) return err;
+  return launch_join(args.a, dtype, width, kRows, (int)units, 1, stream);
+}
+
+}  // namespace ma
