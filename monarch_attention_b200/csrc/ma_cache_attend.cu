@@ -402,7 +402,9 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<D, NT>::kCtas) attend_kerne
           }
         }
       const float4 scales = *reinterpret_cast<const float4*>(keys + 2 * kSlice * D);
-      const float ks[2] = {scales.x, scales.y}, vs[2] = {scales.z, scales.w}, vl[2] = {__log2f(scales.z), __log2f(scales.w)};
+      const float ks[2] = {scales.x, scales.y}, vs[2] = {scales.z, scales.w};
+      // (a scale of zero is as good as 2^-100: its keys have weights, which the reference has to stand for)
+      const float vl[2] = {fmaxf(__log2f(scales.z), -100.0f), fmaxf(__log2f(scales.w), -100.0f)};
       uint32_t weights[2][NT][2];
       const bool whole = t0 >= full_low && t0 + kSlice <= full_high;
 #pragma unroll

@@ -3,14 +3,14 @@
 // Bound by the tensor cores and by the exponentials (as many cycles at 128 features: 2 x 256 x 128 x 128 x 2 operations of a step are 2048 cycles,
 // its 256 x 128 exponentials 2048 of the special function units).  A CTA takes 256 rows (tokens times heads of a group) of a key head and
 // walks over its keys, 128 at a step:
-//  * Seven warps bring keys and values: bytes from global memory into registers, half a step ahead, and from there, widened to f16 (exact),
+//  * Eight warps bring keys and values: bytes from global memory into registers, half a step ahead, and from there, widened to f16 (exact),
 //    into swizzled tiles in shared memory.  Two tiles of rows share them, so that the conversion and the shared memory's traffic, which a
 //    single tile would be bound by, count half.
-//  * One warp issues the products: scores S = Q K^T into tensor memory, and O += P V with the weights P read from tensor memory, where they
-//    take the place of their scores.  While the rows of one tile are exponentiated, the products of the other run.
-//  * Two warpgroups have a row a thread: the row's 128 scores go to registers in one go, and the maximum, the weights and their sum need no
-//    other thread.  Scales of blocks are applied as in the kernel for few rows (ma_cache_attend.cu): the keys' to the scores, the
-//    values' to the weights, with a reference that is raised (and O multiplied) only when a weight would pass 2^8.
+//  * Two warpgroups have a row a thread: the row's 128 scores go from tensor memory to registers in one go, and the maximum, the weights and
+//    their sum need no other thread.  Scales of blocks are applied as in the kernel for few rows (ma_cache_attend.cu): the keys' to the
+//    scores, the values' to the weights, with a reference that is raised (and O multiplied) only when a weight would pass 2^8.
+//  * One warp issues the products: O += P V, the weights P read from tensor memory, where they have taken the place of their scores, and
+//    the next step's scores S = Q K^T.  While one tile's rows are exponentiated the other's products run.
 // Every wait is bounded; one that gives up ends the CTA's others, and the next call on the device reports it.
 #include <math_constants.h>
 
@@ -25,9 +25,9 @@ namespace {
 using namespace sm100;
 
 constexpr int kKeys = 128, kTileRows = 128, kRows = 2 * kTileRows;
-constexpr int kThreads = 512, kBringers = 224;  // warps 0-3, 4-7: rows; 8-14: keys and values; 15: products
-constexpr int kRowRegs = 176, kHelperRegs = 80;
-static_assert(256 * (kRowRegs + kHelperRegs) <= kThreads * 128, "setmaxnreg draws on the launch's registers");
+constexpr int kThreads = 640, kBringers = 256;  // warps 0-3, 4-7: rows; 8-15: keys and values; 16: products (17-19 make it a warpgroup)
+constexpr int kLaunchRegs = 96, kRowRegs = 160, kBringerRegs = 56, kIssuerRegs = 40;
+static_assert(256 * (kRowRegs + kBringerRegs) + 128 * kIssuerRegs <= kThreads * kLaunchRegs, "setmaxnreg draws on the launch's registers");
 constexpr int kRing = 8;  // steps whose pages and scales are kept
 constexpr float kSlack = 8.0f;
 
@@ -35,8 +35,8 @@ enum Bar { kQ0, kQ1, kKFull, kKEmpty = kKFull + 2, kVFull = kKEmpty + 2, kVEmpty
 
 // What the rows need of a step's 8 blocks.
 struct alignas(16) Blocks {
-  float k_scale[8], v_scale[8], v_log[8];
-  int page[8];
+  float k_scale[8], v_inverse[8], v_log[8];  // the values' scales as their inverse and logarithm
+  int page[2][8];  // of keys and of values; -1: zeros
 };
 
 template <int D>
@@ -58,25 +58,41 @@ __device__ __forceinline__ void regs_inc() { asm volatile("setmaxnreg.inc.sync.a
 template <int N>
 __device__ __forceinline__ void regs_dec() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
 
-__device__ __forceinline__ uint32_t widen2(uint32_t codes, bool upper) {
+__device__ __forceinline__ uint32_t widen2(uint32_t codes) {
   uint32_t r;
-  asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, lo;\n\t}" : "=r"(r) : "r"(upper ? codes >> 16 : codes));
+  asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, lo;\n\t}" : "=r"(r) : "r"(codes));
   return r;
 }
-// 16 codes as two 16-byte chunks of a row: `chunk` and the one after it, in either order (lanes on different panels start with different ones,
-// so that they do not meet in a bank).
-__device__ __forceinline__ void put_codes(uint32_t panel, uint32_t row, uint32_t chunk, bool second_first, const uint4& c) {
-  uint32_t w[8] = {widen2(c.x, false), widen2(c.x, true), widen2(c.y, false), widen2(c.y, true),
-                   widen2(c.z, false), widen2(c.z, true), widen2(c.w, false), widen2(c.w, true)};
-  const uint32_t a = panel + swz(row, chunk), b = panel + swz(row, chunk + 1);
-  st_shared_v4(second_first ? b : a, second_first ? w[4] : w[0], second_first ? w[5] : w[1], second_first ? w[6] : w[2], second_first ? w[7] : w[3]);
-  st_shared_v4(second_first ? a : b, second_first ? w[0] : w[4], second_first ? w[1] : w[5], second_first ? w[2] : w[6], second_first ? w[3] : w[7]);
+__device__ __forceinline__ uint32_t widen2_upper(uint32_t codes) {
+  uint32_t r;
+  asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, hi;\n\t}" : "=r"(r) : "r"(codes));
+  return r;
+}
+// 2^x on the multipliers, for x up to 2^7: the special function units are what the weights wait for.  x = n + f with f in [-1/2, 1/2], 2^f by a
+// polynomial of degree 5 (minimax in the relative error, 2^-23.6; found by exchange), n added to the exponent.
+constexpr int kByProducts = 1;  // of 4 pairs of weights, these
+__device__ __forceinline__ float2 exp2_by_products(float2 x) {
+  x = make_float2(fmaxf(x.x, -126.0f), fmaxf(x.y, -126.0f));
+  const float2 round = make_float2(12582912.0f, 12582912.0f);  // 1.5 * 2^23: its last bits are n
+  const float2 t = add2(x, round), f = sub2(x, sub2(t, round));
+  auto both = [](float c) { return make_float2(c, c); };
+  float2 p = fma2(f, both(1.3277939e-3f), both(9.6757580e-3f));
+  p = fma2(p, f, both(5.5507097e-2f));
+  p = fma2(p, f, both(2.4022114e-1f));
+  p = fma2(p, f, both(6.9314694e-1f));
+  p = fma2(p, f, both(1.0000001f));
+  return make_float2(__int_as_float(__float_as_int(p.x) + (__float_as_int(t.x) << 23)), __int_as_float(__float_as_int(p.y) + (__float_as_int(t.y) << 23)));
+}
+// 16 codes as two 16-byte chunks of a row.
+__device__ __forceinline__ void put_codes(uint32_t panel, uint32_t row, uint32_t chunk, const uint4& c) {
+  st_shared_v4(panel + swz(row, chunk), widen2(c.x), widen2_upper(c.x), widen2(c.y), widen2_upper(c.y));
+  st_shared_v4(panel + swz(row, chunk + 1), widen2(c.z), widen2_upper(c.z), widen2(c.w), widen2_upper(c.w));
 }
 
 template <typename T, int D>
 __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_constant__ PromptArgs args) {
   using L = Layout<D>;
-  constexpr int kPanel = 128 * 128, kPieces = kKeys * D / 16, kPer = (kPieces + kBringers - 1) / kBringers, kPiecesPerRow = D / 16;
+  constexpr int kPanel = 128 * 128;  // bytes of 128 rows of 64 features
   constexpr uint32_t kTmemS = 0, kTmemO = 256;  // columns: S (and P) of both tiles, then O of both
   extern __shared__ uint8_t smem_raw[];
   const AttendArgs& a = args.a;
@@ -127,7 +143,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  if (warp == 15) {
+  if (warp == 16) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(base + L::kFlags + 4), "r"(512) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
@@ -186,80 +202,83 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
       mbar_arrive(bar(kQ0 + tile));
       const int place = len - count + token;
       const int high = !real ? 0 : a.causal ? place + 1 : len, low = a.window > 0 ? place - a.window + 1 : 0;
-      for (int i = 0; i < steps; ++i) {
+      for (int i = 0; i < steps && ok; ++i) {
         ok = wait(kS0 + tile, i);
         if (!ok) break;
         tc_fence_after();
-        float v[4][32];
-#pragma unroll
-        for (int q = 0; q < 4; ++q) tmem_ld32_nowait(t_s + 32 * q, v[q]);
-#pragma unroll
-        for (int q = 0; q < 4; ++q) tmem_wait_ld(v[q]);
         const Blocks& b = blocks[i & (kRing - 1)];
         const int t0 = lo + i * kKeys;
-        auto f = [&](int j) { return a.softcap > 0.0f ? 1.0f : factor * b.k_scale[j]; };  // (scores in units of log2 e) = f * S
-        if (a.softcap > 0.0f) {
+        uint32_t y[4][16];
+        float more;
+        // The weights are found with the reference as it is, next to the maximum that says whether it would do; where not, once more.
+#pragma unroll 1
+        for (;;) {
+          float v[4][32];
 #pragma unroll
-          for (int q = 0; q < 4; ++q)
+          for (int q = 0; q < 4; ++q) tmem_ld32_nowait(t_s + 32 * q, v[q]);
 #pragma unroll
-            for (int j = 0; j < 32; ++j)
-              v[q][j] = a.softcap * kLog2e * (1.0f - __fdividef(2.0f, ex2(v[q][j] * factor * b.k_scale[2 * q + j / 16] * (2.0f / a.softcap)) + 1.0f));
-        }
-        if (t0 < low || t0 + kKeys > high) {
+          for (int q = 0; q < 4; ++q) tmem_wait_ld(v[q]);
+          auto f = [&](int j) { return a.softcap > 0.0f ? 1.0f : factor * b.k_scale[j]; };  // (scores in units of log2 e) = f * S
+          if (a.softcap > 0.0f) {
 #pragma unroll
-          for (int q = 0; q < 4; ++q)
+            for (int q = 0; q < 4; ++q)
 #pragma unroll
-            for (int j = 0; j < 32; ++j)
-              if (t0 + 32 * q + j < low || t0 + 32 * q + j >= high) v[q][j] = -CUDART_INF_F;
-        }
-        float most = -CUDART_INF_F;
+              for (int j = 0; j < 32; ++j)
+                v[q][j] = a.softcap * kLog2e * (1.0f - __fdividef(2.0f, ex2(v[q][j] * factor * b.k_scale[2 * q + j / 16] * (2.0f / a.softcap)) + 1.0f));
+          }
+          if (t0 < low || t0 + kKeys > high) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const float* x = &v[j / 2][(j & 1) * 16];
-          float m0 = max3(x[0], x[1], x[2]), m1 = max3(x[3], x[4], x[5]);
-          m0 = max3(m0, x[6], x[7]);
-          m1 = max3(m1, x[8], x[9]);
-          m0 = max3(m0, x[10], x[11]);
-          m1 = max3(m1, x[12], x[13]);
-          m0 = max3(m0, x[14], x[15]);
-          most = fmaxf(most, fmaxf(m0, m1) * f(j) + b.v_log[j]);
-        }
-        if (__any_sync(0xffffffffu, most > top + kSlack)) {
+            for (int q = 0; q < 4; ++q)
+#pragma unroll
+              for (int j = 0; j < 32; ++j)
+                if (t0 + 32 * q + j < low || t0 + 32 * q + j >= high) v[q][j] = -CUDART_INF_F;
+          }
+          const float ref = top == -CUDART_INF_F ? 0.0f : top;
+          float most = -CUDART_INF_F;
+          more = 0.0f;
+          // weights times the values' scale; the sum of the weights takes it out again, block by block
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            float* x = &v[j / 2][(j & 1) * 16];
+            float m0 = max3(x[0], x[1], x[2]), m1 = max3(x[3], x[4], x[5]);
+            m0 = max3(m0, x[6], x[7]);
+            m1 = max3(m1, x[8], x[9]);
+            m0 = max3(m0, x[10], x[11]);
+            m1 = max3(m1, x[12], x[13]);
+            m0 = max3(m0, x[14], x[15]);
+            const float fj = f(j), log = b.v_log[j], shift = log - ref;
+            most = fmaxf(most, fmaf(fmaxf(m0, m1), fj, log));
+            float2 part = make_float2(0.0f, 0.0f);
+#pragma unroll
+            for (int k = 0; k < 16; k += 2) {
+              float2 p = fma2(make_float2(x[k], x[k + 1]), make_float2(fj, fj), make_float2(shift, shift));
+              p = k % 8 < 8 - 2 * kByProducts ? make_float2(ex2(p.x), ex2(p.y)) : exp2_by_products(p);
+              part = k == 0 ? p : add2(part, p);
+              y[j / 2][(j & 1) * 8 + k / 2] = pack2<__half>(p.x, p.y);
+            }
+            more = fmaf(part.x + part.y, b.v_inverse[j], more);
+          }
+          if (!__any_sync(0xffffffffu, most > top + kSlack)) break;
           const float before = top;
           top = fmaxf(top, most);
           const float shrink = ex2(before - (top == -CUDART_INF_F ? 0.0f : top));
           sum *= shrink;
           if (i > 0) {  // (the scores of this step are there, so the products of the one before are done)
 #pragma unroll 1
-            for (int q = 0; q < D / 16; ++q) {  // (few at a time: the scores are in registers)
+            for (int q = 0; q < D / 16; ++q) {
               float o[16];
-              uint32_t y[16];
+              uint32_t z[16];
               tmem_ld16_nowait(t_o + 16 * q, o);
               tmem_wait_ld16(o);
 #pragma unroll
-              for (int j = 0; j < 16; ++j) y[j] = __float_as_uint(o[j] * shrink);
-              tmem_st16(t_o + 16 * q, y);
+              for (int j = 0; j < 16; ++j) z[j] = __float_as_uint(o[j] * shrink);
+              tmem_st16(t_o + 16 * q, z);
             }
           }
         }
-        const float ref = top == -CUDART_INF_F ? 0.0f : top;
-        const float2 minus = make_float2(-ref, -ref);
-        float2 part[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
+        sum += more;
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          uint32_t y[16];
-#pragma unroll
-          for (int j = 0; j < 32; j += 2) {
-            const float fj = f(2 * q + j / 16), vj = b.v_scale[2 * q + j / 16];
-            float2 p = fma2(make_float2(v[q][j], v[q][j + 1]), make_float2(fj, fj), minus);
-            p = make_float2(ex2(p.x), ex2(p.y));
-            part[(j >> 1) & 1] = add2(part[(j >> 1) & 1], p);
-            p = mul2(p, make_float2(vj, vj));
-            y[j / 2] = pack2<__half>(p.x, p.y);
-          }
-          tmem_st16(t_s + 16 * q, y);
-        }
-        sum += (part[0].x + part[0].y) + (part[1].x + part[1].y);
+        for (int q = 0; q < 4; ++q) tmem_st16(t_s + 16 * q, y[q]);
         tmem_wait_st();
         tc_fence_before();
         mbar_arrive(bar(kP0 + tile));
@@ -271,7 +290,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
     }
     // --- result: rows without a key, and of padding, are zero
     if (ok) {
-      const float inverse = real && sum > 0.0f ? 1.0f / sum : 0.0f;
+      const float inverse = real && top > -CUDART_INF_F ? 1.0f / sum : 0.0f;  // (no key, no reference)
       const size_t slot = ((size_t)unit * args.pieces + piece) * kRows + tile * kTileRows + r;
       T* const dst = reinterpret_cast<T*>(const_cast<void*>(a.out.ptr)) + e * a.out.se + h * a.out.sh + token * a.out.sn;
 #pragma unroll
@@ -299,11 +318,9 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
     }
     if (args.pieces > 1 && tid == 0 && piece == 0)
       a.split[unit] = make_int4((e * c.heads + head) * a.row_blocks + block, unit * args.pieces, (unit + 1) * args.pieces - 1, 0);
-  } else {
-    regs_dec<kHelperRegs>();
-  }
-  if (warp >= 8 && warp < 15) {
+  } else if (warp < 16) {
     // =========================== keys and values =====================================================================
+    regs_dec<kBringerRegs>();
     const int t = tid - 256, page_mask = (1 << c.page_shift) - 1;
     // Threads 0-7 look after a block each: its page two steps ahead of its scales, those a step ahead of the bytes.
     auto page_at = [&](int i) {
@@ -318,10 +335,12 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
     };
     auto put_blocks = [&](int i, int page, float ks, float vs) {
       Blocks& b = blocks[i & (kRing - 1)];
-      b.page[t] = page;
-      b.k_scale[t] = ks;
-      b.v_scale[t] = vs;
-      b.v_log[t] = __log2f(vs);
+      // (a scale of zero is one of one before zeros: a mask is minus infinity times the keys' scale, a weight is divided by the values')
+      b.page[0][t] = ks == 0.0f ? -1 : page;
+      b.page[1][t] = vs == 0.0f ? -1 : page;
+      b.k_scale[t] = ks == 0.0f ? 1.0f : ks;
+      b.v_inverse[t] = vs == 0.0f ? 1.0f : 1.0f / vs;
+      b.v_log[t] = vs == 0.0f ? 0.0f : __log2f(vs);
     };
     auto meet = [&]() { asm volatile("bar.sync 1, %0;" ::"n"(kBringers) : "memory"); };
     int page_next = -1;
@@ -333,28 +352,28 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
       page_next = page_at(2);
     }
     meet();
-    uint4 raw[2][kPer];  // keys and values on their way
+    // A thread has a 16-byte piece of 4 in each panel of rows t / 4 and t / 4 + 64: eight threads write 4 pieces of two rows, an even and an
+    // odd one, whose chunks the swizzle puts on different banks.
+    constexpr int kPanels = D / 64;
+    uint4 raw[2][2][kPanels];  // keys and values on their way
     auto load = [&](int which, int i) {
       const uint8_t* const all = which ? c.v : c.k;
       const uint32_t sp = which ? a.v16[0] : a.k16[0], sh = which ? a.v16[1] : a.k16[1], st = which ? a.v16[2] : a.k16[2];
       const Blocks& b = blocks[i & (kRing - 1)];
 #pragma unroll
-      for (int j = 0; j < kPer; ++j) {
-        const int at = t + j * kBringers, row = at / kPiecesPerRow, token = lo + i * kKeys + row;
-        raw[which][j] = make_uint4(0, 0, 0, 0);
-        if (at >= kPieces || token >= len) continue;
-        const int page = b.page[row / kScaleBlock];
-        if (page >= 0)
-          raw[which][j] = *reinterpret_cast<const uint4*>(
-              all + 16 * ((uint32_t)page * (uint64_t)sp + (uint32_t)head * (uint64_t)sh + (uint32_t)(token & page_mask) * (uint64_t)st + at % kPiecesPerRow));
+      for (int j = 0; j < 2; ++j) {
+        const int row = (t >> 2) + 64 * j, token = lo + i * kKeys + row, page = b.page[which][row / kScaleBlock];
+        const uint8_t* const src = all + 16 * ((uint32_t)page * (uint64_t)sp + (uint32_t)head * (uint64_t)sh + (uint32_t)(token & page_mask) * (uint64_t)st + (t & 3));
+#pragma unroll
+        for (int x = 0; x < kPanels; ++x)
+          raw[which][j][x] = token < len && page >= 0 ? *reinterpret_cast<const uint4*>(src + 64 * x) : make_uint4(0, 0, 0, 0);
       }
     };
     auto put = [&](int which, uint32_t to) {
 #pragma unroll
-      for (int j = 0; j < kPer; ++j) {
-        const int at = t + j * kBringers, row = at / kPiecesPerRow, p = at % kPiecesPerRow;
-        if (at < kPieces) put_codes(to + (p >> 2) * kPanel, row, 2 * (p & 3), p >> 2 & 1, raw[which][j]);
-      }
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int x = 0; x < kPanels; ++x) put_codes(to + x * kPanel, (t >> 2) + 64 * j, 2 * (t & 3), raw[which][j][x]);
       fence_async_smem();
     };
     if (steps > 0) {
@@ -389,39 +408,40 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
       }
       meet();
     }
-  } else if (warp == 15) {
+  } else {
+    regs_dec<kIssuerRegs>();
+  }
+  if (warp == 16) {
     // =========================== products ============================================================================
     constexpr uint32_t kScores = instr_desc(0, 0, 0, kKeys, kTileRows), kSums = instr_desc(0, 0, 1, D, kTileRows);
-    const uint32_t q0 = smem_desc_lo(base + L::kQ, 16), k0 = smem_desc_lo(base + L::kK, 16), v0 = smem_desc_lo(base + L::kV, kPanel);
-    constexpr uint32_t kTileUnits = L::kTileBytes >> 4;
+    constexpr uint32_t kTileUnits = L::kTileBytes >> 4, kPanelUnits = kPanel >> 4;
     auto scores = [&](int tile, int i) {
-      const uint32_t da = q0 + tile * kTileUnits, db = k0 + (i & 1) * kTileUnits;
+      const uint32_t da = smem_desc_lo(base + L::kQ, 16) + tile * kTileUnits, db = smem_desc_lo(base + L::kK, 16) + (i & 1) * kTileUnits;
 #pragma unroll
       for (int kk = 0; kk < D / 16; ++kk)
-        mma_f16_lo(tmem + kTmemS + tile * 128, da + (kk >> 2) * (kPanel >> 4) + (kk & 3) * 2, db + (kk >> 2) * (kPanel >> 4) + (kk & 3) * 2, kScores, kk > 0);
+        mma_f16_lo(tmem + kTmemS + tile * 128, da + (kk >> 2) * kPanelUnits + (kk & 3) * 2, db + (kk >> 2) * kPanelUnits + (kk & 3) * 2, kScores, kk > 0);
       mma_commit(bar(kS0 + tile));
     };
     auto sums = [&](int tile, int i) {
-      const uint32_t db = v0 + (i & 1) * kTileUnits;
+      const uint32_t db = smem_desc_lo(base + L::kV, kPanel) + (i & 1) * kTileUnits;
 #pragma unroll
       for (int kk = 0; kk < kKeys / 16; ++kk)
         mma_f16_ts(tmem + kTmemO + tile * 128, tmem + kTmemS + tile * 128 + kk * 8, db + kk * 128, kSums, i > 0 || kk > 0);
     };
     const int tiles = two ? 2 : 1;
-    bool ok = steps > 0;
-    for (int tile = 0; tile < tiles && ok; ++tile) ok = wait(kQ0 + tile, 0);
-    ok = ok && wait(kKFull, 0);
-    if (ok) {
+    bool ok = steps > 0 && wait(kKFull, 0);
+    for (int tile = 0; tile < tiles && ok; ++tile) {
+      ok = wait(kQ0 + tile, 0);
+      if (!ok) break;
       tc_fence_after();
       if (elect_one()) {
-        for (int tile = 0; tile < tiles; ++tile) scores(tile, 0);
-        mma_commit(bar(kKEmpty));
+        scores(tile, 0);
+        if (tile == tiles - 1) mma_commit(bar(kKEmpty));
       }
       __syncwarp();
     }
     for (int i = 0; i < steps && ok; ++i) {
-      ok = wait(kVFull + (i & 1), i >> 1);
-      if (i + 1 < steps) ok = ok && wait(kKFull + (i + 1 & 1), (i + 1) >> 1);
+      ok = wait(kVFull + (i & 1), i >> 1) && (i + 1 == steps || wait(kKFull + ((i + 1) & 1), (i + 1) >> 1));
       for (int tile = 0; tile < tiles && ok; ++tile) {
         ok = wait(kP0 + tile, i);
         if (!ok) break;
@@ -431,7 +451,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
           if (tile == tiles - 1) mma_commit(bar(kVEmpty + (i & 1)));
           if (i + 1 < steps) {
             scores(tile, i + 1);
-            if (tile == tiles - 1) mma_commit(bar(kKEmpty + (i + 1 & 1)));
+            if (tile == tiles - 1) mma_commit(bar(kKEmpty + ((i + 1) & 1)));
           } else if (tile == tiles - 1) {
             mma_commit(bar(kO));
           }
@@ -444,7 +464,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
   tc_fence_before();
   __syncthreads();
   if (tid == 0 && *abort_flag != 0 && args.wait_status != nullptr) *reinterpret_cast<volatile int*>(args.wait_status) = 800;
-  if (warp == 15) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+  if (warp == 16) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
 }
 
 }  // namespace
@@ -487,7 +507,7 @@ cudaError_t launch_prompt(AttendArgs a, int dtype, int width, void* workspace, l
     cudaFuncAttributes fa;
     err = cudaFuncGetAttributes(&fa, fn);
     if (err != cudaSuccess) return err;
-    if (fa.numRegs * kThreads < 256 * (kRowRegs + kHelperRegs) || fa.numRegs > kRowRegs || fa.numRegs < kHelperRegs) return cudaErrorLaunchOutOfResources;
+    if (fa.numRegs != kLaunchRegs) return cudaErrorLaunchOutOfResources;
     if (dev < 64) done.fetch_or(1ull << dev, std::memory_order_relaxed);
   }
   err = allow_dynamic_smem(fn, smem);

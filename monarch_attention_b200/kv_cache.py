@@ -30,7 +30,7 @@ _NO_ROTARY = (None, 0, 0, 1.0)
 class PagedKV(NamedTuple):
     """The pool: ``k``, ``v`` (pages, heads, page size, width) float8_e4m3fn and ``k_scale``, ``v_scale`` (pages, heads, page size / 16) float32.
 
-    The 16 tokens of a block of a head stand for ``code * scale``.  The width is 64 or 128, the page size a power of two from 16 on; strides
+    The 16 tokens of a block of a head stand for ``code * scale`` (scales are not negative, and zero or from 2^-40 to 2^60).  The width is 64 or 128, the page size a power of two from 16 on; strides
     are free as long as rows start on 16-byte boundaries (a pool of (pages, page size, heads, width) is passed as a permuted view).
     """
 

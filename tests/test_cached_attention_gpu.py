@@ -91,6 +91,37 @@ def test_windows_caps_and_scales(Hk, D, N, window, softcap, scale, dtype):
     check(out, q, cache, table, lengths, counts, page, True, scale, softcap, window)
 
 
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("E,H,Hk,N,D,page,lengths,counts,causal,window,softcap,scale", [
+    (1, 4, 1, 64, 128, 64, [5000], None, True, 0, 0.0, None), (2, 8, 2, 33, 64, 32, [3000, 40], [33, 5], True, 0, 0.0, None),
+    (1, 2, 2, 130, 128, 128, [4100], None, False, 0, 10.0, None), (2, 6, 1, 90, 64, 16, [2500, 1], [90, 1], True, 700, 0.0, None),
+    (1, 1, 1, 600, 128, 64, [600], None, True, 0, 0.0, None), (3, 5, 1, 257, 64, 64, [257, 2000, 300], [257, 0, 100], True, 0, 0.0, -0.2),
+    (1, 8, 8, 1100, 64, 64, [1100], None, True, 33, 0.0, None), (1, 3, 1, 77, 128, 32, [1023], None, True, 0, 0.0, 0.0)])
+def test_prompts(E, H, Hk, N, D, page, lengths, counts, causal, window, softcap, scale, dtype):
+    """Many rows: one tile or two of them, keys in one piece or several, sequences of one token, without tokens, or shorter than the rest."""
+    import monarch_attention_b200 as ma
+    cache, table = filled(E, max(lengths) // page + 2, Hk, D, page, lengths, "tokens")
+    q = queries(E, H, N, D, dtype, "tokens")
+    dev = [None if x is None else torch.tensor(x, dtype=torch.int32, device="cuda") for x in (lengths, counts)]
+    out = ma.cached_attention_b200(q, cache, table, *dev, causal=causal, window=window, softcap=softcap, scale=scale)
+    check(out, q, cache, table, lengths, counts, page, causal, scale, softcap, window)
+
+
+@pytest.mark.parametrize("N", [1, 20, 80])
+def test_blocks_of_other_quantisers(N):
+    """Scales that are no powers of two, and zero (with codes that are not): what counts is code * scale."""
+    import monarch_attention_b200 as ma
+    cache, table = filled(2, 6, 2, 128, 64, [300, 90 + N])
+    g = torch.Generator(device="cuda").manual_seed(4)
+    for s in (cache.k_scale, cache.v_scale):
+        s.mul_(0.6 + torch.rand(s.shape, generator=g, device="cuda"))
+        s[torch.rand(s.shape, generator=g, device="cuda") < 0.3] = 0.0
+    q = queries(2, 8, N, 128, BF, "heads")
+    lengths = [300, 90 + N]
+    out = ma.cached_attention_b200(q, cache, table, torch.tensor(lengths, dtype=torch.int32, device="cuda"))
+    check(out, q, cache, table, lengths, None, 64)
+
+
 def test_more_queries_than_keys_leaves_the_first_rows_empty():
     """Tokens at positions before the sequence's first see nothing and are zero."""
     import monarch_attention_b200 as ma
