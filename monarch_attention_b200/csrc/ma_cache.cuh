@@ -67,7 +67,7 @@ struct AttendArgs {
   int whole_heads;          // 1: no head is split
 };
 // Bytes of scratch, and how many row tiles and CTAs the call takes.
-size_t attend_workspace(int E, int N, int H, int kv_heads, int width, long long longest);
+size_t attend_workspace(int E, int N, int H, int kv_heads, int width, int window, long long longest);
 cudaError_t launch_attend(AttendArgs a, int dtype, int width, void* workspace, long long longest, int* wait_status, cudaStream_t stream);
 // The pieces of `entries` heads and blocks of tile_rows rows (a.split, a.part_o, a.part_ml; a head's pieces `stride` slots apart) into a.out.
 cudaError_t launch_join(const AttendArgs& a, int dtype, int width, int tile_rows, int entries, int stride, cudaStream_t stream);

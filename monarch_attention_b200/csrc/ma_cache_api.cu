@@ -116,7 +116,7 @@ int ma_b200_cache_append(const ma_b200_append* p, void* stream) {
 
 size_t ma_b200_cache_attend_workspace_bytes(const ma_b200_attend* p) {
   if (check_attend_shape(p) != MA_B200_OK) return 0;
-  return ma::attend_workspace(p->E, p->N, p->H, p->cache.heads, p->cache.width, longest(p->sequences, p->cache.page_size));
+  return ma::attend_workspace(p->E, p->N, p->H, p->cache.heads, p->cache.width, p->window, longest(p->sequences, p->cache.page_size));
 }
 
 int ma_b200_cache_attend(const ma_b200_attend* p, void* workspace, size_t workspace_bytes, void* stream) {
@@ -128,7 +128,7 @@ int ma_b200_cache_attend(const ma_b200_attend* p, void* workspace, size_t worksp
   if (p->window < 0 || (p->window > 0 && !p->causal)) return invalid("window must not be negative, and needs causal");
   if (!isfinite(p->scale) || !(p->softcap >= 0.0f) || !isfinite(p->softcap)) return invalid("scale and softcap must be finite, softcap not negative");
   const long long most = longest(p->sequences, p->cache.page_size);
-  const size_t need = ma::attend_workspace(p->E, p->N, p->H, p->cache.heads, p->cache.width, most);
+  const size_t need = ma::attend_workspace(p->E, p->N, p->H, p->cache.heads, p->cache.width, p->window, most);
   if (workspace == nullptr || reinterpret_cast<uintptr_t>(workspace) % 256 != 0) return invalid("workspace is NULL or not 256-byte aligned");
   if (workspace_bytes < need)
     return fail_with(MA_B200_WORKSPACE_TOO_SMALL, "workspace has " + std::to_string(workspace_bytes) + " bytes, need " + std::to_string(need));

@@ -30,18 +30,19 @@ using sm100::kLog2e;
 using sm100::smem_u32;
 
 constexpr float kSlack = 8.0f;  // weights are at most 2^8 of the reference: f16 holds them as exactly as those up to 1
-constexpr int kWarps = 4, kSlice = 32, kStep = kWarps * kSlice;  // tokens of a warp and of a CTA at a time
+constexpr int kSlice = 32;  // tokens of a warp at a time
 
-template <int D, int NT>
+template <int D, int NT, int W>
 struct Shape {
-  static constexpr int kStages = D == 128 ? 2 : 3;
+  static constexpr int kStep = W * kSlice;  // tokens of a CTA at a time
+  static constexpr int kStages = W == 4 ? (D == 128 ? 2 : 3) : (D == 128 ? 3 : 4);
   static constexpr int kStageBytes = 2 * kSlice * D + 16;  // keys, values and their two scales each
   static constexpr int kRows = 8 * NT;
   static constexpr bool kSharedRows = NT > 1;  // the query rows' operands are in shared memory: there are no registers for them
-  static constexpr int kRing = kWarps * kStages * kStageBytes;
+  static constexpr int kRing = W * kStages * kStageBytes;
   static constexpr int kOperandBytes = kSharedRows ? kRows * D * 2 : 0;
   static constexpr int kSmem = kRing + kOperandBytes;
-  static constexpr int kCtas = NT > 2 ? 2 : 3;  // of an SM: what registers and shared memory allow
+  static constexpr int kCtas = W > 4 ? 1 : NT > 2 ? 2 : 3;  // of an SM: what registers and shared memory allow
 };
 
 // Byte offset of 16-byte piece `piece` of token t in a slice: pieces are permuted so that neither the reads of the keys (8 rows x 4 pieces)
@@ -92,6 +93,7 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
 struct Sequence {
   int len, count, lo, steps;  // keys [lo, len) are looked at, in `steps` steps (one at least)
 };
+template <int kStep>
 __device__ __forceinline__ Sequence sequence(const AttendArgs& a, int e) {
   Sequence s;
   sequence_of(a.cache, e, a.N, &s.len, &s.count);
@@ -123,6 +125,7 @@ struct Place {
   int e, head, block, step;  // block: of rows
   Sequence s;
 };
+template <int kStep>
 __device__ __forceinline__ void advance(const AttendArgs& a, Place* p) {
   if (++p->step < p->s.steps) return;
   p->step = 0;
@@ -130,19 +133,20 @@ __device__ __forceinline__ void advance(const AttendArgs& a, Place* p) {
   p->block = 0;
   if (++p->head < a.cache.heads) return;
   p->head = 0;
-  if (++p->e < a.E) p->s = sequence(a, p->e);
+  if (++p->e < a.E) p->s = sequence<kStep>(a, p->e);
 }
 
-template <typename T, int D, int NT>
-__global__ void __launch_bounds__(kWarps * 32, Shape<D, NT>::kCtas) attend_kernel(const __grid_constant__ AttendArgs a) {
-  using S = Shape<D, NT>;
+template <typename T, int D, int NT, int W>
+__global__ void __launch_bounds__(W * 32, Shape<D, NT, W>::kCtas) attend_kernel(const __grid_constant__ AttendArgs a) {
+  using S = Shape<D, NT, W>;
+  constexpr int kStep = S::kStep;
   constexpr int kWords = D / 16;   // 32-bit words of a key row that a lane holds; also products of 16 features, and feature tiles of 16
   constexpr int kValueWords = D / 32;
   extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ long long warp_sum[kWarps];
+  __shared__ long long warp_sum[W];
   __shared__ __align__(16) float row_scale[S::kRows];
   __shared__ __align__(16) int2 row_keys[S::kRows];  // keys [x, y) that a row sees
-  __shared__ float2 tops[kWarps][S::kRows];           // running maximum and sum of each warp
+  __shared__ float2 tops[W][S::kRows];           // running maximum and sum of each warp
   __shared__ int where_e;
   __shared__ long long where_at;
   const CacheArgs& c = a.cache;
@@ -159,22 +163,22 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<D, NT>::kCtas) attend_kerne
     const long long heads = (long long)a.E * units, u0 = blockIdx.x * heads / ctas, u1 = (blockIdx.x + 1) * heads / ctas;
     now.e = (int)(u0 / units);
     unit = (int)(u0 - (long long)now.e * units);
-    now.s = sequence(a, now.e);
+    now.s = sequence<kStep>(a, now.e);
     now.step = 0;
     for (long long u = u0; u < u1;) {
       const int e = (int)(u / units);
       const long long next = min(u1, (long long)(e + 1) * units);
-      steps += (int)(next - u) * sequence(a, e).steps;
+      steps += (int)(next - u) * sequence<kStep>(a, e).steps;
       u = next;
     }
     int x, y;
-    for (int e = blockIdx.x * kWarps * 32 + tid; e < a.E; e += gridDim.x * kWarps * 32)
+    for (int e = blockIdx.x * W * 32 + tid; e < a.E; e += gridDim.x * W * 32)
       if (!sequence_of(c, e, a.N, &x, &y)) report(c.status, kBadLength);
   } else {  // prefix sums over the sequences, a run of them per thread
-    const int run = (a.E + kWarps * 32 - 1) / (kWarps * 32);
+    const int run = (a.E + W * 32 - 1) / (W * 32);
     long long mine = 0;
     for (int e = tid * run; e < min(a.E, (tid + 1) * run); ++e) {
-      mine += sequence(a, e).steps;
+      mine += sequence<kStep>(a, e).steps;
       int x, y;
       if (blockIdx.x == 0 && !sequence_of(c, e, a.N, &x, &y)) report(c.status, kBadLength);
     }
@@ -187,7 +191,7 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<D, NT>::kCtas) attend_kerne
     if (lane == 31) warp_sum[w] = upto;
     __syncthreads();
     for (int i = 0; i < w; ++i) upto += warp_sum[i];
-    for (int i = 0; i < kWarps; ++i) total += warp_sum[i];
+    for (int i = 0; i < W; ++i) total += warp_sum[i];
     total *= units;
     ctas = min(ctas, total);
     if (blockIdx.x >= ctas) {
@@ -202,7 +206,7 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<D, NT>::kCtas) attend_kerne
       long long at = (upto - mine) * units;
       int e = tid * run;
       for (;; ++e) {
-        const long long n = (long long)sequence(a, e).steps * units;
+        const long long n = (long long)sequence<kStep>(a, e).steps * units;
         if (begin < at + n) break;
         at += n;
       }
@@ -211,7 +215,7 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<D, NT>::kCtas) attend_kerne
     }
     __syncthreads();
     now.e = where_e;
-    now.s = sequence(a, now.e);
+    now.s = sequence<kStep>(a, now.e);
     unit = where_at < 0x7fffffff ? (int)where_at / now.s.steps : (int)(where_at / now.s.steps);
     now.step = (int)(where_at - (long long)unit * now.s.steps);
   }
@@ -270,7 +274,7 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<D, NT>::kCtas) attend_kerne
   for (int i = 0; i < S::kStages - 1; ++i) {
     if (i < steps) {
       fetch(i);
-      advance(a, &ahead);
+      advance<kStep>(a, &ahead);
       if (i + 1 < steps) look_up();
     }
     copies_commit();
@@ -360,7 +364,7 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<D, NT>::kCtas) attend_kerne
     __syncwarp();
     if (i + S::kStages - 1 < steps) {
       fetch(stage == 0 ? S::kStages - 1 : stage - 1);
-      advance(a, &ahead);
+      advance<kStep>(a, &ahead);
       if (i + S::kStages < steps) look_up();
     }
     copies_commit();
@@ -499,8 +503,8 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<D, NT>::kCtas) attend_kerne
 
     const bool last_of_head = now.step + 1 == now.s.steps;
     if (last_of_head || i + 1 == steps) {
-      // --- the four warps' sums into one: each brings its own to the common maximum and leaves it in its ring, in the stage that it has just
-      // used up, a tile of rows at a time (by turns in its two halves); warp w then adds up rows 2 w and 2 w + 1
+      // --- the warps' sums into one: each brings its own to the common maximum and leaves it in its ring, in the stage that it has just
+      // used up, a tile of rows at a time (by turns in its two halves); warp w < 4 then adds up rows 2 w and 2 w + 1
       fresh = true;
 #pragma unroll
       for (int n = 0; n < NT; ++n)
@@ -520,7 +524,7 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<D, NT>::kCtas) attend_kerne
         for (int j = 0; j < 2; ++j) {
           float most = -CUDART_INF_F;
 #pragma unroll
-          for (int v = 0; v < kWarps; ++v) most = fmaxf(most, tops[v][n * 8 + 2 * q4 + j].x);
+          for (int v = 0; v < W; ++v) most = fmaxf(most, tops[v][n * 8 + 2 * q4 + j].x);
           const float x = ex2(top[n][j] - (most == -CUDART_INF_F ? 0.0f : most));
 #pragma unroll
           for (int m = 0; m < kWords; ++m) {
@@ -532,22 +536,22 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<D, NT>::kCtas) attend_kerne
         // 8 neighbouring features of a row a lane (64 features: 4), in the places where the lanes of the product had them
         constexpr int kRun = D / 16;
         const int j = lane >> 4, u = lane & 15, r = n * 8 + 2 * w + j;
-        if (row0 + r < a.N * a.group) {
+        if (w < 4 && row0 + r < a.N * a.group) {
           float x[kRun];
 #pragma unroll
           for (int f = 0; f < kRun; ++f) x[f] = 0.0f;
 #pragma unroll
-          for (int v = 0; v < kWarps; ++v) {
+          for (int v = 0; v < W; ++v) {
             const float* theirs = reinterpret_cast<const float*>(smem + (v * S::kStages + stage) * S::kStageBytes);
 #pragma unroll
             for (int f = 0; f < kRun; ++f) x[f] += theirs[(n & 1) * 8 * D + (((u & 1) * (kWords / 2) + f / 2) * 4 + j + 2 * (f & 1)) * 32 + (u >> 1) * 4 + w];
           }
           float most = -CUDART_INF_F, all = 0.0f;
 #pragma unroll
-          for (int v = 0; v < kWarps; ++v) most = fmaxf(most, tops[v][r].x);
+          for (int v = 0; v < W; ++v) most = fmaxf(most, tops[v][r].x);
           const float base = most == -CUDART_INF_F ? 0.0f : most;
 #pragma unroll
-          for (int v = 0; v < kWarps; ++v) all += tops[v][r].y * ex2(tops[v][r].x - base);
+          for (int v = 0; v < W; ++v) all += tops[v][r].y * ex2(tops[v][r].x - base);
           if (alone) {
             const int token = (row0 + r) / a.group, h = now.head * a.group + row0 + r - token * a.group;
             const float inverse = token < now.s.count && all > 0.0f ? 1.0f / all : 0.0f;
@@ -579,7 +583,7 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<D, NT>::kCtas) attend_kerne
       later = true;
     }
     stage = stage + 1 == S::kStages ? 0 : stage + 1;
-    advance(a, &now);
+    advance<kStep>(a, &now);
   }
 }
 
@@ -705,37 +709,55 @@ __global__ void __launch_bounds__(256) join_rows_kernel(const __grid_constant__ 
 }
 
 int row_tiles(int rows) { return rows <= 32 ? (rows + 7) / 8 : 4; }
-int ctas_per_sm(int nt) { return nt > 2 ? Shape<128, 4>::kCtas : Shape<128, 1>::kCtas; }
-
 constexpr long long kPromptRows = 65;  // from as many rows on, the tcgen05 kernel
 
-constexpr int kWholeSteps = 4;  // heads of up to as many steps are not split
-
-// CTAs of a call: what the GPU holds at once, and no more than the steps that the lengths can have.
-long long grid_of(int E, int N, int H, int kv_heads, int width, long long longest) {
+// How a call is shared out.
+struct Plan {
+  int nt, warps;
+  bool whole;       // heads are not split, and there is nothing to join
+  long long grid;
+};
+Plan plan_of(int E, int N, int H, int kv_heads, int window, long long longest) {
   const int rows = H / kv_heads * N, nt = row_tiles(rows);
   const long long units = (long long)E * kv_heads * ((rows + 8 * nt - 1) / (8 * nt));
-  const long long steps = longest <= kWholeSteps * kStep ? units : units * ((longest + kStep - 1) / kStep);
-  const long long most = (long long)ctas_per_sm(nt) * sm_count();
-  return steps < most ? steps : most;
+  const long long looked_at = (long long)window + N + kScaleBlock;  // keys of a sequence, at most
+  if (window > 0 && longest > looked_at) longest = looked_at;
+  // A head of a few steps stays with one CTA: a second kernel costs 3 to 4 us.  Where there are no more heads than SMs, each has a CTA of
+  // eight warps and steps of 256 tokens, of 1.5 (64 features) to 2.3 us; with half as many heads or more the SMs are busy either way.
+  // us, whole / split, 12 heads of 64: 500 tokens 7.4 / 9.1, 1000 10.5 / 9.5, 2000 16.1 / 9.9; 96 heads: 1000 10.6 / 13.6, 2000 16.2 / 16.5; 144
+  // heads, 2000 16.5 / 19.7; 128 heads of 128 features, 2000 22.9 / 23.0, 4000 40.5 / 37.2.
+  if (units <= sm_count() && longest <= (2 * units >= sm_count() ? 2048 : 768)) return {nt, 8, true, units};
+  const long long most = (nt > 2 ? Shape<128, 4, 4>::kCtas : Shape<128, 1, 4>::kCtas) * (long long)sm_count();
+  constexpr int kStep = Shape<128, 1, 4>::kStep;
+  const bool whole = longest <= 4 * kStep;
+  const long long steps = whole ? units : units * ((longest + kStep - 1) / kStep);
+  return {nt, 4, whole, steps < most ? steps : most};
 }
 
-template <typename T, int D, int NT>
-cudaError_t launch(AttendArgs& a, long long grid, cudaStream_t stream) {
-  const void* fn = (const void*)attend_kernel<T, D, NT>;
-  constexpr size_t smem = Shape<D, NT>::kSmem;
+template <typename T, int D, int NT, int W>
+cudaError_t launch(AttendArgs& a, const Plan& plan, cudaStream_t stream) {
+  const void* fn = (const void*)attend_kernel<T, D, NT, W>;
+  constexpr size_t smem = Shape<D, NT, W>::kSmem;
   cudaError_t err = allow_dynamic_smem(fn, smem);
   if (err != cudaSuccess) return err;
   void* args[] = {(void*)&a};
-  err = launch_kernel(fn, dim3((unsigned)grid), dim3(kWarps * 32), args, smem, stream);
-  if (err != cudaSuccess || a.whole_heads) return err;
+  err = launch_kernel(fn, dim3((unsigned)plan.grid), dim3(W * 32), args, smem, stream);
+  if (err != cudaSuccess || plan.whole) return err;
   int tile_rows = 8 * NT;
   void* join_args[] = {(void*)&a, (void*)&tile_rows};
   const unsigned rows = a.group * a.N < tile_rows ? a.group * a.N : tile_rows;
-  const long long entries = a.split_by_head ? (long long)a.E * a.cache.heads * a.row_blocks : grid;
+  const long long entries = a.split_by_head ? (long long)a.E * a.cache.heads * a.row_blocks : plan.grid;
   // few heads have many pieces each: their rows are cut into parts of 32 features
   if (entries * rows < 2 * sm_count()) return launch_kernel((const void*)join_kernel<T, D>, dim3((unsigned)entries, rows, D / 32), dim3(256), join_args, 0, stream);
   return launch_join(a, std::is_same<T, __half>::value ? MA_B200_F16 : MA_B200_BF16, D, tile_rows, (int)entries, 2, stream);
+}
+template <typename T, int D>
+cudaError_t launch_rows(AttendArgs& a, const Plan& plan, cudaStream_t stream) {
+  if (plan.warps == 8)
+    return plan.nt == 1 ? launch<T, D, 1, 8>(a, plan, stream) : plan.nt == 2 ? launch<T, D, 2, 8>(a, plan, stream) :
+           plan.nt == 3 ? launch<T, D, 3, 8>(a, plan, stream) : launch<T, D, 4, 8>(a, plan, stream);
+  return plan.nt == 1 ? launch<T, D, 1, 4>(a, plan, stream) : plan.nt == 2 ? launch<T, D, 2, 4>(a, plan, stream) :
+         plan.nt == 3 ? launch<T, D, 3, 4>(a, plan, stream) : launch<T, D, 4, 4>(a, plan, stream);
 }
 
 }  // namespace
@@ -749,35 +771,30 @@ cudaError_t launch_join(const AttendArgs& a, int dtype, int width, int tile_rows
   return launch_kernel(fn, dim3((unsigned)(((long long)entries * rows + 7) / 8)), dim3(256), args, 0, stream);
 }
 
-size_t attend_workspace(int E, int N, int H, int kv_heads, int width, long long longest) {
+size_t attend_workspace(int E, int N, int H, int kv_heads, int width, int window, long long longest) {
   if (H / kv_heads * (long long)N >= kPromptRows) return prompt_workspace(E, N, H, kv_heads, width, longest);
-  const long long grid = grid_of(E, N, H, kv_heads, width, longest), rows = 8 * row_tiles(H / kv_heads * N);
-  const size_t entries = ((size_t)grid * sizeof(int4) + 255) / 256 * 256;
-  return entries + (size_t)grid * 2 * rows * (width + 2) * sizeof(float);
+  const Plan plan = plan_of(E, N, H, kv_heads, window, longest);
+  if (plan.whole) return 256;
+  const size_t entries = ((size_t)plan.grid * sizeof(int4) + 255) / 256 * 256;
+  return entries + (size_t)plan.grid * 2 * 8 * plan.nt * (width + 2) * sizeof(float);
 }
 
 cudaError_t launch_attend(AttendArgs a, int dtype, int width, void* workspace, long long longest, int* wait_status, cudaStream_t stream) {
   const long long strides[6] = {a.cache.k_sp, a.cache.k_sh, a.cache.k_st, a.cache.v_sp, a.cache.v_sh, a.cache.v_st};
   for (int i = 0; i < 6; ++i) (i < 3 ? a.k16[i] : a.v16[i - 3]) = (uint32_t)(strides[i] / 16);
   if (a.group * (long long)a.N >= kPromptRows) return launch_prompt(a, dtype, width, workspace, longest, wait_status, stream);
-  const int rows = a.group * a.N, nt = row_tiles(rows);
-  const long long grid = grid_of(a.E, a.N, a.H, a.cache.heads, width, longest);
-  a.row_blocks = (rows + 8 * nt - 1) / (8 * nt);
+  const Plan plan = plan_of(a.E, a.N, a.H, a.cache.heads, a.window, longest);
+  const int tile_rows = 8 * plan.nt;
+  a.row_blocks = (a.group * a.N + tile_rows - 1) / tile_rows;
   char* at = reinterpret_cast<char*>(workspace);
   a.split = reinterpret_cast<int4*>(at);
-  at += ((size_t)grid * sizeof(int4) + 255) / 256 * 256;
-  a.part_o = reinterpret_cast<float*>(at);
-  a.part_ml = a.part_o + (size_t)grid * 2 * 8 * nt * width;
-  a.split_by_head = (long long)a.E * a.cache.heads * a.row_blocks <= grid;
-  // A head of a few steps stays with one CTA: a second kernel costs 3 us, a step 0.7.
-  a.whole_heads = longest <= kWholeSteps * kStep;
+  a.part_o = reinterpret_cast<float*>(at + ((size_t)plan.grid * sizeof(int4) + 255) / 256 * 256);
+  a.part_ml = a.part_o + (size_t)plan.grid * 2 * tile_rows * width;
+  a.whole_heads = plan.whole;
+  a.split_by_head = (long long)a.E * a.cache.heads * a.row_blocks <= plan.grid;
   const bool bf = dtype == MA_B200_BF16;
-#define MA_ATTEND(T, D) \
-  (nt == 1 ? launch<T, D, 1>(a, grid, stream) : nt == 2 ? launch<T, D, 2>(a, grid, stream) : \
-   nt == 3 ? launch<T, D, 3>(a, grid, stream) : launch<T, D, 4>(a, grid, stream))
-  if (width == 128) return bf ? MA_ATTEND(__nv_bfloat16, 128) : MA_ATTEND(__half, 128);
-  return bf ? MA_ATTEND(__nv_bfloat16, 64) : MA_ATTEND(__half, 64);
-#undef MA_ATTEND
+  if (width == 128) return bf ? launch_rows<__nv_bfloat16, 128>(a, plan, stream) : launch_rows<__half, 128>(a, plan, stream);
+  return bf ? launch_rows<__nv_bfloat16, 64>(a, plan, stream) : launch_rows<__half, 64>(a, plan, stream);
 }
 
 }  // namespace ma
