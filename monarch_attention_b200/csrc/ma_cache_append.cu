@@ -137,6 +137,22 @@ __global__ void __launch_bounds__(kThreads, 2) append_kernel(const __grid_consta
   // slots [first, last) of the block take new tokens
   const int first = max(start - base, 0), last = min(max(len - base, 0), kScaleBlock);
   const bool any = first < last;
+  const bool fresh = slot >= first && slot < last;  // the lane's token is new
+  const int n = base + slot - start;                // the call's number of it
+  const int stride = gridDim.y * kTeams * kHeads, g_first = blockIdx.y * kTeams * kHeads;
+  uint4 raw[2][kHeads];
+  auto load = [&](int h0) {
+#pragma unroll
+    for (int kind = 0; kind < 2; ++kind)
+#pragma unroll
+      for (int h = 0; h < kHeads; ++h) {
+        const View4& view = kind == 0 ? a.k : a.v;
+        raw[kind][h] = make_uint4(0, 0, 0, 0);
+        if (fresh && h0 + h < c.heads)
+          raw[kind][h] = *reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(view.ptr) + e * view.se + (h0 + h) * view.sh + n * view.sn + f0);
+      }
+  };
+  load(g_first + team * kHeads);  // (on their way while the sines are computed)
   if (any)
     for (int i = first * pairs + tid; i < last * pairs; i += kThreads) table[i] = rotary_turn(a.rotary, i % pairs, base + i / pairs);
   if (tid < 3 * kTeams * 2 * kHeads) (&most[0][0][0][0])[tid] = 0;
@@ -144,28 +160,21 @@ __global__ void __launch_bounds__(kThreads, 2) append_kernel(const __grid_consta
   if (any && page < 0 && tid == 0 && blockIdx.y == 0) report(c.status, kBadPage);
   const int in_page = base & ((1 << c.page_shift) - 1);
   __syncthreads();
-  const bool fresh = slot >= first && slot < last;  // the lane's token is new
-  const int n = base + slot - start;                // the call's number of it
   const Turn turn = turn_of<D>(a.rotary, table + slot * pairs, fresh, lane, f0);
 
   // --- keys and values, kHeads at a time
-  const int stride = gridDim.y * kTeams * kHeads;
   if (page >= 0) {
     int round = 0;
-    for (int g0 = blockIdx.y * kTeams * kHeads; g0 < c.heads; g0 += stride, round = round == 2 ? 0 : round + 1) {  // (the same for all teams)
+    for (int g0 = g_first; g0 < c.heads; g0 += stride, round = round == 2 ? 0 : round + 1) {  // (the same for all teams)
       const int h0 = g0 + team * kHeads;
-      uint4 raw[2][kHeads];
+      if (g0 != g_first) load(h0);
       float before[2][kHeads];
 #pragma unroll
       for (int kind = 0; kind < 2; ++kind)
 #pragma unroll
         for (int h = 0; h < kHeads; ++h) {
-          const View4& view = kind == 0 ? a.k : a.v;
-          raw[kind][h] = make_uint4(0, 0, 0, 0);
           before[kind][h] = 0.0f;
-          if (h0 + h >= c.heads) continue;
-          if (fresh) raw[kind][h] = *reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(view.ptr) + e * view.se + (h0 + h) * view.sh + n * view.sn + f0);
-          if (first > 0)  // the block has older tokens, and a scale
+          if (first > 0 && h0 + h < c.heads)  // the block has older tokens, and a scale
             before[kind][h] = (kind == 0 ? c.k_scale + page * c.ks_sp + (h0 + h) * c.ks_sh : c.v_scale + page * c.vs_sp + (h0 + h) * c.vs_sh)[in_page / kScaleBlock];
         }
 #pragma unroll

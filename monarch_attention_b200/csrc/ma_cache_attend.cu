@@ -718,17 +718,23 @@ struct Plan {
   long long grid;
 };
 Plan plan_of(int E, int N, int H, int kv_heads, int window, long long longest) {
-  const int rows = H / kv_heads * N, nt = row_tiles(rows);
-  const long long units = (long long)E * kv_heads * ((rows + 8 * nt - 1) / (8 * nt));
+  const int rows = H / kv_heads * N;
   const long long looked_at = (long long)window + N + kScaleBlock;  // keys of a sequence, at most
   if (window > 0 && longest > looked_at) longest = looked_at;
+  constexpr int kStep = Shape<128, 1, 4>::kStep;
+  // Up to four tiles of 8 rows share a key's conversion; but three or four of them are a long chain for a warp, and where the steps are few
+  // anyway, two blocks of rows that both read the keys are done sooner.  us, with as many tiles as there are rows / two: 16 sequences
+  // of 20 rows x 4 heads, window 1024, 20.7 / 17.3, of 32 rows and up to 4096 tokens 38.3 / 34.6; 32 of 32 rows and up to 8000 82 / 86, one of
+  // 20 rows and 131000 tokens 32 / 43.
+  int nt = row_tiles(rows);
+  if (nt > 2 && (long long)E * kv_heads * ((rows + 8 * nt - 1) / (8 * nt)) * ((longest + kStep - 1) / kStep) <= 16LL * sm_count()) nt = 2;
+  const long long units = (long long)E * kv_heads * ((rows + 8 * nt - 1) / (8 * nt));
   // A head of a few steps stays with one CTA: a second kernel costs 3 to 4 us.  Where there are no more heads than SMs, each has a CTA of
   // eight warps and steps of 256 tokens, of 1.5 (64 features) to 2.3 us; with half as many heads or more the SMs are busy either way.
   // us, whole / split, 12 heads of 64: 500 tokens 7.4 / 9.1, 1000 10.5 / 9.5, 2000 16.1 / 9.9; 96 heads: 1000 10.6 / 13.6, 2000 16.2 / 16.5; 144
   // heads, 2000 16.5 / 19.7; 128 heads of 128 features, 2000 22.9 / 23.0, 4000 40.5 / 37.2.
   if (units <= sm_count() && longest <= (2 * units >= sm_count() ? 2048 : 768)) return {nt, 8, true, units};
   const long long most = (nt > 2 ? Shape<128, 4, 4>::kCtas : Shape<128, 1, 4>::kCtas) * (long long)sm_count();
-  constexpr int kStep = Shape<128, 1, 4>::kStep;
   const bool whole = longest <= 4 * kStep;
   const long long steps = whole ? units : units * ((longest + kStep - 1) / kStep);
   return {nt, 4, whole, steps < most ? steps : most};
