@@ -120,7 +120,7 @@ template <typename T, int D>
 __global__ void __launch_bounds__(kThreads, 2) append_kernel(const __grid_constant__ AppendArgs a) {
   constexpr int kLanes = D / F, kRows = 32 / kLanes;               // rows of a warp at once
   constexpr int kTeam = kScaleBlock / kRows, kTeams = kWarps / kTeam;  // warps that hold the 16 tokens of a head between them
-  constexpr int kHeads = 4;                                        // of keys, and of values, that a team has in flight
+  constexpr int kHeads = 2;                                        // of keys, and of values, that a team has in flight
   __shared__ float2 table[kScaleBlock * D / 2];
   __shared__ unsigned int most[3][kTeams][2][kHeads];
   const CacheArgs& c = a.cache;
@@ -152,7 +152,19 @@ __global__ void __launch_bounds__(kThreads, 2) append_kernel(const __grid_consta
           raw[kind][h] = *reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(view.ptr) + e * view.se + (h0 + h) * view.sh + n * view.sn + f0);
       }
   };
+  constexpr int kInFlight = 8;
+  const int q_first = (blockIdx.y * kTeams + team) * kInFlight;
+  uint4 rows[kInFlight];  // of queries
+  auto load_q = [&](int h0) {
+    const T* const src = reinterpret_cast<const T*>(a.q.ptr) + e * a.q.se + n * a.q.sn + f0;
+#pragma unroll
+    for (int i = 0; i < kInFlight; ++i) {
+      rows[i] = make_uint4(0, 0, 0, 0);
+      if (fresh && h0 + i < a.H) rows[i] = *reinterpret_cast<const uint4*>(src + (h0 + i) * a.q.sh);
+    }
+  };
   load(g_first + team * kHeads);  // (on their way while the sines are computed)
+  load_q(q_first);
   if (any)
     for (int i = first * pairs + tid; i < last * pairs; i += kThreads) table[i] = rotary_turn(a.rotary, i % pairs, base + i / pairs);
   if (tid < 3 * kTeams * 2 * kHeads) (&most[0][0][0][0])[tid] = 0;
@@ -219,20 +231,13 @@ __global__ void __launch_bounds__(kThreads, 2) append_kernel(const __grid_consta
 
   // --- queries; rows behind the sequence's tokens become zeros
   const bool mine = n >= 0 && n < a.N;
-  const T* src = reinterpret_cast<const T*>(a.q.ptr) + e * a.q.se + n * a.q.sn + f0;
-  T* dst = reinterpret_cast<T*>(const_cast<void*>(a.q_out.ptr)) + e * a.q_out.se + n * a.q_out.sn + f0;
-  constexpr int kInFlight = 8;
-  for (int h0 = (blockIdx.y * kTeams + team) * kInFlight; h0 < a.H; h0 += gridDim.y * kTeams * kInFlight) {
-    uint4 raw[kInFlight];
-#pragma unroll
-    for (int i = 0; i < kInFlight; ++i) {
-      raw[i] = make_uint4(0, 0, 0, 0);
-      if (fresh && h0 + i < a.H) raw[i] = *reinterpret_cast<const uint4*>(src + (h0 + i) * a.q.sh);
-    }
+  T* const dst = reinterpret_cast<T*>(const_cast<void*>(a.q_out.ptr)) + e * a.q_out.se + n * a.q_out.sn + f0;
+  for (int h0 = q_first; h0 < a.H; h0 += gridDim.y * kTeams * kInFlight) {
+    if (h0 != q_first) load_q(h0);
 #pragma unroll
     for (int i = 0; i < kInFlight; ++i) {
       float x[F];
-      widen<T>(raw[i], x);
+      widen<T>(rows[i], x);
       if (pairs > 0) apply(a.rotary, turn, x);
       if (mine && h0 + i < a.H) *reinterpret_cast<uint4*>(dst + (h0 + i) * a.q_out.sh) = narrow<T>(x);
     }
@@ -313,7 +318,7 @@ cudaError_t launch_append(const AppendArgs& a, int dtype, int width, cudaStream_
                       : (width == 128 ? (const void*)append_kernel<__half, 128> : (const void*)append_kernel<__half, 64>);
   const long long blocks = (long long)a.E * ((a.N + kScaleBlock - 2) / kScaleBlock + 1);
   // few blocks: their heads are spread over more CTAs, each of which computes the sines again
-  const int per = width == 128 ? 4 : 8;
+  const int per = width == 128 ? 2 : 4;
   const int groups = (a.cache.heads + per - 1) / per;
   const long long wanted = 4LL * sm_count() / blocks + 1;
   return launch_kernel(fn, dim3((unsigned)blocks, (unsigned)(wanted < groups ? wanted : groups)), dim3(kThreads), args, 0, stream);
