@@ -126,7 +126,8 @@ int ma_b200_cache_attend(const ma_b200_attend* p, void* workspace, size_t worksp
   if ((rc = check_cache(p->cache, p->sequences, p->E, p->H, p->N, p->dtype, &a.cache)) != MA_B200_OK) return rc;
   if ((rc = check_tensor(p->q, "q", 2, 16)) != MA_B200_OK || (rc = check_tensor(p->out, "out", 2, 16)) != MA_B200_OK) return rc;
   if (p->window < 0 || (p->window > 0 && !p->causal)) return invalid("window must not be negative, and needs causal");
-  if (!isfinite(p->scale) || !(p->softcap >= 0.0f) || !isfinite(p->softcap)) return invalid("scale and softcap must be finite, softcap not negative");
+  if (!isfinite(p->scale) || !(p->softcap == 0.0f || p->softcap >= 1e-20f) || !isfinite(p->softcap))
+    return invalid("scale and softcap must be finite, softcap 0 (none) or from 1e-20 on");
   const long long most = longest(p->sequences, p->cache.page_size);
   const size_t need = ma::attend_workspace(p->E, p->N, p->H, p->cache.heads, p->cache.width, p->window, most);
   if (workspace == nullptr || reinterpret_cast<uintptr_t>(workspace) % 256 != 0) return invalid("workspace is NULL or not 256-byte aligned");

@@ -97,7 +97,7 @@ template <int kStep>
 __device__ __forceinline__ Sequence sequence(const AttendArgs& a, int e) {
   Sequence s;
   sequence_of(a.cache, e, a.N, &s.len, &s.count);
-  s.lo = a.window > 0 ? max(s.len - s.count - a.window + 1, 0) & ~(kScaleBlock - 1) : 0;
+  s.lo = a.window > 0 ? max(max(s.len - s.count, 0) - a.window + 1, 0) & ~(kScaleBlock - 1) : 0;
   s.steps = max((s.len - s.lo + kStep - 1) / kStep, 1);
   return s;
 }
@@ -152,7 +152,8 @@ __global__ void __launch_bounds__(W * 32, Shape<D, NT, W>::kCtas) attend_kernel(
   const CacheArgs& c = a.cache;
   const int tid = threadIdx.x, w = tid >> 5, lane = tid & 31, g = lane >> 2, q4 = lane & 3;
   const int units = c.heads * a.row_blocks;
-  stage_begin();  // (the joining kernel may come up where there is room)
+  if (!a.whole_heads) dependents_may_start();  // (the joining kernel may come up where there is room)
+  grid_wait();
 
   // --- this CTA's share of the steps
   Place now;
@@ -339,7 +340,7 @@ __global__ void __launch_bounds__(W * 32, Shape<D, NT, W>::kCtas) attend_kernel(
       }
       if (tid < S::kRows) {
         const int token = (row0 + tid) / a.group, place = now.s.len - now.s.count + token;
-        row_keys[tid] = make_int2(a.window > 0 ? place - a.window + 1 : 0, token >= now.s.count ? 0 : a.causal ? place + 1 : now.s.len);
+        row_keys[tid] = make_int2(a.window > 0 ? max(place, 0) - a.window + 1 : 0, token >= now.s.count ? 0 : a.causal ? place + 1 : now.s.len);
       }
       __syncthreads();
       // rows are in the order of their tokens; those of padding have results of zero whatever they see
@@ -348,7 +349,7 @@ __global__ void __launch_bounds__(W * 32, Shape<D, NT, W>::kCtas) attend_kernel(
       if (a.causal && row0 / a.group < now.s.count) {
         const int last = min((row0 + S::kRows - 1) / a.group, now.s.count - 1);
         full_high = row_keys[0].y;
-        if (a.window > 0) full_low = now.s.len - now.s.count + last - a.window + 1;
+        if (a.window > 0) full_low = max(now.s.len - now.s.count + last, 0) - a.window + 1;
       }
 #pragma unroll
       for (int n = 0; n < NT; ++n) {

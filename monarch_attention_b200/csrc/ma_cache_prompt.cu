@@ -122,7 +122,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
   const bool two = row0 + kTileRows < count * a.group;  // the second tile has rows
   int lo = 0, hi = len;
   if (a.causal) hi = min(len, len - count + last_token + 1);
-  if (a.window > 0) lo = max(len - count + first_token - a.window + 1, 0) & ~(kScaleBlock - 1);
+  if (a.window > 0) lo = max(max(len - count + first_token, 0) - a.window + 1, 0) & ~(kScaleBlock - 1);
   if (first_token >= count) hi = lo;
   const int all_steps = max((hi - lo + kKeys - 1) / kKeys, 0);
   const int step0 = (int)((long long)piece * all_steps / args.pieces), steps = (int)((long long)(piece + 1) * all_steps / args.pieces) - step0;
@@ -201,7 +201,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
       fence_async_smem();
       mbar_arrive(bar(kQ0 + tile));
       const int place = len - count + token;
-      const int high = !real ? 0 : a.causal ? place + 1 : len, low = a.window > 0 ? place - a.window + 1 : 0;
+      const int high = !real ? 0 : a.causal ? place + 1 : len, low = a.window > 0 ? max(place, 0) - a.window + 1 : 0;
       for (int i = 0; i < steps && ok; ++i) {
         ok = wait(kS0 + tile, i);
         if (!ok) break;

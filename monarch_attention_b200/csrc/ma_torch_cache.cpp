@@ -1,6 +1,7 @@
 // Native halves of the rotary positions, the paged cache and the attention over it: input checks, results and
 // workspaces from PyTorch's caching allocator, and the launches through the C ABI.
 #include <ATen/ExpandUtils.h>
+#include <ATen/MemoryOverlap.h>
 #include <torch/csrc/autograd/function.h>
 #include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/saved_variable.h>
@@ -68,7 +69,9 @@ void check_rotated(const Tensor& q, const optional<Tensor>& k, const optional<Te
 Tensor new_like(const Tensor& t) {
   const at::TensorOptions o = at::TensorOptions().dtype(t.scalar_type()).device(t.device());
   if (t.is_non_overlapping_and_dense()) return at::detail::empty_strided_cuda(t.sizes(), t.strides(), o);
-  return at::detail::empty_strided_cuda(t.sizes(), at::infer_dense_strides(t.sizes(), t.strides()), o);
+  const auto strides = at::infer_dense_strides(t.sizes(), t.strides());
+  if (strides.back() != 1 && t.size(-1) != 1) return at::detail::empty_cuda(t.sizes(), o);  // (features next to one another whatever is expanded)
+  return at::detail::empty_strided_cuda(t.sizes(), strides, o);
 }
 
 // Rotated copies of q and k (undefined ones are left out).
@@ -262,6 +265,7 @@ Tensor attend(const Tensor& q_in, const Cache& cache, const Tensor& table, const
     TORCH_CHECK_VALUE(out.sizes() == q_in.sizes() && out.scalar_type() == q_in.scalar_type() && out.device() == q_in.device() && out.stride(3) == 1,
                       "out must have the query's shape, dtype and device and unit inner stride");
     TORCH_CHECK_VALUE(!at::GradMode::is_enabled() || !out.requires_grad(), "out requires a gradient");
+    TORCH_CHECK_VALUE(at::has_internal_overlap(out) != at::MemOverlap::Yes, "the rows of out overlap");
   } else {
     const at::TensorOptions o = at::TensorOptions().dtype(q_in.scalar_type()).device(q_in.device());
     out = token_major ? at::detail::empty_strided_cuda({E, H, N, W}, {N * H * W, W, H * W, 1}, o) : at::detail::empty_cuda({E, H, N, W}, o);

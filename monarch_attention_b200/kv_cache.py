@@ -88,7 +88,8 @@ def cached_attention_b200(query: Tensor, cache: PagedKV, page_table: Tensor, len
     Query head ``h`` reads cache head ``h // (H / heads)``.  ``causal``: a token sees the positions up to its own (the call's tokens have been
     appended before); else all ``lengths`` (an encoder's output).  ``window`` > 0 (causal only): the last ``window`` of those.  Scores are
     multiplied by ``scale`` (None: ``width ** -0.5``) and, with ``softcap`` > 0, become ``softcap * tanh(score / softcap)``.  Rows without
-    a key, and rows of padding, are zero.  What lies in the cache behind a sequence's end is never looked at, NaN included.
+    a key, and rows of padding, are zero.  What lies in the cache behind a sequence's end is never looked at, NaN included; a NaN that was appended as a value reaches
+    all of the call's rows of its sequence and head, masked ones too (zero times NaN).
 
     The result has the query's dtype, and with ``token_major_output`` is a view of an (E, N, H, width) buffer; ``out`` (rows on 16-byte
     boundaries) takes it in place.  Scores and sums are in 32 bits; a bfloat16 query is read in 16-bit steps of 2^-11 of itself and 2^-25 of

@@ -336,3 +336,107 @@ def test_refusals():
     assert ma.cached_attention_b200(q[:0], cache, table[:0], n[:0]).shape == (0, 4, 1, 64)
     assert ma.cached_attention_b200(q[:, :, :0], cache, table, n).shape == (2, 4, 0, 64)
     assert ma.append_kv_b200(cache, k[:, :, :0], k[:, :, :0], table, n) is None
+
+
+@pytest.mark.parametrize("N,G", [(4, 2), (40, 4)])
+def test_windows_as_large_as_integers_go(N, G):
+    """More tokens than the sequence is long, with windows whose arithmetic would leave 32 bits."""
+    import monarch_attention_b200 as ma
+    cache, table = filled(2, 4, 2, 64, 16, [3, 60])
+    q = queries(2, 2 * G, N, 64, BF, "heads")
+    lengths = torch.tensor([3, 60], dtype=torch.int32, device="cuda")
+    want = ma.cached_attention_b200(q, cache, table, lengths)
+    for window in (2 ** 31 - 1, 2 ** 31 - 2, 2 ** 30):
+        assert torch.equal(ma.cached_attention_b200(q, cache, table, lengths, window=window), want)
+    with pytest.raises(ValueError):
+        ma.cached_attention_b200(q, cache, table, lengths, window=2 ** 31)
+
+
+def test_prompts_and_appends_are_captured_and_replayed():
+    import monarch_attention_b200 as ma
+    rotary = ma.RotaryPositions(64, pairs="interleaved")
+    module = ma.CachedAttention(rotary)
+    cache = ma.PagedKV.allocate(40, 2, 64, 32)
+    table = torch.arange(40, dtype=torch.int32, device="cuda").view(2, 20)
+    lengths, counts = torch.tensor([100, 600], dtype=torch.int32, device="cuda"), torch.tensor([100, 50], dtype=torch.int32, device="cuda")
+    q, k, v = (queries(2, h, 100, 64, BF, "tokens", seed=h) for h in (8, 2, 2))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = module(q, k, v, cache, table, lengths, counts)
+    for seed, pair, own in ((5, [100, 600], [100, 50]), (6, [640, 77], [3, 77]), (7, [0, 1], [0, 1])):
+        for t in (q, k, v):
+            t.copy_(queries(*t.shape, BF, "tokens", seed=seed))
+        lengths.copy_(torch.tensor(pair, dtype=torch.int32)), counts.copy_(torch.tensor(own, dtype=torch.int32))
+        before = [t.clone() if t.dtype != torch.float8_e4m3fn else t.view(torch.uint8).clone() for t in cache]
+        graph.replay()
+        torch.cuda.synchronize()
+        got = out.clone()
+        other = ma.PagedKV(*(t.view(torch.float8_e4m3fn) if t.dtype == torch.uint8 else t for t in before))
+        assert torch.equal(got, module(q, k, v, other, table, lengths, counts))
+        assert all(torch.equal(a.view(torch.uint8), b.view(torch.uint8)) for a, b in zip(cache, other))
+
+
+def test_first_calls_of_a_process_are_captured():
+    """What a first call sets up (shared memory, the status word, attributes) does not invalidate a capture."""
+    import os
+    import subprocess
+    import sys
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    code = """
+import torch, monarch_attention_b200 as ma
+r = ma.RotaryPositions(128)
+cache = ma.PagedKV.allocate(16, 2, 128, 64)
+table = torch.arange(16, dtype=torch.int32, device="cuda").view(1, 16)
+q, k, v = (torch.randn(1, h, 64, 128, device="cuda").to(torch.bfloat16) for h in (8, 2, 2))
+n, many = torch.tensor([64], dtype=torch.int32, device="cuda"), torch.tensor([1000], dtype=torch.int32, device="cuda")
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    a, b = ma.rotary_b200(q, k, r)
+    c = ma.append_kv_b200(cache, k, v, table, n, query=q, rotary=r)
+    d = ma.cached_attention_b200(c, cache, table, n)
+    e = ma.cached_attention_b200(c[:, :, -1:], cache, table, many)
+    f = ma.append_kv_b200(cache, k[:, :, :1], v[:, :, :1], table, many, query=q[:, :, :1], rotary=r)
+graph.replay()
+torch.cuda.synchronize()
+assert torch.equal(a, ma.rotary_b200(q, None, r)[0]) and torch.equal(d, ma.cached_attention_b200(c, cache, table, n))
+print("captured")
+"""
+    done = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True, timeout=300)
+    assert done.returncode == 0 and "captured" in done.stdout, done.stderr[-2000:]
+
+
+def test_calls_on_other_streams_and_from_threads():
+    """Calls at once on streams of their own, with a cache for reading in common."""
+    import threading
+
+    import monarch_attention_b200 as ma
+    cache, table = filled(2, 30, 2, 128, 64, [1800, 900])
+    lengths = torch.tensor([1800, 900], dtype=torch.int32, device="cuda")
+    qs = [queries(2, 8, n, 128, BF, "tokens", seed=n) for n in (1, 5, 80)]
+    want = [ma.cached_attention_b200(q, cache, table, lengths) for q in qs]
+    torch.cuda.synchronize()
+    wrong = []
+
+    def work(i):
+        stream = torch.cuda.Stream()
+        with torch.cuda.stream(stream):
+            for j in range(20):
+                q = qs[(i + j) % 3]
+                if not torch.equal(ma.cached_attention_b200(q, cache, table, lengths), want[(i + j) % 3]):
+                    wrong.append((i, j))
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(3)]
+    [t.start() for t in threads]
+    [t.join() for t in threads]
+    assert not wrong
+
+
+def test_the_rows_of_out_do_not_overlap():
+    import monarch_attention_b200 as ma
+    cache, table = filled(2, 4, 2, 64, 16, [3, 60])
+    q = queries(2, 4, 1, 64, BF, "heads")
+    lengths = torch.tensor([3, 60], dtype=torch.int32, device="cuda")
+    with pytest.raises(ValueError):
+        ma.cached_attention_b200(q, cache, table, lengths, out=torch.zeros(1, 4, 1, 64, dtype=BF, device="cuda").expand(2, -1, -1, -1))
+    with pytest.raises(ValueError):
+        ma.cached_attention_b200(q, cache, table, lengths, softcap=1e-30)

@@ -184,3 +184,30 @@ def test_refusals():
 def test_half_steps_are_the_types_own():
     for t, h in HALF_STEP.items():
         assert torch.finfo(t).eps / 2 == h
+
+
+def test_training_step_is_captured_and_replayed():
+    import monarch_attention_b200 as ma
+    r = ma.RotaryPositions(64)
+    q, k = (heads(2, 4, 50, 64, torch.float32, "tokens", s).requires_grad_(True) for s in (1, 2))
+    w = heads(2, 4, 50, 64, torch.float32, "heads", 3)
+    eager = torch.autograd.grad(ma.rotary_b200(q, k, r), (q, k), (w, w))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        grads = torch.autograd.grad(ma.rotary_b200(q, k, r), (q, k), (w, w))
+    for t in grads:
+        t.zero_()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(eager, grads))
+
+
+@pytest.mark.parametrize("expanded", [(3, 4, 5), (3, 1, 5), (1, 4, 5), (1, 1, 5), (3, 4, 1)])
+def test_expanded_inputs_of_all_kinds(expanded):
+    import monarch_attention_b200 as ma
+    r = ma.RotaryPositions(8, pairs="interleaved")
+    x = torch.randn(*expanded, 16, device="cuda").expand(3, 4, 5, 16)
+    y, z = ma.rotary_b200(x, x.transpose(0, 1).contiguous().transpose(0, 1), r)
+    want, size = rotate(x, torch.arange(5), r)
+    close(y, want, rotation_bound(want, size, torch.float32))
+    assert torch.equal(y, z) and y.stride(-1) == 1
