@@ -250,6 +250,7 @@ Tensor attend(const Tensor& q_in, const Cache& cache, const Tensor& table, const
               double softcap, int64_t window, const optional<Tensor>& out_in, bool token_major) {
   check_16bit(q_in, "query");
   const c10::cuda::CUDAGuard guard(q_in.device());
+  raise_for_status(ma_b200_poll_device_status(q_in.device().index()));  // (a bounded wait of an earlier call that gave up)
   raise_for_status(ma_b200_poll_cache_status(q_in.device().index()));
   ma_b200_attend p{};
   p.abi_version = MA_B200_ABI_VERSION;
