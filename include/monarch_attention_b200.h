@@ -371,7 +371,7 @@ MA_B200_API int ma_b200_cache_append(const ma_b200_append* p, void* stream);
 
 /* Softmax attention of q (E, H, N, width; bf16 or f16; query head h reads cache head h / (H / heads)) over the sequences' cached tokens
  * into out.  causal: token n sees positions up to its own, else all `lengths`.  window > 0 (causal only): the last `window`
- * of those.  softcap > 0: scores s become softcap * tanh(s / softcap).  Rows without a key, and rows of padding, are zero. */
+ * of those.  softcap > 0 (1e-20 to 1e30): scores s become softcap * tanh(s / softcap).  Rows without a key, and rows of padding, are zero. */
 typedef struct ma_b200_attend {
   int32_t abi_version;
   int32_t E, H, N;

@@ -2,6 +2,7 @@
 #pragma once
 
 #include "ma_rotary.cuh"
+#include "ma_sm100.cuh"
 
 namespace ma {
 
@@ -43,6 +44,16 @@ __device__ __forceinline__ int page_of(const CacheArgs& c, int e, int position) 
   if (i >= c.table_pages) return -1;
   const int page = c.table[e * c.table_se + i];
   return page >= 0 && page < c.pages ? page : -1;
+}
+
+// softcap * tanh(score / softcap) of a score in units of log2 e, in the same units.  tanh y = 1 - 2 / (exp(2 y) + 1) is off by some 2^-22 whatever y is,
+// too much next to a small y; below 1/8 its series takes over, whose first term left out is 2^-29 of it.
+__device__ __forceinline__ float capped(float x, float softcap) {
+  constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+  const float two = x * (2.0f / softcap), y2 = two * two * (0.25f * kLn2 * kLn2);
+  const float large = softcap * kLog2e * (1.0f - __fdividef(2.0f, sm100::ex2(two) + 1.0f));
+  const float small = x * fmaf(y2, fmaf(y2, fmaf(y2, -17.0f / 315.0f, 2.0f / 15.0f), -1.0f / 3.0f), 1.0f);
+  return y2 < 1.0f / 64.0f ? small : large;
 }
 
 struct AppendArgs {

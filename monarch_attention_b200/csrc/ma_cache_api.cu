@@ -100,6 +100,7 @@ int ma_b200_rotary_apply(const ma_b200_rotation* p, void* stream) {
 int ma_b200_cache_append(const ma_b200_append* p, void* stream) {
   if (p == nullptr) return invalid("problem is NULL");
   if (p->abi_version != MA_B200_ABI_VERSION) return invalid("abi_version mismatch: got " + std::to_string(p->abi_version));
+  if (longest(p->sequences, p->cache.page_size) + p->N + ma::kScaleBlock > 0x7fffffffLL) return invalid("positions would pass 2^31");
   ma::AppendArgs a{};
   int rc = check_cache(p->cache, p->sequences, p->E, p->H, p->N, p->dtype, &a.cache);
   if (rc != MA_B200_OK) return rc;
@@ -122,12 +123,12 @@ size_t ma_b200_cache_attend_workspace_bytes(const ma_b200_attend* p) {
 int ma_b200_cache_attend(const ma_b200_attend* p, void* workspace, size_t workspace_bytes, void* stream) {
   int rc = check_attend_shape(p);
   if (rc != MA_B200_OK) return rc;
+  if (p->window < 0 || (p->window > 0 && !p->causal)) return invalid("window must not be negative, and needs causal");
+  if (!isfinite(p->scale) || !(p->softcap == 0.0f || (p->softcap >= 1e-20f && p->softcap <= 1e30f)))
+    return invalid("scale must be finite, softcap 0 (none) or from 1e-20 to 1e30");
   ma::AttendArgs a{};
   if ((rc = check_cache(p->cache, p->sequences, p->E, p->H, p->N, p->dtype, &a.cache)) != MA_B200_OK) return rc;
   if ((rc = check_tensor(p->q, "q", 2, 16)) != MA_B200_OK || (rc = check_tensor(p->out, "out", 2, 16)) != MA_B200_OK) return rc;
-  if (p->window < 0 || (p->window > 0 && !p->causal)) return invalid("window must not be negative, and needs causal");
-  if (!isfinite(p->scale) || !(p->softcap == 0.0f || p->softcap >= 1e-20f) || !isfinite(p->softcap))
-    return invalid("scale and softcap must be finite, softcap 0 (none) or from 1e-20 on");
   const long long most = longest(p->sequences, p->cache.page_size);
   const size_t need = ma::attend_workspace(p->E, p->N, p->H, p->cache.heads, p->cache.width, p->window, most);
   if (workspace == nullptr || reinterpret_cast<uintptr_t>(workspace) % 256 != 0) return invalid("workspace is NULL or not 256-byte aligned");

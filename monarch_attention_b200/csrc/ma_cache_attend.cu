@@ -421,8 +421,7 @@ __global__ void __launch_bounds__(W * 32, Shape<D, NT, W>::kCtas) attend_kernel(
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             float x = s[mt][n][j] * (ks[mt] * (j & 1 ? rs.y : rs.x));
-            if (a.softcap > 0.0f)  // softcap * tanh(x / softcap): tanh y = 1 - 2 / (exp(2 y) + 1), off by 2^-23 of the cap at most
-              x = a.softcap * kLog2e * (1.0f - __fdividef(2.0f, ex2(x * (2.0f / a.softcap)) + 1.0f));
+            if (a.softcap > 0.0f) x = capped(x, a.softcap);
             s[mt][n][j] = x;
           }
         if (!whole) {
@@ -710,7 +709,10 @@ __global__ void __launch_bounds__(256) join_rows_kernel(const __grid_constant__ 
 }
 
 int row_tiles(int rows) { return rows <= 32 ? (rows + 7) / 8 : 4; }
-constexpr long long kPromptRows = 65;  // from as many rows on, the tcgen05 kernel
+// From as many rows on, the tcgen05 kernel.  us, it / this one, heads of 128 features: 64 sequences x 8 heads x 1024 tokens, 32 rows 116 / 74, 48 rows
+// 122 / 123, 64 rows 118 / 127, 80 rows 124 / 178; 8 x 8 x 2048, 48 rows 35.4 / 35.7, 64 rows 35.3 / 43.4; 1 x 8 x 32768, 32 rows 55 / 43, 64 rows
+// 55 / 61; 1 x 8 x 2048, 48 rows 22 / 16, 64 rows 21 / 20.
+constexpr long long kPromptRows = 49;
 
 // How a call is shared out.
 struct Plan {

@@ -218,13 +218,15 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
           for (int q = 0; q < 4; ++q) tmem_ld32_nowait(t_s + 32 * q, v[q]);
 #pragma unroll
           for (int q = 0; q < 4; ++q) tmem_wait_ld(v[q]);
-          auto f = [&](int j) { return a.softcap > 0.0f ? 1.0f : factor * b.k_scale[j]; };  // (scores in units of log2 e) = f * S
+          // (scores in units of log2 e) = f * S, and never zero: a mask is minus infinity times f, and rows of zeros, small keys and a small
+          // scale together leave 32 bits.  (S is 2^17 at most.)
+          auto f = [&](int j) { return a.softcap > 0.0f ? 1.0f : fmaxf(factor * b.k_scale[j], 1e-37f); };
           if (a.softcap > 0.0f) {
 #pragma unroll
             for (int q = 0; q < 4; ++q)
 #pragma unroll
               for (int j = 0; j < 32; ++j)
-                v[q][j] = a.softcap * kLog2e * (1.0f - __fdividef(2.0f, ex2(v[q][j] * factor * b.k_scale[2 * q + j / 16] * (2.0f / a.softcap)) + 1.0f));
+                v[q][j] = capped(v[q][j] * (factor * b.k_scale[2 * q + j / 16]), a.softcap);
           }
           if (t0 < low || t0 + kKeys > high) {
 #pragma unroll
@@ -488,7 +490,6 @@ cudaError_t launch_prompt(AttendArgs a, int dtype, int width, void* workspace, l
   a.row_blocks = (a.group * a.N + kRows - 1) / kRows;
   const long long units = (long long)a.E * a.cache.heads * a.row_blocks;
   PromptArgs args{a, prompt_pieces(a.E, a.N, a.H, a.cache.heads, longest), wait_status};
-  if (a.scale == 0.0f) args.a.scale = 1e-30f;  // (a mask is minus infinity times the factor)
   char* at = reinterpret_cast<char*>(workspace);
   args.a.split = reinterpret_cast<int4*>(at);
   args.a.part_o = reinterpret_cast<float*>(at + ((size_t)units * sizeof(int4) + 255) / 256 * 256);

@@ -272,6 +272,11 @@ Tensor attend(const Tensor& q_in, const Cache& cache, const Tensor& table, const
     out = token_major ? at::detail::empty_strided_cuda({E, H, N, W}, {N * H * W, W, H * W, 1}, o) : at::detail::empty_cuda({E, H, N, W}, o);
   }
   if (E == 0 || N == 0) return out;
+  if (out_in.has_value()) {
+    // (the query itself may take the result: a row is read by those that write it, before they do)
+    TORCH_CHECK_VALUE(at::get_overlap_status(out, q_in) != at::MemOverlapStatus::Partial, "out and query overlap in part");
+    if (!out.is_inference()) out.unsafeGetTensorImpl()->bump_version();
+  }
   const Tensor q = aligned(q_in, 16);
   p.E = (int32_t)E; p.H = (int32_t)H; p.N = (int32_t)N;
   p.dtype = dtype_code(q.scalar_type());

@@ -71,7 +71,7 @@ def append_kv_b200(cache: PagedKV, key: Tensor, value: Tensor, page_table: Tenso
     rotated copy is returned, with rows of padding as zeros.  A block's scale is the smallest power of two from 2^-40 to 2^60 with which 448 holds the
     block's largest magnitude.  It never falls while the block has older tokens; when it rises they are re-expressed, which is exact but for
     values that become subnormal.  Magnitudes above 448 * 2^60 (infinities) are stored as that, NaN as NaN.  The pages that a call writes to
-    must belong to one sequence each (pages that are only read may be shared).  No gradient: inputs that require one are refused.
+    must stand once in one sequence's row of the table (pages that are only read may be shared).  No gradient: inputs that require one are refused.
     """
     if _append is None:
         _load()
@@ -87,12 +87,12 @@ def cached_attention_b200(query: Tensor, cache: PagedKV, page_table: Tensor, len
 
     Query head ``h`` reads cache head ``h // (H / heads)``.  ``causal``: a token sees the positions up to its own (the call's tokens have been
     appended before); else all ``lengths`` (an encoder's output).  ``window`` > 0 (causal only): the last ``window`` of those.  Scores are
-    multiplied by ``scale`` (None: ``width ** -0.5``) and, with ``softcap`` > 0, become ``softcap * tanh(score / softcap)``.  Rows without
+    multiplied by ``scale`` (None: ``width ** -0.5``) and, with ``softcap`` > 0 (from 1e-20 to 1e30), become ``softcap * tanh(score / softcap)``.  Rows without
     a key, and rows of padding, are zero.  What lies in the cache behind a sequence's end is never looked at, NaN included; a NaN that was appended as a value reaches
     all of the call's rows of its sequence and head, masked ones too (zero times NaN).
 
     The result has the query's dtype, and with ``token_major_output`` is a view of an (E, N, H, width) buffer; ``out`` (rows on 16-byte
-    boundaries) takes it in place.  Scores and sums are in 32 bits; a bfloat16 query is read in 16-bit steps of 2^-11 of itself and 2^-25 of
+    boundaries; the query itself is fine) takes it in place.  Scores and sums are in 32 bits; a bfloat16 query is read in 16-bit steps of 2^-11 of itself and 2^-25 of
     its row's largest magnitude, weights are rounded to 2^-12 of themselves.  The same call gives the same bits; what else is in the batch may
     change the order of a sequence's sums.  No gradient: inputs that require one are refused.
     """

@@ -440,3 +440,66 @@ def test_the_rows_of_out_do_not_overlap():
         ma.cached_attention_b200(q, cache, table, lengths, out=torch.zeros(1, 4, 1, 64, dtype=BF, device="cuda").expand(2, -1, -1, -1))
     with pytest.raises(ValueError):
         ma.cached_attention_b200(q, cache, table, lengths, softcap=1e-30)
+
+
+@pytest.mark.parametrize("N", [1, 9, 40])
+@pytest.mark.parametrize("cap", [1e4, 1e6, 1e30])
+def test_caps_far_above_the_scores(cap, N):
+    """A cap that no score comes near leaves them as they are: its error is a part of the score, not of the cap.
+
+    Scores of s lose s^3 / (3 cap^2), 10^-5 at most, and 2^-18 of themselves in the capping; the bound without a cap has D 2^-24 of the sum of
+    magnitudes, which is more than that, twice."""
+    import monarch_attention_b200 as ma
+    lengths = [500, 40]
+    cache, table = filled(2, 9, 2, 128, 64, lengths)
+    q = queries(2, 8, N, 128, BF, "heads")
+    out = ma.cached_attention_b200(q, cache, table, torch.tensor(lengths, dtype=torch.int32, device="cuda"), softcap=cap)
+    for e, L in enumerate(lengths):
+        k, v = held(cache.k, cache.k_scale, table[e], L, 64), held(cache.v, cache.v_scale, table[e], L, 64)
+        want, bound = attention(q[e], k, v, L - N, True, 128 ** -0.5)
+        close(out[e], want, 2 * bound + 2.0 ** -8 * (want.abs() + 2 * bound), f"cap {cap}")
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("scale", [0.0, 1e-30, 1e-4, -1e-4])
+def test_rows_of_zeros_over_keys_of_zeros(scale, D):
+    """Many rows, some of zeros and some of padding, over blocks of keys of zeros (the smallest scale of all): a mask stays a mask."""
+    import monarch_attention_b200 as ma
+    lengths, counts, N, page = [200, 90], [40, 33], 40, 32
+    table = torch.arange(16, dtype=torch.int32, device="cuda").view(2, 8)
+    dev = [torch.tensor(x, dtype=torch.int32, device="cuda") for x in (lengths, counts)]
+    cache = ma.PagedKV.allocate(16, 2, D, page)
+    k, v, q = (queries(2, h, n, D, BF, "heads", seed=s) for s, h, n in ((1, 2, 200), (2, 2, 200), (3, 8, N)))
+    k[:, :, 16:100] = 0
+    q[:, :, ::3] = 0
+    ma.append_kv_b200(cache, k, v, table, dev[0], dev[0])
+    out = ma.cached_attention_b200(q, cache, table, *dev, scale=scale)
+    check(out, q, cache, table, lengths, counts, page, scale=scale)
+
+
+@pytest.mark.parametrize("G,N,L", [(4, 1, 9000), (8, 6, 300), (4, 80, 3000)])
+def test_the_result_in_the_querys_place(G, N, L):
+    import monarch_attention_b200 as ma
+    cache, table = filled(2, L // 64 + 1, 2, 64, 64, [L, L // 2])
+    lengths = torch.tensor([L, L // 2], dtype=torch.int32, device="cuda")
+    q = queries(2, 2 * G, N, 64, BF, "tokens")
+    want = ma.cached_attention_b200(q, cache, table, lengths)
+    buffer = torch.zeros(q.numel() + 64, device="cuda", dtype=BF)
+    shifted = [buffer[i:i + q.numel()].view(2, 2 * G, N, 64) for i in (0, 64)]
+    with pytest.raises(ValueError):  # rows would be overwritten before others read them
+        ma.cached_attention_b200(shifted[0], cache, table, lengths, out=shifted[1])
+    assert ma.cached_attention_b200(q, cache, table, lengths, out=q) is not None and torch.equal(q, want)
+
+
+def test_a_result_over_what_a_backward_pass_needs_is_noticed():
+    import monarch_attention_b200 as ma
+    cache, table = filled(1, 2, 1, 64, 64, [100])
+    q, w = queries(1, 1, 1, 64, BF, "heads"), torch.ones(1, 1, 1, 64, device="cuda", dtype=BF, requires_grad=True)
+    saved = torch.zeros_like(q)
+    y = (w * saved).sum()
+    with torch.no_grad():
+        ma.cached_attention_b200(q, cache, table, torch.tensor([100], dtype=torch.int32, device="cuda"), out=saved)
+    with pytest.raises(RuntimeError, match="modified by an inplace"):
+        y.backward()
+    with torch.inference_mode():
+        ma.cached_attention_b200(q, cache, table, torch.tensor([100], dtype=torch.int32, device="cuda"), out=torch.zeros_like(q))

@@ -170,3 +170,14 @@ def test_attention_scratch_is_host_arithmetic(lib):
 def test_status_of_a_device_that_had_no_call(lib):
     assert lib.ma_b200_poll_cache_status(0) == _cabi.OK and lib.ma_b200_poll_cache_status(-1) == _cabi.OK
     assert b"page" in lib.ma_b200_status_string(_cabi.DEVICE_BAD_SEQUENCE)
+
+
+def test_positions_stay_below_2_to_the_31(lib):
+    a = _cabi.Append(_cabi.ABI_VERSION, 1, 0, 1000, _cabi.BF16)
+    a.k, a.v, a.cache, a.sequences = tensor(), tensor(), cache_struct(), sequences(table_pages=2 ** 26)
+    assert lib.ma_b200_cache_append(C.byref(a), None) == _cabi.INVALID_ARGUMENT and b"2^31" in lib.ma_b200_last_error()
+
+
+@pytest.mark.parametrize("softcap", [-1.0, 1e-30, 1e31, float("inf"), float("nan")])
+def test_caps_that_leave_32_bits(lib, softcap):
+    assert lib.ma_b200_cache_attend(C.byref(attend(softcap=softcap)), 1 << 20, 1 << 60, None) == _cabi.INVALID_ARGUMENT
