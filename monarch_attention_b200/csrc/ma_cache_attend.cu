@@ -42,7 +42,7 @@ struct Shape {
   static constexpr int kRing = W * kStages * kStageBytes;
   static constexpr int kOperandBytes = kSharedRows ? kRows * D * 2 : 0;
   static constexpr int kSmem = kRing + kOperandBytes;
-  static constexpr int kCtas = W > 4 ? 1 : NT > 2 ? 2 : 3;  // of an SM: what registers and shared memory allow
+  static constexpr int kCtas = W > 4 ? 1 : NT > 2 ? 2 : D == 64 && NT == 1 ? 4 : 3;  // of an SM: what registers and shared memory allow
 };
 
 // Byte offset of 16-byte piece `piece` of token t in a slice: pieces are permuted so that neither the reads of the keys (8 rows x 4 pieces)
@@ -720,7 +720,7 @@ struct Plan {
   bool whole;       // heads are not split, and there is nothing to join
   long long grid;
 };
-Plan plan_of(int E, int N, int H, int kv_heads, int window, long long longest) {
+Plan plan_of(int E, int N, int H, int kv_heads, int width, int window, long long longest) {
   const int rows = H / kv_heads * N;
   const long long looked_at = (long long)window + N + kScaleBlock;  // keys of a sequence, at most
   if (window > 0 && longest > looked_at) longest = looked_at;
@@ -737,9 +737,13 @@ Plan plan_of(int E, int N, int H, int kv_heads, int window, long long longest) {
   // us, whole / split, 12 heads of 64: 500 tokens 7.4 / 9.1, 1000 10.5 / 9.5, 2000 16.1 / 9.9; 96 heads: 1000 10.6 / 13.6, 2000 16.2 / 16.5; 144
   // heads, 2000 16.5 / 19.7; 128 heads of 128 features, 2000 22.9 / 23.0, 4000 40.5 / 37.2.
   if (units <= sm_count() && longest <= (2 * units >= sm_count() ? 2048 : 768)) return {nt, 8, true, units};
-  const long long most = (nt > 2 ? Shape<128, 4, 4>::kCtas : Shape<128, 1, 4>::kCtas) * (long long)sm_count();
   const bool whole = longest <= 4 * kStep;
   const long long steps = whole ? units : units * ((longest + kStep - 1) / kStep);
+  // Rows of 64 features and one tile leave room for a fourth CTA of an SM, where it has some steps.  us, four / three: 32 sequences x 8 heads of 16384
+  // tokens 117.6 / 122.3, of 8192 65.4 / 67.3, of 2048 24.6 / 25.3, of 1024 18.3 / 17.8; 2 heads of 131071 19.1 / 17.2.
+  constexpr int kFour = Shape<64, 1, 4>::kCtas, kThree = Shape<128, 1, 4>::kCtas;
+  const int per_sm = nt > 2 ? Shape<128, 4, 4>::kCtas : width == 64 && nt == 1 && steps >= 6LL * kFour * sm_count() ? kFour : kThree;
+  const long long most = per_sm * (long long)sm_count();
   return {nt, 4, whole, steps < most ? steps : most};
 }
 
@@ -782,7 +786,7 @@ cudaError_t launch_join(const AttendArgs& a, int dtype, int width, int tile_rows
 
 size_t attend_workspace(int E, int N, int H, int kv_heads, int width, int window, long long longest) {
   if (H / kv_heads * (long long)N >= kPromptRows) return prompt_workspace(E, N, H, kv_heads, width, longest);
-  const Plan plan = plan_of(E, N, H, kv_heads, window, longest);
+  const Plan plan = plan_of(E, N, H, kv_heads, width, window, longest);
   if (plan.whole) return 256;
   const size_t entries = ((size_t)plan.grid * sizeof(int4) + 255) / 256 * 256;
   return entries + (size_t)plan.grid * 2 * 8 * plan.nt * (width + 2) * sizeof(float);
@@ -792,7 +796,7 @@ cudaError_t launch_attend(AttendArgs a, int dtype, int width, void* workspace, l
   const long long strides[6] = {a.cache.k_sp, a.cache.k_sh, a.cache.k_st, a.cache.v_sp, a.cache.v_sh, a.cache.v_st};
   for (int i = 0; i < 6; ++i) (i < 3 ? a.k16[i] : a.v16[i - 3]) = (uint32_t)(strides[i] / 16);
   if (a.group * (long long)a.N >= kPromptRows) return launch_prompt(a, dtype, width, workspace, longest, wait_status, stream);
-  const Plan plan = plan_of(a.E, a.N, a.H, a.cache.heads, a.window, longest);
+  const Plan plan = plan_of(a.E, a.N, a.H, a.cache.heads, width, a.window, longest);
   const int tile_rows = 8 * plan.nt;
   a.row_blocks = (a.group * a.N + tile_rows - 1) / tile_rows;
   char* at = reinterpret_cast<char*>(workspace);
