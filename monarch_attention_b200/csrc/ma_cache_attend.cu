@@ -31,11 +31,12 @@ using sm100::smem_u32;
 
 constexpr float kSlack = 8.0f;  // weights are at most 2^8 of the reference: f16 holds them as exactly as those up to 1
 constexpr int kSlice = 32;  // tokens of a warp at a time
+constexpr int kWide = 12;   // warps of a CTA that has an SM to itself: as many as fit in with two tiles of rows
 
 template <int D, int NT, int W>
 struct Shape {
   static constexpr int kStep = W * kSlice;  // tokens of a CTA at a time
-  static constexpr int kStages = W == 4 ? (D == 128 ? 2 : 3) : (D == 128 ? 3 : 4);
+  static constexpr int kStages = D == 128 ? 2 : W == 4 ? 3 : 4;
   static constexpr int kStageBytes = 2 * kSlice * D + 16;  // keys, values and their two scales each
   static constexpr int kRows = 8 * NT;
   static constexpr bool kSharedRows = NT > 1;  // the query rows' operands are in shared memory: there are no registers for them
@@ -733,10 +734,10 @@ Plan plan_of(int E, int N, int H, int kv_heads, int width, int window, long long
   if (nt > 2 && (long long)E * kv_heads * ((rows + 8 * nt - 1) / (8 * nt)) * ((longest + kStep - 1) / kStep) <= 16LL * sm_count()) nt = 2;
   const long long units = (long long)E * kv_heads * ((rows + 8 * nt - 1) / (8 * nt));
   // A head of a few steps stays with one CTA: a second kernel costs 3 to 4 us.  Where there are no more heads than SMs, each has a CTA of
-  // eight warps and steps of 256 tokens, of 1.5 (64 features) to 2.3 us; with half as many heads or more the SMs are busy either way.
-  // us, whole / split, 12 heads of 64: 500 tokens 7.4 / 9.1, 1000 10.5 / 9.5, 2000 16.1 / 9.9; 96 heads: 1000 10.6 / 13.6, 2000 16.2 / 16.5; 144
-  // heads, 2000 16.5 / 19.7; 128 heads of 128 features, 2000 22.9 / 23.0, 4000 40.5 / 37.2.
-  if (units <= sm_count() && longest <= (2 * units >= sm_count() ? 2048 : 768)) return {nt, 8, true, units};
+  // twelve warps and steps of 384 tokens, 1.8 (64 features) to 3 us; the more of the SMs are busy that way, the longer it pays.
+  // us, whole / split, 64 features: 12 heads of 600 tokens 8.0 / 9.5; 84 heads, 1400 11.4 / 13.5, 2000 14.7 / 14.8, 2800 18.8 / 17.7; 144 heads, 1400
+  // 11.6 / 17.1, 4000 23.7 / 26.5; 128 features: 8 heads, 600 10.1 / 10.5, 800 12.6 / 10.4; 64 heads, 1400 15.9 / 18.6; 128 heads, 2800 26.2 / 27.7.
+  if (nt <= 2 && units <= sm_count() && (longest <= 768 || longest * sm_count() <= 4352 * units)) return {nt, kWide, true, units};
   const bool whole = longest <= 4 * kStep;
   const long long steps = whole ? units : units * ((longest + kStep - 1) / kStep);
   // Rows of 64 features and one tile leave room for a fourth CTA of an SM, where it has some steps.  us, four / three: 32 sequences x 8 heads of 16384
@@ -766,9 +767,7 @@ cudaError_t launch(AttendArgs& a, const Plan& plan, cudaStream_t stream) {
 }
 template <typename T, int D>
 cudaError_t launch_rows(AttendArgs& a, const Plan& plan, cudaStream_t stream) {
-  if (plan.warps == 8)
-    return plan.nt == 1 ? launch<T, D, 1, 8>(a, plan, stream) : plan.nt == 2 ? launch<T, D, 2, 8>(a, plan, stream) :
-           plan.nt == 3 ? launch<T, D, 3, 8>(a, plan, stream) : launch<T, D, 4, 8>(a, plan, stream);
+  if (plan.warps == kWide) return plan.nt == 1 ? launch<T, D, 1, kWide>(a, plan, stream) : launch<T, D, 2, kWide>(a, plan, stream);
   return plan.nt == 1 ? launch<T, D, 1, 4>(a, plan, stream) : plan.nt == 2 ? launch<T, D, 2, 4>(a, plan, stream) :
          plan.nt == 3 ? launch<T, D, 3, 4>(a, plan, stream) : launch<T, D, 4, 4>(a, plan, stream);
 }

@@ -503,3 +503,14 @@ def test_a_result_over_what_a_backward_pass_needs_is_noticed():
         y.backward()
     with torch.inference_mode():
         ma.cached_attention_b200(q, cache, table, torch.tensor([100], dtype=torch.int32, device="cuda"), out=torch.zeros_like(q))
+
+
+@pytest.mark.parametrize("E,H,Hk,N,D,dtype", [(12, 12, 12, 1, 64, BF), (16, 32, 8, 1, 128, HF), (18, 32, 8, 3, 128, BF), (70, 8, 2, 4, 64, HF)])
+def test_heads_that_nearly_fill_the_device(E, H, Hk, N, D, dtype):
+    """As many heads as SMs or fewer, of some thousand tokens at most: none is split, and a CTA has twelve warps' slices of several steps."""
+    import monarch_attention_b200 as ma
+    lengths = [(211 * e + 3) % 2100 + N for e in range(E)]
+    cache, table = filled(E, 35, Hk, D, 64, lengths)
+    q = queries(E, H, N, D, dtype, "heads")
+    out = ma.cached_attention_b200(q, cache, table, torch.tensor(lengths, dtype=torch.int32, device="cuda"))
+    check(out, q, cache, table, lengths, None, 64)
