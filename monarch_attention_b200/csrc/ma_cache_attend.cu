@@ -14,7 +14,10 @@
 //    weights change sides by an 8 x 8 transpose between lanes.
 //  * e4m3 is exact in f16, so the products are f16 with 32-bit sums whatever the queries' type; a bf16 row is scaled by a power of two to
 //    magnitudes of 1 to 2 first (exact but for elements 2^-23 below the row's largest).  A block's key scale multiplies its scores; its value
-//    scale goes into the weights, and the running maximum is taken over weight times scale, so that f16 weights are at most 1.
+//    scale goes into the weights, and the running maximum is taken over weight times scale, so that f16 weights are at most 2^kSlack.
+// Measured, a token each: 32 sequences of up to 8192 tokens, 8 heads of 128 features, 270 MB in 59 us; every further byte comes at 6.3 TB/s, 96 %
+// of a copy (64 features: 4.9, the bytes' conversion and the weights bind), and some 12 us go to the start, the unequal finish of the CTAs and the
+// join.  One sequence of 131071 tokens and 2 heads, 67 MB in 23 us; of 500 tokens and 12 heads of 64 features 7.4 us.
 #include <math_constants.h>
 
 #include <type_traits>

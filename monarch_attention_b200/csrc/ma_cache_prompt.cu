@@ -11,6 +11,9 @@
 //    scores, the values' to the weights, with a reference that is raised (and O multiplied) only when a weight would pass 2^8.
 //  * One warp issues the products: O += P V, the weights P read from tensor memory, where they have taken the place of their scores, and
 //    the next step's scores S = Q K^T.  While one tile's rows are exponentiated the other's products run.
+// Measured: 1024 tokens of 2 sequences over 16384 keys, 4 heads of 128 features, 305 us, 870 TFLOP/s, 53 % of a library product; 64 features 490.  No
+// unit is busy for half of the 4500 cycles of a step: the row warps' 2400 and the two products behind them follow one another, twice a step.
+// Slower were: two threads a row (343 us), scores of 64 keys in two buffers (358), scores loaded a quarter at a time (347).
 // Every wait is bounded; one that gives up ends the CTA's others, and the next call on the device reports it.
 #include <math_constants.h>
 
@@ -70,7 +73,7 @@ __device__ __forceinline__ uint32_t widen2_upper(uint32_t codes) {
 }
 // 2^x on the multipliers, for x up to 2^7: the special function units are what the weights wait for.  x = n + f with f in [-1/2, 1/2], 2^f by a
 // polynomial of degree 5 (minimax in the relative error, 2^-23.6; found by exchange), n added to the exponent.
-constexpr int kByProducts = 1;  // of 4 pairs of weights, these
+constexpr int kByProducts = 1;  // of 4 pairs of weights, these (us of 16384 keys: none 325, one 303, two 344)
 __device__ __forceinline__ float2 exp2_by_products(float2 x) {
   x = make_float2(fmaxf(x.x, -126.0f), fmaxf(x.y, -126.0f));
   const float2 round = make_float2(12582912.0f, 12582912.0f);  // 1.5 * 2^23: its last bits are n
