@@ -3,7 +3,7 @@
 // Bound by the tensor cores and by the exponentials (as many cycles at 128 features: 2 x 256 x 128 x 128 x 2 operations of a step are 2048 cycles,
 // its 256 x 128 exponentials 2048 of the special function units).  A CTA takes 256 rows (tokens times heads of a group) of a key head and
 // walks over its keys, 128 at a step:
-//  * Eight warps bring keys and values: bytes from global memory into registers, half a step ahead, and from there, widened to f16 (exact),
+//  * Four warps bring keys and values: bytes from global memory into registers, half a step ahead, and from there, widened to f16 (exact),
 //    into swizzled tiles in shared memory.  Two tiles of rows share them, so that the conversion and the shared memory's traffic, which a
 //    single tile would be bound by, count half.
 //  * Two warpgroups have a row a thread: the row's 128 scores go from tensor memory to registers in one go, and the maximum, the weights and
@@ -11,9 +11,11 @@
 //    scores, the values' to the weights, with a reference that is raised (and O multiplied) only when a weight would pass 2^8.
 //  * One warp issues the products: O += P V, the weights P read from tensor memory, where they have taken the place of their scores, and
 //    the next step's scores S = Q K^T.  While one tile's rows are exponentiated the other's products run.
-// Measured: 1024 tokens of 2 sequences over 16384 keys, 4 heads of 128 features, 305 us, 870 TFLOP/s, 53 % of a library product; 64 features 490.  No
-// unit is busy for half of the 4500 cycles of a step: the row warps' 2400 and the two products behind them follow one another, twice a step.
-// Slower were: two threads a row (343 us), scores of 64 keys in two buffers (358), scores loaded a quarter at a time (347).
+// Measured: 1024 tokens of 2 sequences over 16384 keys, 4 heads of 128 features, 288 us, 920 TFLOP/s, 56 % of a library product; 64 features 505.  A
+// step takes 4300 cycles, of which the row warps' weights are 2300 a tile: without any exponential they would take 80 % of the time, without the
+// conversion of keys and values all of it, and with scores that never wait for the products of the step before (64 features leave the room) 99 %.
+// Slower were (beside 304 us): two threads a row 343, scores of 64 keys in two buffers 358, scores loaded a quarter at a time 347; eight warps that
+// bring keys and values, which leave the rows 160 registers each, took the 304.
 // Every wait is bounded; one that gives up ends the CTA's others, and the next call on the device reports it.
 #include <math_constants.h>
 
@@ -28,9 +30,9 @@ namespace {
 using namespace sm100;
 
 constexpr int kKeys = 128, kTileRows = 128, kRows = 2 * kTileRows;
-constexpr int kThreads = 640, kBringers = 256;  // warps 0-3, 4-7: rows; 8-15: keys and values; 16: products (17-19 make it a warpgroup)
-constexpr int kLaunchRegs = 96, kRowRegs = 160, kBringerRegs = 56, kIssuerRegs = 40;
-static_assert(256 * (kRowRegs + kBringerRegs) + 128 * kIssuerRegs <= kThreads * kLaunchRegs, "setmaxnreg draws on the launch's registers");
+constexpr int kThreads = 512, kBringers = 128;  // warps 0-3, 4-7: rows; 8-11: keys and values; 12: products (13-15 make it a warpgroup)
+constexpr int kLaunchRegs = 128, kRowRegs = 184, kBringerRegs = 104, kIssuerRegs = 40;
+static_assert(256 * kRowRegs + kBringers * kBringerRegs + 128 * kIssuerRegs <= kThreads * kLaunchRegs, "setmaxnreg draws on the launch's registers");
 constexpr int kRing = 8;  // steps whose pages and scales are kept
 constexpr float kSlack = 8.0f;
 
@@ -73,7 +75,7 @@ __device__ __forceinline__ uint32_t widen2_upper(uint32_t codes) {
 }
 // 2^x on the multipliers, for x up to 2^7: the special function units are what the weights wait for.  x = n + f with f in [-1/2, 1/2], 2^f by a
 // polynomial of degree 5 (minimax in the relative error, 2^-23.6; found by exchange), n added to the exponent.
-constexpr int kByProducts = 1;  // of 4 pairs of weights, these (us of 16384 keys: none 325, one 303, two 344)
+constexpr int kByProducts = 1;  // of 4 pairs of weights, these (us of 16384 keys: none 295, one 288, two 320)
 __device__ __forceinline__ float2 exp2_by_products(float2 x) {
   x = make_float2(fmaxf(x.x, -126.0f), fmaxf(x.y, -126.0f));
   const float2 round = make_float2(12582912.0f, 12582912.0f);  // 1.5 * 2^23: its last bits are n
@@ -146,7 +148,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  if (warp == 16) {
+  if (warp == 12) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(base + L::kFlags + 4), "r"(512) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
@@ -323,7 +325,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
     }
     if (args.pieces > 1 && tid == 0 && piece == 0)
       a.split[unit] = make_int4((e * c.heads + head) * a.row_blocks + block, unit * args.pieces, (unit + 1) * args.pieces - 1, 0);
-  } else if (warp < 16) {
+  } else if (warp < 12) {
     // =========================== keys and values =====================================================================
     regs_dec<kBringerRegs>();
     const int t = tid - 256, page_mask = (1 << c.page_shift) - 1;
@@ -357,17 +359,17 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
       page_next = page_at(2);
     }
     meet();
-    // A thread has a 16-byte piece of 4 in each panel of rows t / 4 and t / 4 + 64: eight threads write 4 pieces of two rows, an even and an
+    // A thread has a 16-byte piece of 4 in each panel of rows t / 4 + 32 j: eight threads write 4 pieces of two rows, an even and an
     // odd one, whose chunks the swizzle puts on different banks.
     constexpr int kPanels = D / 64;
-    uint4 raw[2][2][kPanels];  // keys and values on their way
+    uint4 raw[2][4][kPanels];  // keys and values on their way
     auto load = [&](int which, int i) {
       const uint8_t* const all = which ? c.v : c.k;
       const uint32_t sp = which ? a.v16[0] : a.k16[0], sh = which ? a.v16[1] : a.k16[1], st = which ? a.v16[2] : a.k16[2];
       const Blocks& b = blocks[i & (kRing - 1)];
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const int row = (t >> 2) + 64 * j, token = lo + i * kKeys + row, page = b.page[which][row / kScaleBlock];
+      for (int j = 0; j < 4; ++j) {
+        const int row = (t >> 2) + 32 * j, token = lo + i * kKeys + row, page = b.page[which][row / kScaleBlock];
         const uint8_t* const src = all + 16 * ((uint32_t)page * (uint64_t)sp + (uint32_t)head * (uint64_t)sh + (uint32_t)(token & page_mask) * (uint64_t)st + (t & 3));
 #pragma unroll
         for (int x = 0; x < kPanels; ++x)
@@ -376,9 +378,9 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
     };
     auto put = [&](int which, uint32_t to) {
 #pragma unroll
-      for (int j = 0; j < 2; ++j)
+      for (int j = 0; j < 4; ++j)
 #pragma unroll
-        for (int x = 0; x < kPanels; ++x) put_codes(to + x * kPanel, (t >> 2) + 64 * j, 2 * (t & 3), raw[which][j][x]);
+        for (int x = 0; x < kPanels; ++x) put_codes(to + x * kPanel, (t >> 2) + 32 * j, 2 * (t & 3), raw[which][j][x]);
       fence_async_smem();
     };
     if (steps > 0) {
@@ -416,7 +418,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
   } else {
     regs_dec<kIssuerRegs>();
   }
-  if (warp == 16) {
+  if (warp == 12) {
     // =========================== products ============================================================================
     constexpr uint32_t kScores = instr_desc(0, 0, 0, kKeys, kTileRows), kSums = instr_desc(0, 0, 1, D, kTileRows);
     constexpr uint32_t kTileUnits = L::kTileBytes >> 4, kPanelUnits = kPanel >> 4;
@@ -469,7 +471,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
   tc_fence_before();
   __syncthreads();
   if (tid == 0 && *abort_flag != 0 && args.wait_status != nullptr) *reinterpret_cast<volatile int*>(args.wait_status) = 800;
-  if (warp == 16) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+  if (warp == 12) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
 }
 
 }  // namespace
