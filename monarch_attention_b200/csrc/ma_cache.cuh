@@ -77,6 +77,9 @@ struct AttendArgs {
   int split_by_head;        // (1) a head and block of rows
   int whole_heads;          // 1: no head is split
 };
+// Whether a row of the call's token n has a key at all; the others' results are zero, whatever the sums of their tile have caught.
+__device__ __forceinline__ bool sees_keys(const AttendArgs& a, int len, int count, int n) { return n < count && (!a.causal || len - count + n >= 0); }
+
 // Bytes of scratch, and how many row tiles and CTAs the call takes.
 size_t attend_workspace(int E, int N, int H, int kv_heads, int width, int window, long long longest);
 cudaError_t launch_attend(AttendArgs a, int dtype, int width, void* workspace, long long longest, int* wait_status, cudaStream_t stream);

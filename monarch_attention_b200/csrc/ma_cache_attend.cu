@@ -558,7 +558,11 @@ __global__ void __launch_bounds__(W * 32, Shape<D, NT, W>::kCtas) attend_kernel(
           for (int v = 0; v < W; ++v) all += tops[v][r].y * ex2(tops[v][r].x - base);
           if (alone) {
             const int token = (row0 + r) / a.group, h = now.head * a.group + row0 + r - token * a.group;
-            const float inverse = token < now.s.count && all > 0.0f ? 1.0f / all : 0.0f;
+            const float inverse = all > 0.0f ? 1.0f / all : 0.0f;
+            if (!sees_keys(a, now.s.len, now.s.count, token)) {
+#pragma unroll
+              for (int f = 0; f < kRun; ++f) x[f] = 0.0f;
+            }
             T* dst = reinterpret_cast<T*>(const_cast<void*>(a.out.ptr)) + now.e * a.out.se + h * a.out.sh + token * a.out.sn + u * kRun;
             if constexpr (D == 128)
               *reinterpret_cast<uint4*>(dst) = make_uint4(sm100::pack2<T>(x[0] * inverse, x[1] * inverse), sm100::pack2<T>(x[2] * inverse, x[3] * inverse),
@@ -654,7 +658,8 @@ __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ Atten
   }
   int len, count;
   sequence_of(a.cache, e, a.N, &len, &count);
-  const float inverse = token < count && total > 0.0f ? 1.0f / total : 0.0f;
+  const float inverse = total > 0.0f ? 1.0f / total : 0.0f;
+  if (!sees_keys(a, len, count, token)) acc = make_float4(0, 0, 0, 0);
   T* dst = reinterpret_cast<T*>(const_cast<void*>(a.out.ptr)) + e * a.out.se + h * a.out.sh + token * a.out.sn + blockIdx.z * W + lane * 4;
   *reinterpret_cast<uint2*>(dst) = make_uint2(sm100::pack2<T>(acc.x * inverse, acc.y * inverse), sm100::pack2<T>(acc.z * inverse, acc.w * inverse));
 }
@@ -704,7 +709,11 @@ __global__ void __launch_bounds__(256) join_rows_kernel(const __grid_constant__ 
   }
   int len, count;
   sequence_of(a.cache, e, a.N, &len, &count);
-  const float inverse = token < count && total > 0.0f ? 1.0f / total : 0.0f;
+  const float inverse = total > 0.0f ? 1.0f / total : 0.0f;
+  if (!sees_keys(a, len, count, token)) {
+#pragma unroll
+    for (int f = 0; f < kRun; ++f) acc[f] = 0.0f;
+  }
   T* dst = reinterpret_cast<T*>(const_cast<void*>(a.out.ptr)) + e * a.out.se + h * a.out.sh + token * a.out.sn + lane * kRun;
   if constexpr (kRun == 4)
     *reinterpret_cast<uint2*>(dst) = make_uint2(sm100::pack2<T>(acc[0] * inverse, acc[1] * inverse), sm100::pack2<T>(acc[2] * inverse, acc[3] * inverse));
@@ -712,11 +721,10 @@ __global__ void __launch_bounds__(256) join_rows_kernel(const __grid_constant__ 
     *reinterpret_cast<uint32_t*>(dst) = sm100::pack2<T>(acc[0] * inverse, acc[1] * inverse);
 }
 
-int row_tiles(int rows) { return rows <= 32 ? (rows + 7) / 8 : 4; }
-// From as many rows on, the tcgen05 kernel.  us, it / this one, heads of 128 features: 64 sequences x 8 heads x 1024 tokens, 32 rows 116 / 74, 48 rows
-// 122 / 123, 64 rows 118 / 127, 80 rows 124 / 178; 8 x 8 x 2048, 48 rows 35.4 / 35.7, 64 rows 35.3 / 43.4; 1 x 8 x 32768, 32 rows 55 / 43, 64 rows
-// 55 / 61; 1 x 8 x 2048, 48 rows 22 / 16, 64 rows 21 / 20.
-constexpr long long kPromptRows = 49;
+// From as many rows on, the tcgen05 kernel.  us, it / this one, heads of 128 features: 64 sequences x 8 heads x 1024 tokens, 32 rows 96 / 74, 48 rows
+// 97 / 122, 80 rows 99 / 177; 8 x 8 x 2048, 32 rows 28 / 25, 48 rows 29 / 35; 1 x 8 x 32768, 32 rows 44 / 42, 48 rows 45 / 59; 1 x 8 x 2048, 32 rows
+// 18 / 16, 48 rows 19 / 16, 80 rows 20 / 20.
+constexpr long long kPromptRows = 33;
 
 // How a call is shared out.
 struct Plan {
@@ -733,7 +741,7 @@ Plan plan_of(int E, int N, int H, int kv_heads, int width, int window, long long
   // anyway, two blocks of rows that both read the keys are done sooner.  us, with as many tiles as there are rows / two: 16 sequences
   // of 20 rows x 4 heads, window 1024, 20.7 / 17.3, of 32 rows and up to 4096 tokens 38.3 / 34.6; 32 of 32 rows and up to 8000 82 / 86, one of
   // 20 rows and 131000 tokens 32 / 43.
-  int nt = row_tiles(rows);
+  int nt = (rows + 7) / 8;
   if (nt > 2 && (long long)E * kv_heads * ((rows + 8 * nt - 1) / (8 * nt)) * ((longest + kStep - 1) / kStep) <= 16LL * sm_count()) nt = 2;
   const long long units = (long long)E * kv_heads * ((rows + 8 * nt - 1) / (8 * nt));
   // A head of a few steps stays with one CTA: a second kernel costs 3 to 4 us.  Where there are no more heads than SMs, each has a CTA of

@@ -11,8 +11,8 @@
 //    scores, the values' to the weights, with a reference that is raised (and O multiplied) only when a weight would pass 2^8.
 //  * One warp issues the products: O += P V, the weights P read from tensor memory, where they have taken the place of their scores, and
 //    the next step's scores S = Q K^T.  While one tile's rows are exponentiated the other's products run.
-// Measured: 1024 tokens of 2 sequences over 16384 keys, 4 heads of 128 features, 288 us, 920 TFLOP/s, 56 % of a library product; 64 features 505.  A
-// step takes 4300 cycles, of which the row warps' weights are 2300 a tile: without any exponential they would take 80 % of the time, without the
+// Measured: 1024 tokens of 2 sequences over 16384 keys, 4 heads of 128 features, 281 us, 947 TFLOP/s, 57 % of a library product; 64 features 495.  A
+// step takes 4200 cycles, of which the row warps' weights are 2300 a tile: without any exponential they would take 80 % of the time, without the
 // conversion of keys and values all of it, and with scores that never wait for the products of the step before (64 features leave the room) 99 %.
 // Slower were (beside 304 us): two threads a row 343, scores of 64 keys in two buffers 358, scores loaded a quarter at a time 347; eight warps that
 // bring keys and values, which leave the rows 160 registers each, took the 304.
@@ -165,7 +165,9 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
     const bool exists = token < a.N, real = token < count;
     const uint32_t lanes = (uint32_t)(warp & 3) << 21;  // the warp's 32 lanes of tensor memory
     const uint32_t t_s = tmem + kTmemS + tile * 128 + lanes, t_o = tmem + kTmemO + tile * 128 + lanes;
-    const bool works = steps > 0 && (tile == 0 || two);
+    const bool works = steps > 0 && (tile == 0 || two), idle = !__any_sync(0xffffffffu, real);
+    int keyed = sees_keys(a, len, count, token);
+    asm volatile("" : "+r"(keyed));  // (else its four operands take registers through the loop)
     float factor = fabsf(a.scale) * kLog2e, top = -CUDART_INF_F, sum = 0.0f;
     bool ok = true;
     if (works) {
@@ -206,8 +208,14 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
       fence_async_smem();
       mbar_arrive(bar(kQ0 + tile));
       const int place = len - count + token;
-      const int high = !real ? 0 : a.causal ? place + 1 : len, low = a.window > 0 ? max(place, 0) - a.window + 1 : 0;
-      for (int i = 0; i < steps && ok; ++i) {
+      // (rows of padding, whose results are not looked at, ask for no mask)
+      const int high = !real ? 0x7fffffff : a.causal ? place + 1 : len, low = real && a.window > 0 ? max(place, 0) - a.window + 1 : 0;
+      // Warps of nothing but padding leave the schedulers to the others: 64 rows of 64 heads over 16384 keys 189 -> 138 us.
+      for (int i = 0; i < steps && idle && ok; ++i) {
+        ok = wait(kS0 + tile, i);
+        if (ok) mbar_arrive(bar(kP0 + tile));
+      }
+      for (int i = 0; i < steps && !idle; ++i) {
         ok = wait(kS0 + tile, i);
         if (!ok) break;
         tc_fence_after();
@@ -297,15 +305,14 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
     }
     // --- result: rows without a key, and of padding, are zero
     if (ok) {
-      const float inverse = real && top > -CUDART_INF_F ? 1.0f / sum : 0.0f;  // (no key, no reference)
+      const float inverse = top > -CUDART_INF_F ? 1.0f / sum : 0.0f;  // (no key, no reference)
       const size_t slot = ((size_t)unit * args.pieces + piece) * kRows + tile * kTileRows + r;
       T* const dst = reinterpret_cast<T*>(const_cast<void*>(a.out.ptr)) + e * a.out.se + h * a.out.sh + token * a.out.sn;
 #pragma unroll
       for (int q = 0; q < D / 32; ++q) {
         float o[32];
-        if (works) {
-          tmem_ld32(t_o + 32 * q, o);
-        } else {
+        if (works) tmem_ld32(t_o + 32 * q, o);
+        if (!works || !keyed) {
 #pragma unroll
           for (int j = 0; j < 32; ++j) o[j] = 0.0f;
         }

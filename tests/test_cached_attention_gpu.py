@@ -514,3 +514,18 @@ def test_heads_that_nearly_fill_the_device(E, H, Hk, N, D, dtype):
     q = queries(E, H, N, D, dtype, "heads")
     out = ma.cached_attention_b200(q, cache, table, torch.tensor(lengths, dtype=torch.int32, device="cuda"))
     check(out, q, cache, table, lengths, None, 64)
+
+
+@pytest.mark.parametrize("N,L", [(3, 40), (3, 5000), (9, 700), (40, 300), (40, 5000), (150, 300)])
+def test_rows_without_keys_are_zero_beside_nan(N, L):
+    """A NaN among the values reaches the rows that see it; rows of padding and rows in front of the sequence's first token stay zero."""
+    import monarch_attention_b200 as ma
+    lengths, counts = [L, 2], [N - 1, N]
+    cache, table = filled(2, L // 32 + 1, 2, 64, 32, lengths)
+    for e, t in ((0, L // 2), (1, 1)):
+        cache.v.view(torch.uint8)[int(table[e, t // 32]), :, t % 32, 5] = 0x7f
+    q = queries(2, 8, N, 64, BF, "heads")
+    out = ma.cached_attention_b200(q, cache, table, *(torch.tensor(x, dtype=torch.int32, device="cuda") for x in (lengths, counts)))
+    assert not bool(out[0, :, N - 1].any()) and not bool(out[1, :, :N - 2].any())
+    assert bool(out[0, :, :N - 1, 5][:, -1].isnan().all()) and bool(out[1, :, -1, 5].isnan().all())
+    assert bool(out[..., :5].isfinite().all()) and bool(out[..., 6:].isfinite().all())
