@@ -772,7 +772,8 @@ cudaError_t launch(AttendArgs& a, const Plan& plan, cudaStream_t stream) {
   void* join_args[] = {(void*)&a, (void*)&tile_rows};
   const unsigned rows = a.group * a.N < tile_rows ? a.group * a.N : tile_rows;
   const long long entries = a.split_by_head ? (long long)a.E * a.cache.heads * a.row_blocks : plan.grid;
-  // few heads have many pieces each: their rows are cut into parts of 32 features
+  // Few heads have many pieces each: a CTA for 32 features of a row, else a warp for a row.  us of the call, the one / the other: a token of 2 heads of 131071
+  // tokens 23 / 59, of 8 heads of 32768 23 / 31; 64 heads of 32768 (more rows than that) 101 / 99.
   if (entries * rows < 2 * sm_count()) return launch_kernel((const void*)join_kernel<T, D>, dim3((unsigned)entries, rows, D / 32), dim3(256), join_args, 0, stream);
   return launch_join(a, std::is_same<T, __half>::value ? MA_B200_F16 : MA_B200_BF16, D, tile_rows, (int)entries, 2, stream);
 }

@@ -484,8 +484,8 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
 }  // namespace
 
 // Pieces that the keys of 256 rows are cut into: with fewer blocks of rows than SMs, what brings them to all SMs, as long as a piece has
-// four steps at least.  us, pieces / none: 4 heads x 256 rows over 16384 keys 35 / 292, over 4096 29 / 88, over 1500 28 / 41; 32 heads over 16384 110 / 353, 64
-// over 8000 112 / 183.
+// four steps at least.  us, pieces / none: 4 heads x 256 rows over 16384 keys 34 / 275, over 4096 28 / 80, over 1500 27 / 38; 32 heads over 16384 94 / 286, 64
+// over 8000 97 / 150.
 int prompt_pieces(int E, int N, int H, int kv_heads, long long longest) {
   const long long units = (long long)E * kv_heads * (((long long)H / kv_heads * N + kRows - 1) / kRows);
   const long long fill = sm_count() / units, most = longest / (4 * kKeys);
