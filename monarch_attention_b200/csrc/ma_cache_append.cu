@@ -69,20 +69,20 @@ __device__ __forceinline__ float largest(const float (&x)[F]) {
 struct Turn {
   float2 cs[F];  // half: of each feature, the sine with its sign; interleaved: of its four pairs
   int partner;   // lane that holds the other half
-  bool turned;
+  bool turned;   // else the features stay what they are: a product with a sine of zero would make a NaN of the partner's infinity
 };
-// `sines`: those of the position, by pair; not looked at where `real` is false.
+// `sines`: those of the position, by pair; not looked at where `real` is false, which turns nothing.
 template <int D>
 __device__ __forceinline__ Turn turn_of(const RotaryArgs& r, const float2* sines, bool real, int lane, int f0) {
   Turn t;
-  t.turned = f0 < 2 * r.pairs;
+  t.turned = real && f0 < 2 * r.pairs;
   const bool upper = f0 >= r.pairs;
   constexpr int kLanes = D / F;  // of a row
   t.partner = !t.turned || r.interleaved ? lane : (lane & ~(kLanes - 1)) | ((lane & (kLanes - 1)) + (upper ? -r.pairs / F : r.pairs / F));
 #pragma unroll
   for (int i = 0; i < F; ++i) {
     t.cs[i] = make_float2(1.0f, 0.0f);
-    if (!t.turned || !real) continue;
+    if (!t.turned) continue;
     if (!r.interleaved) {
       t.cs[i] = sines[f0 + i - (upper ? r.pairs : 0)];
       if (!upper) t.cs[i].y = -t.cs[i].y;
@@ -95,6 +95,7 @@ __device__ __forceinline__ Turn turn_of(const RotaryArgs& r, const float2* sines
 // Features of a row turned in place (the whole warp takes part).
 __device__ __forceinline__ void apply(const RotaryArgs& r, const Turn& t, float (&x)[F]) {
   if (r.interleaved) {
+    if (!t.turned) return;
 #pragma unroll
     for (int i = 0; i < F; i += 2) {
       const float u = x[i], w = x[i + 1];
@@ -103,11 +104,12 @@ __device__ __forceinline__ void apply(const RotaryArgs& r, const Turn& t, float 
     }
     return;
   }
+  float w[F];
 #pragma unroll
-  for (int i = 0; i < F; ++i) {
-    const float w = __shfl_sync(0xffffffffu, x[i], t.partner);
-    x[i] = x[i] * t.cs[i].x + w * t.cs[i].y;
-  }
+  for (int i = 0; i < F; ++i) w[i] = __shfl_sync(0xffffffffu, x[i], t.partner);
+  if (!t.turned) return;
+#pragma unroll
+  for (int i = 0; i < F; ++i) x[i] = x[i] * t.cs[i].x + w[i] * t.cs[i].y;
 }
 
 // What a call has to know of sequence e; counts that cannot be are taken as none.
@@ -280,7 +282,7 @@ __global__ void __launch_bounds__(kThreads) append_token_kernel(const __grid_con
   __syncthreads();  // (also: the row's lanes have read the older scale)
   float x[F];
   widen<T>(raw, x);
-  if (pairs > 0) apply(a.rotary, turn_of<D>(a.rotary, table, kind != 1, lane, f0), x);  // (values, next to keys in a warp, keep theirs)
+  if (pairs > 0) apply(a.rotary, turn_of<D>(a.rotary, table, kind != 1, lane, f0), x);  // (values, next to keys in a warp, are not turned)
   float amax = largest(x);
 #pragma unroll
   for (int m = kLanes / 2; m > 0; m >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, m));

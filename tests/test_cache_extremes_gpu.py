@@ -1,0 +1,45 @@
+"""The append to the 8-bit cache and the attention over it at the ends of their ranges: infinities, NaN, scales and scores far apart."""
+import math
+
+import pytest
+import torch
+
+from decoder_reference import HALF_STEP, SUBNORMAL, attention, close, held
+from test_cached_attention_gpu import check, filled, queries
+
+pytestmark = pytest.mark.gpu
+BF, HF = torch.bfloat16, torch.float16
+INF, NAN = float("inf"), float("nan")
+
+
+def ints(*x):
+    return torch.tensor(x, dtype=torch.int32, device="cuda")
+
+
+@pytest.mark.parametrize("N", [1, 2, 20])
+@pytest.mark.parametrize("dim", [16, 32, 64, 128])
+@pytest.mark.parametrize("pairs", ["half", "interleaved"])
+@pytest.mark.parametrize("D", [64, 128])
+def test_infinities_and_nan_stay_in_features_that_are_not_rotated(D, pairs, dim, N):
+    """Values, and what lies behind ``dim`` in keys and queries, are passed on feature by feature whatever is in them."""
+    import monarch_attention_b200 as ma
+    if dim > D:
+        pytest.skip("wider than the head")
+    E, H, Hk = 2, 3, 2
+    rotary = ma.RotaryPositions(dim, pairs=pairs)
+    q, k, v = (torch.ones(E, h, N, D, device="cuda", dtype=BF) for h in (H, Hk, Hk))
+    for t, first in ((q, dim), (k, dim), (v, 0)):
+        for i, x in enumerate((INF, NAN, -INF)):
+            at = first + (D - first) * (2 * i + 1) // 7
+            if at < D:
+                t[:, i % t.shape[1], N // 2, at] = x
+    cache = ma.PagedKV.allocate(8, Hk, D, 32)
+    table, lengths = torch.arange(8, dtype=torch.int32, device="cuda").view(E, 4), ints(N + 3, N + 60)
+    out = ma.append_kv_b200(cache, k, v, table, lengths, query=q, rotary=rotary)
+    assert bool(((out == q) | (out.isnan() & q.isnan()))[..., dim:].all()) and bool(out[..., :dim].isfinite().all())
+    for codes, x, first in ((cache.k, k, dim), (cache.v, v, 0)):
+        for e in range(E):
+            place = torch.arange(int(lengths[e]) - N, int(lengths[e]), device="cuda")
+            got = codes.view(torch.uint8)[table[e].long()[place // 32], :, place % 32].view(torch.float8_e4m3fn).float().transpose(0, 1)
+            assert torch.equal(got.isnan(), x[e].isnan())
+            assert bool((got[x[e] == INF] == 448.0).all()) and bool((got[x[e] == -INF] == -448.0).all())
