@@ -58,10 +58,11 @@ template <typename T>
 __device__ __forceinline__ uint4 narrow(const float (&x)[F]) {
   return make_uint4(sm100::pack2<T>(x[0], x[1]), sm100::pack2<T>(x[2], x[3]), sm100::pack2<T>(x[4], x[5]), sm100::pack2<T>(x[6], x[7]));
 }
+// (of the numbers: a NaN, also a row of nothing else, asks for no scale)
 __device__ __forceinline__ float largest(const float (&x)[F]) {
-  float m = fabsf(x[0]);
+  float m = 0.0f;
 #pragma unroll
-  for (int i = 1; i < F; ++i) m = fmaxf(m, fabsf(x[i]));
+  for (int i = 0; i < F; ++i) m = fmaxf(m, fabsf(x[i]));
   return m;
 }
 
@@ -104,12 +105,11 @@ __device__ __forceinline__ void apply(const RotaryArgs& r, const Turn& t, float 
     }
     return;
   }
-  float w[F];
 #pragma unroll
-  for (int i = 0; i < F; ++i) w[i] = __shfl_sync(0xffffffffu, x[i], t.partner);
-  if (!t.turned) return;
-#pragma unroll
-  for (int i = 0; i < F; ++i) x[i] = x[i] * t.cs[i].x + w[i] * t.cs[i].y;
+  for (int i = 0; i < F; ++i) {
+    const float w = __shfl_sync(0xffffffffu, x[i], t.partner);
+    if (t.turned) x[i] = x[i] * t.cs[i].x + w * t.cs[i].y;
+  }
 }
 
 // What a call has to know of sequence e; counts that cannot be are taken as none.

@@ -43,3 +43,26 @@ def test_infinities_and_nan_stay_in_features_that_are_not_rotated(D, pairs, dim,
             got = codes.view(torch.uint8)[table[e].long()[place // 32], :, place % 32].view(torch.float8_e4m3fn).float().transpose(0, 1)
             assert torch.equal(got.isnan(), x[e].isnan())
             assert bool((got[x[e] == INF] == 448.0).all()) and bool((got[x[e] == -INF] == -448.0).all())
+
+
+@pytest.mark.parametrize("N", [1, 2, 20])
+@pytest.mark.parametrize("D", [64, 128])
+def test_a_row_of_nan_leaves_the_others_of_its_block(D, N):
+    """A block's scale is that of its numbers: a token that is NaN throughout is stored as that, and the tokens beside it keep their values."""
+    import monarch_attention_b200 as ma
+    cache = ma.PagedKV.allocate(4, 2, D, 16)
+    table = torch.arange(4, dtype=torch.int32, device="cuda").view(1, 4)
+    x = torch.linspace(1.0, 1.75, 8, device="cuda").to(BF).repeat(D // 8).expand(1, 2, 5, D).contiguous()
+    ma.append_kv_b200(cache, x, -x, table, ints(5))
+    bad = x[:, :, :1].expand(1, 2, N, D).clone()
+    bad[:, 1, N // 2] = NAN
+    ma.append_kv_b200(cache, bad, -bad, table, ints(5 + N))
+    alone = ma.PagedKV.allocate(4, 2, D, 16)
+    ma.append_kv_b200(alone, torch.full_like(x[:, :, :1], NAN), torch.full_like(x[:, :, :1], NAN), table, ints(1))
+    for codes, scales, sign in ((cache.k, cache.k_scale, 1.0), (cache.v, cache.v_scale, -1.0)):
+        got = held(codes, scales, table[0], 5 + N, 16)
+        want = sign * torch.cat((x, bad), 2)[0].to(torch.float8_e4m3fn).double().cpu()   # (the scale is a power of two, so the rounding is the type's)
+        assert torch.equal(got.isnan(), want.isnan())
+        assert torch.equal(got.nan_to_num(0.0), want.nan_to_num(0.0))
+    # with nothing but NaN the smallest scale of all, which the next token raises as far as it asks for
+    assert float(alone.k_scale[0, 0, 0]) == 2.0 ** -40 and bool(alone.k[0, 0, 0].float().isnan().all())
