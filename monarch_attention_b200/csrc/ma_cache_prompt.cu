@@ -73,11 +73,17 @@ __device__ __forceinline__ uint32_t widen2_upper(uint32_t codes) {
   asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, hi;\n\t}" : "=r"(r) : "r"(codes));
   return r;
 }
+// The larger of the two, NaN if one is: a key of NaN takes its rows with it.
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
 // 2^x on the multipliers, for x up to 2^7: the special function units are what the weights wait for.  x = n + f with f in [-1/2, 1/2], 2^f by a
-// polynomial of degree 5 (minimax in the relative error, 2^-23.6; found by exchange), n added to the exponent.
+// polynomial of degree 5 (minimax in the relative error, found by exchange; 2^-22.7 with the coefficients in 32 bits), times 2^n.
 constexpr int kByProducts = 1;  // of 4 pairs of weights, these (us of 16384 keys: none 295, one 288, two 320)
 __device__ __forceinline__ float2 exp2_by_products(float2 x) {
-  x = make_float2(fmaxf(x.x, -126.0f), fmaxf(x.y, -126.0f));
+  x = make_float2(max_nan(x.x, -126.0f), max_nan(x.y, -126.0f));
   const float2 round = make_float2(12582912.0f, 12582912.0f);  // 1.5 * 2^23: its last bits are n
   const float2 t = add2(x, round), f = sub2(x, sub2(t, round));
   auto both = [](float c) { return make_float2(c, c); };
@@ -86,7 +92,8 @@ __device__ __forceinline__ float2 exp2_by_products(float2 x) {
   p = fma2(p, f, both(2.4022114e-1f));
   p = fma2(p, f, both(6.9314694e-1f));
   p = fma2(p, f, both(1.0000001f));
-  return make_float2(__int_as_float(__float_as_int(p.x) + (__float_as_int(t.x) << 23)), __int_as_float(__float_as_int(p.y) + (__float_as_int(t.y) << 23)));
+  // times 2^n, a product, in which a NaN stays one (added to its bits n would make a number of it)
+  return mul2(p, make_float2(__int_as_float((__float_as_int(t.x) << 23) + 0x3f800000), __int_as_float((__float_as_int(t.y) << 23) + 0x3f800000)));
 }
 // 16 codes as two 16-byte chunks of a row.
 __device__ __forceinline__ void put_codes(uint32_t panel, uint32_t row, uint32_t chunk, const uint4& c) {

@@ -66,3 +66,44 @@ def test_a_row_of_nan_leaves_the_others_of_its_block(D, N):
         assert torch.equal(got.nan_to_num(0.0), want.nan_to_num(0.0))
     # with nothing but NaN the smallest scale of all, which the next token raises as far as it asks for
     assert float(alone.k_scale[0, 0, 0]) == 2.0 ** -40 and bool(alone.k[0, 0, 0].float().isnan().all())
+
+
+@pytest.mark.parametrize("place", range(16))
+@pytest.mark.parametrize("N,softcap", [(1, 0.0), (5, 0.0), (40, 0.0), (40, 20.0)])
+def test_a_key_of_nan_reaches_all_rows_that_see_it(N, softcap, place):
+    """Whichever of a block's 16 places it has, and however many rows there are; rows in front of it do not see it."""
+    import monarch_attention_b200 as ma
+    L, D, page = 300, 64, 32
+    cache, table = filled(2, 12, 2, D, page, [L, L])
+    spots = (160 + place, L - N // 2 - 1 if N > 1 else 3)   # in the middle; among the call's own tokens
+    for e, t in enumerate(spots):
+        cache.k.view(torch.uint8)[int(table[e, t // page]), :, t % page, 7] = 0x7f
+    q = queries(2, 8, N, D, BF, "heads")
+    out = ma.cached_attention_b200(q, cache, table, ints(L, L), softcap=softcap)
+    for e, t in enumerate(spots):
+        sees = torch.arange(L - N, L) >= t
+        assert bool(out[e][:, sees.cuda()].isnan().all())
+        if not sees.all():
+            k, v = (held(c, s, table[e], L, page) for c, s in ((cache.k, cache.k_scale), (cache.v, cache.v_scale)))
+            n = int((~sees).sum())
+            want, bound = attention(q[e, :, :n], k[:, :t], v[:, :t], L - N, True, D ** -0.5, softcap)
+            close(out[e, :, :n], want, bound + HALF_STEP[BF] * (want.abs() + bound) + SUBNORMAL[BF])
+
+
+@pytest.mark.parametrize("bad", [NAN, INF])
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("N", [3, 40])
+def test_a_query_of_nan_or_infinity_is_its_own_rows_matter(N, dtype, bad):
+    import monarch_attention_b200 as ma
+    cache, table = filled(1, 8, 2, 128, 64, [400])
+    q = queries(1, 4, N, 128, dtype, "heads")
+    want = ma.cached_attention_b200(q, cache, table, ints(400))
+    broken = q.clone()
+    broken[0, 1, N // 2, 70] = bad
+    out = ma.cached_attention_b200(broken, cache, table, ints(400))
+    assert bool(out[0, 1, N // 2].isnan().all())   # (of scores of plus and minus infinity, or NaN)
+    rest = torch.ones(1, 4, N, dtype=torch.bool, device="cuda")
+    rest[0, 1, N // 2] = False
+    assert bool(out[rest].isfinite().all())
+    # (the other rows of its tile may get another reference and so other roundings of their weights: 2^-11 and the type's)
+    assert bool(((out[rest].float() - want[rest].float()).abs() <= 2 ** -10 * 16 + 2 * HALF_STEP[dtype] * want[rest].float().abs()).all())
