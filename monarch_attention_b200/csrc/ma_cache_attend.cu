@@ -14,7 +14,7 @@
 //    weights change sides by an 8 x 8 transpose between lanes.
 //  * e4m3 is exact in f16, so the products are f16 with 32-bit sums whatever the queries' type; a bf16 row is scaled by a power of two to
 //    magnitudes of 1 to 2 first (exact but for elements 2^-23 below the row's largest).  A block's key scale multiplies its scores; its value
-//    scale goes into the weights, and the running maximum is taken over weight times scale, so that f16 weights are at most 2^kSlack.
+//    scale goes into the weights, and the running maximum is taken over weight times scale, so that f16 weights are at most 2^kSlack (kBelow).
 // Measured, a token each: 32 sequences of up to 8192 tokens, 8 heads of 128 features, 270 MB in 59 us; every further byte comes at 6.3 TB/s, 96 %
 // of a copy (64 features: 4.9, the bytes' conversion and the weights bind), and some 12 us go to the start, the unequal finish of the CTAs and the
 // join.  One sequence of 131071 tokens and 2 heads, 67 MB in 23 us; of 500 tokens and 12 heads of 64 features 7.4 us.
@@ -32,7 +32,9 @@ using sm100::ex2;
 using sm100::kLog2e;
 using sm100::smem_u32;
 
-constexpr float kSlack = 8.0f;  // weights are at most 2^8 of the reference: f16 holds them as exactly as those up to 1
+// Weights in f16 (times their value's scale): the reference is kBelow under the largest when it is set, and raised when one would pass 2^kSlack, so that the largest are
+// 2^7 to 2^15, under the 65504 of the type, and only those below 2^-21 to 2^-29 of the largest have fewer bits than 11.
+constexpr float kBelow = 7.0f, kSlack = 15.0f;
 constexpr int kSlice = 32;  // tokens of a warp at a time
 constexpr int kWide = 12;   // warps of a CTA that has an SM to itself: as many as fit in with two tiles of rows
 
@@ -450,7 +452,7 @@ __global__ void __launch_bounds__(W * 32, Shape<D, NT, W>::kCtas) attend_kernel(
 #pragma unroll
             for (int m = 4; m < 32; m <<= 1) most[j] = fmaxf(most[j], __shfl_xor_sync(0xffffffffu, most[j], m));
             const float before = top[n][j];
-            top[n][j] = fmaxf(before, most[j]);
+            top[n][j] = fmaxf(before, most[j] - kBelow);
             const float shrink = ex2(before - (top[n][j] == -CUDART_INF_F ? 0.0f : top[n][j]));
             sum[n][j] *= shrink;
 #pragma unroll

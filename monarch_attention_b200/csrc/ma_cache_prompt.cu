@@ -8,7 +8,7 @@
 //    single tile would be bound by, count half.
 //  * Two warpgroups have a row a thread: the row's 128 scores go from tensor memory to registers in one go, and the maximum, the weights and
 //    their sum need no other thread.  Scales of blocks are applied as in the kernel for few rows (ma_cache_attend.cu): the keys' to the
-//    scores, the values' to the weights, with a reference that is raised (and O multiplied) only when a weight would pass 2^8.
+//    scores, the values' to the weights, with a reference that is raised (and O multiplied) only when a weight would pass 2^15.
 //  * One warp issues the products: O += P V, the weights P read from tensor memory, where they have taken the place of their scores, and
 //    the next step's scores S = Q K^T.  While one tile's rows are exponentiated the other's products run.
 // Measured: 1024 tokens of 2 sequences over 16384 keys, 4 heads of 128 features, 281 us, 947 TFLOP/s, 57 % of a library product; 64 features 495.  A
@@ -34,7 +34,7 @@ constexpr int kThreads = 512, kBringers = 128;  // warps 0-3, 4-7: rows; 8-11: k
 constexpr int kLaunchRegs = 128, kRowRegs = 184, kBringerRegs = 104, kIssuerRegs = 40;
 static_assert(256 * kRowRegs + kBringers * kBringerRegs + 128 * kIssuerRegs <= kThreads * kLaunchRegs, "setmaxnreg draws on the launch's registers");
 constexpr int kRing = 8;  // steps whose pages and scales are kept
-constexpr float kSlack = 8.0f;
+constexpr float kBelow = 7.0f, kSlack = 15.0f;  // (ma_cache_attend.cu)
 
 enum Bar { kQ0, kQ1, kKFull, kKEmpty = kKFull + 2, kVFull = kKEmpty + 2, kVEmpty = kVFull + 2, kS0 = kVEmpty + 2, kS1, kP0, kP1, kO, kBars };
 
@@ -282,7 +282,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
           }
           if (!__any_sync(0xffffffffu, most > top + kSlack)) break;
           const float before = top;
-          top = fmaxf(top, most);
+          top = fmaxf(top, most - kBelow);
           const float shrink = ex2(before - (top == -CUDART_INF_F ? 0.0f : top));
           sum *= shrink;
           if (i > 0) {  // (the scores of this step are there, so the products of the one before are done)

@@ -107,3 +107,36 @@ def test_a_query_of_nan_or_infinity_is_its_own_rows_matter(N, dtype, bad):
     assert bool(out[rest].isfinite().all())
     # (the other rows of its tile may get another reference and so other roundings of their weights: 2^-11 and the type's)
     assert bool(((out[rest].float() - want[rest].float()).abs() <= 2 ** -10 * 16 + 2 * HALF_STEP[dtype] * want[rest].float().abs()).all())
+
+
+def one_hot_keys(L, D, page, far):
+    """A cache of keys that give scores of 0 (an early token, of value 0) and ``-far`` in units of log2 (all others, of value 1) to the query (1, 0, ..)."""
+    import monarch_attention_b200 as ma
+    pages = -(-L // page)
+    cache = ma.PagedKV.allocate(pages, 1, D, page)
+    cache.k_scale.fill_(1.0), cache.v_scale.fill_(1.0)
+    raw = cache.k.view(torch.uint8)
+    raw[..., 0] = 0xb8                     # -1
+    raw[0, :, 5, 0] = 0
+    cache.v.view(torch.uint8).fill_(0x38)  # 1
+    cache.v.view(torch.uint8)[0, :, 5] = 0
+    return cache, torch.arange(pages, dtype=torch.int32, device="cuda").view(1, pages), far * math.log(2.0)
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("E,N", [(1, 1), (1, 40), (1000, 1), (500, 5), (160, 40)])
+@pytest.mark.parametrize("L,far", [(131071, 25.1), (131071, 24.4), (60000, 25.0), (60000, 27.0), (3000, 22.6), (3000, 26.0)])
+def test_a_long_tail_of_small_weights_is_not_lost(L, far, E, N, dtype):
+    """One key far above all others, whose values are what the result has: tail / (1 + tail), tail = (L - 1) 2^-far.
+
+    The largest weight is 2^7 at least, so that those of the tail are 2^(7 - far) or more and rounded to 2^-25: 2^(far - 32) of themselves, 2^-11 at normal
+    weights.  An addend to a 32-bit sum of products loses up to 2^-25 of the sum: L 2^-25 of it, and sums of weights L 2^-24 of the tail."""
+    import monarch_attention_b200 as ma
+    cache, table, scale = one_hot_keys(L, 64, 128, far)
+    q = torch.zeros(E, 4, N, 64, dtype=dtype, device="cuda")   # (many sequences over the same pages: a head stays with one CTA)
+    q[..., 0] = 1.0
+    out = ma.cached_attention_b200(q, cache, table.expand(E, -1), ints(*[L] * E), causal=False, scale=scale)
+    tail = (L - 1) * 2.0 ** -far
+    want = tail / (1 + tail)
+    bound = want * (2.0 ** (far - 32) + 2.0 ** -11 + L * 2.0 ** -24)
+    close(out, torch.full((E, 4, N, 64), want, dtype=torch.float64), torch.tensor(bound + HALF_STEP[dtype] * (want + bound) + SUBNORMAL[dtype]))
