@@ -35,6 +35,8 @@ constexpr int kLaunchRegs = 128, kRowRegs = 184, kBringerRegs = 104, kIssuerRegs
 static_assert(256 * kRowRegs + kBringers * kBringerRegs + 128 * kIssuerRegs <= kThreads * kLaunchRegs, "setmaxnreg draws on the launch's registers");
 constexpr int kRing = 8;  // steps whose pages and scales are kept
 constexpr float kBelow = 7.0f, kSlack = 15.0f;  // (ma_cache_attend.cu)
+// Scores beyond this (in units of log2) have references in two parts (rows_apart).
+constexpr float kApart = 8192.0f;
 
 enum Bar { kQ0, kQ1, kKFull, kKEmpty = kKFull + 2, kVFull = kKEmpty + 2, kVEmpty = kVFull + 2, kS0 = kVEmpty + 2, kS1, kP0, kP1, kO, kBars };
 
@@ -94,6 +96,95 @@ __device__ __forceinline__ float2 exp2_by_products(float2 x) {
   p = fma2(p, f, both(1.0000001f));
   // times 2^n, a product, in which a NaN stays one (added to its bits n would make a number of it)
   return mul2(p, make_float2(__int_as_float((__float_as_int(t.x) << 23) + 0x3f800000), __int_as_float((__float_as_int(t.y) << 23) + 0x3f800000)));
+}
+// What a row needs for its scores: those of keys [low, high) count.
+struct RowScores {
+  float factor, softcap;
+  int low, high;
+};
+// A step's weights of a row whose scores are far from zero, of the 128 scores at t_s (t0: the first one's key), in place of them, and into the row's sum.
+//
+// The kernel's loop has a weight as the exponential of fma(score, f, log - reference), with the logarithm of the value's scale in the reference: where
+// the last bit of a score is worth more than a unit, such a difference is anything, the weights leave f16 and the logarithm is lost.  Here a score is
+// rounded first and a reference is a score S and a logarithm L: (score - S) + (log - L) is exact for the keys that count, however large S is.
+// It takes twice as long, with a few scores at a time in registers.
+template <int D>
+__device__ __forceinline__ void rows_apart(const RowScores& r, const Blocks& b, int t0, uint32_t t_s, uint32_t t_o, bool has_sums, float* sum, float* S_row, float* L_row) {
+  constexpr int kUnroll = D == 128 ? 1 : 2;  // (what leaves the kernel's loop as it was: us of 2 x 1024 tokens over 16384 keys, 128 features 284 / 288, 64 274 / 268)
+  auto load = [&](int q, float (&x)[32]) {
+    tmem_ld32_nowait(t_s + 32 * q, x);
+    tmem_wait_ld(x);
+#pragma unroll
+    for (int j = 0; j < 32; ++j) {
+      const float f = r.factor * b.k_scale[2 * q + j / 16];
+      x[j] = r.softcap > 0.0f ? capped(x[j] * f, r.softcap) : __fmul_rn(x[j], fmaxf(f, 1e-37f));
+      const int t = t0 + 32 * q + j;
+      if (t < r.low || t >= r.high) x[j] = -CUDART_INF_F;
+    }
+  };
+  float S = *S_row, L = *L_row, best = -CUDART_INF_F, best_log = 0.0f;
+#pragma unroll kUnroll
+  for (int q = 0; q < 4; ++q) {
+    float x[32];
+    load(q, x);
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      float most = x[16 * h];
+#pragma unroll
+      for (int j = 1; j < 16; ++j) most = fmaxf(most, x[16 * h + j]);
+      const float log = b.v_log[2 * q + h];
+      if ((most - best) + (log - best_log) > 0.0f) {
+        best = most;
+        best_log = log;
+      }
+    }
+  }
+  const bool raise = (best - S) + (best_log - L) > kSlack;
+  if (__any_sync(0xffffffffu, raise)) {
+    const float S0 = S, L0 = L;
+    if (raise) {
+      S = best;
+      L = best_log - kBelow;
+    }
+    const float shrink = raise ? ex2((S0 - S) + (L0 - L)) : 1.0f;
+    *sum *= shrink;
+    if (has_sums) {
+#pragma unroll 1
+      for (int q = 0; q < D / 16; ++q) {
+        float o[16];
+        uint32_t z[16];
+        tmem_ld16_nowait(t_o + 16 * q, o);
+        tmem_wait_ld16(o);
+#pragma unroll
+        for (int j = 0; j < 16; ++j) z[j] = __float_as_uint(o[j] * shrink);
+        tmem_st16(t_o + 16 * q, z);
+      }
+    }
+  }
+  *S_row = S;
+  *L_row = L;
+  const float base = S == -CUDART_INF_F ? 0.0f : S;
+  float all = 0.0f;
+#pragma unroll kUnroll
+  for (int q = 0; q < 4; ++q) {  // (the weights of 32 keys take the place of 16 scores that have been read)
+    float x[32];
+    uint32_t y[16];
+    load(q, x);
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const float log = b.v_log[2 * q + h] - L;
+      float part = 0.0f;
+#pragma unroll
+      for (int j = 0; j < 16; j += 2) {
+        const float p0 = ex2((x[16 * h + j] - base) + log), p1 = ex2((x[16 * h + j + 1] - base) + log);
+        part += p0 + p1;
+        y[8 * h + j / 2] = pack2<__half>(p0, p1);
+      }
+      all = fmaf(part, b.v_inverse[2 * q + h], all);
+    }
+    tmem_st16(t_s + 16 * q, y);
+  }
+  *sum += all;
 }
 // 16 codes as two 16-byte chunks of a row.
 __device__ __forceinline__ void put_codes(uint32_t panel, uint32_t row, uint32_t chunk, const uint4& c) {
@@ -175,7 +266,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
     const bool works = steps > 0 && (tile == 0 || two), idle = !__any_sync(0xffffffffu, real);
     int keyed = sees_keys(a, len, count, token);
     asm volatile("" : "+r"(keyed));  // (else its four operands take registers through the loop)
-    float factor = fabsf(a.scale) * kLog2e, top = -CUDART_INF_F, sum = 0.0f;
+    float factor = fabsf(a.scale) * kLog2e, top = -CUDART_INF_F, top_log = 0.0f, sum = 0.0f;  // top_log: of references in two parts
     bool ok = true;
     if (works) {
       // the query row in f16, brought to magnitudes of 1 to 2 by a power of two (bf16), with the sign of the scale
@@ -222,7 +313,8 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
         ok = wait(kS0 + tile, i);
         if (ok) mbar_arrive(bar(kP0 + tile));
       }
-      for (int i = 0; i < steps && !idle; ++i) {
+      int i = 0;
+      for (; i < steps && !idle; ++i) {
         ok = wait(kS0 + tile, i);
         if (!ok) break;
         tc_fence_after();
@@ -239,7 +331,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
 #pragma unroll
           for (int q = 0; q < 4; ++q) tmem_wait_ld(v[q]);
           // (scores in units of log2 e) = f * S, and never zero: a mask is minus infinity times f, and rows of zeros, small keys and a small
-          // scale together leave 32 bits.  (S is 2^17 at most.)
+          // scale together leave 32 bits.  (S is 2^17 at most of bf16 rows, 2^32 of f16.)
           auto f = [&](int j) { return a.softcap > 0.0f ? 1.0f : fmaxf(factor * b.k_scale[j], 1e-37f); };
           if (a.softcap > 0.0f) {
 #pragma unroll
@@ -281,6 +373,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
             more = fmaf(part.x + part.y, b.v_inverse[j], more);
           }
           if (!__any_sync(0xffffffffu, most > top + kSlack)) break;
+          if (__any_sync(0xffffffffu, fabsf(most) > kApart && most > -CUDART_INF_F)) goto apart;
           const float before = top;
           top = fmaxf(top, most - kBelow);
           const float shrink = ex2(before - (top == -CUDART_INF_F ? 0.0f : top));
@@ -305,6 +398,22 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
         tc_fence_before();
         mbar_arrive(bar(kP0 + tile));
       }
+      // From the first step on in which a row of the warp has a score far from zero, its rows go this way: a path of its own, of which the loop above knows a jump
+      // and no state (a flag in its place: 4 to 6 % on all calls; the same inside the loop: 15).
+      if (false) {
+      apart:
+#pragma unroll 1
+        for (bool there = true;; there = false) {  // (the first step's scores have been waited for)
+          if (!there) ok = wait(kS0 + tile, i);
+          if (!ok) break;
+          tc_fence_after();
+          rows_apart<D>({factor, a.softcap, low, high}, blocks[i & (kRing - 1)], lo + i * kKeys, t_s, t_o, i > 0, &sum, &top, &top_log);
+          tmem_wait_st();
+          tc_fence_before();
+          mbar_arrive(bar(kP0 + tile));
+          if (++i == steps) break;
+        }
+      }
       if (ok) {
         ok = wait(kO, 0);
         tc_fence_after();
@@ -312,6 +421,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
     }
     // --- result: rows without a key, and of padding, are zero
     if (ok) {
+      const float unit_of = ex2(top_log);  // (a piece's reference is one number)
       const float inverse = top > -CUDART_INF_F ? 1.0f / sum : 0.0f;  // (no key, no reference)
       const size_t slot = ((size_t)unit * args.pieces + piece) * kRows + tile * kTileRows + r;
       T* const dst = reinterpret_cast<T*>(const_cast<void*>(a.out.ptr)) + e * a.out.se + h * a.out.sh + token * a.out.sn;
@@ -332,10 +442,10 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
                            pack2<T>(o[j + 4] * inverse, o[j + 5] * inverse), pack2<T>(o[j + 6] * inverse, o[j + 7] * inverse));
         } else {
 #pragma unroll
-          for (int j = 0; j < 32; j += 4) *reinterpret_cast<float4*>(a.part_o + slot * D + 32 * q + j) = make_float4(o[j], o[j + 1], o[j + 2], o[j + 3]);
+          for (int j = 0; j < 32; j += 4) *reinterpret_cast<float4*>(a.part_o + slot * D + 32 * q + j) = make_float4(o[j] * unit_of, o[j + 1] * unit_of, o[j + 2] * unit_of, o[j + 3] * unit_of);
         }
       }
-      if (args.pieces > 1 && exists) *reinterpret_cast<float2*>(a.part_ml + 2 * slot) = make_float2(top, sum);
+      if (args.pieces > 1 && exists) *reinterpret_cast<float2*>(a.part_ml + 2 * slot) = make_float2(top, sum * unit_of);
     }
     if (args.pieces > 1 && tid == 0 && piece == 0)
       a.split[unit] = make_int4((e * c.heads + head) * a.row_blocks + block, unit * args.pieces, (unit + 1) * args.pieces - 1, 0);

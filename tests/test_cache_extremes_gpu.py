@@ -140,3 +140,50 @@ def test_a_long_tail_of_small_weights_is_not_lost(L, far, E, N, dtype):
     want = tail / (1 + tail)
     bound = want * (2.0 ** (far - 32) + 2.0 ** -11 + L * 2.0 ** -24)
     close(out, torch.full((E, 4, N, 64), want, dtype=torch.float64), torch.tensor(bound + HALF_STEP[dtype] * (want + bound) + SUBNORMAL[dtype]))
+
+
+def one_hot(q, k, v, first, scale, softcap=0.0):
+    """Values of the best key of each row, and whether it stands so far above the others that nothing else counts, whatever 32-bit sums do to scores."""
+    q, D = q.double().cpu(), q.shape[-1]
+    k, v = (t.repeat_interleave(q.shape[0] // t.shape[0], 0) for t in (k, v))
+    s, size = q @ k.mT * scale, q.abs() @ k.abs().mT * abs(scale)
+    if softcap:
+        s, size = softcap * torch.tanh(s / softcap), size + softcap
+    seen = torch.arange(k.shape[1]) <= first + torch.arange(q.shape[1])[:, None]
+    top, best = s.masked_fill(~seen, -math.inf).topk(2, -1)
+    # (D + 8) 2^-24 of the sum of magnitudes each, D 2^-25 more of a row brought to f16; 100 more is 2^-144 of the weight
+    clear = top[..., 0] - top[..., 1] > 2 * (1.5 * D + 8) * 2.0 ** -24 * size.amax(-1) + 100
+    return v.gather(1, best[..., :1].expand(-1, -1, D)), clear
+
+
+@pytest.mark.parametrize("dtype,size", [(BF, 3e4), (BF, 1e8), (BF, 1e20), (BF, 1e30), (HF, 3e2), (HF, 6e4 / 5)])
+@pytest.mark.parametrize("N", [1, 20, 80])
+@pytest.mark.parametrize("scale", [128 ** -0.5, 1e4])
+@pytest.mark.parametrize("L", [300, 5000])
+def test_scores_of_any_magnitude(L, scale, N, dtype, size):
+    """Scores that decide for one key give that key's value, with few rows and with many, keys in one piece or in several."""
+    import monarch_attention_b200 as ma
+    cache, table = filled(1, L // 64 + 2, 1, 128, 64, [L])
+    q = (queries(1, 8, N, 128, torch.float32, "heads").clamp(-5, 5) * size).to(dtype)
+    out = ma.cached_attention_b200(q, cache, table, ints(L), scale=scale)[0].double().cpu()
+    k, v = (held(c, s, table[0], L, 64) for c, s in ((cache.k, cache.k_scale), (cache.v, cache.v_scale)))
+    want, clear = one_hot(q[0], k, v, L - N, scale)
+    assert bool(clear.any()) and bool(out.isfinite().all())
+    # the weight in f16, its sum in 32 bits and the rounding of the result
+    assert bool(((out - want).abs() <= (2.0 ** -11 + 2.0 ** -20 + HALF_STEP[dtype]) * want.abs() + SUBNORMAL[dtype])[clear].all())
+    # what is not clear lies between the values
+    most, least = v.amax((0, 1)), v.amin((0, 1))
+    assert bool((out <= most + 2.0 ** -7 * most.abs()).all()) and bool((out >= least - 2.0 ** -7 * least.abs()).all())
+
+
+@pytest.mark.parametrize("softcap", [1e5, 1e9, 1e30])
+@pytest.mark.parametrize("N", [1, 20, 80])
+def test_large_caps_of_large_scores(N, softcap):
+    import monarch_attention_b200 as ma
+    cache, table = filled(1, 6, 1, 128, 64, [300])
+    q = (queries(1, 8, N, 128, BF, "heads").float() * softcap / 10).to(BF)
+    out = ma.cached_attention_b200(q, cache, table, ints(300), scale=0.1, softcap=softcap)[0].double().cpu()
+    k, v = (held(c, s, table[0], 300, 64) for c, s in ((cache.k, cache.k_scale), (cache.v, cache.v_scale)))
+    want, clear = one_hot(q[0], k, v, 300 - N, 0.1, softcap)
+    assert bool(clear.any()) and bool(out.isfinite().all())
+    assert bool(((out - want).abs() <= (2.0 ** -11 + 2.0 ** -20 + 2.0 ** -8) * want.abs())[clear].all())
