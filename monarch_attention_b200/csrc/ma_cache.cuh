@@ -6,7 +6,8 @@
 
 namespace ma {
 
-constexpr int kScaleBlock = 16;  // tokens that share a scale
+constexpr int kScaleBlock = 16;       // tokens that share a scale
+constexpr float kLeastLog = -40.0f;   // of a scale that is not zero, to base 2
 
 // Strides in elements of each tensor; the features of a row lie next to one another.
 struct CacheArgs {

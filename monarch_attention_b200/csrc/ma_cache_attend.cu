@@ -414,8 +414,8 @@ __global__ void __launch_bounds__(W * 32, Shape<D, NT, W>::kCtas) attend_kernel(
         }
       const float4 scales = *reinterpret_cast<const float4*>(keys + 2 * kSlice * D);
       const float ks[2] = {scales.x, scales.y}, vs[2] = {scales.z, scales.w};
-      // (a scale of zero is as good as 2^-100: its keys have weights, which the reference has to stand for)
-      const float vl[2] = {fmaxf(__log2f(scales.z), -100.0f), fmaxf(__log2f(scales.w), -100.0f)};
+      // (values of scale zero count as of the smallest scale there is: their keys have weights, which the reference has to stand for, but no more than that)
+      const float vl[2] = {fmaxf(__log2f(scales.z), kLeastLog), fmaxf(__log2f(scales.w), kLeastLog)};
       uint32_t weights[2][NT][2];
       const bool whole = t0 >= full_low && t0 + kSlice <= full_high;
 #pragma unroll

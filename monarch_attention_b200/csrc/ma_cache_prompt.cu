@@ -466,12 +466,13 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
     };
     auto put_blocks = [&](int i, int page, float ks, float vs) {
       Blocks& b = blocks[i & (kRing - 1)];
-      // (a scale of zero is one of one before zeros: a mask is minus infinity times the keys' scale, a weight is divided by the values')
+      // (a scale of zero is another one before zeros, since a mask is minus infinity times the keys' scale and a weight is divided by the values': one for keys,
+      // the smallest that there is for values, whose weights are not to be above those of any other block's)
       b.page[0][t] = ks == 0.0f ? -1 : page;
       b.page[1][t] = vs == 0.0f ? -1 : page;
       b.k_scale[t] = ks == 0.0f ? 1.0f : ks;
-      b.v_inverse[t] = vs == 0.0f ? 1.0f : 1.0f / vs;
-      b.v_log[t] = vs == 0.0f ? 0.0f : __log2f(vs);
+      b.v_inverse[t] = vs == 0.0f ? exp2f(-kLeastLog) : 1.0f / vs;
+      b.v_log[t] = vs == 0.0f ? kLeastLog : __log2f(vs);
     };
     auto meet = [&]() { asm volatile("bar.sync 1, %0;" ::"n"(kBringers) : "memory"); };
     int page_next = -1;

@@ -187,3 +187,17 @@ def test_large_caps_of_large_scores(N, softcap):
     want, clear = one_hot(q[0], k, v, 300 - N, 0.1, softcap)
     assert bool(clear.any()) and bool(out.isfinite().all())
     assert bool(((out - want).abs() <= (2.0 ** -11 + 2.0 ** -20 + 2.0 ** -8) * want.abs())[clear].all())
+
+
+@pytest.mark.parametrize("exponent", [-20, -30, -39, 0, 50])
+@pytest.mark.parametrize("N", [1, 3, 4, 20, 40])
+@pytest.mark.parametrize("L", [300, 5000])
+def test_zero_scales_beside_values_of_any_size(L, N, exponent):
+    """Blocks of scale zero hold zeros; the others' values count in full beside them, however small they are."""
+    import monarch_attention_b200 as ma
+    cache, table = filled(1, L // 64 + 2, 2, 64, 64, [L])
+    g = torch.Generator(device="cuda").manual_seed(3)
+    cache.v_scale.fill_(2.0 ** exponent)
+    cache.v_scale[torch.rand(cache.v_scale.shape, generator=g, device="cuda") < 0.5] = 0.0
+    q = queries(1, 8, N, 64, BF, "heads")
+    check(ma.cached_attention_b200(q, cache, table, ints(L)), q, cache, table, [L], None, 64)
