@@ -371,7 +371,8 @@ MA_B200_API int ma_b200_cache_append(const ma_b200_append* p, void* stream);
 
 /* Softmax attention of q (E, H, N, width; bf16 or f16; query head h reads cache head h / (H / heads)) over the sequences' cached tokens
  * into out.  causal: token n sees positions up to its own, else all `lengths`.  window > 0 (causal only): the last `window`
- * of those.  softcap > 0 (1e-20 to 1e30): scores s become softcap * tanh(s / softcap).  Rows without a key, and rows of padding, are zero. */
+ * of those.  softcap > 0 (1e-20 to 1e30): scores s become softcap * tanh(s / softcap).  Rows without a key, and rows of padding, are zero.
+ * Where scores pass 2^27 and there are 32 rows or fewer to a cache head (N * H / heads), scales of values are to be from 2^-14 to 2^15. */
 typedef struct ma_b200_attend {
   int32_t abi_version;
   int32_t E, H, N;

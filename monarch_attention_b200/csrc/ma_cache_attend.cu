@@ -34,6 +34,9 @@ using sm100::smem_u32;
 
 // Weights in f16 (times their value's scale): the reference is kBelow under the largest when it is set, and raised when one would pass 2^kSlack, so that the largest are
 // 2^7 to 2^15, under the 65504 of the type, and only those below 2^-21 to 2^-29 of the largest have fewer bits than 11.
+// (Beside a score of 2^27 and more the logarithm of a value's scale is lost from the reference, and a weight is anything from the scale itself to 2^(7 +- 16).  A
+// reference of two numbers, score and logarithm, as the kernel for many rows has it there, costs every call of this one 3 to 5 %, and the shortest 0.8 us of 6.7:
+// in the loop, as a rare branch in it and as a call from there.  So there the scales are asked to be from 2^-14 to 2^15.)
 constexpr float kBelow = 7.0f, kSlack = 15.0f;
 constexpr int kSlice = 32;  // tokens of a warp at a time
 constexpr int kWide = 12;   // warps of a CTA that has an SM to itself: as many as fit in with two tiles of rows

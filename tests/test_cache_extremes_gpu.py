@@ -201,3 +201,42 @@ def test_zero_scales_beside_values_of_any_size(L, N, exponent):
     cache.v_scale[torch.rand(cache.v_scale.shape, generator=g, device="cuda") < 0.5] = 0.0
     q = queries(1, 8, N, 64, BF, "heads")
     check(ma.cached_attention_b200(q, cache, table, ints(L)), q, cache, table, [L], None, 64)
+
+
+@pytest.mark.parametrize("N,exponents", [(N, e) for N in (20, 40) for e in ((-40, -40), (60, 60), (-40, 60), (-30, -20), (10, 30))] +
+                         [(N, e) for N in (1, 3, 4) for e in ((-14, -14), (15, 15), (-14, 15))])
+@pytest.mark.parametrize("size", [1e6, 1e9, 1e12, 1e30])
+@pytest.mark.parametrize("L", [300, 5000])
+def test_large_scores_over_values_of_other_scales(L, size, N, exponents):
+    """A value's scale is a part of its weight, however far beyond it the scores are: any scale with many rows, 2^-14 to 2^15 with few."""
+    import monarch_attention_b200 as ma
+    cache, table = filled(1, L // 64 + 2, 1, 64, 64, [L])
+    g = torch.Generator(device="cuda").manual_seed(3)
+    cache.v_scale.copy_(torch.exp2(torch.randint(exponents[0], exponents[1] + 1, cache.v_scale.shape, generator=g, device="cuda").float()))
+    q = (queries(1, 8, N, 64, BF, "heads").float() * size).to(BF)
+    out = ma.cached_attention_b200(q, cache, table, ints(L))[0].double().cpu()
+    k, v = (held(c, s, table[0], L, 64) for c, s in ((cache.k, cache.k_scale), (cache.v, cache.v_scale)))
+    want, clear = one_hot(q[0], k, v, L - N, 0.125)
+    assert bool(clear.any()) and bool(out.isfinite().all())
+    assert bool(((out - want).abs() <= (2.0 ** -11 + 2.0 ** -20 + 2.0 ** -8) * want.abs())[clear].all())
+
+
+@pytest.mark.parametrize("N", [1, 3, 4, 20, 40])
+@pytest.mark.parametrize("L", [200, 5000])
+@pytest.mark.parametrize("size", [1.0, 2.0 ** 20, 2.0 ** 30, 2.0 ** 100])
+def test_equal_keys_share_the_weight_whatever_the_scores(size, L, N):
+    """All keys are one and the same, so the result is the mean of the values, and the scales of the blocks are apart.
+
+    Weights are equal, so each is as far off as another; 2^-11 of a weight in f16, L 2^-24 of the largest value, sums 2^-20."""
+    import monarch_attention_b200 as ma
+    cache, table = filled(1, L // 64 + 2, 1, 64, 64, [L])
+    cache.k_scale.fill_(0.25)
+    cache.k.view(torch.uint8).fill_(0x38)
+    g = torch.Generator(device="cuda").manual_seed(3)
+    cache.v_scale.copy_(torch.exp2(torch.randint(-6, 7, cache.v_scale.shape, generator=g, device="cuda").float()))
+    q = torch.full((1, 4, N, 64), size, dtype=BF, device="cuda")
+    q[:, 1] *= -1
+    out = ma.cached_attention_b200(q, cache, table, ints(L), causal=False)[0]
+    v = held(cache.v, cache.v_scale, table[0], L, 64)[0]
+    bound = (2.0 ** -11 + 2.0 ** -20) * v.abs().mean(0) + 2.0 ** -24 * v.abs().amax()
+    close(out, v.mean(0).expand(4, N, 64), bound + 2.0 ** -8 * (v.mean(0).abs() + bound))
