@@ -448,8 +448,9 @@ __global__ void __launch_bounds__(W * 32, Shape<D, NT, W>::kCtas) attend_kernel(
 #pragma unroll
           for (int j = 0; j < 4; ++j) most[j & 1] = fmaxf(most[j & 1], s[mt][n][j] + vl[mt]);
         // The rows' reference is raised only when a weight would pass 2^kSlack: seldom once a head's first keys have been seen, and until then
-        // no lane has to know the others' scores.
-        if (__any_sync(0xffffffffu, most[0] > top[n][0] + kSlack || most[1] > top[n][1] + kSlack)) {
+        // no lane has to know the others' scores.  (A difference, which is exact; a reference plus kSlack is rounded to the last bit of a large reference, and a weight could
+        // pass 2^16.)
+        if (__any_sync(0xffffffffu, most[0] - top[n][0] > kSlack || most[1] - top[n][1] > kSlack)) {
 #pragma unroll
           for (int j = 0; j < 2; ++j) {
 #pragma unroll

@@ -240,3 +240,28 @@ def test_equal_keys_share_the_weight_whatever_the_scores(size, L, N):
     v = held(cache.v, cache.v_scale, table[0], L, 64)[0]
     bound = (2.0 ** -11 + 2.0 ** -20) * v.abs().mean(0) + 2.0 ** -24 * v.abs().amax()
     close(out, v.mean(0).expand(4, N, 64), bound + 2.0 ** -8 * (v.mean(0).abs() + bound))
+
+
+@pytest.mark.parametrize("e", range(18, 28))
+@pytest.mark.parametrize("delta", [8.0, 14.0, 15.0, 15.5, 16.0, 17.0, 24.0])
+@pytest.mark.parametrize("N", [1, 3, 40])
+def test_a_little_above_the_reference_at_large_scores(N, delta, e):
+    """Later keys that are 2^delta above earlier ones, at scores of 2^e where the last bit of a 32-bit score is 2^(e - 23): weights stay in f16.
+
+    In units of log2 all scores are off by that bit, so the earlier keys' share of 2^-delta by a factor of two to it; values are 1 and 2."""
+    import monarch_attention_b200 as ma
+    L, D = 512, 64
+    cache = ma.PagedKV.allocate(8, 1, D, 64)
+    cache.k_scale.fill_(1.0), cache.v_scale.fill_(1.0)
+    k, v = cache.k.view(torch.uint8), cache.v.view(torch.uint8)
+    k[..., 0] = 0x38          # 1: 2^e to all
+    k[4:, :, :, 1] = 0x38     # and delta to the later half
+    v[:4], v[4:] = 0x38, 0x40
+    q = torch.zeros(1, 4, N, D, dtype=BF, device="cuda")
+    q[..., 0], q[..., 1] = 2.0 ** e, delta
+    out = ma.cached_attention_b200(q, cache, torch.arange(8, dtype=torch.int32, device="cuda").view(1, 8), ints(L), causal=False, scale=math.log(2.0))
+    out = out.double().cpu()
+    assert bool(out.isfinite().all())
+    least, most = (2 - 1 / (1 + 2.0 ** x) for x in (delta - 2.0 ** (e - 22), delta + 2.0 ** (e - 22)))
+    slack = 2.0 ** -8 * 2 + 2.0 ** -10
+    assert bool((out >= least - slack).all()) and bool((out <= most + slack).all())
