@@ -318,7 +318,7 @@ __global__ void __launch_bounds__(W * 32, Shape<D, NT, W>::kCtas) attend_kernel(
           }
           amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
           amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-          const int exponent = min(max((int)(__float_as_uint(amax) >> 23), 27), 227);  // biased
+          const int exponent = min(max((int)(__float_as_uint(amax) >> 23), 27), 253);  // biased
           const float down = __uint_as_float((uint32_t)(254 - exponent) << 23);
           factor *= __uint_as_float((uint32_t)exponent << 23);
 #pragma unroll

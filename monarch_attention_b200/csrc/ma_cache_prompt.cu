@@ -286,7 +286,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
             amax = fmaxf(amax, fmaxf(fabsf(x.x), fabsf(x.y)));
           }
         }
-        const int exponent = min(max((int)(__float_as_uint(amax) >> 23), 27), 227);  // biased
+        const int exponent = min(max((int)(__float_as_uint(amax) >> 23), 27), 253);  // biased
         down = __uint_as_float((uint32_t)(254 - exponent) << 23);
         factor *= __uint_as_float((uint32_t)exponent << 23);
       }

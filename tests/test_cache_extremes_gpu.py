@@ -265,3 +265,17 @@ def test_a_little_above_the_reference_at_large_scores(N, delta, e):
     least, most = (2 - 1 / (1 + 2.0 ** x) for x in (delta - 2.0 ** (e - 22), delta + 2.0 ** (e - 22)))
     slack = 2.0 ** -8 * 2 + 2.0 ** -10
     assert bool((out >= least - slack).all()) and bool((out <= most + slack).all())
+
+
+@pytest.mark.parametrize("size", [1e33, 1e35, 1e36])
+@pytest.mark.parametrize("N", [1, 3, 4, 20, 40])
+def test_queries_near_the_end_of_32_bits(N, size):
+    """bf16 goes to 3e38: rows are brought to f16 by their own exponent whatever it is, as long as the scores are numbers of 32 bits."""
+    import monarch_attention_b200 as ma
+    cache, table = filled(1, 6, 1, 128, 64, [300])
+    q = (queries(1, 8, N, 128, BF, "heads").float() * size).to(BF)
+    out = ma.cached_attention_b200(q, cache, table, ints(300))[0].double().cpu()
+    k, v = (held(c, s, table[0], 300, 64) for c, s in ((cache.k, cache.k_scale), (cache.v, cache.v_scale)))
+    want, clear = one_hot(q[0], k, v, 300 - N, 128 ** -0.5)
+    assert bool(clear.any()) and bool(out.isfinite().all())
+    assert bool(((out - want).abs() <= (2.0 ** -11 + 2.0 ** -20 + 2.0 ** -8) * want.abs())[clear].all())
