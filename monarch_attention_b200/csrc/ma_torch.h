@@ -37,6 +37,9 @@ inline ma_b200_tensor view4(const at::Tensor& t) {
 
 inline at::Tensor unit_inner(const at::Tensor& t) { return t.stride(-1) == 1 || t.size(-1) == 1 ? t : t.contiguous(); }
 
+// Whether forward-mode differentiation has a tangent for t.
+inline bool has_tangent(const at::Tensor& t) { return t.defined() && t._fw_grad(0).defined(); }
+
 // Entry points of ma_torch_cache.cpp.
 PyObject* py_rotary(PyObject*, PyObject* const* args, Py_ssize_t n);
 PyObject* py_append(PyObject*, PyObject* const* args, Py_ssize_t n);

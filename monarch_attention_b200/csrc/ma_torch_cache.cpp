@@ -139,8 +139,7 @@ std::pair<Tensor, Tensor> rotate_with_history(const Tensor& x, const Tensor& y, 
   return out;
 }
 
-// (Either of q and k may be undefined.)
-std::pair<Tensor, Tensor> rotate_any(const Tensor& q, const Tensor& k, const Rotary& r, const optional<Tensor>& positions, bool inverse) {
+std::pair<Tensor, Tensor> rotate_reverse(const Tensor& q, const Tensor& k, const Rotary& r, const optional<Tensor>& positions, bool inverse) {
   const bool grad = at::GradMode::is_enabled();
   const bool gq = grad && q.defined() && q.requires_grad(), gk = grad && k.defined() && k.requires_grad();
   if (!gq && !gk) return rotate(q, k, r, positions, inverse);
@@ -148,6 +147,22 @@ std::pair<Tensor, Tensor> rotate_any(const Tensor& q, const Tensor& k, const Rot
   // one of the two has no gradient: its result is not to hang on the other's graph
   if (gq) return {rotate_with_history(q, Tensor(), r, positions, inverse).first, k.defined() ? rotate(Tensor(), k, r, positions, inverse).second : k};
   return {q.defined() ? rotate(q, Tensor(), r, positions, inverse).first : q, rotate_with_history(k, Tensor(), r, positions, inverse).first};
+}
+
+// (Either of q and k may be undefined.)  In forward mode a result's tangent is the rotated tangent.
+std::pair<Tensor, Tensor> rotate_any(const Tensor& q, const Tensor& k, const Rotary& r, const optional<Tensor>& positions, bool inverse) {
+  const auto out = rotate_reverse(q, k, r, positions, inverse);
+  if (!has_tangent(q) && !has_tangent(k)) return out;
+  auto tangent = [](const Tensor& t) {
+    Tensor d = has_tangent(t) ? t._fw_grad(0) : Tensor();
+    if (d.defined() && d._is_zerotensor()) d = at::zeros(d.sizes(), d.options());  // (which has no memory)
+    return d;
+  };
+  const Tensor dq = tangent(q), dk = tangent(k);
+  const auto d = rotate_any(dq, dk, r, positions, inverse);
+  if (dq.defined()) out.first._set_fw_grad(d.first, 0, false);
+  if (dk.defined()) out.second._set_fw_grad(d.second, 0, false);
+  return out;
 }
 
 // ---------------------------------------------------------------------------------------------- paged cache

@@ -91,7 +91,8 @@ def rotary_b200(query: Tensor, key: Tensor | None, rotary: RotaryPositions, posi
     ``positions``: int32 or int64 of shape (N) or (E, N) on the same device, negative ones allowed; None: 0 .. N-1.  ``inverse`` turns
     back (the transpose: a magnitude other than one is multiplied once more).  float32, bfloat16 and float16, any strides (an inner
     stride other than one costs a copy); results keep the order of their input's strides.  Arithmetic is in 32 bits, rounded
-    once.  Differentiable in both, any number of times.
+    once.  Differentiable in both, any number of times, in reverse and
+    in forward mode.
     """
     if not isinstance(rotary, RotaryPositions):
         raise TypeError("rotary must be a RotaryPositions")
