@@ -182,6 +182,9 @@ PyObject* py_forward(PyObject*, PyObject* const* args, Py_ssize_t n) {
   {
     pybind11::gil_scoped_release no_gil;
     check_inputs(q, k, v, mask_in);
+    check_no_tangent(q, "query");
+    check_no_tangent(k, "key");
+    check_no_tangent(v, "value");
     const bool grad = at::GradMode::is_enabled() && (q.requires_grad() || k.requires_grad() || v.requires_grad());
     TORCH_CHECK_VALUE(!grad || !out.defined(), "out= cannot be combined with inputs that require a gradient");
     if (!grad) {

@@ -39,6 +39,9 @@ inline at::Tensor unit_inner(const at::Tensor& t) { return t.stride(-1) == 1 || 
 
 // Whether forward-mode differentiation has a tangent for t.
 inline bool has_tangent(const at::Tensor& t) { return t.defined() && t._fw_grad(0).defined(); }
+inline void check_no_tangent(const at::Tensor& t, const char* name) {
+  TORCH_CHECK_NOT_IMPLEMENTED(!has_tangent(t), name, " has a tangent: there is no forward-mode derivative of this operator");
+}
 
 // Entry points of ma_torch_cache.cpp.
 PyObject* py_rotary(PyObject*, PyObject* const* args, Py_ssize_t n);

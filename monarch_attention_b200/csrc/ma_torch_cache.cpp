@@ -216,6 +216,7 @@ void check_16bit(const Tensor& t, const char* name) {
   TORCH_CHECK(t.is_cuda(), "monarch_attention_b200 runs on CUDA tensors only (there is no CPU path)");
   TORCH_CHECK_VALUE(t.scalar_type() == at::kBFloat16 || t.scalar_type() == at::kHalf, "unsupported dtype ", t.scalar_type(), " (bfloat16 or float16)");
   TORCH_CHECK_VALUE(!at::GradMode::is_enabled() || !t.requires_grad(), name, " requires a gradient: the cached operators have none (torch.no_grad())");
+  check_no_tangent(t, name);
   TORCH_CHECK_VALUE(t.size(0) <= INT32_MAX && t.size(1) <= INT32_MAX && t.size(2) <= INT32_MAX, name, " is too large");
 }
 

@@ -1,4 +1,4 @@
-"""Forward-mode derivatives of the rotation."""
+"""Forward-mode derivatives: the rotation has them, the attentions and the append refuse what they would lose."""
 import pytest
 import torch
 import torch.autograd.forward_ad as fwAD
@@ -66,3 +66,27 @@ def test_a_tangent_of_zeros_that_has_no_memory():
         y, _ = ma.rotary_b200(fwAD.make_dual(q, torch._efficientzerotensor(q.shape, device="cuda")), None, r)
         primal, tangent = fwAD.unpack_dual(y)
         assert torch.equal(primal, ma.rotary_b200(q, None, r)[0]) and tangent.shape == q.shape and not bool(tangent.any())
+
+
+def test_what_has_no_forward_derivative_is_refused():
+    """A tangent that would be lost without a word: the attention of the encoder, the append, the attention over the cache."""
+    import monarch_attention_b200 as ma
+    module = ma.MonarchAttention(16, 2, ma.PadType.post)
+    x = [torch.randn(1, 2, 64, 64, device="cuda") for _ in range(3)]
+    cache = ma.PagedKV.allocate(4, 2, 64, 16)
+    table, lengths = torch.arange(4, dtype=torch.int32, device="cuda").view(1, 4), torch.full((1,), 5, dtype=torch.int32, device="cuda")
+    t = torch.randn(1, 2, 5, 64, device="cuda").to(torch.bfloat16)
+    with fwAD.dual_level():
+        for i in range(3):
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                module(*(fwAD.make_dual(a, torch.ones_like(a)) if i == j else a for j, a in enumerate(x)))
+        d = fwAD.make_dual(t, torch.ones_like(t))
+        for call in (lambda: ma.append_kv_b200(cache, d, t, table, lengths), lambda: ma.append_kv_b200(cache, t, d, table, lengths),
+                     lambda: ma.append_kv_b200(cache, t, t, table, lengths, query=d), lambda: ma.cached_attention_b200(d, cache, table, lengths)):
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                call()
+        assert module(*x).shape == x[0].shape   # (a dual level alone asks for nothing)
+        ma.append_kv_b200(cache, t, t, table, lengths)
+    with torch.no_grad(), fwAD.dual_level():   # (forward mode goes on without the reverse)
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            ma.cached_attention_b200(fwAD.make_dual(t, torch.ones_like(t)), cache, table, lengths)
