@@ -259,6 +259,9 @@ Tensor append(const Cache& cache, const Tensor& k_in, const Tensor& v_in, const 
     p.rotary = &r;
   }
   raise_for_status(ma_b200_cache_append(&p, c10::cuda::getCurrentCUDAStream().stream()));
+  // (what a graph has saved of the pool is not what it was)
+  for (const Tensor* t : {&cache.k, &cache.v, &cache.k_scale, &cache.v_scale})
+    if (!t->is_inference()) t->unsafeGetTensorImpl()->bump_version();
   return q_out;
 }
 

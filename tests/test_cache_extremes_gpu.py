@@ -279,3 +279,23 @@ def test_queries_near_the_end_of_32_bits(N, size):
     want, clear = one_hot(q[0], k, v, 300 - N, 128 ** -0.5)
     assert bool(clear.any()) and bool(out.isfinite().all())
     assert bool(((out - want).abs() <= (2.0 ** -11 + 2.0 ** -20 + 2.0 ** -8) * want.abs())[clear].all())
+
+
+def test_an_append_is_a_change_of_the_pool():
+    """A backward pass that needs what the pool held before says so, as after any operation in place."""
+    import monarch_attention_b200 as ma
+    cache = ma.PagedKV.allocate(2, 1, 64, 16)
+    table = torch.arange(2, dtype=torch.int32, device="cuda").view(1, 2)
+    k = queries(1, 1, 1, 64, BF, "heads")
+    w = torch.ones_like(cache.v_scale).requires_grad_(True)
+    y = (w * cache.v_scale).sum()
+    before = [t._version for t in cache]
+    with torch.no_grad():
+        ma.append_kv_b200(cache, k, k, table, ints(1))
+    assert all(t._version > n for t, n in zip(cache, before))
+    with pytest.raises(RuntimeError, match="modified by an inplace"):
+        y.backward()
+    with torch.inference_mode():
+        pool = ma.PagedKV.allocate(2, 1, 64, 16)
+        ma.append_kv_b200(pool, k, k, table, ints(1))
+    assert torch.equal(pool.k.view(torch.uint8), cache.k.view(torch.uint8)) and torch.equal(pool.k_scale, cache.k_scale)
