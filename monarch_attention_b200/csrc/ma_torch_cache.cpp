@@ -176,6 +176,10 @@ ma_b200_cache cache_struct(const Cache& c, const at::Device& device) {
   TORCH_CHECK_VALUE(c.k.scalar_type() == at::kFloat8_e4m3fn && c.v.scalar_type() == at::kFloat8_e4m3fn, "the cache's k and v must be float8_e4m3fn");
   TORCH_CHECK_VALUE(c.k.device() == device && c.v.device() == device && c.k_scale.device() == device && c.v_scale.device() == device,
                     "the cache must be on the query's or key's device");
+  for (const Tensor* t : {&c.k, &c.v, &c.k_scale, &c.v_scale}) {
+    TORCH_CHECK_VALUE(!at::GradMode::is_enabled() || !t->requires_grad(), "the cache requires a gradient: the cached operators have none (torch.no_grad())");
+    check_no_tangent(*t, "the cache");
+  }
   TORCH_CHECK_VALUE(c.k.stride(3) == 1 && c.v.stride(3) == 1, "the features of the cache's k and v must lie next to one another");
   for (const Tensor* s : {&c.k_scale, &c.v_scale}) {
     TORCH_CHECK_VALUE(s->scalar_type() == at::kFloat && s->dim() == 3 && s->size(0) == c.k.size(0) && s->size(1) == c.k.size(1) &&

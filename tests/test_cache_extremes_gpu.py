@@ -299,3 +299,17 @@ def test_an_append_is_a_change_of_the_pool():
         pool = ma.PagedKV.allocate(2, 1, 64, 16)
         ma.append_kv_b200(pool, k, k, table, ints(1))
     assert torch.equal(pool.k.view(torch.uint8), cache.k.view(torch.uint8)) and torch.equal(pool.k_scale, cache.k_scale)
+
+
+@pytest.mark.parametrize("part", ["k_scale", "v_scale"])
+def test_a_pool_that_requires_a_gradient_is_refused(part):
+    import monarch_attention_b200 as ma
+    cache = ma.PagedKV.allocate(2, 1, 64, 16)
+    cache = cache._replace(**{part: getattr(cache, part).clone().requires_grad_(True)})
+    table = torch.arange(2, dtype=torch.int32, device="cuda").view(1, 2)
+    k = queries(1, 1, 1, 64, BF, "heads")
+    for call in (lambda: ma.append_kv_b200(cache, k, k, table, ints(1)), lambda: ma.cached_attention_b200(k, cache, table, ints(1))):
+        with pytest.raises(ValueError, match="requires a gradient"):
+            call()
+        with torch.no_grad():
+            call()
