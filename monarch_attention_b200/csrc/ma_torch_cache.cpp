@@ -282,6 +282,8 @@ Tensor attend(const Tensor& q_in, const Cache& cache, const Tensor& table, const
                     q_in.sizes(), " does not match the cache's ", p.cache.heads, " heads of ", p.cache.width);
   p.sequences = sequences_struct(table, lengths, counts, q_in.size(0), q_in.device());
   TORCH_CHECK_VALUE(window >= 0 && window <= INT32_MAX, "window must not be negative");
+  // (before it becomes a number of 32 bits, where a smaller one is zero: none)
+  TORCH_CHECK_VALUE(softcap == 0.0 || (softcap >= 1e-20 && softcap <= 1e30), "softcap must be 0 (none) or from 1e-20 to 1e30");
   const int64_t E = q_in.size(0), H = q_in.size(1), N = q_in.size(2), W = q_in.size(3);
   Tensor out;
   if (out_in.has_value()) {

@@ -313,3 +313,11 @@ def test_a_pool_that_requires_a_gradient_is_refused(part):
             call()
         with torch.no_grad():
             call()
+
+
+@pytest.mark.parametrize("softcap", [1e-50, -1e-50, 1e-21, -1.0, 1e31, NAN])
+def test_caps_that_would_be_none_in_32_bits_are_refused(softcap):
+    import monarch_attention_b200 as ma
+    cache, table = filled(1, 2, 1, 64, 16, [20])
+    with pytest.raises(ValueError, match="softcap"):
+        ma.cached_attention_b200(queries(1, 1, 1, 64, BF, "heads"), cache, table, ints(20), softcap=softcap)
