@@ -159,6 +159,10 @@ class MonarchAttention(nn.Module):
     unknown name raises ``ValueError`` exactly as the reference does.
     """
 
+    # Set to a RotaryPositions to have queries and keys rotated at positions 0 .. N-1 before the attention.
+    # (Of the class, so that modules that were pickled without it have it too.)
+    rotary = None
+
     def __init__(self, block_size, num_steps, pad_type, impl="b200"):
         super().__init__()
         self.block_size = block_size
@@ -171,8 +175,6 @@ class MonarchAttention(nn.Module):
         # Set to True to get the result as a view of a (batch, tokens, heads, width) buffer (see
         # monarch_attention_b200); only the default implementation honours it.
         self.token_major_output = False
-        # Set to a RotaryPositions to have queries and keys rotated at positions 0 .. N-1 before the attention.
-        self.rotary = None
 
     def forward(self, query, key, value, attention_mask=None):
         if self.rotary is not None:
