@@ -31,7 +31,8 @@ class RotaryPositions:
     * ``"linear"``: all frequencies divided by ``factor`` (positions are interpolated);
     * ``"ntk"``: ``base`` multiplied by ``factor ** (dim / (dim - 2))``: the slowest pair is divided by ``factor``, the fastest kept;
     * ``"yarn"``: by parts: pairs of more than 32 turns in ``trained_length`` kept, of less than one divided by ``factor``, those
-      between mixed linearly in their number of turns; sines and cosines multiplied by ``0.1 ln(factor) + 1``.
+      between mixed linearly in their number of turns; sines and cosines multiplied by ``0.1 ln(factor) + 1``; ``factor`` from 1 on.  (Some
+      checkpoints were trained with a mixture that is linear in the pair's number between two borders; that is another rotation.)
 
     The object holds no device memory: it is made once and serves any device, stream and position.
     """
@@ -48,6 +49,8 @@ class RotaryPositions:
             raise ValueError(f"unknown scaling {scaling!r}")
         if scaling is not None and not (factor > 0.0 and math.isfinite(factor)):
             raise ValueError("factor must be positive")
+        if scaling == "yarn" and factor < 1.0:
+            raise ValueError("the 'yarn' scaling needs a factor of at least 1")
         if scaling == "ntk" and dim == 2:
             raise ValueError("the 'ntk' scaling needs more than one pair")
         self.dim, self.base, self.pairs, self.scaling, self.factor = int(dim), float(base), pairs, scaling, float(factor)

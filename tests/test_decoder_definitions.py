@@ -1,4 +1,5 @@
 """Definitions of the decoder's side that need no GPU: modules from before, rotations that are none."""
+import pytest
 import torch
 
 import monarch_attention_b200 as ma
@@ -12,3 +13,11 @@ def test_a_module_pickled_without_a_rotary_has_none():
     old.__setstate__({k: v for k, v in module.__dict__.items() if k != "rotary"})
     x = torch.ones(1, 1, 2, 4)
     assert old.rotary is None and torch.equal(old(x, x, x), 3 * x) and torch.equal(module(x, x, x), 3 * x)
+
+
+@pytest.mark.parametrize("factor", [0.99, 0.5, 1e-5])
+def test_yarn_is_for_longer_contexts(factor):
+    """Below one its multiplier of sines would shrink scores, and end below zero."""
+    with pytest.raises(ValueError, match="factor"):
+        ma.RotaryPositions(64, scaling="yarn", factor=factor, trained_length=4096)
+    assert ma.RotaryPositions(64, scaling="yarn", factor=1.0, trained_length=4096).magnitude == 1.0
