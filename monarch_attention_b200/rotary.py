@@ -56,16 +56,21 @@ class RotaryPositions:
         self.dim, self.base, self.pairs, self.scaling, self.factor = int(dim), float(base), pairs, scaling, float(factor)
         self.trained_length = trained_length
         self.magnitude = 1.0
-        b = self.base * self.factor ** (dim / (dim - 2)) if scaling == "ntk" else self.base
-        f = [b ** (-2.0 * i / dim) for i in range(dim // 2)]
-        if scaling == "linear":
-            f = [x / self.factor for x in f]
-        elif scaling == "yarn":
-            if not trained_length or trained_length <= 0:
-                raise ValueError("the 'yarn' scaling needs trained_length")
-            kept = [min(1.0, max(0.0, (trained_length * x / (2 * math.pi) - 1.0) / 31.0)) for x in f]
-            f = [x * (g + (1.0 - g) / self.factor) for x, g in zip(f, kept)]
-            self.magnitude = 0.1 * math.log(self.factor) + 1.0
+        try:
+            b = self.base * self.factor ** (dim / (dim - 2)) if scaling == "ntk" else self.base
+            f = [b ** (-2.0 * i / dim) for i in range(dim // 2)]
+            if scaling == "linear":
+                f = [x / self.factor for x in f]
+            elif scaling == "yarn":
+                if not trained_length or trained_length <= 0:
+                    raise ValueError("the 'yarn' scaling needs trained_length")
+                kept = [min(1.0, max(0.0, (trained_length * x / (2 * math.pi) - 1.0) / 31.0)) for x in f]
+                f = [x * (g + (1.0 - g) / self.factor) for x, g in zip(f, kept)]
+                self.magnitude = 0.1 * math.log(self.factor) + 1.0
+        except (OverflowError, ZeroDivisionError):
+            b, f = math.inf, []
+        if not all(math.isfinite(x) for x in (b, *f)):
+            raise ValueError("the frequencies are no finite numbers")
         #: radians per position of each pair
         self.frequencies = tuple(f)
         turns = [round(Fraction(x) / (2 * _PI) * 2 ** 64) % 2 ** 64 for x in f]

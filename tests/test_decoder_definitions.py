@@ -21,3 +21,9 @@ def test_yarn_is_for_longer_contexts(factor):
     with pytest.raises(ValueError, match="factor"):
         ma.RotaryPositions(64, scaling="yarn", factor=factor, trained_length=4096)
     assert ma.RotaryPositions(64, scaling="yarn", factor=1.0, trained_length=4096).magnitude == 1.0
+
+
+@pytest.mark.parametrize("kw", [dict(base=1e300, scaling="ntk", factor=1e300), dict(base=1e200, scaling="ntk", factor=1e150), dict(base=1e-200, scaling="ntk", factor=1e-200), dict(base=1e-320), dict(base=1e-300, scaling="linear", factor=1e-100)])
+def test_frequencies_that_are_no_numbers_are_refused(kw):
+    with pytest.raises(ValueError, match="frequencies"):
+        ma.RotaryPositions(64, **kw)
