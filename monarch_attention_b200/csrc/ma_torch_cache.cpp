@@ -1,10 +1,11 @@
 // Native halves of the rotary positions, the paged cache and the attention over it: input checks, results and
 // workspaces from PyTorch's caching allocator, and the launches through the C ABI.
 #include <ATen/ExpandUtils.h>
-#include <ATen/MemoryOverlap.h>
 #include <torch/csrc/autograd/function.h>
 #include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/saved_variable.h>
+
+#include <algorithm>
 
 #include "ma_torch.h"
 
@@ -25,6 +26,52 @@ optional<Tensor> optional_of(PyObject* x, const char* name) {
 
 void check_python() {
   if (PyErr_Occurred()) throw python_error();
+}
+
+// ---------------------------------------------------------------------------------------------- who writes where
+
+// A tensor's dimensions of more than one element, the largest stride first.
+struct Places {
+  struct Dim {
+    int64_t size, stride;
+    bool operator==(const Dim& o) const { return size == o.size && stride == o.stride; }
+  };
+  c10::SmallVector<Dim, 4> dims;
+  const char *begin, *end;  // bytes from its first element to behind its last
+  int64_t item;
+
+  explicit Places(const Tensor& t) : begin(static_cast<const char*>(t.data_ptr())), item(t.element_size()) {
+    int64_t last = 0;
+    for (int64_t i = 0; i < t.dim(); ++i) {
+      if (t.size(i) > 1) dims.push_back({t.size(i), t.stride(i)});
+      last += (t.size(i) - 1) * t.stride(i);
+    }
+    std::sort(dims.begin(), dims.end(), [](const Dim& a, const Dim& b) { return a.stride > b.stride; });
+    end = begin + (t.numel() > 0 ? (last + 1) * item : 0);
+  }
+  // Each stride passes over all that the smaller ones reach, so that no two elements are in one place.  (Others may have that too; they are not taken.)
+  bool distinct() const {
+    int64_t reach = 0;
+    for (size_t i = dims.size(); i-- > 0;) {
+      if (dims[i].stride <= reach) return false;
+      reach += (dims[i].size - 1) * dims[i].stride;
+    }
+    return true;
+  }
+  // Two elements of dims[i ..] are `distance` apart.
+  bool differ_by(int64_t distance, size_t i = 0) const {
+    if (i == dims.size()) return distance == 0;
+    int64_t n = distance / dims[i].stride - (distance % dims[i].stride < 0);
+    for (int64_t k = n; k <= n + 1; ++k)
+      if (k > -dims[i].size && k < dims[i].size && differ_by(distance - k * dims[i].stride, i + 1)) return true;
+    return false;
+  }
+};
+// Whether an element of a is in the place of one of b, both with distinct elements; true as well where that is not seen from equal strides.
+bool meet(const Places& a, const Places& b) {
+  if (a.end <= b.begin || b.end <= a.begin) return false;
+  const int64_t distance = b.begin - a.begin;
+  return !(a.dims == b.dims) || a.item != b.item || distance % a.item != 0 || a.differ_by(distance / a.item);
 }
 
 // ---------------------------------------------------------------------------------------------- rotary positions
@@ -291,18 +338,20 @@ Tensor attend(const Tensor& q_in, const Cache& cache, const Tensor& table, const
     TORCH_CHECK_VALUE(out.sizes() == q_in.sizes() && out.scalar_type() == q_in.scalar_type() && out.device() == q_in.device() && out.stride(3) == 1,
                       "out must have the query's shape, dtype and device and unit inner stride");
     TORCH_CHECK_VALUE(!at::GradMode::is_enabled() || !out.requires_grad(), "out requires a gradient");
-    TORCH_CHECK_VALUE(at::has_internal_overlap(out) != at::MemOverlap::Yes, "the rows of out overlap");
+    TORCH_CHECK_VALUE(Places(out).distinct(), "the rows of out overlap");
   } else {
     const at::TensorOptions o = at::TensorOptions().dtype(q_in.scalar_type()).device(q_in.device());
     out = token_major ? at::detail::empty_strided_cuda({E, H, N, W}, {N * H * W, W, H * W, 1}, o) : at::detail::empty_cuda({E, H, N, W}, o);
   }
   if (E == 0 || N == 0) return out;
+  const Tensor q = aligned(q_in, 16);
   if (out_in.has_value()) {
     // (the query itself may take the result: a row is read by those that write it, before they do)
-    TORCH_CHECK_VALUE(at::get_overlap_status(out, q_in) != at::MemOverlapStatus::Partial, "out and query overlap in part");
+    bool same = out.data_ptr() == q.data_ptr();
+    for (int i = 0; i < 4; ++i) same = same && (out.size(i) == 1 || out.stride(i) == q.stride(i));
+    TORCH_CHECK_VALUE(same || !meet(Places(out), Places(q)), "out and query overlap in part");
     if (!out.is_inference()) out.unsafeGetTensorImpl()->bump_version();
   }
-  const Tensor q = aligned(q_in, 16);
   p.E = (int32_t)E; p.H = (int32_t)H; p.N = (int32_t)N;
   p.dtype = dtype_code(q.scalar_type());
   p.causal = causal;

@@ -92,7 +92,7 @@ def cached_attention_b200(query: Tensor, cache: PagedKV, page_table: Tensor, len
     all of the call's rows of its sequence and head, masked ones too (zero times NaN).
 
     The result has the query's dtype, and with ``token_major_output`` is a view of an (E, N, H, width) buffer; ``out`` (rows on 16-byte
-    boundaries; the query itself is fine) takes it in place.  Scores and sums are in 32 bits; a bfloat16 query is read in 16-bit steps of 2^-11 of itself and 2^-25 of
+    boundaries; the query itself, or rows beside its own in a common buffer, are fine, rows over one another or over others of the query's are refused) takes it in place.  Scores and sums are in 32 bits; a bfloat16 query is read in 16-bit steps of 2^-11 of itself and 2^-25 of
     its row's largest magnitude.  Weights, each times its value's scale, are rounded to 2^-11 of themselves or 2^-32 of their row's largest, whichever is more; what is
     below 2^-25 of a sum so far may be lost from it, as 32 bits have it.  Where scores pass 2^27 and there are 32 rows or fewer to a cache head (tokens times
     query heads of it), scales of values are to be from 2^-14 to 2^15.  The same call gives the same bits; what else is in the batch may

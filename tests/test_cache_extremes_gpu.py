@@ -321,3 +321,28 @@ def test_caps_that_would_be_none_in_32_bits_are_refused(softcap):
     cache, table = filled(1, 2, 1, 64, 16, [20])
     with pytest.raises(ValueError, match="softcap"):
         ma.cached_attention_b200(queries(1, 1, 1, 64, BF, "heads"), cache, table, ints(20), softcap=softcap)
+
+
+@pytest.mark.parametrize("N,H", [(4, 4), (40, 4)])
+def test_a_result_in_a_buffer_with_the_query(N, H):
+    """In its place or beside it, row for row, it is taken; over rows that others still read it is refused, whatever the strides are."""
+    import monarch_attention_b200 as ma
+    L, D = 300, 64
+    cache, table = filled(2, 6, 2, D, 64, [L, L])
+    n = ints(L, L)
+    whole = torch.zeros(2 * (N + 1) * 3 * H * D + N * D, dtype=BF, device="cuda")
+    buffer = whole[:2 * (N + 1) * 3 * H * D].view(2, N + 1, 3, H, D)
+    buffer[:, :N, 0] = queries(2, H, N, D, BF, "heads").transpose(1, 2)
+    part = lambda i, first=0: buffer[:, first:first + N, i].transpose(1, 2)   # noqa: E731
+    q = part(0)
+    want = ma.cached_attention_b200(q, cache, table, n)
+    for bad in (part(0, 1), part(0).transpose(1, 2) if N == H else part(0, 1), buffer.view(2, -1)[:, H * D // 2:].as_strided(q.shape, q.stride()),
+                buffer.as_strided(q.shape, (q.stride(0), D, 3 * H * D + D, 1))):
+        with pytest.raises(ValueError, match="overlap"):
+            ma.cached_attention_b200(q, cache, table, n, out=bad)
+    with pytest.raises(ValueError, match="overlap"):   # rows of the result over one another
+        ma.cached_attention_b200(q, cache, table, n, out=torch.zeros(2 * H * N * D, dtype=BF, device="cuda").as_strided(q.shape, (H * N * D // 2, N * D // 2, D // 2, 1)))
+    for i in (1, 2, 0):
+        assert torch.equal(ma.cached_attention_b200(q, cache, table, n, out=part(i)), want)
+        assert not bool(buffer[:, N].any())
+    assert torch.equal(part(1), want) and torch.equal(part(2), want)
