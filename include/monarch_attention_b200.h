@@ -357,7 +357,8 @@ typedef struct ma_b200_sequences {
  * (dim a multiple of 16).  A block's scale is the smallest power of two from 2^-40 to 2^60 with which 448 holds its largest magnitude, and never
  * falls while the block has older tokens; those are re-expressed when it rises.  Values are rounded to nearest even; magnitudes
  * above 448 * 2^60 are stored as that, NaN as NaN.  If H > 0, q (E, H, N, width) is rotated into q_out (which may be q) in the same
- * launch, rows of padding as zeros.  The pages that a call writes must belong to one sequence each. */
+ * launch, rows of padding as zeros.  The pages that a call writes must belong to one sequence each, and pages,
+ * heads and tokens of k, of v and of their scales must not overlap. */
 typedef struct ma_b200_append {
   int32_t abi_version;
   int32_t E, H, N;

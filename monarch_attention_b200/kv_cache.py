@@ -71,7 +71,8 @@ def append_kv_b200(cache: PagedKV, key: Tensor, value: Tensor, page_table: Tenso
     rotated copy is returned, with rows of padding as zeros.  A block's scale is the smallest power of two from 2^-40 to 2^60 with which 448 holds the
     block's largest magnitude.  It never falls while the block has older tokens; when it rises they are re-expressed, which is exact but for
     values that become subnormal.  Magnitudes above 448 * 2^60 (infinities) are stored as that, NaN as NaN.  The pages that a call writes to
-    must stand once in one sequence's row of the table (pages that are only read may be shared).  No gradient: inputs that require one are refused.
+    must stand once in one sequence's row of the table (pages that are only read may be shared), and the pool's pages, heads and tokens must not
+    overlap (keys and values may lie in one buffer, with the same strides).  No gradient: inputs that require one are refused.
     """
     if _append is None:
         _load()

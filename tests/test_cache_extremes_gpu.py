@@ -346,3 +346,27 @@ def test_a_result_in_a_buffer_with_the_query(N, H):
         assert torch.equal(ma.cached_attention_b200(q, cache, table, n, out=part(i)), want)
         assert not bool(buffer[:, N].any())
     assert torch.equal(part(1), want) and torch.equal(part(2), want)
+
+
+def test_pools_whose_parts_are_over_one_another_are_not_written():
+    import monarch_attention_b200 as ma
+    table = torch.arange(2, dtype=torch.int32, device="cuda").view(1, 2)
+    k = queries(1, 2, 20, 64, BF, "heads")
+    good = ma.PagedKV.allocate(4, 2, 64, 32)
+    byte, e4m3 = torch.uint8, torch.float8_e4m3fn
+    for bad in (dict(v=good.k), dict(v_scale=good.k_scale), dict(k=good.k[:1].expand(4, 2, 32, 64)), dict(v=good.v[:, :1].expand(4, 2, 32, 64)),
+                dict(k_scale=good.k_scale[:, :1].expand(4, 2, 2)), dict(k=good.k.view(byte).view(-1).as_strided((4, 2, 32, 64), (4096, 1024, 64, 1)).view(e4m3)),
+                dict(k=good.k[:3], v=good.k[1:], k_scale=good.k_scale[:3], v_scale=good.v_scale[:3])):
+        with pytest.raises(ValueError, match="overlap"):
+            ma.append_kv_b200(good._replace(**bad), k, k, table, ints(20))
+    # one buffer for keys and values, page by page or token by token, is a pool like any other; reading shared pages is, too
+    ma.append_kv_b200(good, k, -k, table, ints(20))
+    q = queries(1, 4, 1, 64, BF, "heads")
+    want = ma.cached_attention_b200(q, good, table, ints(20))
+    for codes, scales in ((torch.zeros(4, 2, 2, 32, 64, dtype=byte, device="cuda").view(e4m3).unbind(1), torch.zeros(4, 2, 2, 2, device="cuda").unbind(1)),
+                          ([t.permute(0, 2, 1, 3) for t in torch.zeros(4, 32, 2, 2, 64, dtype=byte, device="cuda").view(e4m3).unbind(2)],
+                           torch.zeros(2, 4, 2, 2, device="cuda").unbind(0))):
+        pool = ma.PagedKV(*codes, *scales)
+        ma.append_kv_b200(pool, k, -k, table, ints(20))
+        assert torch.equal(ma.cached_attention_b200(q, pool, table, ints(20)), want)
+    ma.cached_attention_b200(q, good._replace(v=good.k), table, ints(20))
