@@ -9,8 +9,9 @@ Which tokens a call is about is said the same way everywhere: ``page_table`` (E,
 sequence; ``lengths`` (E) int32, the tokens of each sequence, those of the call among them; ``counts`` (E) int32 or None, how many of
 the call's N tokens are a sequence's own (the rest is padding behind them).  Token n of the call stands at position
 ``lengths[e] - counts[e] + n``.  The three are read on the GPU, so that nothing waits for the host and calls can be captured in a
-graph.  A length that the table has no room for, a count above N (or above the length) or a page outside the cache is not followed: what
-it concerns is left out or undefined, and a later call on the device raises ``RuntimeError``.
+graph.  A length that the table has no room for, a count above N or a page outside the cache is not followed: what
+it concerns is left out or undefined, and a later call on the device raises ``RuntimeError``.  A count above the length is one of these when
+appending; in the attention, rows in front of a sequence's first token see no key and are zero.
 """
 from __future__ import annotations
 
