@@ -389,6 +389,11 @@ typedef struct ma_b200_attend {
 MA_B200_API size_t ma_b200_cache_attend_workspace_bytes(const ma_b200_attend* p);
 MA_B200_API int ma_b200_cache_attend(const ma_b200_attend* p, void* workspace, size_t workspace_bytes, void* stream);
 
+/* Test hook: the same call, in bf16 and of 33 rows or more to a cache head (N * H / heads), with a wait of every thread block that has keys run out.  The result is
+ * undefined, ma_b200_poll_device_status() reports MA_B200_DEVICE_WAIT_EXPIRED, and the next ordinary call is unaffected.  Nothing faults, traps or
+ * spins without bound. */
+MA_B200_API int ma_b200_selftest_attend_wait_expiry(const ma_b200_attend* p, void* workspace, size_t workspace_bytes, void* stream);
+
 /* Without synchronising anything: has a kernel of the cache on `device` met a length, count or page outside its range since the last
  * poll?  MA_B200_OK, or MA_B200_DEVICE_BAD_SEQUENCE once per incident; trails the GPU by at most the kernels in flight. */
 MA_B200_API int ma_b200_poll_cache_status(int device);

@@ -30,7 +30,7 @@ EXPORTS = (
     "ma_b200_poll_device_status", "ma_b200_selftest_wait_expiry", "ma_b200_selftest_generic_general_form",
     "ma_b200_backward_workspace_bytes", "ma_b200_backward", "ma_b200_forward_typed_mask", "ma_b200_backward_typed_mask",
     "ma_b200_rotary_apply", "ma_b200_cache_append", "ma_b200_cache_attend_workspace_bytes", "ma_b200_cache_attend",
-    "ma_b200_poll_cache_status",
+    "ma_b200_poll_cache_status", "ma_b200_selftest_attend_wait_expiry",
 )
 
 
@@ -166,6 +166,8 @@ def load() -> C.CDLL:
     lib.ma_b200_cache_attend_workspace_bytes.restype = C.c_size_t
     lib.ma_b200_cache_attend.argtypes = [C.POINTER(Attend), C.c_void_p, C.c_size_t, C.c_void_p]
     lib.ma_b200_cache_attend.restype = C.c_int
+    lib.ma_b200_selftest_attend_wait_expiry.argtypes = [C.POINTER(Attend), C.c_void_p, C.c_size_t, C.c_void_p]
+    lib.ma_b200_selftest_attend_wait_expiry.restype = C.c_int
     lib.ma_b200_poll_cache_status.argtypes = [C.c_int]
     lib.ma_b200_poll_cache_status.restype = C.c_int
     lib.ma_b200_host_last_error.argtypes = []

@@ -81,13 +81,14 @@ struct AttendArgs {
 // Whether a row of the call's token n has a key at all; the others' results are zero, whatever the sums of their tile have caught.
 __device__ __forceinline__ bool sees_keys(const AttendArgs& a, int len, int count, int n) { return n < count && (!a.causal || len - count + n >= 0); }
 
-// Bytes of scratch, and how many row tiles and CTAs the call takes.
+// Bytes of scratch.
 size_t attend_workspace(int E, int N, int H, int kv_heads, int width, int window, long long longest);
-cudaError_t launch_attend(AttendArgs a, int dtype, int width, void* workspace, long long longest, int* wait_status, cudaStream_t stream);
+// (wait_expiry, a self-test: a wait of the kernel for many rows runs out.)
+cudaError_t launch_attend(AttendArgs a, int dtype, int width, void* workspace, long long longest, int* wait_status, bool wait_expiry, cudaStream_t stream);
 // The pieces of `entries` heads and blocks of tile_rows rows (a.split, a.part_o, a.part_ml; a head's pieces `stride` slots apart) into a.out.
 cudaError_t launch_join(const AttendArgs& a, int dtype, int width, int tile_rows, int entries, int stride, cudaStream_t stream);
 // The kernel for many rows (ma_cache_prompt.cu).
 size_t prompt_workspace(int E, int N, int H, int kv_heads, int width, long long longest);
-cudaError_t launch_prompt(AttendArgs a, int dtype, int width, void* workspace, long long longest, int* wait_status, cudaStream_t stream);
+cudaError_t launch_prompt(AttendArgs a, int dtype, int width, void* workspace, long long longest, int* wait_status, bool wait_expiry, cudaStream_t stream);
 
 }  // namespace ma

@@ -77,6 +77,29 @@ int launched(cudaError_t ce, const char* what) {
   return MA_B200_OK;
 }
 
+int attend(const ma_b200_attend* p, void* workspace, size_t workspace_bytes, void* stream, bool wait_expiry) {
+  int rc = check_attend_shape(p);
+  if (rc != MA_B200_OK) return rc;
+  if (p->window < 0 || (p->window > 0 && !p->causal)) return invalid("window must not be negative, and needs causal");
+  if (!isfinite(p->scale) || !(p->softcap == 0.0f || (p->softcap >= 1e-20f && p->softcap <= 1e30f)))
+    return invalid("scale must be finite, softcap 0 (none) or from 1e-20 to 1e30");
+  ma::AttendArgs a{};
+  if ((rc = check_cache(p->cache, p->sequences, p->E, p->H, p->N, p->dtype, &a.cache)) != MA_B200_OK) return rc;
+  if ((rc = check_tensor(p->q, "q", 2, 16)) != MA_B200_OK || (rc = check_tensor(p->out, "out", 2, 16)) != MA_B200_OK) return rc;
+  const long long most = longest(p->sequences, p->cache.page_size);
+  const size_t need = ma::attend_workspace(p->E, p->N, p->H, p->cache.heads, p->cache.width, p->window, most);
+  if (workspace == nullptr || reinterpret_cast<uintptr_t>(workspace) % 256 != 0) return invalid("workspace is NULL or not 256-byte aligned");
+  if (workspace_bytes < need)
+    return fail_with(MA_B200_WORKSPACE_TOO_SMALL, "workspace has " + std::to_string(workspace_bytes) + " bytes, need " + std::to_string(need));
+  int dev = 0;
+  (void)cudaGetDevice(&dev);
+  int* const wait_status = ma::host_status_word(dev, 0);
+  a.q = view(p->q); a.out = view(p->out);
+  a.E = p->E; a.N = p->N; a.H = p->H; a.group = p->H / p->cache.heads;
+  a.causal = p->causal != 0; a.window = p->window; a.scale = p->scale; a.softcap = p->softcap;
+  return launched(ma::launch_attend(a, p->dtype, p->cache.width, workspace, most, wait_status, wait_expiry, reinterpret_cast<cudaStream_t>(stream)), "attention over the cache");
+}
+
 }  // namespace
 
 extern "C" {
@@ -121,26 +144,12 @@ size_t ma_b200_cache_attend_workspace_bytes(const ma_b200_attend* p) {
 }
 
 int ma_b200_cache_attend(const ma_b200_attend* p, void* workspace, size_t workspace_bytes, void* stream) {
-  int rc = check_attend_shape(p);
-  if (rc != MA_B200_OK) return rc;
-  if (p->window < 0 || (p->window > 0 && !p->causal)) return invalid("window must not be negative, and needs causal");
-  if (!isfinite(p->scale) || !(p->softcap == 0.0f || (p->softcap >= 1e-20f && p->softcap <= 1e30f)))
-    return invalid("scale must be finite, softcap 0 (none) or from 1e-20 to 1e30");
-  ma::AttendArgs a{};
-  if ((rc = check_cache(p->cache, p->sequences, p->E, p->H, p->N, p->dtype, &a.cache)) != MA_B200_OK) return rc;
-  if ((rc = check_tensor(p->q, "q", 2, 16)) != MA_B200_OK || (rc = check_tensor(p->out, "out", 2, 16)) != MA_B200_OK) return rc;
-  const long long most = longest(p->sequences, p->cache.page_size);
-  const size_t need = ma::attend_workspace(p->E, p->N, p->H, p->cache.heads, p->cache.width, p->window, most);
-  if (workspace == nullptr || reinterpret_cast<uintptr_t>(workspace) % 256 != 0) return invalid("workspace is NULL or not 256-byte aligned");
-  if (workspace_bytes < need)
-    return fail_with(MA_B200_WORKSPACE_TOO_SMALL, "workspace has " + std::to_string(workspace_bytes) + " bytes, need " + std::to_string(need));
-  int dev = 0;
-  (void)cudaGetDevice(&dev);
-  int* const wait_status = ma::host_status_word(dev, 0);
-  a.q = view(p->q); a.out = view(p->out);
-  a.E = p->E; a.N = p->N; a.H = p->H; a.group = p->H / p->cache.heads;
-  a.causal = p->causal != 0; a.window = p->window; a.scale = p->scale; a.softcap = p->softcap;
-  return launched(ma::launch_attend(a, p->dtype, p->cache.width, workspace, most, wait_status, reinterpret_cast<cudaStream_t>(stream)), "attention over the cache");
+  return attend(p, workspace, workspace_bytes, stream, false);
+}
+
+int ma_b200_selftest_attend_wait_expiry(const ma_b200_attend* p, void* workspace, size_t workspace_bytes, void* stream) {
+  if (p != nullptr && p->dtype != MA_B200_BF16) return fail_with(MA_B200_UNSUPPORTED, "the self-test is of bf16");
+  return attend(p, workspace, workspace_bytes, stream, true);
 }
 
 int ma_b200_poll_cache_status(int device) {

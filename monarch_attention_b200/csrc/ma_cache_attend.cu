@@ -809,10 +809,10 @@ size_t attend_workspace(int E, int N, int H, int kv_heads, int width, int window
   return entries + (size_t)plan.grid * 2 * 8 * plan.nt * (width + 2) * sizeof(float);
 }
 
-cudaError_t launch_attend(AttendArgs a, int dtype, int width, void* workspace, long long longest, int* wait_status, cudaStream_t stream) {
+cudaError_t launch_attend(AttendArgs a, int dtype, int width, void* workspace, long long longest, int* wait_status, bool wait_expiry, cudaStream_t stream) {
   const long long strides[6] = {a.cache.k_sp, a.cache.k_sh, a.cache.k_st, a.cache.v_sp, a.cache.v_sh, a.cache.v_st};
   for (int i = 0; i < 6; ++i) (i < 3 ? a.k16[i] : a.v16[i - 3]) = (uint32_t)(strides[i] / 16);
-  if (a.group * (long long)a.N >= kPromptRows) return launch_prompt(a, dtype, width, workspace, longest, wait_status, stream);
+  if (a.group * (long long)a.N >= kPromptRows) return launch_prompt(a, dtype, width, workspace, longest, wait_status, wait_expiry, stream);
   const Plan plan = plan_of(a.E, a.N, a.H, a.cache.heads, width, a.window, longest);
   const int tile_rows = 8 * plan.nt;
   a.row_blocks = (a.group * a.N + tile_rows - 1) / tile_rows;

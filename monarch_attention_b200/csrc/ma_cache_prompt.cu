@@ -38,7 +38,7 @@ constexpr float kBelow = 7.0f, kSlack = 15.0f;  // (ma_cache_attend.cu)
 // Scores beyond this (in units of log2) have references in two parts (rows_apart).
 constexpr float kApart = 8192.0f;
 
-enum Bar { kQ0, kQ1, kKFull, kKEmpty = kKFull + 2, kVFull = kKEmpty + 2, kVEmpty = kVFull + 2, kS0 = kVEmpty + 2, kS1, kP0, kP1, kO, kBars };
+enum Bar { kQ0, kQ1, kKFull, kKEmpty = kKFull + 2, kVFull = kKEmpty + 2, kVEmpty = kVFull + 2, kS0 = kVEmpty + 2, kS1, kP0, kP1, kO, kDrain, kBars };
 
 // What the rows need of a step's 8 blocks.
 struct alignas(16) Blocks {
@@ -108,9 +108,11 @@ struct RowScores {
 // the last bit of a score is worth more than a unit, such a difference is anything, the weights leave f16 and the logarithm is lost.  Here a score is
 // rounded first and a reference is a score S and a logarithm L: (score - S) + (log - L) is exact for the keys that count, however large S is.
 // It takes twice as long, with a few scores at a time in registers.
-template <int D>
+template <typename T, int D>
 __device__ __forceinline__ void rows_apart(const RowScores& r, const Blocks& b, int t0, uint32_t t_s, uint32_t t_o, bool has_sums, float* sum, float* S_row, float* L_row) {
-  constexpr int kUnroll = D == 128 ? 1 : 2;  // (what leaves the kernel's loop as it was: us of 2 x 1024 tokens over 16384 keys, 128 features 284 / 288, 64 274 / 268)
+  // (What leaves the kernel's loop as it was; us of 2 x 1024 tokens over 16384 keys with 1 / 2 / 4: 128 features, bf16 281 / 288 / 285, f16 285 / 282 / 278; 64
+  // features, bf16 273 / 266 / 277, f16 275 / 270 / 271.)
+  constexpr int kUnroll = D == 64 ? 2 : std::is_same<T, __half>::value ? 4 : 1;
   auto load = [&](int q, float (&x)[32]) {
     tmem_ld32_nowait(t_s + 32 * q, x);
     tmem_wait_ld(x);
@@ -192,7 +194,8 @@ __device__ __forceinline__ void put_codes(uint32_t panel, uint32_t row, uint32_t
   st_shared_v4(panel + swz(row, chunk + 1), widen2(c.z), widen2_upper(c.z), widen2(c.w), widen2_upper(c.w));
 }
 
-template <typename T, int D>
+// kExpire: of the self-test, in which the values of a CTA's first step never arrive.
+template <typename T, int D, bool kExpire = false>
 __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_constant__ PromptArgs args) {
   using L = Layout<D>;
   constexpr int kPanel = 128 * 128;  // bytes of 128 rows of 64 features
@@ -207,8 +210,9 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
   const int tid = threadIdx.x, warp = tid >> 5;
   auto bar = [&](int i) { return base + L::kBarriers + 8 * i; };
   // (the vote brings the lanes of a warp back together, and of one mind)
-  auto wait = [&](int b, uint32_t phase) {
-    const bool r = __all_sync(0xffffffffu, mbar_wait_abortable(bar(b), phase & 1u, abort_flag));
+  constexpr int kTries = kExpire ? 4096 : 1 << 21;
+  auto wait = [&](int b, uint32_t phase, int tries = 1 << 21) {
+    const bool r = __all_sync(0xffffffffu, mbar_wait_abortable(bar(b), phase & 1u, abort_flag, tries));
     if (!r) *abort_flag = 1;
     return r;
   };
@@ -243,6 +247,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
       mbar_init(bar(kP0 + i), 128);
     }
     mbar_init(bar(kO), 1);
+    mbar_init(bar(kDrain), 1);
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -407,7 +412,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
           if (!there) ok = wait(kS0 + tile, i);
           if (!ok) break;
           tc_fence_after();
-          rows_apart<D>({factor, a.softcap, low, high}, blocks[i & (kRing - 1)], lo + i * kKeys, t_s, t_o, i > 0, &sum, &top, &top_log);
+          rows_apart<T, D>({factor, a.softcap, low, high}, blocks[i & (kRing - 1)], lo + i * kKeys, t_s, t_o, i > 0, &sum, &top, &top_log);
           tmem_wait_st();
           tc_fence_before();
           mbar_arrive(bar(kP0 + tile));
@@ -531,7 +536,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
       ok = ok && (i < 2 || wait(kVEmpty + stage, (i >> 1) - 1));
       if (ok) {
         put(1, base + L::kV + stage * L::kTileBytes);
-        mbar_arrive(bar(kVFull + stage));
+        if (!kExpire || i > 0) mbar_arrive(bar(kVFull + stage));
       }
       if (i + 1 < steps) load(1, i + 1);
       if (t < 8) {
@@ -573,7 +578,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
       __syncwarp();
     }
     for (int i = 0; i < steps && ok; ++i) {
-      ok = wait(kVFull + (i & 1), i >> 1) && (i + 1 == steps || wait(kKFull + ((i + 1) & 1), (i + 1) >> 1));
+      ok = wait(kVFull + (i & 1), i >> 1, kTries) && (i + 1 == steps || wait(kKFull + ((i + 1) & 1), (i + 1) >> 1));
       for (int tile = 0; tile < tiles && ok; ++tile) {
         ok = wait(kP0 + tile, i);
         if (!ok) break;
@@ -595,7 +600,15 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
 
   tc_fence_before();
   __syncthreads();
-  if (tid == 0 && *abort_flag != 0 && args.wait_status != nullptr) *reinterpret_cast<volatile int*>(args.wait_status) = 800;
+  if (*abort_flag != 0) {
+    if (tid == 0 && args.wait_status != nullptr) *reinterpret_cast<volatile int*>(args.wait_status) = 800;
+    // products that were issued have read their operands and written tensor memory before the CTA leaves
+    if (warp == 12 && elect_one()) {
+      mma_commit(bar(kDrain));
+      (void)mbar_wait(bar(kDrain), 0);
+    }
+    __syncwarp();
+  }
   if (warp == 12) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
 }
 
@@ -617,7 +630,7 @@ size_t prompt_workspace(int E, int N, int H, int kv_heads, int width, long long 
   return (units * sizeof(int4) + 255) / 256 * 256 + units * pieces * kRows * (width + 2) * sizeof(float);
 }
 
-cudaError_t launch_prompt(AttendArgs a, int dtype, int width, void* workspace, long long longest, int* wait_status, cudaStream_t stream) {
+cudaError_t launch_prompt(AttendArgs a, int dtype, int width, void* workspace, long long longest, int* wait_status, bool wait_expiry, cudaStream_t stream) {
   a.row_blocks = (a.group * a.N + kRows - 1) / kRows;
   const long long units = (long long)a.E * a.cache.heads * a.row_blocks;
   PromptArgs args{a, prompt_pieces(a.E, a.N, a.H, a.cache.heads, longest), wait_status};
@@ -628,13 +641,14 @@ cudaError_t launch_prompt(AttendArgs a, int dtype, int width, void* workspace, l
   const bool bf = dtype == MA_B200_BF16;
   const void* fn = width == 128 ? (bf ? (const void*)prompt_kernel<__nv_bfloat16, 128> : (const void*)prompt_kernel<__half, 128>)
                                 : (bf ? (const void*)prompt_kernel<__nv_bfloat16, 64> : (const void*)prompt_kernel<__half, 64>);
+  if (wait_expiry) fn = width == 128 ? (const void*)prompt_kernel<__nv_bfloat16, 128, true> : (const void*)prompt_kernel<__nv_bfloat16, 64, true>;
   const size_t smem = width == 128 ? Layout<128>::kSmem : Layout<64>::kSmem;
   // a build whose launch does not cover the roles' registers must not start: setmaxnreg would wait for them without end
-  static std::atomic<unsigned long long> checked[4];
+  static std::atomic<unsigned long long> checked[6];
   int dev = 0;
   cudaError_t err = cudaGetDevice(&dev);
   if (err != cudaSuccess) return err;
-  std::atomic<unsigned long long>& done = checked[(width == 128) * 2 + bf];
+  std::atomic<unsigned long long>& done = checked[(width == 128) * 3 + (wait_expiry ? 2 : bf)];
   if (dev >= 64 || !(done.load(std::memory_order_relaxed) >> dev & 1)) {
     cudaFuncAttributes fa;
     err = cudaFuncGetAttributes(&fa, fn);

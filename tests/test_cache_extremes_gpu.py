@@ -370,3 +370,37 @@ def test_pools_whose_parts_are_over_one_another_are_not_written():
         ma.append_kv_b200(pool, k, -k, table, ints(20))
         assert torch.equal(ma.cached_attention_b200(q, pool, table, ints(20)), want)
     ma.cached_attention_b200(q, good._replace(v=good.k), table, ints(20))
+
+
+@pytest.mark.parametrize("E,Hk,N,L,D", [(1, 2, 40, 300, 64), (2, 4, 100, 5000, 128), (40, 4, 300, 600, 64)])
+def test_a_wait_that_runs_out_ends_the_call_and_is_reported(E, Hk, N, L, D):
+    """Many rows, with keys in one piece and in several: the values of each block of threads' first step never arrive.  All end by themselves, the next call
+    raises, and the one after is an ordinary call."""
+    import ctypes as C
+
+    from monarch_attention_b200 import _cabi
+    import monarch_attention_b200 as ma
+    lib, H, page = _cabi.load(), 4 * Hk, 64
+    cache, table = filled(E, L // page + 1, Hk, D, page, [L] * E)
+    q, n = queries(E, H, N, D, BF, "heads"), ints(*[L] * E)
+    good = ma.cached_attention_b200(q, cache, table, n)
+    out = torch.empty_like(q)
+    p = _cabi.Attend(_cabi.ABI_VERSION, E, H, N, _cabi.BF16, 1, 0, D ** -0.5, 0.0)
+    p.q, p.out = (_cabi.Tensor4(t.data_ptr(), *t.stride()[:3]) for t in (q, out))
+    p.cache = _cabi.Cache(*(t.data_ptr() for t in cache), *cache.k.shape, *cache.k.stride()[:3], *cache.v.stride()[:3], *cache.k_scale.stride()[:2],
+                          *cache.v_scale.stride()[:2])
+    p.sequences = _cabi.Sequences(table.data_ptr(), table.stride(0), table.shape[1], n.data_ptr(), None)
+    ws = torch.empty(lib.ma_b200_cache_attend_workspace_bytes(C.byref(p)), dtype=torch.uint8, device="cuda")
+    stream = torch.cuda.current_stream().cuda_stream
+    assert lib.ma_b200_cache_attend(C.byref(p), ws.data_ptr(), ws.numel(), stream) == _cabi.OK
+    assert torch.equal(out, good) and lib.ma_b200_poll_device_status(0) == _cabi.OK
+    start, end = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+    start.record()
+    assert lib.ma_b200_selftest_attend_wait_expiry(C.byref(p), ws.data_ptr(), ws.numel(), stream) == _cabi.OK
+    end.record()
+    torch.cuda.synchronize()
+    assert start.elapsed_time(end) < 2000   # (waits of 4096 tries, a round of blocks after another)
+    with pytest.raises(RuntimeError, match="gave up"):
+        ma.cached_attention_b200(q, cache, table, n)
+    assert lib.ma_b200_poll_device_status(0) == _cabi.OK
+    assert torch.equal(ma.cached_attention_b200(q, cache, table, n), good)
