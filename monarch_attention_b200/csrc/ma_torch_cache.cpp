@@ -285,10 +285,13 @@ Tensor append(const Cache& cache, const Tensor& k_in, const Tensor& v_in, const 
   TORCH_CHECK_VALUE(k_in.size(1) == p.cache.heads && k_in.size(3) == p.cache.width, "key shape ", k_in.sizes(), " does not match the cache's ",
                     p.cache.heads, " heads of ", p.cache.width);
   p.sequences = sequences_struct(table, lengths, counts, k_in.size(0), k_in.device());
-  const Places places[4] = {Places(cache.k), Places(cache.v), Places(cache.k_scale), Places(cache.v_scale)};
-  TORCH_CHECK_VALUE(places[0].distinct() && places[1].distinct() && places[2].distinct() && places[3].distinct() && !meet(places[0], places[1]) &&
-                        !meet(places[2], places[3]),
-                    "what the append writes must not overlap: pages, heads or tokens of the cache are over one another, or keys over values");
+  for (const auto& [a, b] : {std::pair<const Tensor&, const Tensor&>(cache.k, cache.v), std::pair<const Tensor&, const Tensor&>(cache.k_scale, cache.v_scale)}) {
+    const char *at = static_cast<const char*>(a.data_ptr()), *bt = static_cast<const char*>(b.data_ptr());
+    if (a.is_contiguous() && b.is_contiguous() && (at + a.nbytes() <= bt || bt + b.nbytes() <= at)) continue;  // (as allocated: 0.2 us less of the host's 6.5)
+    const Places x(a), y(b);
+    TORCH_CHECK_VALUE(x.distinct() && y.distinct() && !meet(x, y),
+                      "what the append writes must not overlap: pages, heads or tokens of the cache are over one another, or keys over values");
+  }
   const size_t lane = 16;
   Tensor q, q_out;
   if (query.has_value()) {
