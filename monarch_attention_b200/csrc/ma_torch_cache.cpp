@@ -51,6 +51,7 @@ struct Places {
   }
   // Each stride passes over all that the smaller ones reach, so that no two elements are in one place.  (Others may have that too; they are not taken.)
   bool distinct() const {
+    if (begin == end) return true;
     int64_t reach = 0;
     for (size_t i = dims.size(); i-- > 0;) {
       if (dims[i].stride <= reach) return false;

@@ -404,3 +404,11 @@ def test_a_wait_that_runs_out_ends_the_call_and_is_reported(E, Hk, N, L, D):
         ma.cached_attention_b200(q, cache, table, n)
     assert lib.ma_b200_poll_device_status(0) == _cabi.OK
     assert torch.equal(ma.cached_attention_b200(q, cache, table, n), good)
+
+
+def test_results_of_no_tokens():
+    import monarch_attention_b200 as ma
+    cache, table = filled(2, 2, 2, 64, 16, [20, 3])
+    q = torch.empty_strided((2, 4, 0, 64), (0, 0, 0, 1), dtype=BF, device="cuda")
+    out = ma.cached_attention_b200(q, cache, table, ints(20, 3), out=q)
+    assert out.shape == q.shape and ma.append_kv_b200(cache, q[:, :2], q[:, :2], table, ints(20, 3)) is None
