@@ -12,9 +12,9 @@
 //    memory; rows stay in registers in 16 bits until the scale is known.  Bound by memory.
 //  * Single tokens: a row is all there is of a block, so rows of different heads are spread over the warps, and nothing is exchanged
 //    between them.  Bound by latency: the row's load does not wait for the length and the page.
-// Measured: 8 prompts of up to 1999 tokens, 4 heads of 128 features and 16 query heads, 123 MB in 32 us, 3.8 TB/s; the SMs issue in 55 % of their
+// Measured: 8 prompts of up to 1999 tokens, 4 heads of 128 features and 16 query heads, 123 MB in 32 us, 3.8 TB/s; the SMs issue in 52 % of their
 // cycles, 16 warps of 128 registers each.  (24 warps of 80 registers, or four heads in flight, take longer.)  One token of 256 sequences of 8 + 32
-// heads 5.5 us, of 8 sequences 3.4, of which a launch is 2.5.
+// heads 4.7 us back to back, of 8 sequences 2.5, which is a launch.
 #include <cuda_fp8.h>
 
 #include "ma_cache.cuh"

@@ -11,8 +11,8 @@
 //    scores, the values' to the weights, with a reference that is raised (and O multiplied) only when a weight would pass 2^15.
 //  * One warp issues the products: O += P V, the weights P read from tensor memory, where they have taken the place of their scores, and
 //    the next step's scores S = Q K^T.  While one tile's rows are exponentiated the other's products run.
-// Measured: 1024 tokens of 2 sequences over 16384 keys, 4 heads of 128 features, 281 us, 947 TFLOP/s, 57 % of a library product; 64 features 495.  A
-// step takes 4200 cycles, of which the row warps' weights are 2300 a tile: without any exponential they would take 80 % of the time, without the
+// Measured: 1024 tokens of 2 sequences over 16384 keys, 4 heads of 128 features, 281 us, 947 TFLOP/s, 57 % of a library product; 64 features 495.  (A call
+// lasts as long as its longest sequence: one of 16384 beside one of 1024 takes the same 281.)  A step takes 4200 cycles, of which the row warps' weights are 2300 a tile: without any exponential they would take 80 % of the time, without the
 // conversion of keys and values all of it, and with scores that never wait for the products of the step before (64 features leave the room) 99 %.
 // Slower were (beside 304 us): two threads a row 343, scores of 64 keys in two buffers 358, scores loaded a quarter at a time 347; eight warps that
 // bring keys and values, which leave the rows 160 registers each, took the 304.
@@ -107,7 +107,7 @@ struct RowScores {
 // The kernel's loop has a weight as the exponential of fma(score, f, log - reference), with the logarithm of the value's scale in the reference: where
 // the last bit of a score is worth more than a unit, such a difference is anything, the weights leave f16 and the logarithm is lost.  Here a score is
 // rounded first and a reference is a score S and a logarithm L: (score - S) + (log - L) is exact for the keys that count, however large S is.
-// It takes twice as long, with a few scores at a time in registers.
+// A few scores are in registers at a time, read and scaled twice: 1276 us for the loop's 281 (2 x 1024 tokens over 16384 keys of 128 features).
 template <typename T, int D>
 __device__ __forceinline__ void rows_apart(const RowScores& r, const Blocks& b, int t0, uint32_t t_s, uint32_t t_o, bool has_sums, float* sum, float* S_row, float* L_row) {
   // (What leaves the kernel's loop as it was; us of 2 x 1024 tokens over 16384 keys with 1 / 2 / 4: 128 features, bf16 281 / 288 / 285, f16 285 / 282 / 278; 64
@@ -404,7 +404,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
         mbar_arrive(bar(kP0 + tile));
       }
       // From the first step on in which a row of the warp has a score far from zero, its rows go this way: a path of its own, of which the loop above knows a jump
-      // and no state (a flag in its place: 4 to 6 % on all calls; the same inside the loop: 15).
+      // and no state (a flag in its place costs 4 to 6 % of all calls, the same inside the loop 15).
       if (false) {
       apart:
 #pragma unroll 1
