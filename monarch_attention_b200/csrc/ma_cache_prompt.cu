@@ -12,8 +12,9 @@
 //  * One warp issues the products: O += P V, the weights P read from tensor memory, where they have taken the place of their scores, and
 //    the next step's scores S = Q K^T.  While one tile's rows are exponentiated the other's products run.
 // Measured: 1024 tokens of 2 sequences over 16384 keys, 4 heads of 128 features, 281 us, 947 TFLOP/s, 57 % of a library product; 64 features 495.  (A call
-// lasts as long as its longest sequence: one of 16384 beside one of 1024 takes the same 281.)  A step takes 4200 cycles, of which the row warps' weights are 2300 a tile: without any exponential they would take 80 % of the time, without the
-// conversion of keys and values all of it, and with scores that never wait for the products of the step before (64 features leave the room) 99 %.
+// lasts as long as its longest sequence: one of 16384 beside one of 1024 takes the same 281.)  A step takes 4200 cycles, of which the row warps' weights are
+// 2300 a tile: without any exponential they would take 80 % of the time, without the conversion of keys and values all of it, and with scores that never
+// wait for the products of the step before (64 features leave the room) 99 %.
 // Slower were (beside 304 us): two threads a row 343, scores of 64 keys in two buffers 358, scores loaded a quarter at a time 347; eight warps that
 // bring keys and values, which leave the rows 160 registers each, took the 304.
 // Every wait is bounded; one that gives up ends the CTA's others, and the next call on the device reports it.
@@ -447,7 +448,8 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
                            pack2<T>(o[j + 4] * inverse, o[j + 5] * inverse), pack2<T>(o[j + 6] * inverse, o[j + 7] * inverse));
         } else {
 #pragma unroll
-          for (int j = 0; j < 32; j += 4) *reinterpret_cast<float4*>(a.part_o + slot * D + 32 * q + j) = make_float4(o[j] * unit_of, o[j + 1] * unit_of, o[j + 2] * unit_of, o[j + 3] * unit_of);
+          for (int j = 0; j < 32; j += 4)
+            *reinterpret_cast<float4*>(a.part_o + slot * D + 32 * q + j) = make_float4(o[j] * unit_of, o[j + 1] * unit_of, o[j + 2] * unit_of, o[j + 3] * unit_of);
         }
       }
       if (args.pieces > 1 && exists) *reinterpret_cast<float2*>(a.part_ml + 2 * slot) = make_float2(top, sum * unit_of);

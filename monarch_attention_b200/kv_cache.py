@@ -90,14 +90,15 @@ def cached_attention_b200(query: Tensor, cache: PagedKV, page_table: Tensor, len
     Query head ``h`` reads cache head ``h // (H / heads)``.  ``causal``: a token sees the positions up to its own (the call's tokens have been
     appended before); else all ``lengths`` (an encoder's output).  ``window`` > 0 (causal only): the last ``window`` of those.  Scores are
     multiplied by ``scale`` (None: ``width ** -0.5``) and, with ``softcap`` > 0 (from 1e-20 to 1e30), become ``softcap * tanh(score / softcap)``.  Rows without
-    a key, and rows of padding, are zero.  What lies in the cache behind a sequence's end is never looked at, NaN included; a NaN that was appended as a value reaches
-    all of the call's rows of its sequence and head, masked ones too (zero times NaN).
+    a key, and rows of padding, are zero.  What lies in the cache behind a sequence's end is never looked at, NaN included; a NaN that was appended as a key
+    makes NaN of the rows that see it, as a value it reaches all of the call's rows of its sequence and head, masked ones too (zero times NaN).
 
     The result has the query's dtype, and with ``token_major_output`` is a view of an (E, N, H, width) buffer; ``out`` (rows on 16-byte
-    boundaries; the query itself, or rows beside its own in a common buffer, are fine, rows over one another or over others of the query's are refused) takes it in place.  Scores and sums are in 32 bits; a bfloat16 query is read in 16-bit steps of 2^-11 of itself and 2^-25 of
-    its row's largest magnitude.  Weights, each times its value's scale, are rounded to 2^-11 of themselves or 2^-32 of their row's largest, whichever is more; what is
-    below 2^-25 of a sum so far may be lost from it, as 32 bits have it.  Where scores pass 2^27 and there are 32 rows or fewer to a cache head (tokens times
-    query heads of it), scales of values are to be from 2^-14 to 2^15.  The same call gives the same bits; what else is in the batch may
+    boundaries) takes it in place: the query itself, or rows beside its own in a common buffer, are fine; rows over one another or over others of the
+    query's are refused.  Scores and sums are in 32 bits; a bfloat16 query is read in 16-bit steps of 2^-11 of itself and 2^-25 of its row's
+    largest magnitude.  Weights, each times its value's scale, are rounded to 2^-11 of themselves or 2^-32 of their row's largest, whichever is more; what
+    is below 2^-25 of a sum so far may be lost from it, as 32 bits have it.  Where scores pass 2^27 and there are 32 rows or fewer to a cache head
+    (tokens times query heads of it), scales of values are to be from 2^-14 to 2^15.  The same call gives the same bits; what else is in the batch may
     change the order of a sequence's sums.  No gradient: inputs that require one are refused.
     """
     if _attend is None:

@@ -412,3 +412,19 @@ def test_results_of_no_tokens():
     q = torch.empty_strided((2, 4, 0, 64), (0, 0, 0, 1), dtype=BF, device="cuda")
     out = ma.cached_attention_b200(q, cache, table, ints(20, 3), out=q)
     assert out.shape == q.shape and ma.append_kv_b200(cache, q[:, :2], q[:, :2], table, ints(20, 3)) is None
+
+
+@pytest.mark.parametrize("exponents", [(-40, -40), (60, 60), (-40, 60), (-30, -20)])
+@pytest.mark.parametrize("N", [1, 3, 4])
+@pytest.mark.parametrize("size", [1e4, 1e5, 1e6, 1e7])
+def test_few_rows_with_scores_below_their_limit_over_values_of_any_scale(size, N, exponents):
+    import monarch_attention_b200 as ma
+    cache, table = filled(1, 6, 1, 64, 64, [300])
+    g = torch.Generator(device="cuda").manual_seed(3)
+    cache.v_scale.copy_(torch.exp2(torch.randint(exponents[0], exponents[1] + 1, cache.v_scale.shape, generator=g, device="cuda").float()))
+    q = (queries(1, 8, N, 64, BF, "heads").float() * size).to(BF)
+    out = ma.cached_attention_b200(q, cache, table, ints(300))[0].double().cpu()
+    k, v = (held(c, s, table[0], 300, 64) for c, s in ((cache.k, cache.k_scale), (cache.v, cache.v_scale)))
+    want, clear = one_hot(q[0], k, v, 300 - N, 0.125)
+    assert bool(clear.any()) and bool(out.isfinite().all())
+    assert bool(((out - want).abs() <= (2.0 ** -11 + 2.0 ** -20 + 2.0 ** -8) * want.abs())[clear].all())
