@@ -439,14 +439,15 @@ def _run_plain_fork(s):
 
     uses = uses - count(table, holds) + count(theirs, kept)
     wanted = (column < need[:, None]) & ~kept
-    free = torch.sort((uses != 0).to(torch.uint8), stable=True).indices   # free pages, the lowest first
-    given = free[(wanted.flatten().long().cumsum(0) - 1).clamp(0, pages - 1)].view(E, P)
-    new = torch.where(kept, theirs, torch.where(wanted, given, -1))
-    uses = uses + count(given, wanted)
-    # a page that is partly filled and stays with another row
+    # a page that is partly filled and stays with another row is copied, and not given out in this call
     at = full.clamp_max(P - 1)[:, None]
     tokens = length - full * page
     copies = goes_on & (tokens > 0) & ~kept.gather(1, at)[:, 0]
+    read = count(theirs.gather(1, at).expand(E, P), copies[:, None] & (column == 0))
+    free = torch.sort((uses + read != 0).to(torch.uint8), stable=True).indices   # free pages, the lowest first
+    given = free[(wanted.flatten().long().cumsum(0) - 1).clamp(0, pages - 1)].view(E, P)
+    new = torch.where(kept, theirs, torch.where(wanted, given, -1))
+    uses = uses + count(given, wanted)
     src, dst = theirs.gather(1, at)[:, 0][copies], new.gather(1, at)[:, 0][copies]
     slot = torch.arange(page, device=dev)
     block = (slot < ((tokens[copies] + BLOCK - 1) // BLOCK * BLOCK)[:, None]).view(1, -1, 1, page, 1)
