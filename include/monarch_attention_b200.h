@@ -47,7 +47,7 @@ enum {
   MA_B200_CUDA_ERROR = 3,       /* a CUDA runtime / driver call failed (see last_error)       */
   MA_B200_DEVICE_WAIT_EXPIRED = 4, /* a bounded on-device wait gave up; output is undefined   */
   MA_B200_WORKSPACE_TOO_SMALL = 5,
-  MA_B200_DEVICE_BAD_SEQUENCE = 6 /* a kernel met a length, count or page outside its range (see ma_b200_poll_cache_status) */
+  MA_B200_DEVICE_BAD_SEQUENCE = 6 /* a kernel met a length, count, page or the like outside its range (see ma_b200_poll_cache_status) */
 };
 
 /* Element types.  q and k share qk_dtype; v and out share v_dtype. */
@@ -388,6 +388,60 @@ typedef struct ma_b200_attend {
  * overlap in time need one each. */
 MA_B200_API size_t ma_b200_cache_attend_workspace_bytes(const ma_b200_attend* p);
 MA_B200_API int ma_b200_cache_attend(const ma_b200_attend* p, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Trees of drafted tokens: a sequence's tokens of the call are several continuations at once.  parents (E, N) int32: the call's number of each
+ * token's parent, an earlier one, or -1; another value counts as -1 and is reported by ma_b200_poll_cache_status.  A token lies in the cache at the
+ * place that it has in the call, and stands at the position lengths[e] - counts[e] + d, d the number of its ancestors. */
+#define MA_B200_TREE_TOKENS 512 /* most tokens of a call */
+typedef struct ma_b200_tree {
+  const int32_t* parents;
+  int64_t stride; /* of a sequence, in elements; tokens lie next to one another */
+} ma_b200_tree;
+/* ma_b200_cache_append with keys and queries rotated at the tokens' positions. */
+MA_B200_API int ma_b200_cache_append_tree(const ma_b200_append* p, const ma_b200_tree* tree, void* stream);
+/* ma_b200_cache_attend (causal; the same workspace): a token sees what is cached in front of the call, its ancestors and itself; a window is of positions. */
+MA_B200_API int ma_b200_cache_attend_tree(const ma_b200_attend* p, const ma_b200_tree* tree, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Which tokens of a tree stand, and the caches of all layers (HOST array, one shape and strides) closed up over them.  drafted and answers (E, N; int32, or
+ * int64 with ids_i64): the call's tokens, and what the model answered each with.  Token 0 of a sequence stands; another one does if its parent does and its
+ * drafted value is the parent's answer (the first of several).  Those that stand move to the slots lengths[e] - counts[e] + 0, 1, ..; a block that
+ * tokens move into gets the scale that an append of them would have given it.  Written: new_lengths (E), path (E, N contiguous; the tokens that
+ * stand, -1 behind), answer (E; of the last of them, -1 where there is none).  They must not overlap what is read.  A count above N or the length stands for none. */
+typedef struct ma_b200_accept {
+  int32_t abi_version;
+  int32_t E, N, layers;
+  const ma_b200_cache* caches;
+  ma_b200_sequences sequences;
+  ma_b200_tree tree;
+  const void *drafted, *answers;
+  int64_t drafted_stride, answers_stride;
+  int32_t ids_i64;
+  int32_t *new_lengths, *path;
+  void* answer;
+} ma_b200_accept;
+MA_B200_API int ma_b200_cache_accept(const ma_b200_accept* p, void* stream);
+
+/* Sequences that go on from others, end, or get room.  page_uses (pages) int32 counts the rows of page_table (E, table_pages) int32 that hold each page; a row's
+ * pages are those in front of its first negative entry.  Row e takes what row source[e] held (-1: nothing; NULL: each row its own): full pages are shared, a page
+ * that is partly filled, and pages behind, stay with row source[e] itself where it goes on from itself, else with the first row that goes on from it,
+ * unless another row holds them too; the others get a copy, in all layers' caches (HOST array, one shape and strides).  Each row ends with pages for its
+ * length and room[e] (room_all where room is NULL) tokens more; new ones are the lowest that are free, in the order of rows and places.  All rows change
+ * at once.  page_uses, page_table and lengths are written.  A source, length or room outside its range and a pool without enough free pages (rows then
+ * end where their pages do) are reported by ma_b200_poll_cache_status.  Workspace: 256-byte aligned, without initialisation. */
+typedef struct ma_b200_fork {
+  int32_t abi_version;
+  int32_t E, layers;
+  const ma_b200_cache* caches;
+  int32_t* page_uses;
+  int32_t* page_table;
+  int64_t table_stride;
+  int32_t table_pages;
+  int32_t* lengths;
+  const int32_t *source, *room;
+  int32_t room_all;
+} ma_b200_fork;
+MA_B200_API size_t ma_b200_cache_fork_workspace_bytes(const ma_b200_fork* p);
+MA_B200_API int ma_b200_cache_fork(const ma_b200_fork* p, void* workspace, size_t workspace_bytes, void* stream);
 
 /* Test hook: the same call, in bf16 and of 33 rows or more to a cache head (N * H / heads), with a wait of every thread block that has keys run out.  The result is
  * undefined, ma_b200_poll_device_status() reports MA_B200_DEVICE_WAIT_EXPIRED, and the next ordinary call is unaffected.  Nothing faults, traps or

@@ -31,6 +31,7 @@ EXPORTS = (
     "ma_b200_backward_workspace_bytes", "ma_b200_backward", "ma_b200_forward_typed_mask", "ma_b200_backward_typed_mask",
     "ma_b200_rotary_apply", "ma_b200_cache_append", "ma_b200_cache_attend_workspace_bytes", "ma_b200_cache_attend",
     "ma_b200_poll_cache_status", "ma_b200_selftest_attend_wait_expiry",
+    "ma_b200_cache_append_tree", "ma_b200_cache_attend_tree", "ma_b200_cache_accept", "ma_b200_cache_fork_workspace_bytes", "ma_b200_cache_fork",
 )
 
 
@@ -87,6 +88,21 @@ class Attend(C.Structure):
     _fields_ = [(n, C.c_int32) for n in ("abi_version", "E", "H", "N", "dtype", "causal", "window")] + \
                [("scale", C.c_float), ("softcap", C.c_float)] + [(n, Tensor4) for n in ("q", "out")] + \
                [("cache", Cache), ("sequences", Sequences)]
+
+
+class Tree(C.Structure):
+    _fields_ = [("parents", C.c_void_p), ("stride", C.c_int64)]
+
+
+class Accept(C.Structure):
+    _fields_ = [(n, C.c_int32) for n in ("abi_version", "E", "N", "layers")] + [("caches", C.POINTER(Cache)), ("sequences", Sequences), ("tree", Tree)] + \
+               [(n, C.c_void_p) for n in ("drafted", "answers")] + [(n, C.c_int64) for n in ("drafted_stride", "answers_stride")] + \
+               [("ids_i64", C.c_int32)] + [(n, C.c_void_p) for n in ("new_lengths", "path", "answer")]
+
+
+class Fork(C.Structure):
+    _fields_ = [(n, C.c_int32) for n in ("abi_version", "E", "layers")] + [("caches", C.POINTER(Cache)), ("page_uses", C.c_void_p), ("page_table", C.c_void_p)] + \
+               [("table_stride", C.c_int64), ("table_pages", C.c_int32)] + [(n, C.c_void_p) for n in ("lengths", "source", "room")] + [("room_all", C.c_int32)]
 
 
 class WorkspaceLayout(C.Structure):
@@ -168,6 +184,16 @@ def load() -> C.CDLL:
     lib.ma_b200_cache_attend.restype = C.c_int
     lib.ma_b200_selftest_attend_wait_expiry.argtypes = [C.POINTER(Attend), C.c_void_p, C.c_size_t, C.c_void_p]
     lib.ma_b200_selftest_attend_wait_expiry.restype = C.c_int
+    lib.ma_b200_cache_append_tree.argtypes = [C.POINTER(Append), C.POINTER(Tree), C.c_void_p]
+    lib.ma_b200_cache_append_tree.restype = C.c_int
+    lib.ma_b200_cache_attend_tree.argtypes = [C.POINTER(Attend), C.POINTER(Tree), C.c_void_p, C.c_size_t, C.c_void_p]
+    lib.ma_b200_cache_attend_tree.restype = C.c_int
+    lib.ma_b200_cache_accept.argtypes = [C.POINTER(Accept), C.c_void_p]
+    lib.ma_b200_cache_accept.restype = C.c_int
+    lib.ma_b200_cache_fork_workspace_bytes.argtypes = [C.POINTER(Fork)]
+    lib.ma_b200_cache_fork_workspace_bytes.restype = C.c_size_t
+    lib.ma_b200_cache_fork.argtypes = [C.POINTER(Fork), C.c_void_p, C.c_size_t, C.c_void_p]
+    lib.ma_b200_cache_fork.restype = C.c_int
     lib.ma_b200_poll_cache_status.argtypes = [C.c_int]
     lib.ma_b200_poll_cache_status.restype = C.c_int
     lib.ma_b200_host_last_error.argtypes = []

@@ -24,7 +24,7 @@ struct CacheArgs {
   int* status;         // mapped host word: what was wrong with a table, length or count
 };
 
-enum CacheFault { kBadLength = 1, kBadPage = 2 };
+enum CacheFault { kBadLength = 1, kBadPage = 2, kBadParent = 3, kBadSource = 4, kNoPage = 5 };
 
 __device__ __forceinline__ void report(int* status, int code) {
   if (status != nullptr) *reinterpret_cast<volatile int*>(status) = code;
@@ -47,6 +47,16 @@ __device__ __forceinline__ int page_of(const CacheArgs& c, int e, int position) 
   return page >= 0 && page < c.pages ? page : -1;
 }
 
+constexpr int kTreeTokens = 512;  // most tokens of a tree
+
+// Parent of token n of a tree (a row of `parents`): an earlier token, or -1; another value counts as -1.
+__device__ __forceinline__ int parent_of(const int* parents, int n, int* status) {
+  const int p = parents[n];
+  if (p >= -1 && p < n) return p;
+  report(status, kBadParent);
+  return -1;
+}
+
 // softcap * tanh(score / softcap) of a score in units of log2 e, in the same units.  tanh y = 1 - 2 / (exp(2 y) + 1) is off by some 2^-22 whatever y is,
 // too much next to a small y; below 1/8 its series takes over, whose first term left out is 2^-29 of it.
 __device__ __forceinline__ float capped(float x, float softcap) {
@@ -62,8 +72,46 @@ struct AppendArgs {
   View4 k, v, q, q_out;
   int E, N, H;  // H: query heads, 0 = none
   RotaryArgs rotary;
+  const int* parents;  // (E, N) of a tree, whose tokens are rotated at the positions of their depth, or nullptr
+  long long parents_se;
 };
 cudaError_t launch_append(const AppendArgs& a, int dtype, int width, cudaStream_t stream);
+
+// The caches of several layers: one shape, the same strides (in CacheArgs), other pointers.
+struct LayerPointers {
+  uint8_t *k, *v;
+  float *k_scale, *v_scale;
+};
+constexpr int kMostLayers = 32;  // of a launch
+
+struct AcceptArgs {
+  CacheArgs cache;  // (without pointers to a pool)
+  LayerPointers layer[kMostLayers];
+  int layers, E, N;
+  const int* parents;  // (E, N)
+  long long parents_se;
+  const void *drafted, *answers;  // (E, N) int32 or (ids64) int64
+  long long drafted_se, answers_se;
+  int ids64;
+  int *lengths_out, *path_out;  // (E), (E, N); nullptr: not written
+  void* answer_out;             // (E)
+};
+cudaError_t launch_accept(const AcceptArgs& a, int width, cudaStream_t stream);
+
+struct ForkArgs {
+  CacheArgs cache;  // (without pointers to a pool; the table and the lengths are written)
+  LayerPointers layer[kMostLayers];
+  int layers, E;
+  int* uses;            // (pages)
+  int *table, *lengths;
+  const int *source, *room;  // (E) or nullptr: each row itself, room_all tokens
+  int room_all;
+  int* workspace;
+};
+size_t fork_workspace(int E, int table_pages, int pages);
+cudaError_t launch_fork(const ForkArgs& a, int width, cudaStream_t stream);
+// The copies of the same call in other layers.
+cudaError_t launch_fork_copies(const ForkArgs& a, int width, cudaStream_t stream);
 
 struct AttendArgs {
   CacheArgs cache;
@@ -77,6 +125,8 @@ struct AttendArgs {
   int4* split;              // where heads have been split: an entry a CTA or
   int split_by_head;        // (1) a head and block of rows
   int whole_heads;          // 1: no head is split
+  const int* parents;       // (E, N) of a tree, or nullptr
+  long long parents_se;
 };
 // Whether a row of the call's token n has a key at all; the others' results are zero, whatever the sums of their tile have caught.
 __device__ __forceinline__ bool sees_keys(const AttendArgs& a, int len, int count, int n) { return n < count && (!a.causal || len - count + n >= 0); }
@@ -85,6 +135,8 @@ __device__ __forceinline__ bool sees_keys(const AttendArgs& a, int len, int coun
 size_t attend_workspace(int E, int N, int H, int kv_heads, int width, int window, long long longest);
 // (wait_expiry, a self-test: a wait of the kernel for many rows runs out.)
 cudaError_t launch_attend(AttendArgs a, int dtype, int width, void* workspace, long long longest, int* wait_status, bool wait_expiry, cudaStream_t stream);
+// The kernel for few rows over trees (ma_cache_attend_tree.cu): `nt` tiles of 8 rows, `warps` warps a CTA.
+cudaError_t launch_few_tree(AttendArgs& a, int dtype, int width, int nt, int warps, long long grid, cudaStream_t stream);
 // The pieces of `entries` heads and blocks of tile_rows rows (a.split, a.part_o, a.part_ml; a head's pieces `stride` slots apart) into a.out.
 cudaError_t launch_join(const AttendArgs& a, int dtype, int width, int tile_rows, int entries, int stride, cudaStream_t stream);
 // The kernel for many rows (ma_cache_prompt.cu).

@@ -15,9 +15,7 @@
 // Measured: 8 prompts of up to 1999 tokens, 4 heads of 128 features and 16 query heads, 123 MB in 32 us, 3.8 TB/s; the SMs issue in 52 % of their
 // cycles, 16 warps of 128 registers each.  (24 warps of 80 registers, or four heads in flight, take longer.)  One token of 256 sequences of 8 + 32
 // heads 4.7 us back to back, of 8 sequences 2.5, which is a launch.
-#include <cuda_fp8.h>
-
-#include "ma_cache.cuh"
+#include "ma_cache_codes.cuh"
 #include "ma_sm100.cuh"
 
 namespace ma {
@@ -26,24 +24,7 @@ namespace {
 constexpr int kWarps = 8, kThreads = 32 * kWarps;
 constexpr int F = 8;  // features of a lane
 
-// The smallest n in [-40, 60] with amax <= 448 * 2^n, as 2^n: 448 = 1.75 * 2^8, so a mantissa above 1.75 takes one more.
-__device__ __forceinline__ float scale_for(float amax) {
-  const int n = (int)((__float_as_uint(amax) + 0x1fffffu) >> 23) - 127 - 8;
-  return __uint_as_float((uint32_t)(min(max(n, -40), 60) + 127) << 23);
-}
-
-__device__ __forceinline__ uint32_t four_codes(float a, float b, float c, float d) {
-  return (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3) |
-         (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(c, d), __NV_SATFINITE, __NV_E4M3) << 16;
-}
 __device__ __forceinline__ uint2 to_codes(const float (&x)[F]) { return make_uint2(four_codes(x[0], x[1], x[2], x[3]), four_codes(x[4], x[5], x[6], x[7])); }
-// Codes of a block whose scale has risen by 1 / ratio.
-__device__ __forceinline__ uint32_t moved(uint32_t codes, float ratio) {
-  const float2 lo = __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)codes, __NV_E4M3)));
-  const float2 hi = __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(codes >> 16), __NV_E4M3)));
-  return four_codes(lo.x * ratio, lo.y * ratio, hi.x * ratio, hi.y * ratio);
-}
-
 template <typename T>
 __device__ __forceinline__ void widen(const uint4& raw, float (&x)[F]) {
   const uint32_t words[4] = {raw.x, raw.y, raw.z, raw.w};
@@ -121,13 +102,16 @@ __device__ __forceinline__ void span_of(const CacheArgs& c, int e, int N, bool r
   *count = 0;
 }
 
-template <typename T, int D>
+// kTree: the call's tokens are a tree (a.parents): they lie in the cache as they come, and are rotated at the positions of their depth.
+template <typename T, int D, bool kTree>
 __global__ void __launch_bounds__(kThreads, 2) append_kernel(const __grid_constant__ AppendArgs a) {
   constexpr int kLanes = D / F, kRows = 32 / kLanes;               // rows of a warp at once
   constexpr int kTeam = kScaleBlock / kRows, kTeams = kWarps / kTeam;  // warps that hold the 16 tokens of a head between them
   constexpr int kHeads = 2;                                        // of keys, and of values, that a team has in flight
   __shared__ float2 table[kScaleBlock * D / 2];
   __shared__ unsigned int most[3][kTeams][2][kHeads];
+  __shared__ int16_t parents[kTree ? kTreeTokens : 1];
+  __shared__ int places[kTree ? kScaleBlock : 1];
   const CacheArgs& c = a.cache;
   const int tid = threadIdx.x, lane = tid & 31, f0 = (lane & (kLanes - 1)) * F;
   const int team = (tid >> 5) / kTeam, slot = ((tid >> 5) % kTeam) * kRows + lane / kLanes;  // the lane's token of the block
@@ -170,8 +154,19 @@ __global__ void __launch_bounds__(kThreads, 2) append_kernel(const __grid_consta
   };
   load(g_first + team * kHeads);  // (on their way while the sines are computed)
   load_q(q_first);
+  if constexpr (kTree) {
+    const int behind = min(base + last - start, count);  // (a token's ancestors are in front of it)
+    for (int i = tid; any && i < behind; i += kThreads) parents[i] = (int16_t)parent_of(a.parents + e * a.parents_se, i, c.status);
+    __syncthreads();
+    if (any && tid >= first && tid < last) {
+      int depth = -1;
+      for (int i = base + tid - start; i >= 0; i = parents[i]) ++depth;
+      places[tid] = start + depth;
+    }
+    __syncthreads();
+  }
   if (any)
-    for (int i = first * pairs + tid; i < last * pairs; i += kThreads) table[i] = rotary_turn(a.rotary, i % pairs, base + i / pairs);
+    for (int i = first * pairs + tid; i < last * pairs; i += kThreads) table[i] = rotary_turn(a.rotary, i % pairs, kTree ? places[i / pairs] : base + i / pairs);
   if (tid < 3 * kTeams * 2 * kHeads) (&most[0][0][0][0])[tid] = 0;
   const int page = any ? page_of(c, e, base) : -1;
   if (any && page < 0 && tid == 0 && blockIdx.y == 0) report(c.status, kBadPage);
@@ -315,14 +310,18 @@ cudaError_t launch_append(const AppendArgs& a, int dtype, int width, cudaStream_
   void* args[] = {(void*)&a};
   const bool bf = dtype == MA_B200_BF16;
   // us, the kernel for single tokens / the other: 8 sequences of 4 heads 3.5 / 9.9, 256 of 8 heads 5.4 / 20.1
+  // (The one token of a tree is at the position of its place.)
   if (a.N == 1) {
     const int rows = kWarps * 32 * F / width;  // of a CTA
     const void* fn = bf ? (width == 128 ? (const void*)append_token_kernel<__nv_bfloat16, 128> : (const void*)append_token_kernel<__nv_bfloat16, 64>)
                         : (width == 128 ? (const void*)append_token_kernel<__half, 128> : (const void*)append_token_kernel<__half, 64>);
     return launch_kernel(fn, dim3(a.E, (2 * a.cache.heads + a.H + rows - 1) / rows), dim3(kThreads), args, 0, stream);
   }
-  const void* fn = bf ? (width == 128 ? (const void*)append_kernel<__nv_bfloat16, 128> : (const void*)append_kernel<__nv_bfloat16, 64>)
-                      : (width == 128 ? (const void*)append_kernel<__half, 128> : (const void*)append_kernel<__half, 64>);
+  const void* fn = bf ? (width == 128 ? (const void*)append_kernel<__nv_bfloat16, 128, false> : (const void*)append_kernel<__nv_bfloat16, 64, false>)
+                      : (width == 128 ? (const void*)append_kernel<__half, 128, false> : (const void*)append_kernel<__half, 64, false>);
+  if (a.parents != nullptr && a.rotary.pairs > 0)  // (where nothing is rotated a tree's tokens are like any others)
+    fn = bf ? (width == 128 ? (const void*)append_kernel<__nv_bfloat16, 128, true> : (const void*)append_kernel<__nv_bfloat16, 64, true>)
+            : (width == 128 ? (const void*)append_kernel<__half, 128, true> : (const void*)append_kernel<__half, 64, true>);
   const long long blocks = (long long)a.E * ((a.N + kScaleBlock - 2) / kScaleBlock + 1);
   // Few blocks: their heads are spread over more CTAs, each of which computes the sines again; four for each SM where a block's sines are few, else one.
   // us, all heads together / four / one: 17 tokens of 8 sequences 11.2 / 7.8 / 7.7; 5 tokens of 64 sequences and 12 heads of 64 features 10.2 / 8.3 / 9.5; a

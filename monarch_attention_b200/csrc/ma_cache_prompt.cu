@@ -53,7 +53,10 @@ struct Layout {
   static constexpr int kQ = 0, kK = 2 * kTileBytes, kV = kK + 2 * kTileBytes, kBlocks = kV + 2 * kTileBytes;
   static constexpr int kBarriers = kBlocks + kRing * (int)sizeof(Blocks), kFlags = kBarriers + 8 * kBars, kBytes = kFlags + 16;
   static constexpr int kSmem = kBytes + 1024;  // (tiles start on 1024-byte boundaries)
+  // of trees: the rows' lines, a bit for each of the call's tokens (word by word, a row next to the other), and their parents
+  static constexpr int kLines = kBytes, kLineWords = kTreeTokens / 32, kParents = kLines + kLineWords * kRows * 4, kTreeSmem = kParents + kTreeTokens * 2 + 1024;
 };
+static_assert(Layout<128>::kTreeSmem <= 227 * 1024 && kTreeTokens <= kThreads, "a thread brings a parent");
 
 struct PromptArgs {
   AttendArgs a;
@@ -103,26 +106,37 @@ struct RowScores {
   float factor, softcap;
   int low, high;
 };
+// Of 32 keys from t on, those that a row of a tree sees: of those in front of the call (from `low` on), and of the call's own, which begin at `start`, the ones of its
+// line.  (None of these is in front of `low`: a token's place in the call is its depth or more.)
+__device__ __forceinline__ uint32_t tree_keys(const uint32_t* line, int words, int start, int low, int t) {
+  const int at = t - start, i = at >> 5, s = at & 31;  // (at is -32 or more where it matters)
+  const uint32_t w0 = i >= 0 && i < words ? line[i * kRows] : 0, w1 = i >= -1 && i + 1 < words ? line[(i + 1) * kRows] : 0;
+  uint32_t m = at <= -32 ? 0xffffffffu : __funnelshift_r(at < 0 ? 0xffffffffu : w0, w1, s);
+  const int hidden = low - t;
+  if (hidden > 0) m = hidden >= 32 ? 0 : m & (0xffffffffu << hidden);
+  return m;
+}
 // A step's weights of a row whose scores are far from zero, of the 128 scores at t_s (t0: the first one's key), in place of them, and into the row's sum.
 //
 // The kernel's loop has a weight as the exponential of fma(score, f, log - reference), with the logarithm of the value's scale in the reference: where
 // the last bit of a score is worth more than a unit, such a difference is anything, the weights leave f16 and the logarithm is lost.  Here a score is
 // rounded first and a reference is a score S and a logarithm L: (score - S) + (log - L) is exact for the keys that count, however large S is.
 // A few scores are in registers at a time, read and scaled twice: 1276 us for the loop's 281 (2 x 1024 tokens over 16384 keys of 128 features).
-template <typename T, int D>
-__device__ __forceinline__ void rows_apart(const RowScores& r, const Blocks& b, int t0, uint32_t t_s, uint32_t t_o, bool has_sums, float* sum, float* S_row, float* L_row) {
+template <typename T, int D, bool kTree>
+__device__ __forceinline__ void rows_apart(const RowScores& r, const uint32_t* line, int words, const Blocks& b, int t0, uint32_t t_s, uint32_t t_o, bool has_sums, float* sum, float* S_row, float* L_row) {
   // (What leaves the kernel's loop as it was; us of 2 x 1024 tokens over 16384 keys with 1 / 2 / 4: 128 features, bf16 281 / 288 / 285, f16 285 / 282 / 278; 64
   // features, bf16 273 / 266 / 277, f16 275 / 270 / 271.)
   constexpr int kUnroll = D == 64 ? 2 : std::is_same<T, __half>::value ? 4 : 1;
   auto load = [&](int q, float (&x)[32]) {
     tmem_ld32_nowait(t_s + 32 * q, x);
     tmem_wait_ld(x);
+    const uint32_t keys = kTree ? tree_keys(line, words, r.high, r.low, t0 + 32 * q) : 0;
 #pragma unroll
     for (int j = 0; j < 32; ++j) {
       const float f = r.factor * b.k_scale[2 * q + j / 16];
       x[j] = r.softcap > 0.0f ? capped(x[j] * f, r.softcap) : __fmul_rn(x[j], fmaxf(f, 1e-37f));
       const int t = t0 + 32 * q + j;
-      if (t < r.low || t >= r.high) x[j] = -CUDART_INF_F;
+      if (kTree ? !(keys >> j & 1) : t < r.low || t >= r.high) x[j] = -CUDART_INF_F;
     }
   };
   float S = *S_row, L = *L_row, best = -CUDART_INF_F, best_log = 0.0f;
@@ -196,7 +210,8 @@ __device__ __forceinline__ void put_codes(uint32_t panel, uint32_t row, uint32_t
 }
 
 // kExpire: of the self-test, in which the values of a CTA's first step never arrive.
-template <typename T, int D, bool kExpire = false>
+// kTree: the call's tokens are a tree (a.parents).
+template <typename T, int D, bool kExpire = false, bool kTree = false>
 __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_constant__ PromptArgs args) {
   using L = Layout<D>;
   constexpr int kPanel = 128 * 128;  // bytes of 128 rows of 64 features
@@ -230,7 +245,8 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
   const bool two = row0 + kTileRows < count * a.group;  // the second tile has rows
   int lo = 0, hi = len;
   if (a.causal) hi = min(len, len - count + last_token + 1);
-  if (a.window > 0) lo = max(max(len - count + first_token, 0) - a.window + 1, 0) & ~(kScaleBlock - 1);
+  // (a tree's token stands anywhere between the first one's position and that of its place)
+  if (a.window > 0) lo = max(max(len - count + (kTree ? 0 : first_token), 0) - a.window + 1, 0) & ~(kScaleBlock - 1);
   if (first_token >= count) hi = lo;
   const int all_steps = max((hi - lo + kKeys - 1) / kKeys, 0);
   const int step0 = (int)((long long)piece * all_steps / args.pieces), steps = (int)((long long)(piece + 1) * all_steps / args.pieces) - step0;
@@ -255,6 +271,10 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
   if (warp == 12) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(base + L::kFlags + 4), "r"(512) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  int16_t* const parents = reinterpret_cast<int16_t*>(smem + L::kParents);
+  if constexpr (kTree) {
+    if (tid < count) parents[tid] = (int16_t)parent_of(a.parents + e * a.parents_se, tid, c.status);
   }
   tc_fence_before();
   __syncthreads();
@@ -311,9 +331,20 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
       }
       fence_async_smem();
       mbar_arrive(bar(kQ0 + tile));
-      const int place = len - count + token;
-      // (rows of padding, whose results are not looked at, ask for no mask)
-      const int high = !real ? 0x7fffffff : a.causal ? place + 1 : len, low = real && a.window > 0 ? max(place, 0) - a.window + 1 : 0;
+      int place = len - count + token;
+      uint32_t* const line = reinterpret_cast<uint32_t*>(smem + L::kLines) + tid;  // (of trees; tid is the row's number in the CTA)
+      const int words = kTree ? (a.N + 31) >> 5 : 0;
+      if constexpr (kTree) {
+        if (real) {
+          for (int i = 0; i < words; ++i) line[i * kRows] = 0;
+          int depth = 0;
+          for (int n = token; n >= 0; n = parents[n], ++depth)
+            if (a.window == 0 || depth < a.window) line[(n >> 5) * kRows] |= 1u << (n & 31);
+          place = len - count + depth - 1;
+        }
+      }
+      // (rows of padding, whose results are not looked at, ask for no mask; of a tree, keys from `high` on are looked up)
+      const int high = !real ? 0x7fffffff : kTree ? len - count : a.causal ? place + 1 : len, low = real && a.window > 0 ? max(place, 0) - a.window + 1 : 0;
       // Warps of nothing but padding leave the schedulers to the others: 64 rows of 64 heads over 16384 keys 189 -> 138 us.
       for (int i = 0; i < steps && idle && ok; ++i) {
         ok = wait(kS0 + tile, i);
@@ -348,10 +379,12 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
           }
           if (t0 < low || t0 + kKeys > high) {
 #pragma unroll
-            for (int q = 0; q < 4; ++q)
+            for (int q = 0; q < 4; ++q) {
+              const uint32_t keys = kTree ? tree_keys(line, words, high, low, t0 + 32 * q) : 0;
 #pragma unroll
               for (int j = 0; j < 32; ++j)
-                if (t0 + 32 * q + j < low || t0 + 32 * q + j >= high) v[q][j] = -CUDART_INF_F;
+                if (kTree ? !(keys >> j & 1) : t0 + 32 * q + j < low || t0 + 32 * q + j >= high) v[q][j] = -CUDART_INF_F;
+            }
           }
           const float ref = top == -CUDART_INF_F ? 0.0f : top;
           float most = -CUDART_INF_F;
@@ -413,7 +446,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
           if (!there) ok = wait(kS0 + tile, i);
           if (!ok) break;
           tc_fence_after();
-          rows_apart<T, D>({factor, a.softcap, low, high}, blocks[i & (kRing - 1)], lo + i * kKeys, t_s, t_o, i > 0, &sum, &top, &top_log);
+          rows_apart<T, D, kTree>({factor, a.softcap, low, high}, line, words, blocks[i & (kRing - 1)], lo + i * kKeys, t_s, t_o, i > 0, &sum, &top, &top_log);
           tmem_wait_st();
           tc_fence_before();
           mbar_arrive(bar(kP0 + tile));
@@ -643,14 +676,17 @@ cudaError_t launch_prompt(AttendArgs a, int dtype, int width, void* workspace, l
   const bool bf = dtype == MA_B200_BF16;
   const void* fn = width == 128 ? (bf ? (const void*)prompt_kernel<__nv_bfloat16, 128> : (const void*)prompt_kernel<__half, 128>)
                                 : (bf ? (const void*)prompt_kernel<__nv_bfloat16, 64> : (const void*)prompt_kernel<__half, 64>);
+  const bool tree = a.parents != nullptr;
+  if (tree) fn = width == 128 ? (bf ? (const void*)prompt_kernel<__nv_bfloat16, 128, false, true> : (const void*)prompt_kernel<__half, 128, false, true>)
+                              : (bf ? (const void*)prompt_kernel<__nv_bfloat16, 64, false, true> : (const void*)prompt_kernel<__half, 64, false, true>);
   if (wait_expiry) fn = width == 128 ? (const void*)prompt_kernel<__nv_bfloat16, 128, true> : (const void*)prompt_kernel<__nv_bfloat16, 64, true>;
-  const size_t smem = width == 128 ? Layout<128>::kSmem : Layout<64>::kSmem;
+  const size_t smem = width == 128 ? (tree ? Layout<128>::kTreeSmem : Layout<128>::kSmem) : tree ? Layout<64>::kTreeSmem : Layout<64>::kSmem;
   // a build whose launch does not cover the roles' registers must not start: setmaxnreg would wait for them without end
-  static std::atomic<unsigned long long> checked[6];
+  static std::atomic<unsigned long long> checked[10];
   int dev = 0;
   cudaError_t err = cudaGetDevice(&dev);
   if (err != cudaSuccess) return err;
-  std::atomic<unsigned long long>& done = checked[(width == 128) * 3 + (wait_expiry ? 2 : bf)];
+  std::atomic<unsigned long long>& done = checked[(width == 128) * 5 + (wait_expiry ? 4 : 2 * tree + bf)];
   if (dev >= 64 || !(done.load(std::memory_order_relaxed) >> dev & 1)) {
     cudaFuncAttributes fa;
     err = cudaFuncGetAttributes(&fa, fn);

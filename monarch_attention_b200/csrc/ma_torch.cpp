@@ -205,10 +205,14 @@ PyMethodDef methods[] = {{"forward", reinterpret_cast<PyCFunction>(reinterpret_c
                           "rotary(q, k | None, turns, dim, pairs, magnitude, positions | None, inverse) -> (Tensor, Tensor | None)"},
                          {"append", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(py_append)), METH_FASTCALL,
                           "append(k_cache, v_cache, k_scale, v_scale, k, v, page_table, lengths, counts | None, query | None, turns | None, dim, "
-                          "pairs, magnitude) -> Tensor | None"},
+                          "pairs, magnitude, parents | None) -> Tensor | None"},
                          {"attend", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(py_attend)), METH_FASTCALL,
                           "attend(q, k_cache, v_cache, k_scale, v_scale, page_table, lengths, counts | None, causal, scale, softcap, window, "
-                          "out | None, token_major) -> Tensor"},
+                          "out | None, token_major, parents | None) -> Tensor"},
+                         {"accept", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(py_accept)), METH_FASTCALL,
+                          "accept(caches, page_table, lengths, counts | None, parents, drafted, answers) -> (Tensor, Tensor, Tensor)"},
+                         {"fork", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(py_fork)), METH_FASTCALL,
+                          "fork(caches, page_uses, page_table, lengths, source | None, room) -> None"},
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_native", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

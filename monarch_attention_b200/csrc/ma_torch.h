@@ -47,5 +47,7 @@ inline void check_no_tangent(const at::Tensor& t, const char* name) {
 PyObject* py_rotary(PyObject*, PyObject* const* args, Py_ssize_t n);
 PyObject* py_append(PyObject*, PyObject* const* args, Py_ssize_t n);
 PyObject* py_attend(PyObject*, PyObject* const* args, Py_ssize_t n);
+PyObject* py_accept(PyObject*, PyObject* const* args, Py_ssize_t n);
+PyObject* py_fork(PyObject*, PyObject* const* args, Py_ssize_t n);
 
 }  // namespace ma_torch

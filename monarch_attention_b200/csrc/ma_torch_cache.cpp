@@ -6,6 +6,8 @@
 #include <torch/csrc/autograd/saved_variable.h>
 
 #include <algorithm>
+#include <array>
+#include <vector>
 
 #include "ma_torch.h"
 
@@ -256,6 +258,14 @@ ma_b200_sequences sequences_struct(const Tensor& table, const Tensor& lengths, c
           counts.has_value() ? counts->data_ptr<int32_t>() : nullptr};
 }
 
+// The parents of a tree's tokens.
+ma_b200_tree tree_struct(const Tensor& parents, int64_t E, int64_t N, const at::Device& device) {
+  TORCH_CHECK_VALUE(parents.scalar_type() == at::kInt && parents.dim() == 2 && parents.size(0) == E && parents.size(1) == N && parents.device() == device,
+                    "parents must be int32 of shape (batch, tokens) on the query's or key's device, got ", parents.scalar_type(), " ", parents.sizes());
+  TORCH_CHECK_VALUE(parents.stride(1) == 1 || N <= 1, "the rows of parents must be contiguous");
+  return {parents.data_ptr<int32_t>(), parents.stride(0)};
+}
+
 // Rows that the kernels can read as they are, else a copy.
 Tensor aligned(const Tensor& t, size_t bytes) {
   bool fine = t.stride(-1) == 1 && reinterpret_cast<uintptr_t>(t.data_ptr()) % bytes == 0;
@@ -273,7 +283,7 @@ void check_16bit(const Tensor& t, const char* name) {
 }
 
 Tensor append(const Cache& cache, const Tensor& k_in, const Tensor& v_in, const Tensor& table, const Tensor& lengths, const optional<Tensor>& counts,
-              const optional<Tensor>& query, const Rotary* rotary) {
+              const optional<Tensor>& query, const Rotary* rotary, const optional<Tensor>& parents) {
   check_16bit(k_in, "key");
   check_16bit(v_in, "value");
   TORCH_CHECK_VALUE(v_in.sizes() == k_in.sizes() && v_in.scalar_type() == k_in.scalar_type() && v_in.device() == k_in.device(),
@@ -286,6 +296,8 @@ Tensor append(const Cache& cache, const Tensor& k_in, const Tensor& v_in, const 
   TORCH_CHECK_VALUE(k_in.size(1) == p.cache.heads && k_in.size(3) == p.cache.width, "key shape ", k_in.sizes(), " does not match the cache's ",
                     p.cache.heads, " heads of ", p.cache.width);
   p.sequences = sequences_struct(table, lengths, counts, k_in.size(0), k_in.device());
+  ma_b200_tree tree{};
+  if (parents.has_value()) tree = tree_struct(*parents, k_in.size(0), k_in.size(2), k_in.device());
   for (const auto& [a, b] : {std::pair<const Tensor&, const Tensor&>(cache.k, cache.v), std::pair<const Tensor&, const Tensor&>(cache.k_scale, cache.v_scale)}) {
     const char *at = static_cast<const char*>(a.data_ptr()), *bt = static_cast<const char*>(b.data_ptr());
     if (a.is_contiguous() && b.is_contiguous() && (at + a.nbytes() <= bt || bt + b.nbytes() <= at)) continue;  // (as allocated: 0.2 us less of the host's 6.5)
@@ -317,7 +329,8 @@ Tensor append(const Cache& cache, const Tensor& k_in, const Tensor& v_in, const 
     r = rotary_struct(*rotary);
     p.rotary = &r;
   }
-  raise_for_status(ma_b200_cache_append(&p, c10::cuda::getCurrentCUDAStream().stream()));
+  const auto stream = c10::cuda::getCurrentCUDAStream().stream();
+  raise_for_status(parents.has_value() ? ma_b200_cache_append_tree(&p, &tree, stream) : ma_b200_cache_append(&p, stream));
   // (what a graph has saved of the pool is not what it was)
   for (const Tensor* t : {&cache.k, &cache.v, &cache.k_scale, &cache.v_scale})
     if (!t->is_inference()) t->unsafeGetTensorImpl()->bump_version();
@@ -325,7 +338,7 @@ Tensor append(const Cache& cache, const Tensor& k_in, const Tensor& v_in, const 
 }
 
 Tensor attend(const Tensor& q_in, const Cache& cache, const Tensor& table, const Tensor& lengths, const optional<Tensor>& counts, bool causal, double scale,
-              double softcap, int64_t window, const optional<Tensor>& out_in, bool token_major) {
+              double softcap, int64_t window, const optional<Tensor>& out_in, bool token_major, const optional<Tensor>& parents) {
   check_16bit(q_in, "query");
   const c10::cuda::CUDAGuard guard(q_in.device());
   raise_for_status(ma_b200_poll_device_status(q_in.device().index()));  // (a bounded wait of an earlier call that gave up)
@@ -340,6 +353,11 @@ Tensor attend(const Tensor& q_in, const Cache& cache, const Tensor& table, const
   // (before it becomes a number of 32 bits, where a smaller one is zero: none)
   TORCH_CHECK_VALUE(softcap == 0.0 || (softcap >= 1e-20 && softcap <= 1e30), "softcap must be 0 (none) or from 1e-20 to 1e30");
   const int64_t E = q_in.size(0), H = q_in.size(1), N = q_in.size(2), W = q_in.size(3);
+  ma_b200_tree tree{};
+  if (parents.has_value()) {
+    tree = tree_struct(*parents, E, N, q_in.device());
+    TORCH_CHECK_VALUE(causal, "parents need causal: a tree's tokens see their ancestors");
+  }
   Tensor out;
   if (out_in.has_value()) {
     out = *out_in;
@@ -371,8 +389,157 @@ Tensor attend(const Tensor& q_in, const Cache& cache, const Tensor& table, const
   const size_t need = ma_b200_cache_attend_workspace_bytes(&p);
   if (need == 0) raise_for_status(MA_B200_INVALID_ARGUMENT);
   const c10::DataPtr ws = c10::cuda::CUDACachingAllocator::get()->allocate(need);
-  raise_for_status(ma_b200_cache_attend(&p, ws.get(), need, c10::cuda::getCurrentCUDAStream().stream()));
+  const auto stream = c10::cuda::getCurrentCUDAStream().stream();
+  raise_for_status(parents.has_value() ? ma_b200_cache_attend_tree(&p, &tree, ws.get(), need, stream) : ma_b200_cache_attend(&p, ws.get(), need, stream));
   return out;
+}
+
+// ---------------------------------------------------------------------------------------------- caches of several layers
+
+using Layer = std::array<Tensor, 4>;  // k, v, k_scale, v_scale
+
+std::vector<Layer> layers_of(PyObject* x) {
+  PyObject* const seq = PySequence_Fast(x, "caches must be a PagedKV or a sequence of them");
+  if (seq == nullptr) throw python_error();
+  const THPObjectPtr owner(seq);
+  std::vector<Layer> layers;
+  const Py_ssize_t n = PySequence_Fast_GET_SIZE(seq);
+  layers.reserve(n);
+  static const char* const names[4] = {"cache.k", "cache.v", "cache.k_scale", "cache.v_scale"};
+  for (Py_ssize_t i = 0; i < n; ++i) {
+    PyObject* const c = PySequence_Fast_GET_ITEM(seq, i);
+    TORCH_CHECK_TYPE(PyTuple_Check(c) && PyTuple_GET_SIZE(c) == 4, "caches must be a PagedKV or a sequence of them");
+    Layer& l = layers.emplace_back();
+    for (int j = 0; j < 4; ++j) l[j] = tensor_of(PyTuple_GET_ITEM(c, j), names[j]);
+  }
+  TORCH_CHECK_VALUE(n > 0, "caches must hold a cache");
+  return layers;
+}
+
+// No two elements of all layers' keys and values are in one place, nor of their scales.  (As allocated, the tensors lie one behind the other: that is seen from
+// where they begin and end.)
+void check_apart(const std::vector<Layer>& layers) {
+  for (int part = 0; part < 4; part += 2) {
+    c10::SmallVector<std::pair<const char*, const char*>, 128> at;
+    bool apart = true;
+    for (const Layer& l : layers)
+      for (int j = part; j < part + 2; ++j) {
+        const char* const begin = static_cast<const char*>(l[j].data_ptr());
+        apart = apart && l[j].is_non_overlapping_and_dense();
+        at.emplace_back(begin, begin + l[j].nbytes());
+      }
+    std::sort(at.begin(), at.end());
+    for (size_t i = 1; i < at.size(); ++i) apart = apart && at[i].first >= at[i - 1].second;
+    if (apart) continue;
+    std::vector<Places> places;
+    for (const Layer& l : layers)
+      for (int j = part; j < part + 2; ++j) places.emplace_back(l[j]);
+    for (size_t i = 0; i < places.size(); ++i) {
+      bool fine = places[i].distinct();
+      for (size_t j = 0; j < i; ++j) fine = fine && !meet(places[j], places[i]);
+      TORCH_CHECK_VALUE(fine, "the caches must not overlap: pages, heads or tokens are over one another, keys over values, or a layer over another");
+    }
+  }
+}
+
+std::vector<ma_b200_cache> cache_structs(const std::vector<Layer>& layers, const at::Device& device) {
+  std::vector<ma_b200_cache> caches;
+  caches.reserve(layers.size());
+  for (const Layer& l : layers) caches.push_back(cache_struct(Cache{l[0], l[1], l[2], l[3]}, device));
+  check_apart(layers);
+  return caches;
+}
+void mark_changed(const std::vector<Layer>& layers) {
+  for (const Layer& l : layers)
+    for (const Tensor& t : l)
+      if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
+void check_cuda(const Tensor& t) { TORCH_CHECK(t.is_cuda(), "monarch_attention_b200 runs on CUDA tensors only (there is no CPU path)"); }
+
+std::array<Tensor, 3> accept(const std::vector<Layer>& layers, const Tensor& table, const Tensor& lengths, const optional<Tensor>& counts, const Tensor& parents,
+                             const Tensor& drafted, const Tensor& answers) {
+  TORCH_CHECK_VALUE(drafted.dim() == 2 && (drafted.scalar_type() == at::kInt || drafted.scalar_type() == at::kLong), "drafted must be int32 or int64 of shape (batch, tokens)");
+  check_cuda(drafted);
+  const at::Device device = drafted.device();
+  TORCH_CHECK_VALUE(answers.sizes() == drafted.sizes() && answers.scalar_type() == drafted.scalar_type() && answers.device() == device,
+                    "answers must have the shape, dtype and device of drafted");
+  const int64_t E = drafted.size(0), N = drafted.size(1);
+  TORCH_CHECK_VALUE(N <= 1 || (drafted.stride(1) == 1 && answers.stride(1) == 1), "the rows of drafted and answers must be contiguous");
+  TORCH_CHECK_VALUE(E <= INT32_MAX && N <= INT32_MAX, "too many sequences or tokens");
+  const c10::cuda::CUDAGuard guard(device);
+  raise_for_status(ma_b200_poll_cache_status(device.index()));
+  const std::vector<ma_b200_cache> caches = cache_structs(layers, device);
+  ma_b200_accept p{};
+  p.abi_version = MA_B200_ABI_VERSION;
+  p.E = (int32_t)E; p.N = (int32_t)N; p.layers = (int32_t)layers.size();
+  p.caches = caches.data();
+  p.sequences = sequences_struct(table, lengths, counts, E, device);
+  p.tree = tree_struct(parents, E, N, device);
+  const at::TensorOptions ints = at::TensorOptions().dtype(at::kInt).device(device);
+  if (E == 0 || N == 0) return {lengths.clone(), at::empty({E, N}, ints), at::full({E}, -1, drafted.options())};
+  std::array<Tensor, 3> out{at::detail::empty_cuda({E}, ints), at::detail::empty_cuda({E, N}, ints), at::detail::empty_cuda({E}, ints.dtype(drafted.scalar_type()))};
+  p.drafted = drafted.data_ptr();
+  p.answers = answers.data_ptr();
+  p.drafted_stride = drafted.stride(0);
+  p.answers_stride = answers.stride(0);
+  p.ids_i64 = drafted.scalar_type() == at::kLong;
+  p.new_lengths = out[0].data_ptr<int32_t>();
+  p.path = out[1].data_ptr<int32_t>();
+  p.answer = out[2].data_ptr();
+  raise_for_status(ma_b200_cache_accept(&p, c10::cuda::getCurrentCUDAStream().stream()));
+  mark_changed(layers);
+  return out;
+}
+
+void fork(const std::vector<Layer>& layers, const Tensor& uses, const Tensor& table, const Tensor& lengths, const optional<Tensor>& source,
+          const optional<Tensor>& room, int64_t room_all) {
+  check_cuda(table);
+  const at::Device device = table.device();
+  const c10::cuda::CUDAGuard guard(device);
+  raise_for_status(ma_b200_poll_cache_status(device.index()));
+  const std::vector<ma_b200_cache> caches = cache_structs(layers, device);
+  TORCH_CHECK_VALUE(table.dim() == 2, "page_table must be int32 of shape (batch, pages of a sequence)");
+  const int64_t E = table.size(0);
+  const ma_b200_sequences s = sequences_struct(table, lengths, std::nullopt, E, device);
+  TORCH_CHECK_VALUE(uses.scalar_type() == at::kInt && uses.dim() == 1 && uses.size(0) == caches[0].pages && uses.is_contiguous() && uses.device() == device,
+                    "page_uses must be contiguous int32 of shape (pages) on the table's device");
+  for (const auto& [t, name] : {std::pair<const optional<Tensor>&, const char*>(source, "source"), std::pair<const optional<Tensor>&, const char*>(room, "room")})
+    if (t.has_value())
+      TORCH_CHECK_VALUE(t->scalar_type() == at::kInt && t->dim() == 1 && t->size(0) == E && t->is_contiguous() && t->device() == device, name,
+                        " must be contiguous int32 of shape (batch) on the table's device");
+  TORCH_CHECK_VALUE(room.has_value() || (room_all >= 0 && room_all <= INT32_MAX), "room must not be negative");
+  if (E == 0) return;
+  TORCH_CHECK_VALUE(E <= INT32_MAX && (E == 1 || table.stride(0) >= table.size(1)), "the rows of page_table overlap");
+  // what is written lies apart from all else
+  auto bytes = [&](const Tensor& t) {
+    const char* const begin = static_cast<const char*>(t.data_ptr());
+    return std::pair<const char*, const char*>(begin, begin + (t.dim() == 2 ? (E - 1) * t.stride(0) + t.size(1) : t.numel()) * t.element_size());
+  };
+  const std::pair<const char*, const char*> written[3] = {bytes(uses), bytes(table), bytes(lengths)};
+  auto apart = [](const auto& a, const auto& b) { return a.second <= b.first || b.second <= a.first; };
+  bool fine = apart(written[0], written[1]) && apart(written[0], written[2]) && apart(written[1], written[2]);
+  for (const auto& w : written) fine = fine && (!source.has_value() || apart(w, bytes(*source))) && (!room.has_value() || apart(w, bytes(*room)));
+  TORCH_CHECK_VALUE(fine, "page_uses, page_table and lengths, which are written, must not overlap one another, source or room");
+  ma_b200_fork p{};
+  p.abi_version = MA_B200_ABI_VERSION;
+  p.E = (int32_t)E; p.layers = (int32_t)layers.size();
+  p.caches = caches.data();
+  p.page_uses = uses.data_ptr<int32_t>();
+  p.page_table = table.data_ptr<int32_t>();
+  p.table_stride = s.table_stride;
+  p.table_pages = s.table_pages;
+  p.lengths = lengths.data_ptr<int32_t>();
+  p.source = source.has_value() ? source->data_ptr<int32_t>() : nullptr;
+  p.room = room.has_value() ? room->data_ptr<int32_t>() : nullptr;
+  p.room_all = (int32_t)room_all;
+  const size_t need = ma_b200_cache_fork_workspace_bytes(&p);
+  if (need == 0) raise_for_status(MA_B200_INVALID_ARGUMENT);
+  const c10::DataPtr ws = c10::cuda::CUDACachingAllocator::get()->allocate(need);
+  raise_for_status(ma_b200_cache_fork(&p, ws.get(), need, c10::cuda::getCurrentCUDAStream().stream()));
+  mark_changed(layers);
+  for (const Tensor* t : {&uses, &table, &lengths})
+    if (!t->is_inference()) t->unsafeGetTensorImpl()->bump_version();
 }
 
 PyObject* wrap_or_none(Tensor t) {
@@ -406,17 +573,17 @@ PyObject* py_rotary(PyObject*, PyObject* const* args, Py_ssize_t n) {
 
 PyObject* py_append(PyObject*, PyObject* const* args, Py_ssize_t n) {
   HANDLE_TH_ERRORS
-  TORCH_CHECK_TYPE(n == 14, "append() takes 14 arguments");
+  TORCH_CHECK_TYPE(n == 15, "append() takes 15 arguments");
   const Cache cache{tensor_of(args[0], "cache.k"), tensor_of(args[1], "cache.v"), tensor_of(args[2], "cache.k_scale"), tensor_of(args[3], "cache.v_scale")};
   const Tensor &k = tensor_of(args[4], "key"), &v = tensor_of(args[5], "value"), &table = tensor_of(args[6], "page_table"),
                &lengths = tensor_of(args[7], "lengths");
-  const optional<Tensor> counts = optional_of(args[8], "counts"), query = optional_of(args[9], "query");
+  const optional<Tensor> counts = optional_of(args[8], "counts"), query = optional_of(args[9], "query"), parents = optional_of(args[14], "parents");
   optional<Rotary> rotary;
   if (args[10] != Py_None) rotary = rotary_of(args[10], args[11], args[12], args[13]);
   Tensor out;
   {
     pybind11::gil_scoped_release no_gil;
-    out = append(cache, k, v, table, lengths, counts, query, rotary.has_value() ? &*rotary : nullptr);
+    out = append(cache, k, v, table, lengths, counts, query, rotary.has_value() ? &*rotary : nullptr, parents);
   }
   return wrap_or_none(std::move(out));
   END_HANDLE_TH_ERRORS
@@ -424,11 +591,11 @@ PyObject* py_append(PyObject*, PyObject* const* args, Py_ssize_t n) {
 
 PyObject* py_attend(PyObject*, PyObject* const* args, Py_ssize_t n) {
   HANDLE_TH_ERRORS
-  TORCH_CHECK_TYPE(n == 14, "attend() takes 14 arguments");
+  TORCH_CHECK_TYPE(n == 15, "attend() takes 15 arguments");
   const Tensor& q = tensor_of(args[0], "query");
   const Cache cache{tensor_of(args[1], "cache.k"), tensor_of(args[2], "cache.v"), tensor_of(args[3], "cache.k_scale"), tensor_of(args[4], "cache.v_scale")};
   const Tensor &table = tensor_of(args[5], "page_table"), &lengths = tensor_of(args[6], "lengths");
-  const optional<Tensor> counts = optional_of(args[7], "counts"), out_in = optional_of(args[12], "out");
+  const optional<Tensor> counts = optional_of(args[7], "counts"), out_in = optional_of(args[12], "out"), parents = optional_of(args[14], "parents");
   const bool causal = PyObject_IsTrue(args[8]) == 1, token_major = PyObject_IsTrue(args[13]) == 1;
   const double scale = PyFloat_AsDouble(args[9]), softcap = PyFloat_AsDouble(args[10]);
   const int64_t window = PyLong_AsLongLong(args[11]);
@@ -436,9 +603,47 @@ PyObject* py_attend(PyObject*, PyObject* const* args, Py_ssize_t n) {
   Tensor out;
   {
     pybind11::gil_scoped_release no_gil;
-    out = attend(q, cache, table, lengths, counts, causal, scale, softcap, window, out_in, token_major);
+    out = attend(q, cache, table, lengths, counts, causal, scale, softcap, window, out_in, token_major, parents);
   }
   return wrap_or_none(std::move(out));
+  END_HANDLE_TH_ERRORS
+}
+
+PyObject* py_accept(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  TORCH_CHECK_TYPE(n == 7, "accept() takes 7 arguments");
+  const std::vector<Layer> layers = layers_of(args[0]);
+  const Tensor &table = tensor_of(args[1], "page_table"), &lengths = tensor_of(args[2], "lengths"), &parents = tensor_of(args[4], "parents"),
+               &drafted = tensor_of(args[5], "drafted"), &answers = tensor_of(args[6], "answers");
+  const optional<Tensor> counts = optional_of(args[3], "counts");
+  std::array<Tensor, 3> out;
+  {
+    pybind11::gil_scoped_release no_gil;
+    out = accept(layers, table, lengths, counts, parents, drafted, answers);
+  }
+  PyObject* result = PyTuple_New(3);
+  if (result == nullptr) throw python_error();
+  for (int i = 0; i < 3; ++i) PyTuple_SET_ITEM(result, i, THPVariable_Wrap(std::move(out[i])));
+  return result;
+  END_HANDLE_TH_ERRORS
+}
+
+PyObject* py_fork(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  TORCH_CHECK_TYPE(n == 6, "fork() takes 6 arguments");
+  const std::vector<Layer> layers = layers_of(args[0]);
+  const Tensor &uses = tensor_of(args[1], "page_uses"), &table = tensor_of(args[2], "page_table"), &lengths = tensor_of(args[3], "lengths");
+  const optional<Tensor> source = optional_of(args[4], "source");
+  optional<Tensor> room;
+  int64_t room_all = 0;
+  if (THPVariable_Check(args[5])) room = THPVariable_Unpack(args[5]);
+  else room_all = PyLong_AsLongLong(args[5]);
+  check_python();
+  {
+    pybind11::gil_scoped_release no_gil;
+    fork(layers, uses, table, lengths, source, room, room_all);
+  }
+  Py_RETURN_NONE;
   END_HANDLE_TH_ERRORS
 }
 

@@ -65,7 +65,7 @@ def _load() -> None:
 
 
 def append_kv_b200(cache: PagedKV, key: Tensor, value: Tensor, page_table: Tensor, lengths: Tensor, counts: Tensor | None = None, *,
-                   query: Tensor | None = None, rotary: RotaryPositions | None = None) -> Tensor | None:
+                   query: Tensor | None = None, rotary: RotaryPositions | None = None, parents: Tensor | None = None) -> Tensor | None:
     """Writes ``key`` and ``value`` (E, heads, N, width; bfloat16 or float16) into the cache at the call's positions.
 
     With ``rotary`` (``dim`` a multiple of 16) keys are rotated at their positions on the way, and so is ``query`` (E, H, N, width), whose
@@ -74,17 +74,21 @@ def append_kv_b200(cache: PagedKV, key: Tensor, value: Tensor, page_table: Tenso
     values that become subnormal.  Magnitudes above 448 * 2^60 (infinities) are stored as that, NaN as NaN.  The pages that a call writes to
     must stand once in one sequence's row of the table (pages that are only read may be shared), and the pool's pages, heads and tokens must not
     overlap (keys and values may lie in one buffer, with the same strides).  No gradient: inputs that require one are refused.
+
+    ``parents`` (E, N; int32, N up to 512): the tokens are a tree, several continuations of a sequence at once.  Each names its parent, an earlier token of the call, or -1.  A
+    token lies in the cache at its place in the call, and is rotated at the position of its depth: ``lengths[e] - counts[e]`` and the number of its ancestors.
     """
     if _append is None:
         _load()
     if rotary is not None and not isinstance(rotary, RotaryPositions):
         raise TypeError("rotary must be a RotaryPositions or None")
-    return _append(*cache, key, value, page_table, lengths, counts, query, *(rotary._native if rotary is not None else _NO_ROTARY))
+    return _append(*cache, key, value, page_table, lengths, counts, query, *(rotary._native if rotary is not None else _NO_ROTARY),
+                   parents)
 
 
 def cached_attention_b200(query: Tensor, cache: PagedKV, page_table: Tensor, lengths: Tensor, counts: Tensor | None = None, *,
                           causal: bool = True, scale: float | None = None, softcap: float = 0.0, window: int = 0,
-                          out: Tensor | None = None, token_major_output: bool = False) -> Tensor:
+                          parents: Tensor | None = None, out: Tensor | None = None, token_major_output: bool = False) -> Tensor:
     """Softmax attention of ``query`` (E, H, N, width; bfloat16 or float16) over the cached tokens of its sequences.
 
     Query head ``h`` reads cache head ``h // (H / heads)``.  ``causal``: a token sees the positions up to its own (the call's tokens have been
@@ -92,6 +96,10 @@ def cached_attention_b200(query: Tensor, cache: PagedKV, page_table: Tensor, len
     multiplied by ``scale`` (None: ``width ** -0.5``) and, with ``softcap`` > 0 (from 1e-20 to 1e30), become ``softcap * tanh(score / softcap)``.  Rows without
     a key, and rows of padding, are zero.  What lies in the cache behind a sequence's end is never looked at, NaN included; a NaN that was appended as a key
     makes NaN of the rows that see it, as a value it reaches all of the call's rows of its sequence and head, masked ones too (zero times NaN).
+
+    ``parents`` (E, N; int32, N up to 512; causal only): the call's tokens are a tree, appended with the same parents.  A token sees what is cached in front of
+    the call, its ancestors and itself; a window counts positions, which go by depth.  A parent that is no earlier token of the call counts as -1, none, and a
+    later call raises.
 
     The result has the query's dtype, and with ``token_major_output`` is a view of an (E, N, H, width) buffer; ``out`` (rows on 16-byte
     boundaries) takes it in place: the query itself, or rows beside its own in a common buffer, are fine; rows over one another or over others of the
@@ -104,15 +112,16 @@ def cached_attention_b200(query: Tensor, cache: PagedKV, page_table: Tensor, len
     if _attend is None:
         _load()
     return _attend(query, *cache, page_table, lengths, counts, causal, query.shape[-1] ** -0.5 if scale is None else scale, softcap, window,
-                   out, token_major_output)
+                   out, token_major_output, parents)
 
 
 class CachedAttention(nn.Module):
     """The attention of a decoder layer: new tokens into the cache, then attention over all of it.
 
-    ``forward(query, key, value, cache, page_table, lengths, counts=None)`` has query, key and value of one step (a prompt, a piece of
+    ``forward(query, key, value, cache, page_table, lengths, counts=None, parents=None)`` has query, key and value of one step (a prompt, a piece of
     one, or a token) in the (E, H, N, width) views that :class:`MonarchAttention` takes, key and value with the cache's heads.  With
     ``key`` and ``value`` None nothing is appended and the query is not rotated: attention to an encoder's output that is in the cache already.
+    With ``parents`` the step's tokens are a tree of drafted ones (:func:`accept_drafts_b200` then keeps those that the model confirms).
     """
 
     def __init__(self, rotary: RotaryPositions | None = None, causal: bool = True, scale: float | None = None, softcap: float = 0.0,
@@ -124,15 +133,15 @@ class CachedAttention(nn.Module):
         # Set to True to get the result as a view of a (batch, tokens, heads, width) buffer, as MonarchAttention has it.
         self.token_major_output = False
 
-    def forward(self, query, key, value, cache, page_table, lengths, counts=None):
+    def forward(self, query, key, value, cache, page_table, lengths, counts=None, parents=None):
         if (key is None) != (value is None):
             raise ValueError("key and value must be given together")
         if key is not None:
             rotated = append_kv_b200(cache, key, value, page_table, lengths, counts, query=query if self.rotary is not None else None,
-                                     rotary=self.rotary)
+                                     rotary=self.rotary, parents=parents)
             query = rotated if self.rotary is not None else query
         return cached_attention_b200(query, cache, page_table, lengths, counts, causal=self.causal, scale=self.scale, softcap=self.softcap,
-                                     window=self.window, token_major_output=self.token_major_output)
+                                     window=self.window, parents=parents, token_major_output=self.token_major_output)
 
     def extra_repr(self) -> str:
         return f"rotary={self.rotary}, causal={self.causal}, softcap={self.softcap}, window={self.window}"
