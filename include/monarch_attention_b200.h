@@ -399,7 +399,8 @@ typedef struct ma_b200_tree {
 } ma_b200_tree;
 /* ma_b200_cache_append with keys and queries rotated at the tokens' positions. */
 MA_B200_API int ma_b200_cache_append_tree(const ma_b200_append* p, const ma_b200_tree* tree, void* stream);
-/* ma_b200_cache_attend (causal; the same workspace): a token sees what is cached in front of the call, its ancestors and itself; a window is of positions. */
+/* ma_b200_cache_attend (causal): a token sees what is cached in front of the call, its ancestors and itself; a window is of positions. */
+MA_B200_API size_t ma_b200_cache_attend_tree_workspace_bytes(const ma_b200_attend* p);
 MA_B200_API int ma_b200_cache_attend_tree(const ma_b200_attend* p, const ma_b200_tree* tree, void* workspace, size_t workspace_bytes, void* stream);
 
 /* Which tokens of a tree stand, and the caches of all layers (HOST array, one shape and strides) closed up over them.  drafted and answers (E, N; int32, or

@@ -31,7 +31,7 @@ EXPORTS = (
     "ma_b200_backward_workspace_bytes", "ma_b200_backward", "ma_b200_forward_typed_mask", "ma_b200_backward_typed_mask",
     "ma_b200_rotary_apply", "ma_b200_cache_append", "ma_b200_cache_attend_workspace_bytes", "ma_b200_cache_attend",
     "ma_b200_poll_cache_status", "ma_b200_selftest_attend_wait_expiry",
-    "ma_b200_cache_append_tree", "ma_b200_cache_attend_tree", "ma_b200_cache_accept", "ma_b200_cache_fork_workspace_bytes", "ma_b200_cache_fork",
+    "ma_b200_cache_append_tree", "ma_b200_cache_attend_tree", "ma_b200_cache_attend_tree_workspace_bytes", "ma_b200_cache_accept", "ma_b200_cache_fork_workspace_bytes", "ma_b200_cache_fork",
 )
 
 
@@ -188,6 +188,8 @@ def load() -> C.CDLL:
     lib.ma_b200_cache_append_tree.restype = C.c_int
     lib.ma_b200_cache_attend_tree.argtypes = [C.POINTER(Attend), C.POINTER(Tree), C.c_void_p, C.c_size_t, C.c_void_p]
     lib.ma_b200_cache_attend_tree.restype = C.c_int
+    lib.ma_b200_cache_attend_tree_workspace_bytes.argtypes = [C.POINTER(Attend)]
+    lib.ma_b200_cache_attend_tree_workspace_bytes.restype = C.c_size_t
     lib.ma_b200_cache_accept.argtypes = [C.POINTER(Accept), C.c_void_p]
     lib.ma_b200_cache_accept.restype = C.c_int
     lib.ma_b200_cache_fork_workspace_bytes.argtypes = [C.POINTER(Fork)]

@@ -135,12 +135,15 @@ __device__ __forceinline__ bool sees_keys(const AttendArgs& a, int len, int coun
 size_t attend_workspace(int E, int N, int H, int kv_heads, int width, int window, long long longest);
 // (wait_expiry, a self-test: a wait of the kernel for many rows runs out.)
 cudaError_t launch_attend(AttendArgs a, int dtype, int width, void* workspace, long long longest, int* wait_status, bool wait_expiry, cudaStream_t stream);
+// The same over a tree (a.parents).
+size_t attend_tree_workspace(int E, int N, int H, int kv_heads, int width, int window, long long longest);
 // The kernel for few rows over trees (ma_cache_attend_tree.cu): `nt` tiles of 8 rows, `warps` warps a CTA.
 cudaError_t launch_few_tree(AttendArgs& a, int dtype, int width, int nt, int warps, long long grid, cudaStream_t stream);
 // The pieces of `entries` heads and blocks of tile_rows rows (a.split, a.part_o, a.part_ml; a head's pieces `stride` slots apart) into a.out.
 cudaError_t launch_join(const AttendArgs& a, int dtype, int width, int tile_rows, int entries, int stride, cudaStream_t stream);
 // The kernel for many rows (ma_cache_prompt.cu).
 size_t prompt_workspace(int E, int N, int H, int kv_heads, int width, long long longest);
+size_t prompt_tree_workspace(int E, int N, int H, int kv_heads, int width, long long longest);
 cudaError_t launch_prompt(AttendArgs a, int dtype, int width, void* workspace, long long longest, int* wait_status, bool wait_expiry, cudaStream_t stream);
 
 }  // namespace ma

@@ -135,7 +135,7 @@ int attend(const ma_b200_attend* p, const ma_b200_tree* tree, void* workspace, s
   if ((rc = check_cache(p->cache, p->sequences, p->E, p->H, p->N, p->dtype, &a.cache)) != MA_B200_OK) return rc;
   if ((rc = check_tensor(p->q, "q", 2, 16)) != MA_B200_OK || (rc = check_tensor(p->out, "out", 2, 16)) != MA_B200_OK) return rc;
   const long long most = longest(p->sequences, p->cache.page_size);
-  const size_t need = ma::attend_workspace(p->E, p->N, p->H, p->cache.heads, p->cache.width, p->window, most);
+  const size_t need = (tree != nullptr ? ma::attend_tree_workspace : ma::attend_workspace)(p->E, p->N, p->H, p->cache.heads, p->cache.width, p->window, most);
   if (workspace == nullptr || reinterpret_cast<uintptr_t>(workspace) % 256 != 0) return invalid("workspace is NULL or not 256-byte aligned");
   if (workspace_bytes < need)
     return fail_with(MA_B200_WORKSPACE_TOO_SMALL, "workspace has " + std::to_string(workspace_bytes) + " bytes, need " + std::to_string(need));
@@ -199,6 +199,11 @@ int ma_b200_cache_append_tree(const ma_b200_append* p, const ma_b200_tree* tree,
 size_t ma_b200_cache_attend_workspace_bytes(const ma_b200_attend* p) {
   if (check_attend_shape(p) != MA_B200_OK) return 0;
   return ma::attend_workspace(p->E, p->N, p->H, p->cache.heads, p->cache.width, p->window, longest(p->sequences, p->cache.page_size));
+}
+
+size_t ma_b200_cache_attend_tree_workspace_bytes(const ma_b200_attend* p) {
+  if (check_attend_shape(p) != MA_B200_OK) return 0;
+  return ma::attend_tree_workspace(p->E, p->N, p->H, p->cache.heads, p->cache.width, p->window, longest(p->sequences, p->cache.page_size));
 }
 
 int ma_b200_cache_attend(const ma_b200_attend* p, void* workspace, size_t workspace_bytes, void* stream) {

@@ -1,5 +1,5 @@
 // Attention over the cache: the pieces of split heads are joined here, and a call goes to the kernel for few rows (ma_cache_attend.inc) or
-// the one for many (ma_cache_prompt.inc).
+// the one for many (ma_cache_prompt.cu).
 #include "ma_cache_attend.inc"
 
 namespace ma {
@@ -199,6 +199,10 @@ size_t attend_workspace(int E, int N, int H, int kv_heads, int width, int window
   if (plan.whole) return 256;
   const size_t entries = ((size_t)plan.grid * sizeof(int4) + 255) / 256 * 256;
   return entries + (size_t)plan.grid * 2 * 8 * plan.nt * (width + 2) * sizeof(float);
+}
+
+size_t attend_tree_workspace(int E, int N, int H, int kv_heads, int width, int window, long long longest) {
+  return H / kv_heads * (long long)N >= kPromptRows ? prompt_tree_workspace(E, N, H, kv_heads, width, longest) : attend_workspace(E, N, H, kv_heads, width, window, longest);
 }
 
 cudaError_t launch_attend(AttendArgs a, int dtype, int width, void* workspace, long long longest, int* wait_status, bool wait_expiry, cudaStream_t stream) {

@@ -31,15 +31,23 @@ namespace {
 using namespace sm100;
 
 constexpr int kKeys = 128, kTileRows = 128, kRows = 2 * kTileRows;
-constexpr int kThreads = 512, kBringers = 128;  // warps 0-3, 4-7: rows; 8-11: keys and values; 12: products (13-15 make it a warpgroup)
-constexpr int kLaunchRegs = 128, kRowRegs = 184, kBringerRegs = 104, kIssuerRegs = 40;
-static_assert(256 * kRowRegs + kBringers * kBringerRegs + 128 * kIssuerRegs <= kThreads * kLaunchRegs, "setmaxnreg draws on the launch's registers");
-constexpr int kRing = 8;  // steps whose pages and scales are kept
+constexpr int kThreads = 512, kBringers = 128;  // warps 0-3, 4-7: rows; 8-11: keys and values; 12: products; 13: pages and scales (14, 15 make it a warpgroup)
+constexpr int kMostRing = 16, kGroup = 4, kGroups = kMostRing / kGroup;  // steps whose pages and scales are kept; so many are looked up at a time by a warp of their own
+// Pages and scales are looked up by a warp of their own, some ten steps ahead (kAhead), or a step at a time by eight of the threads that bring keys and values.  us, the one / the
+// other: 64 features, 2 x 1024 tokens over 16384 keys 260 / 268 (f16 256 / 272), 8 x 64 tokens over 4096 37 / 44; 128 features 281 / 284 (f16 287 / 280), 46 / 46, 300 tokens 19.5 / 18.6:
+// there the products and the exponentials bind, and the rows can use the registers.  Trees, which have fewer rows, always.
+template <int D, bool kTree>
+struct Roles {
+  static constexpr bool kAhead = D == 64 || kTree;
+  static constexpr int kRing = kAhead ? kMostRing : 8;
+  static constexpr int kLaunchRegs = 128, kRowRegs = kAhead ? 176 : 184, kBringerRegs = 104, kOtherRegs = kAhead ? 56 : 40;
+  static_assert(256 * kRowRegs + kBringers * kBringerRegs + 128 * kOtherRegs <= kThreads * kLaunchRegs, "setmaxnreg draws on the launch's registers");
+};
 constexpr float kBelow = 7.0f, kSlack = 15.0f;  // (ma_cache_attend.cu)
 // Scores beyond this (in units of log2) have references in two parts (rows_apart).
 constexpr float kApart = 8192.0f;
 
-enum Bar { kQ0, kQ1, kKFull, kKEmpty = kKFull + 2, kVFull = kKEmpty + 2, kVEmpty = kVFull + 2, kS0 = kVEmpty + 2, kS1, kP0, kP1, kO, kDrain, kBars };
+enum Bar { kQ0, kQ1, kKFull, kKEmpty = kKFull + 2, kVFull = kKEmpty + 2, kVEmpty = kVFull + 2, kS0 = kVEmpty + 2, kS1, kP0, kP1, kO, kDrain, kKnown, kFree = kKnown + kGroups, kBars = kFree + kGroups };
 
 // What the rows need of a step's 8 blocks.
 struct alignas(16) Blocks {
@@ -51,7 +59,7 @@ template <int D>
 struct Layout {
   static constexpr int kTileBytes = 128 * D * 2;  // 128 rows in f16: panels of 64 features
   static constexpr int kQ = 0, kK = 2 * kTileBytes, kV = kK + 2 * kTileBytes, kBlocks = kV + 2 * kTileBytes;
-  static constexpr int kBarriers = kBlocks + kRing * (int)sizeof(Blocks), kFlags = kBarriers + 8 * kBars, kBytes = kFlags + 16;
+  static constexpr int kBarriers = kBlocks + kMostRing * (int)sizeof(Blocks), kFlags = kBarriers + 8 * kBars, kBytes = kFlags + 16;
   static constexpr int kSmem = kBytes + 1024;  // (tiles start on 1024-byte boundaries)
   // of trees: the rows' lines, a bit for each of the call's tokens (word by word, a row next to the other), and their parents
   static constexpr int kLines = kBytes, kLineWords = kTreeTokens / 32, kParents = kLines + kLineWords * kRows * 4, kTreeSmem = kParents + kTreeTokens * 2 + 1024;
@@ -60,7 +68,8 @@ static_assert(Layout<128>::kTreeSmem <= 227 * 1024 && kTreeTokens <= kThreads, "
 
 struct PromptArgs {
   AttendArgs a;
-  int pieces;        // that the keys of a CTA's rows are cut into
+  int pieces;        // that the keys of a CTA's rows are cut into; 0 (trees): as many as make all CTAs' about equal
+  int turns;         // (trees) 1: both tiles have the same rows, and take the steps in turns
   int* wait_status;  // mapped host word: a wait that gave up
 };
 
@@ -209,11 +218,81 @@ __device__ __forceinline__ void put_codes(uint32_t panel, uint32_t row, uint32_t
   st_shared_v4(panel + swz(row, chunk + 1), widen2(c.z), widen2_upper(c.z), widen2(c.w), widen2_upper(c.w));
 }
 
+// Trees, with no more heads and blocks of rows than CTAs: the keys of each are cut into pieces of no more than C steps, C the smallest for which there are enough CTAs.  A warp finds C and
+// what is CTA `cta`'s: sequence (-1: nothing), pieces of each of its heads and blocks, which piece, and of which of them.
+__device__ __forceinline__ void even_pieces(const AttendArgs& a, int ctas, int cta, int lane, int (&shares)[4]) {
+  const int units = a.cache.heads * a.row_blocks;  // of a sequence
+  auto steps_of = [&](int e) {
+    int len, count;
+    sequence_of(a.cache, e, a.N, &len, &count);
+    const int lo = a.window > 0 ? max(max(len - count, 0) - a.window + 1, 0) & ~(kScaleBlock - 1) : 0;
+    return max((len - lo + kKeys - 1) / kKeys, 1);
+  };
+  constexpr int kMost = 5;  // of a lane: 32 * 5 sequences are more than there are SMs
+  int steps[kMost], longest = 1;
+#pragma unroll
+  for (int i = 0; i < kMost; ++i) {
+    const int e = lane + 32 * i;
+    steps[i] = e < a.E ? steps_of(e) : 0;
+    longest = max(longest, steps[i]);
+  }
+  auto pieces_with = [&](int most) {
+    int n = 0;
+#pragma unroll
+    for (int i = 0; i < kMost; ++i) n += (steps[i] + most - 1) / most;
+    return __reduce_add_sync(0xffffffffu, n) * units;
+  };
+  int low = 1, high = __reduce_max_sync(0xffffffffu, longest);
+  while (low < high) {
+    const int mid = (low + high) >> 1;
+    if (pieces_with(mid) <= ctas) high = mid;
+    else low = mid + 1;
+  }
+  int at = 0, found_e = -1, found_pieces = 1, found = 0;
+#pragma unroll
+  for (int i = 0; i < kMost; ++i) {
+    const int n = (steps[i] + low - 1) / low;
+    int upto = n * units;
+#pragma unroll
+    for (int m = 1; m < 32; m <<= 1) {
+      const int o = __shfl_up_sync(0xffffffffu, upto, m);
+      if (lane >= m) upto += o;
+    }
+    const int first = at + upto - n * units;
+    if (cta >= first && cta < first + n * units) {
+      found_e = lane + 32 * i;
+      found_pieces = n;
+      found = cta - first;
+    }
+    at += __shfl_sync(0xffffffffu, upto, 31);
+  }
+  const unsigned who = __ballot_sync(0xffffffffu, found_e >= 0);
+  if (who == 0 ? lane == 0 : found_e >= 0) {
+    shares[0] = found_e;
+    shares[1] = found_pieces;
+    shares[2] = found % found_pieces;
+    shares[3] = found / found_pieces;
+  }
+}
+
+// A block of a step, by its page (-1: nothing) and scales.
+__device__ __forceinline__ void put_block(Blocks& b, int block, int page, float ks, float vs) {
+  // (a scale of zero is another one before zeros, since a mask is minus infinity times the keys' scale and a weight is divided by the values': one for keys,
+  // the smallest that there is for values, whose weights are not to be above those of any other block's)
+  b.page[0][block] = ks == 0.0f ? -1 : page;
+  b.page[1][block] = vs == 0.0f ? -1 : page;
+  b.k_scale[block] = ks == 0.0f ? 1.0f : ks;
+  b.v_inverse[block] = vs == 0.0f ? exp2f(-kLeastLog) : 1.0f / vs;
+  b.v_log[block] = vs == 0.0f ? kLeastLog : __log2f(vs);
+}
+
 // kExpire: of the self-test, in which the values of a CTA's first step never arrive.
 // kTree: the call's tokens are a tree (a.parents).
 template <typename T, int D, bool kExpire = false, bool kTree = false>
 __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_constant__ PromptArgs args) {
   using L = Layout<D>;
+  using R = Roles<D, kTree>;
+  constexpr int kRing = R::kRing;
   constexpr int kPanel = 128 * 128;  // bytes of 128 rows of 64 features
   constexpr uint32_t kTmemS = 0, kTmemO = 256;  // columns: S (and P) of both tiles, then O of both
   extern __shared__ uint8_t smem_raw[];
@@ -235,21 +314,40 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
 
   grid_wait();
   // --- the CTA's rows and keys; row blocks with more keys come first
-  const int piece = blockIdx.x % args.pieces, unit = blockIdx.x / args.pieces;  // unit: (block from the last on, sequence, head)
-  const int e_head = unit % (a.E * c.heads), block = a.row_blocks - 1 - unit / (a.E * c.heads);
-  const int e = e_head / c.heads, head = e_head % c.heads, row0 = block * kRows;
+  int pieces = args.pieces, piece, unit, e, head, block;
+  if (!kTree || pieces > 0) {
+    piece = blockIdx.x % pieces;
+    unit = blockIdx.x / pieces;  // (block from the last on, sequence, head)
+    const int e_head = unit % (a.E * c.heads);
+    block = a.row_blocks - 1 - unit / (a.E * c.heads);
+    e = e_head / c.heads;
+    head = e_head % c.heads;
+  } else {
+    __shared__ int shares[4];
+    if (warp == 0) even_pieces(a, gridDim.x, blockIdx.x, tid, shares);
+    __syncthreads();
+    e = shares[0];
+    if (e < 0) return;  // (a CTA too many)
+    pieces = shares[1];
+    piece = shares[2];
+    head = shares[3] / a.row_blocks;
+    block = shares[3] - head * a.row_blocks;
+    unit = (e * c.heads + head) * a.row_blocks + block;
+  }
+  const int row0 = block * kRows;
   int len, count;
   const bool fine = sequence_of(c, e, a.N, &len, &count);
   if (!fine && tid == 0) report(c.status, kBadLength);
   const int first_token = row0 / a.group, last_token = min((row0 + kRows - 1) / a.group, count - 1);
-  const bool two = row0 + kTileRows < count * a.group;  // the second tile has rows
+  const bool turns = kTree && args.turns;
+  const bool two = turns || row0 + kTileRows < count * a.group;  // the second tile has rows
   int lo = 0, hi = len;
   if (a.causal) hi = min(len, len - count + last_token + 1);
   // (a tree's token stands anywhere between the first one's position and that of its place)
   if (a.window > 0) lo = max(max(len - count + (kTree ? 0 : first_token), 0) - a.window + 1, 0) & ~(kScaleBlock - 1);
   if (first_token >= count) hi = lo;
   const int all_steps = max((hi - lo + kKeys - 1) / kKeys, 0);
-  const int step0 = (int)((long long)piece * all_steps / args.pieces), steps = (int)((long long)(piece + 1) * all_steps / args.pieces) - step0;
+  const int step0 = (int)((long long)piece * all_steps / pieces), steps = (int)((long long)(piece + 1) * all_steps / pieces) - step0;
   lo += step0 * kKeys;
 
   if (tid == 0) {
@@ -265,6 +363,12 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
     }
     mbar_init(bar(kO), 1);
     mbar_init(bar(kDrain), 1);
+    if constexpr (R::kAhead) {
+      for (int i = 0; i < kGroups; ++i) {
+        mbar_init(bar(kKnown + i), 32);
+        mbar_init(bar(kFree + i), 1);
+      }
+    }
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -283,13 +387,16 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
 
   if (warp < 8) {
     // =========================== a row a thread ======================================================================
-    regs_inc<kRowRegs>();
-    const int tile = warp >> 2, r = tid & 127, row = row0 + tile * kTileRows + r;
+    regs_inc<R::kRowRegs>();
+    const int tile = warp >> 2, r = tid & 127, row = row0 + (turns ? 0 : tile * kTileRows) + r;
+    // the tile's steps: all of them, or every other one; a step's phase is how manieth it is
+    const int i0 = turns ? tile : 0, stride = turns ? 2 : 1, shift = turns ? 1 : 0;
     const int token = row / a.group, h = head * a.group + row - token * a.group;
     const bool exists = token < a.N, real = token < count;
     const uint32_t lanes = (uint32_t)(warp & 3) << 21;  // the warp's 32 lanes of tensor memory
     const uint32_t t_s = tmem + kTmemS + tile * 128 + lanes, t_o = tmem + kTmemO + tile * 128 + lanes;
-    const bool works = steps > 0 && (tile == 0 || two), idle = !__any_sync(0xffffffffu, real);
+    bool works = steps > 0 && (tile == 0 || two);
+    const bool idle = !__any_sync(0xffffffffu, real);
     int keyed = sees_keys(a, len, count, token);
     asm volatile("" : "+r"(keyed));  // (else its four operands take registers through the loop)
     float factor = fabsf(a.scale) * kLog2e, top = -CUDART_INF_F, top_log = 0.0f, sum = 0.0f;  // top_log: of references in two parts
@@ -346,13 +453,13 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
       // (rows of padding, whose results are not looked at, ask for no mask; of a tree, keys from `high` on are looked up)
       const int high = !real ? 0x7fffffff : kTree ? len - count : a.causal ? place + 1 : len, low = real && a.window > 0 ? max(place, 0) - a.window + 1 : 0;
       // Warps of nothing but padding leave the schedulers to the others: 64 rows of 64 heads over 16384 keys 189 -> 138 us.
-      for (int i = 0; i < steps && idle && ok; ++i) {
-        ok = wait(kS0 + tile, i);
+      for (int i = i0; i < steps && idle && ok; i += stride) {
+        ok = wait(kS0 + tile, i >> shift);
         if (ok) mbar_arrive(bar(kP0 + tile));
       }
-      int i = 0;
-      for (; i < steps && !idle; ++i) {
-        ok = wait(kS0 + tile, i);
+      int i = i0;
+      for (; i < steps && !idle; i += stride) {
+        ok = wait(kS0 + tile, i >> shift);
         if (!ok) break;
         tc_fence_after();
         const Blocks& b = blocks[i & (kRing - 1)];
@@ -417,7 +524,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
           top = fmaxf(top, most - kBelow);
           const float shrink = ex2(before - (top == -CUDART_INF_F ? 0.0f : top));
           sum *= shrink;
-          if (i > 0) {  // (the scores of this step are there, so the products of the one before are done)
+          if (i >= stride) {  // (the scores of this step are there, so the products of the one before are done)
 #pragma unroll 1
             for (int q = 0; q < D / 16; ++q) {
               float o[16];
@@ -443,14 +550,14 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
       apart:
 #pragma unroll 1
         for (bool there = true;; there = false) {  // (the first step's scores have been waited for)
-          if (!there) ok = wait(kS0 + tile, i);
+          if (!there) ok = wait(kS0 + tile, i >> shift);
           if (!ok) break;
           tc_fence_after();
-          rows_apart<T, D, kTree>({factor, a.softcap, low, high}, line, words, blocks[i & (kRing - 1)], lo + i * kKeys, t_s, t_o, i > 0, &sum, &top, &top_log);
+          rows_apart<T, D, kTree>({factor, a.softcap, low, high}, line, words, blocks[i & (kRing - 1)], lo + i * kKeys, t_s, t_o, i >= stride, &sum, &top, &top_log);
           tmem_wait_st();
           tc_fence_before();
           mbar_arrive(bar(kP0 + tile));
-          if (++i == steps) break;
+          if ((i += stride) >= steps) break;
         }
       }
       if (ok) {
@@ -460,9 +567,11 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
     }
     // --- result: rows without a key, and of padding, are zero
     if (ok) {
+      if (turns && i0 >= steps) works = false;  // (no step was this tile's)
       const float unit_of = ex2(top_log);  // (a piece's reference is one number)
       const float inverse = top > -CUDART_INF_F ? 1.0f / sum : 0.0f;  // (no key, no reference)
-      const size_t slot = ((size_t)unit * args.pieces + piece) * kRows + tile * kTileRows + r;
+      // (even pieces have a place for each CTA)
+      const size_t slot = (kTree && args.pieces == 0 ? (size_t)blockIdx.x : (size_t)unit * pieces + piece) * kRows + tile * kTileRows + r;
       T* const dst = reinterpret_cast<T*>(const_cast<void*>(a.out.ptr)) + e * a.out.se + h * a.out.sh + token * a.out.sn;
 #pragma unroll
       for (int q = 0; q < D / 32; ++q) {
@@ -473,7 +582,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
           for (int j = 0; j < 32; ++j) o[j] = 0.0f;
         }
         if (!exists) continue;
-        if (args.pieces == 1) {
+        if (pieces == 1 && !turns) {
 #pragma unroll
           for (int j = 0; j < 32; j += 8)
             *reinterpret_cast<uint4*>(dst + 32 * q + j) =
@@ -485,13 +594,19 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
             *reinterpret_cast<float4*>(a.part_o + slot * D + 32 * q + j) = make_float4(o[j] * unit_of, o[j + 1] * unit_of, o[j + 2] * unit_of, o[j + 3] * unit_of);
         }
       }
-      if (args.pieces > 1 && exists) *reinterpret_cast<float2*>(a.part_ml + 2 * slot) = make_float2(top, sum * unit_of);
+      if ((pieces > 1 || turns) && exists) *reinterpret_cast<float2*>(a.part_ml + 2 * slot) = make_float2(top, sum * unit_of);
     }
-    if (args.pieces > 1 && tid == 0 && piece == 0)
-      a.split[unit] = make_int4((e * c.heads + head) * a.row_blocks + block, unit * args.pieces, (unit + 1) * args.pieces - 1, 0);
+    if ((args.pieces != 1 || turns) && tid == 0 && piece == 0) {
+      int first = kTree && args.pieces == 0 ? blockIdx.x : unit * pieces, last = first + pieces - 1;
+      if (turns) {  // (each tile's rows are a piece)
+        first = 2 * first;
+        last = 2 * last + 1;
+      }
+      a.split[unit] = make_int4(pieces > 1 || turns ? (e * c.heads + head) * a.row_blocks + block : -1, first, last, 0);
+    }
   } else if (warp < 12) {
     // =========================== keys and values =====================================================================
-    regs_dec<kBringerRegs>();
+    regs_dec<R::kBringerRegs>();
     const int t = tid - 256, page_mask = (1 << c.page_shift) - 1;
     // Threads 0-7 look after a block each: its page two steps ahead of its scales, those a step ahead of the bytes.
     auto page_at = [&](int i) {
@@ -504,26 +619,17 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
     auto scale_at = [&](const float* scales, long long sp, long long sh, int i, int page) {
       return page < 0 ? 1.0f : scales[page * sp + head * sh + ((lo + i * kKeys + t * kScaleBlock) & page_mask) / kScaleBlock];
     };
-    auto put_blocks = [&](int i, int page, float ks, float vs) {
-      Blocks& b = blocks[i & (kRing - 1)];
-      // (a scale of zero is another one before zeros, since a mask is minus infinity times the keys' scale and a weight is divided by the values': one for keys,
-      // the smallest that there is for values, whose weights are not to be above those of any other block's)
-      b.page[0][t] = ks == 0.0f ? -1 : page;
-      b.page[1][t] = vs == 0.0f ? -1 : page;
-      b.k_scale[t] = ks == 0.0f ? 1.0f : ks;
-      b.v_inverse[t] = vs == 0.0f ? exp2f(-kLeastLog) : 1.0f / vs;
-      b.v_log[t] = vs == 0.0f ? kLeastLog : __log2f(vs);
-    };
+    auto put_blocks = [&](int i, int page, float ks, float vs) { put_block(blocks[i & (kRing - 1)], t, page, ks, vs); };
     auto meet = [&]() { asm volatile("bar.sync 1, %0;" ::"n"(kBringers) : "memory"); };
     int page_next = -1;
-    if (t < 8) {
+    if (!R::kAhead && t < 8) {
       for (int i = 0; i < 2; ++i) {
         const int page = page_at(i);
         put_blocks(i, page, scale_at(c.k_scale, c.ks_sp, c.ks_sh, i, page), scale_at(c.v_scale, c.vs_sp, c.vs_sh, i, page));
       }
       page_next = page_at(2);
     }
-    meet();
+    if (!R::kAhead) meet();
     // A thread has a 16-byte piece of 4 in each panel of rows t / 4 + 32 j: eight threads write 4 pieces of two rows, an even and an
     // odd one, whose chunks the swizzle puts on different banks.
     constexpr int kPanels = D / 64;
@@ -548,40 +654,65 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
         for (int x = 0; x < kPanels; ++x) put_codes(to + x * kPanel, (t >> 2) + 32 * j, 2 * (t & 3), raw[which][j][x]);
       fence_async_smem();
     };
-    if (steps > 0) {
-      load(0, 0);
-      load(1, 0);
-    }
-    bool ok = true;  // (whatever happens, all meet at each step)
-    for (int i = 0; i < steps; ++i) {
-      float ks = 1.0f, vs = 1.0f;
-      int page_after = -1;
-      if (t < 8) {
-        ks = scale_at(c.k_scale, c.ks_sp, c.ks_sh, i + 2, page_next);
-        vs = scale_at(c.v_scale, c.vs_sp, c.vs_sh, i + 2, page_next);
-        page_after = page_at(i + 3);
-      }
-      const int stage = i & 1;
-      ok = ok && (i < 2 || wait(kKEmpty + stage, (i >> 1) - 1));
+    if constexpr (R::kAhead) {
+      bool ok = steps > 0 && wait(kKnown, 0);
       if (ok) {
+        load(0, 0);
+        load(1, 0);
+      }
+      for (int i = 0; i < steps && ok; ++i) {
+        const int stage = i & 1;
+        ok = i < 2 || wait(kKEmpty + stage, (i >> 1) - 1);
+        if (!ok) break;
         put(0, base + L::kK + stage * L::kTileBytes);
         mbar_arrive(bar(kKFull + stage));
-      }
-      if (i + 1 < steps) load(0, i + 1);
-      ok = ok && (i < 2 || wait(kVEmpty + stage, (i >> 1) - 1));
-      if (ok) {
+        if (i + 1 < steps) {
+          if ((i + 1) % kGroup == 0) ok = wait(kKnown + (i + 1) / kGroup % kGroups, (i + 1) / kRing);
+          if (!ok) break;
+          load(0, i + 1);
+        }
+        ok = i < 2 || wait(kVEmpty + stage, (i >> 1) - 1);
+        if (!ok) break;
         put(1, base + L::kV + stage * L::kTileBytes);
         if (!kExpire || i > 0) mbar_arrive(bar(kVFull + stage));
+        if (i + 1 < steps) load(1, i + 1);
       }
-      if (i + 1 < steps) load(1, i + 1);
-      if (t < 8) {
-        put_blocks(i + 2, page_next, ks, vs);
-        page_next = page_after;
+    } else {
+      if (steps > 0) {
+        load(0, 0);
+        load(1, 0);
       }
-      meet();
+      bool ok = true;  // (whatever happens, all meet at each step)
+      for (int i = 0; i < steps; ++i) {
+        float ks = 1.0f, vs = 1.0f;
+        int page_after = -1;
+        if (t < 8) {
+          ks = scale_at(c.k_scale, c.ks_sp, c.ks_sh, i + 2, page_next);
+          vs = scale_at(c.v_scale, c.vs_sp, c.vs_sh, i + 2, page_next);
+          page_after = page_at(i + 3);
+        }
+        const int stage = i & 1;
+        ok = ok && (i < 2 || wait(kKEmpty + stage, (i >> 1) - 1));
+        if (ok) {
+          put(0, base + L::kK + stage * L::kTileBytes);
+          mbar_arrive(bar(kKFull + stage));
+        }
+        if (i + 1 < steps) load(0, i + 1);
+        ok = ok && (i < 2 || wait(kVEmpty + stage, (i >> 1) - 1));
+        if (ok) {
+          put(1, base + L::kV + stage * L::kTileBytes);
+          if (!kExpire || i > 0) mbar_arrive(bar(kVFull + stage));
+        }
+        if (i + 1 < steps) load(1, i + 1);
+        if (t < 8) {
+          put_blocks(i + 2, page_next, ks, vs);
+          page_next = page_after;
+        }
+        meet();
+      }
     }
   } else {
-    regs_dec<kIssuerRegs>();
+    regs_dec<R::kOtherRegs>();
   }
   if (warp == 12) {
     // =========================== products ============================================================================
@@ -594,15 +725,41 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
         mma_f16_lo(tmem + kTmemS + tile * 128, da + (kk >> 2) * kPanelUnits + (kk & 3) * 2, db + (kk >> 2) * kPanelUnits + (kk & 3) * 2, kScores, kk > 0);
       mma_commit(bar(kS0 + tile));
     };
-    auto sums = [&](int tile, int i) {
+    auto sums = [&](int tile, int i, bool first) {
       const uint32_t db = smem_desc_lo(base + L::kV, kPanel) + (i & 1) * kTileUnits;
 #pragma unroll
       for (int kk = 0; kk < kKeys / 16; ++kk)
-        mma_f16_ts(tmem + kTmemO + tile * 128, tmem + kTmemS + tile * 128 + kk * 8, db + kk * 128, kSums, i > 0 || kk > 0);
+        mma_f16_ts(tmem + kTmemO + tile * 128, tmem + kTmemS + tile * 128 + kk * 8, db + kk * 128, kSums, !first || kk > 0);
     };
     const int tiles = two ? 2 : 1;
     bool ok = steps > 0 && wait(kKFull, 0);
-    for (int tile = 0; tile < tiles && ok; ++tile) {
+    if (turns) {
+      auto next = [&](int i) {  // scores of step i, in place of weights whose products are in front of them
+        if (!wait(kKFull + (i & 1), i >> 1) || (i < 2 && !wait(kQ0 + i, 0))) return false;
+        tc_fence_after();
+        if (elect_one()) {
+          scores(i & 1, i);
+          mma_commit(bar(kKEmpty + (i & 1)));
+        }
+        __syncwarp();
+        return true;
+      };
+      ok = ok && next(0) && (steps < 2 || next(1));
+      for (int i = 0; i < steps && ok; ++i) {
+        ok = wait(kVFull + (i & 1), i >> 1) && wait(kP0 + (i & 1), i >> 1);
+        if (!ok) break;
+        if (R::kAhead && i % kGroup == kGroup - 1 && (tid & 31) == 0) mbar_arrive(bar(kFree + i / kGroup % kGroups));
+        tc_fence_after();
+        if (elect_one()) {
+          sums(i & 1, i, i < 2);
+          mma_commit(bar(kVEmpty + (i & 1)));
+          if (i + 1 == steps) mma_commit(bar(kO));
+        }
+        __syncwarp();
+        ok = i + 2 >= steps || next(i + 2);
+      }
+    }
+    for (int tile = 0; tile < tiles && ok && !turns; ++tile) {
       ok = wait(kQ0 + tile, 0);
       if (!ok) break;
       tc_fence_after();
@@ -612,14 +769,15 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
       }
       __syncwarp();
     }
-    for (int i = 0; i < steps && ok; ++i) {
+    for (int i = 0; i < steps && ok && !turns; ++i) {
       ok = wait(kVFull + (i & 1), i >> 1, kTries) && (i + 1 == steps || wait(kKFull + ((i + 1) & 1), (i + 1) >> 1));
       for (int tile = 0; tile < tiles && ok; ++tile) {
         ok = wait(kP0 + tile, i);
         if (!ok) break;
+        if (R::kAhead && tile == tiles - 1 && i % kGroup == kGroup - 1 && (tid & 31) == 0) mbar_arrive(bar(kFree + i / kGroup % kGroups));
         tc_fence_after();
         if (elect_one()) {
-          sums(tile, i);
+          sums(tile, i, i == 0);
           if (tile == tiles - 1) mma_commit(bar(kVEmpty + (i & 1)));
           if (i + 1 < steps) {
             scores(tile, i + 1);
@@ -630,6 +788,30 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
         }
         __syncwarp();
       }
+    }
+  }
+
+  if (R::kAhead && warp == 13) {
+    // =========================== pages and scales ====================================================================
+    // A lane has a block of 16 keys of one of a group's steps; both reads of the group's 32 blocks are on their way together, far ahead of the bytes.
+    const int page_mask = (1 << c.page_shift) - 1, lane = tid & 31, own = lane >> 3, block = lane & 7;
+    for (int n0 = 0; n0 < steps; n0 += kGroup) {
+      const int at = lo + (n0 + own) * kKeys + block * kScaleBlock, slot = n0 / kGroup % kGroups;
+      int page = -1;
+      float ks = 1.0f, vs = 1.0f;
+      if (n0 + own < steps && at < len) {
+        page = page_of(c, e, at);
+        if (page >= 0) {
+          const int i = (at & page_mask) / kScaleBlock;
+          ks = c.k_scale[page * c.ks_sp + head * c.ks_sh + i];
+          vs = c.v_scale[page * c.vs_sp + head * c.vs_sh + i];
+        } else {
+          report(c.status, kBadPage);
+        }
+      }
+      if (n0 >= kRing && !wait(kFree + slot, n0 / kRing - 1)) break;
+      put_block(blocks[(n0 + own) & (kRing - 1)], block, page, ks, vs);
+      mbar_arrive(bar(kKnown + slot));
     }
   }
 
@@ -658,6 +840,34 @@ int prompt_pieces(int E, int N, int H, int kv_heads, long long longest) {
   return (int)(fill < 2 || most < 2 ? 1 : fill < most ? fill : most);
 }
 
+// How a tree's rows and keys are shared out.
+struct TreePlan {
+  bool turns, even;
+  int pieces;      // (not even)
+  long long units, grid;
+};
+TreePlan tree_plan(int E, int N, int H, int kv_heads, long long longest) {
+  const long long rows = (long long)H / kv_heads * N, units = (long long)E * kv_heads * ((rows + kRows - 1) / kRows);
+  TreePlan p{};
+  p.units = units;
+  // Even pieces, on a CTA for each SM.  us, even / the same number for all: 8 sequences of up to 8192 tokens, 8 heads of 244 rows, 67.9 / 94.1.
+  p.even = units <= sm_count() && sm_count() <= 160 && longest > 4 * kKeys;
+  p.pieces = p.even ? 0 : prompt_pieces(E, N, H, kv_heads, longest);
+  p.grid = p.even ? sm_count() : units * p.pieces;
+  // Rows of one tile take the other for every other step, where a CTA has steps enough for what the join of twice the pieces costs, and a head not so many pieces that it is long.  us, in
+  // turns / not: 16 sequences of 8192 tokens, 4 heads of 64 rows 67 / 78 (128 rows 76 / 82; 64 features, 64 rows 54 / 63), 24 of 2000 and 48 rows 41 / 44; 32 of 1024 and 8
+  // heads of 64 rows 58 / 49, of 4096 128 / 136 (128 rows 150 / 140); one of 131071 tokens and 2 heads 68 / 57.
+  const long long steps = units * ((longest + kKeys - 1) / kKeys) / p.grid;
+  p.turns = rows <= kTileRows && units >= 16 && (p.even ? steps >= (rows <= 64 ? 10 : 24) : rows <= 64 && steps >= 16);
+  return p;
+}
+
+size_t prompt_tree_workspace(int E, int N, int H, int kv_heads, int width, long long longest) {
+  const TreePlan p = tree_plan(E, N, H, kv_heads, longest);
+  if (p.pieces == 1 && !p.turns) return 256;
+  return ((size_t)p.units * sizeof(int4) + 255) / 256 * 256 + (size_t)p.grid * kRows * (width + 2) * sizeof(float);
+}
+
 size_t prompt_workspace(int E, int N, int H, int kv_heads, int width, long long longest) {
   const long long pieces = prompt_pieces(E, N, H, kv_heads, longest);
   if (pieces == 1) return 256;
@@ -668,11 +878,13 @@ size_t prompt_workspace(int E, int N, int H, int kv_heads, int width, long long 
 cudaError_t launch_prompt(AttendArgs a, int dtype, int width, void* workspace, long long longest, int* wait_status, bool wait_expiry, cudaStream_t stream) {
   a.row_blocks = (a.group * a.N + kRows - 1) / kRows;
   const long long units = (long long)a.E * a.cache.heads * a.row_blocks;
-  PromptArgs args{a, prompt_pieces(a.E, a.N, a.H, a.cache.heads, longest), wait_status};
+  const TreePlan p = a.parents != nullptr ? tree_plan(a.E, a.N, a.H, a.cache.heads, longest) : TreePlan{};
+  PromptArgs args{a, a.parents != nullptr ? p.pieces : prompt_pieces(a.E, a.N, a.H, a.cache.heads, longest), p.turns, wait_status};
+  const long long grid = a.parents != nullptr ? p.grid : units * args.pieces;
   char* at = reinterpret_cast<char*>(workspace);
   args.a.split = reinterpret_cast<int4*>(at);
   args.a.part_o = reinterpret_cast<float*>(at + ((size_t)units * sizeof(int4) + 255) / 256 * 256);
-  args.a.part_ml = args.a.part_o + (size_t)units * args.pieces * kRows * width;
+  args.a.part_ml = args.a.part_o + (size_t)grid * kRows * width;
   const bool bf = dtype == MA_B200_BF16;
   const void* fn = width == 128 ? (bf ? (const void*)prompt_kernel<__nv_bfloat16, 128> : (const void*)prompt_kernel<__half, 128>)
                                 : (bf ? (const void*)prompt_kernel<__nv_bfloat16, 64> : (const void*)prompt_kernel<__half, 64>);
@@ -691,15 +903,15 @@ cudaError_t launch_prompt(AttendArgs a, int dtype, int width, void* workspace, l
     cudaFuncAttributes fa;
     err = cudaFuncGetAttributes(&fa, fn);
     if (err != cudaSuccess) return err;
-    if (fa.numRegs != kLaunchRegs) return cudaErrorLaunchOutOfResources;
+    if (fa.numRegs != Roles<64, false>::kLaunchRegs) return cudaErrorLaunchOutOfResources;
     if (dev < 64) done.fetch_or(1ull << dev, std::memory_order_relaxed);
   }
   err = allow_dynamic_smem(fn, smem);
   if (err != cudaSuccess) return err;
   void* params[] = {(void*)&args};
-  err = launch_kernel(fn, dim3((unsigned)(units * args.pieces)), dim3(kThreads), params, smem, stream);
-  if (err != cudaSuccess || args.pieces == 1) return err;
-  return launch_join(args.a, dtype, width, kRows, (int)units, 1, stream);
+  err = launch_kernel(fn, dim3((unsigned)grid), dim3(kThreads), params, smem, stream);
+  if (err != cudaSuccess || (args.pieces == 1 && !args.turns)) return err;
+  return launch_join(args.a, dtype, width, args.turns ? kTileRows : kRows, (int)units, 1, stream);
 }
 
 }  // namespace ma

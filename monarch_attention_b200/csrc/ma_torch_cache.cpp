@@ -386,7 +386,7 @@ Tensor attend(const Tensor& q_in, const Cache& cache, const Tensor& table, const
   p.softcap = (float)softcap;
   p.q = view4(q);
   p.out = view4(out);
-  const size_t need = ma_b200_cache_attend_workspace_bytes(&p);
+  const size_t need = parents.has_value() ? ma_b200_cache_attend_tree_workspace_bytes(&p) : ma_b200_cache_attend_workspace_bytes(&p);
   if (need == 0) raise_for_status(MA_B200_INVALID_ARGUMENT);
   const c10::DataPtr ws = c10::cuda::CUDACachingAllocator::get()->allocate(need);
   const auto stream = c10::cuda::getCurrentCUDAStream().stream();

@@ -67,6 +67,17 @@ def test_trees_keep_the_checks_of_the_calls_without(lib):
     assert lib.ma_b200_cache_append_tree(C.byref(append(dtype=_cabi.F32)), C.byref(tree()), None) == _cabi.INVALID_ARGUMENT
 
 
+def test_scratch_of_trees_is_host_arithmetic(lib):
+    size = lambda **kw: lib.ma_b200_cache_attend_tree_workspace_bytes(C.byref(attend(**kw)))  # noqa: E731
+    assert size() == size(N=8) == 256 and size(N=200) == 256                       # short sequences: nothing is split
+    few, many = size(N=8, seq=sequences(table_pages=1000)), size(N=200, seq=sequences(table_pages=1000))
+    assert few == lib.ma_b200_cache_attend_workspace_bytes(C.byref(attend(N=8, seq=sequences(table_pages=1000)))) > 256
+    assert many >= 148 * 256 * (128 + 2) * 4                                       # a piece for each SM
+    assert size(H=3) == 0 and size(E=0) == 0
+    p = attend(N=200, seq=sequences(table_pages=1000))
+    assert lib.ma_b200_cache_attend_tree(C.byref(p), C.byref(tree()), 1 << 20, many - 1, None) in (_cabi.WORKSPACE_TOO_SMALL, _cabi.CUDA_ERROR)   # (no device here)
+
+
 @pytest.mark.parametrize("kw", BAD_CACHES)
 def test_caches_are_checked(lib, kw):
     for c in (caches(**kw), (_cabi.Cache * 2)(cache_struct(), cache_struct(**kw))):

@@ -63,7 +63,7 @@ def test_windows_are_of_positions(N, window, softcap, kind, dtype):
 
 @pytest.mark.parametrize("H,Hk,N,lengths,counts,window,softcap", [(4, 4, 1, [700], None, 0, 0.0), (8, 2, 8, [4000, 20], [8, 6], 0, 10.0), (4, 4, 32, [900], None, 50, 0.0), (2, 1, 100, [5000, 100], None, 0, 0.0),
                                                                  (1, 1, 500, [600], None, 300, 0.0)])
-def test_a_chain_has_the_bits_of_ordinary_tokens(H, Hk, N, lengths, counts, window, softcap):
+def test_a_chain_is_what_ordinary_tokens_are(H, Hk, N, lengths, counts, window, softcap):
     import monarch_attention_b200 as ma
     E = len(lengths)
     cache, table = filled(E, max(lengths) // 64 + 2, Hk, 128, 64, lengths)
@@ -71,12 +71,9 @@ def test_a_chain_has_the_bits_of_ordinary_tokens(H, Hk, N, lengths, counts, wind
     kw = dict(window=window, softcap=softcap)
     parents = trees(E, N, "chain")
     out = ma.cached_attention_b200(q, cache, table, *sizes, parents=parents, **kw)
-    if window and N * H // Hk > 256:
-        # From the second block of 256 rows on, the keys of a window begin at the block's first position, which for a tree may be any from the call's first on: steps of 128 keys
-        # are cut elsewhere, and 32-bit sums in another order have other last bits.
-        check(out, q, cache, table, lengths, counts, 64, parents, **kw)
-    else:
+    if N * H // Hk <= 8:   # the same kernel, with another mask
         assert torch.equal(out, ma.cached_attention_b200(q, cache, table, *sizes, **kw))
+    check(out, q, cache, table, lengths, counts, 64, parents, **kw)
 
 
 @pytest.mark.parametrize("N", [6, 60])
