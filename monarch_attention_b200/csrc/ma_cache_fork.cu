@@ -22,6 +22,7 @@ namespace ma {
 namespace {
 
 constexpr int kThreads = 1024, kWarps = kThreads / 32, kMostCtas = 8;
+constexpr int kCached = 1024;  // rows whose numbers each CTA keeps in shared memory
 
 // Parts of the workspace, in ints.
 struct ForkLayout {
@@ -40,8 +41,14 @@ struct ForkLayout {
   }
 };
 
+// Of a row: where it goes on from, pages that it held, that it keeps, that it ends with, and the number of its first new one.
+struct Row {
+  int source, held, kept, need, first;
+};
+
 __device__ __forceinline__ int page_in(const CacheArgs& c, int entry) { return entry >= 0 && entry < c.pages ? entry : -1; }
 
+static_assert(kWarps == 32, "a lane has a warp's sum");
 // The sum of x over the threads in front of this one, and (in *all) over all; every thread takes part.
 __device__ __forceinline__ int sum_before(int x, int* scratch, int* all) {
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
@@ -54,13 +61,15 @@ __device__ __forceinline__ int sum_before(int x, int* scratch, int* all) {
   __syncthreads();  // (the scratch of a call before this one has been read)
   if (lane == 31) scratch[w] = upto;
   __syncthreads();
-  int before = 0, sum = 0;
-  for (int i = 0; i < kWarps; ++i) {
-    if (i < w) before += scratch[i];
-    sum += scratch[i];
+  int warps = scratch[lane];
+#pragma unroll
+  for (int m = 1; m < 32; m <<= 1) {
+    const int o = __shfl_up_sync(0xffffffffu, warps, m);
+    if (lane >= m) warps += o;
   }
-  *all = sum;
-  return before + upto - x;
+  *all = __shfl_sync(0xffffffffu, warps, 31);
+  const int before = __shfl_sync(0xffffffffu, warps, max(w - 1, 0));
+  return (w > 0 ? before : 0) + upto - x;
 }
 
 __global__ void __launch_bounds__(kThreads, 1) fork_kernel(const __grid_constant__ ForkArgs a) {
@@ -144,84 +153,127 @@ __global__ void __launch_bounds__(kThreads, 1) fork_kernel(const __grid_constant
   cluster.sync();
 
   // --- 3
-  for (unsigned i = me; i < entries; i += all) {
-    const int e = (int)(i / (unsigned)P), j = (int)(i - (unsigned)e * P), s = source_of(e), kept = __ldcg(&plan[e].y);
-    const bool had = j < __ldcg(held + e), keeps = j < kept;
-    if (s == e && keeps) continue;
-    if (had) atomicSub(&a.uses[a.table[e * c.table_se + j]], 1);
-    if (keeps) {
-      const int page = a.table[s * c.table_se + j];
-      atomicAdd(&a.uses[page], 1);
-      staged[i] = page;
+  // What the last steps need of a row, in each CTA's shared memory (of the first kCached): reads that depend on one another are what these steps consist of.
+  __shared__ Row rows[kCached];
+  int wanted = 0;
+  for (int e0 = 0; e0 < E; e0 += kThreads) {
+    const int e = e0 + tid;
+    int wants = 0, part;
+    Row r{};
+    if (e < E) {
+      const int4 p = __ldcg(plan + e);
+      r = Row{source_of(e), __ldcg(held + e), p.y, p.z, 0};
+      wants = max(p.z - p.y, 0);
+    }
+    r.first = wanted + sum_before(wants, scratch, &part);
+    if (e < kCached && e < E) rows[e] = r;
+    else if (e < E) first[e] = r.first;  // (each CTA the same)
+    wanted += part;
+  }
+  __syncthreads();
+  auto row = [&](int e) {
+    if (e < kCached) return rows[e];
+    const int4 p = __ldcg(plan + e);
+    return Row{source_of(e), __ldcg(held + e), p.y, p.z, first[e]};
+  };
+  for (unsigned i0 = me; i0 < entries; i0 += all * kInFlight) {
+    int mine[kInFlight], theirs[kInFlight];  // pages given up and taken, -1: none
+#pragma unroll
+    for (int k = 0; k < kInFlight; ++k) {
+      const unsigned i = i0 + k * all;
+      mine[k] = theirs[k] = -1;
+      if (i >= entries) continue;
+      const int e = (int)(i / (unsigned)P), j = (int)(i - (unsigned)e * P);
+      const Row r = row(e);
+      const bool keeps = j < r.kept;
+      if (r.source == e && keeps) continue;
+      if (j < r.held) mine[k] = a.table[e * c.table_se + j];
+      if (keeps) theirs[k] = a.table[r.source * c.table_se + j];
+    }
+#pragma unroll
+    for (int k = 0; k < kInFlight; ++k) {
+      if (theirs[k] >= 0) staged[i0 + k * all] = theirs[k];
+      if (mine[k] == theirs[k]) continue;  // (as where a row goes on again from one that it shares its pages with)
+      if (mine[k] >= 0) atomicSub(&a.uses[mine[k]], 1);
+      if (theirs[k] >= 0) atomicAdd(&a.uses[theirs[k]], 1);
     }
   }
   for (int e = me; e < E; e += all) {  // (a page that is copied is not given out)
     const int page = __ldcg(&plan[e].w);
     if (page >= 0) atomicAdd(&a.uses[page], 1);
   }
-  if (rank == 0) {
-    int sum = 0;
-    for (int e0 = 0; e0 < E; e0 += kThreads) {
-      const int e = e0 + tid;
-      int wants = 0, part;
-      if (e < E) wants = max(__ldcg(&plan[e].z) - __ldcg(&plan[e].y), 0);
-      const int mine = sum_before(wants, scratch, &part);
-      if (e < E) first[e] = sum + mine;
-      sum += part;
-    }
-    if (tid == 0) ws[1] = sum;
-  }
   cluster.sync();
 
   // --- 4: a CTA's part of the pool, of which a thread has a run
-  const int wanted = __ldcg(ws + 1);
   const int run = (int)(((long long)c.pages + all - 1) / all);
   const long long page0 = (long long)me * run, page1 = min(page0 + run, (long long)c.pages);
-  int unused = 0, part, mine = 0;
+  int part, mine = 0, free_pages = 0;
+  unsigned unused = 0;  // of the run's first 32, a bit each
   if (wanted > 0) {
-    for (long long p = page0; p < page1; ++p) unused += __ldcg(a.uses + p) == 0;
-    mine = sum_before(unused, scratch, &part);
+    int n = 0;
+#pragma unroll 4
+    for (long long p = page0; p < page1; ++p) {
+      const bool is = __ldcg(a.uses + p) == 0;
+      n += is;
+      if (is && p - page0 < 32) unused |= 1u << (p - page0);
+    }
+    mine = sum_before(n, scratch, &part);
     if (tid == 0) ws[8 + rank] = part;
   }
   cluster.sync();
 
   // --- 5
-  int free_pages = 0;
   if (wanted > 0) {
-    for (int i = 0; i < ctas; ++i) {
-      const int n = __ldcg(ws + 8 + i);
+#pragma unroll
+    for (int i = 0; i < kMostCtas; ++i) {
+      const int n = i < ctas ? __ldcg(ws + 8 + i) : 0;
       if (i < rank) mine += n;
       free_pages += n;
     }
     if (wanted > free_pages && me == 0) report(c.status, kNoPage);
-    for (long long p = page0; p < page1 && mine < wanted; ++p)
-      if (__ldcg(a.uses + p) == 0) {
-        free_list[mine++] = (int)p;
-        a.uses[p] = 1;
-      }
+    auto give = [&](long long p) {
+      if (mine >= wanted) return;
+      free_list[mine++] = (int)p;
+      a.uses[p] = 1;
+    };
+    for (unsigned bits = unused; bits != 0; bits &= bits - 1) give(page0 + __ffs(bits) - 1);
+    for (long long p = page0 + 32; p < page1 && mine < wanted; ++p)
+      if (__ldcg(a.uses + p) == 0) give(p);
   }
   cluster.sync();
-  for (unsigned i = me; i < entries; i += all) {
-    const int e = (int)(i / (unsigned)P), j = (int)(i - (unsigned)e * P);
-    const int kept = __ldcg(&plan[e].y), need = __ldcg(&plan[e].z);
-    int page = -1;
-    if (j < kept) {
-      if (source_of(e) == e) continue;
-      page = staged[i];
-    } else if (j < need) {
-      const int n = __ldcg(first + e) + j - kept;
-      if (n < free_pages) page = __ldcg(free_list + n);
+  for (unsigned i0 = me; i0 < entries; i0 += all * kInFlight) {
+    int page[kInFlight];
+    int* at_entry[kInFlight];
+#pragma unroll
+    for (int k = 0; k < kInFlight; ++k) {
+      const unsigned i = i0 + k * all;
+      at_entry[k] = nullptr;
+      page[k] = -1;
+      if (i >= entries) continue;
+      const int e = (int)(i / (unsigned)P), j = (int)(i - (unsigned)e * P);
+      const Row r = row(e);
+      if (j < r.kept) {
+        if (r.source == e) continue;
+        page[k] = staged[i];
+      } else if (j < r.need) {
+        const int n = r.first + j - r.kept;
+        if (n < free_pages) page[k] = __ldcg(free_list + n);
+      }
+      at_entry[k] = a.table + e * c.table_se + j;
     }
-    a.table[e * c.table_se + j] = page;
+#pragma unroll
+    for (int k = 0; k < kInFlight; ++k)
+      if (at_entry[k] != nullptr) *at_entry[k] = page[k];
   }
   for (int e = me; e < E; e += all) {
     const int4 p = __ldcg(plan + e);
+    const int new_page = row(e).first;
     // (where the pages did not suffice, a row ends with the last that it has)
-    const int got = min(max(free_pages - __ldcg(first + e), 0), max(p.z - p.y, 0));
+    const int got = min(max(free_pages - new_page, 0), max(p.z - p.y, 0));
     a.lengths[e] = (int)min((long long)p.x, (long long)(p.y + got) << c.page_shift);
     if (p.w < 0) continue;
     atomicSub(&a.uses[p.w], 1);
-    if (got > 0) copies[atomicAdd(ws, 1)] = make_int4(p.w, __ldcg(free_list + __ldcg(first + e)), p.x & (page_size - 1), 0);
+    if (got > 0) copies[atomicAdd(ws, 1)] = make_int4(p.w, __ldcg(free_list + new_page), p.x & (page_size - 1), 0);
   }
 }
 

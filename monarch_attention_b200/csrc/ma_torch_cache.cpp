@@ -443,9 +443,22 @@ void check_apart(const std::vector<Layer>& layers) {
 }
 
 std::vector<ma_b200_cache> cache_structs(const std::vector<Layer>& layers, const at::Device& device) {
-  std::vector<ma_b200_cache> caches;
-  caches.reserve(layers.size());
-  for (const Layer& l : layers) caches.push_back(cache_struct(Cache{l[0], l[1], l[2], l[3]}, device));
+  const Layer& first = layers[0];
+  std::vector<ma_b200_cache> caches(layers.size(), cache_struct(Cache{first[0], first[1], first[2], first[3]}, device));
+  const bool grad = at::GradMode::is_enabled();
+  for (size_t i = 1; i < layers.size(); ++i) {
+    const Layer& l = layers[i];
+    for (int j = 0; j < 4; ++j) {
+      TORCH_CHECK_VALUE(l[j].scalar_type() == first[j].scalar_type() && l[j].device() == device && l[j].sizes() == first[j].sizes() && l[j].strides() == first[j].strides(),
+                        "the layers' caches must have one shape, dtype and device and the same strides");
+      TORCH_CHECK_VALUE(!grad || !l[j].requires_grad(), "the cache requires a gradient: the cached operators have none (torch.no_grad())");
+      check_no_tangent(l[j], "the cache");
+    }
+    caches[i].k = l[0].data_ptr();
+    caches[i].v = l[1].data_ptr();
+    caches[i].k_scale = l[2].data_ptr<float>();
+    caches[i].v_scale = l[3].data_ptr<float>();
+  }
   check_apart(layers);
   return caches;
 }
