@@ -328,7 +328,12 @@ cudaError_t launch_append(const AppendArgs& a, int dtype, int width, cudaStream_
   // prompt of 1999 and 4 heads 11.0 / 9.9 / 10.0; two of them 17.6 / 17.6 / 14.1, four 27 / 32 / 27.
   const int per = width == 128 ? 2 : 4;
   const int groups = (a.cache.heads + per - 1) / per;
-  const long long ctas = (a.N < kScaleBlock ? 4LL : 1LL) * sm_count(), wanted = (ctas + blocks - 1) / blocks;
+  // Trees come by the batch: where their blocks are one to two for each SM, of which it holds two, and of many heads, the heads are spread so that the second round is not
+  // nearly empty.  us, spread / not: 64 sequences of 61 tokens, 8 + 32 heads of 128 features 27 / 29 (without padding 36 / 42), 32 of them 15 / 22, 64 of 25 tokens and 12 + 12 heads of 64 features
+  // 12 / 13; 128 of 20 tokens (384 blocks) 13.8 / 12.6.
+  const long long sms = sm_count();
+  const bool spread = a.parents != nullptr && blocks > sms && 5 * blocks <= 11 * sms && 2 * a.cache.heads + a.H >= 32;
+  const long long ctas = spread ? 3 * sms : (a.N < kScaleBlock ? 4LL : 1LL) * sms, wanted = (ctas + blocks - 1) / blocks;
   return launch_kernel(fn, dim3((unsigned)blocks, (unsigned)(wanted < groups ? wanted : groups)), dim3(kThreads), args, 0, stream);
 }
 
