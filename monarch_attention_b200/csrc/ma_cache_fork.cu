@@ -14,6 +14,8 @@
 //   5  the free pages that are wanted, the lowest first, into a list; from there into the rows
 // The pages' contents are copied by a second kernel, all layers at once, a warp taking the keys and values of 16 tokens of a head.  Pages that are read there are not given
 // out in the same call.
+// The first is bound by latency: some 15 reads one after another and six barriers.  Measured: 4 rows of 33 pages 7.8 us, 128 rows of 17 15, 8 rows of 3752 15 (23 with atomics for
+// pages that stay).  The second by memory: 70 half pages of 16 layers, 8 heads of 128 features, 127 MB in 20.5 us, 6.2 TB/s.
 #include <cooperative_groups.h>
 
 #include "ma_cache.cuh"
@@ -327,6 +329,7 @@ cudaError_t launch_fork_copies(const ForkArgs& a, int width, cudaStream_t stream
 
 cudaError_t launch_fork(const ForkArgs& a, int width, cudaStream_t stream) {
   void* args[] = {(void*)&a};
+  // (few entries and pages: one CTA, whose barriers are its own)
   const long long work = (long long)a.E * a.cache.table_pages + a.cache.pages;
   const int ctas = work <= 4 * kThreads ? 1 : kMostCtas;
   const cudaError_t err = launch_kernel((const void*)fork_kernel, dim3(ctas), dim3(kThreads), args, 0, stream, ctas);

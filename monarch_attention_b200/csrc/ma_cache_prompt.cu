@@ -9,14 +9,22 @@
 //  * Two warpgroups have a row a thread: the row's 128 scores go from tensor memory to registers in one go, and the maximum, the weights and
 //    their sum need no other thread.  Scales of blocks are applied as in the kernel for few rows (ma_cache_attend.cu): the keys' to the
 //    scores, the values' to the weights, with a reference that is raised (and O multiplied) only when a weight would pass 2^15.
+//  * Pages and scales of a step's blocks are looked up some ten steps ahead by a warp of their own, or by eight of those threads (Roles says where).
 //  * One warp issues the products: O += P V, the weights P read from tensor memory, where they have taken the place of their scores, and
 //    the next step's scores S = Q K^T.  While one tile's rows are exponentiated the other's products run.
-// Measured: 1024 tokens of 2 sequences over 16384 keys, 4 heads of 128 features, 281 us, 947 TFLOP/s, 57 % of a library product; 64 features 495.  (A call
+// Measured: 1024 tokens of 2 sequences over 16384 keys, 4 heads of 128 features, 281 us, 947 TFLOP/s, 57 % of a library product; 64 features 526.  (A call
 // lasts as long as its longest sequence: one of 16384 beside one of 1024 takes the same 281.)  A step takes 4200 cycles, of which the row warps' weights are
 // 2300 a tile: without any exponential they would take 80 % of the time, without the conversion of keys and values all of it, and with scores that never
 // wait for the products of the step before (64 features leave the room) 99 %.
 // Slower were (beside 304 us): two threads a row 343, scores of 64 keys in two buffers 358, scores loaded a quarter at a time 347; eight warps that
 // bring keys and values, which leave the rows 160 registers each, took the 304.
+// Trees of drafted tokens (kTree) have some ten to some hundred rows, over one range of keys:
+//  * A row's ancestors among the call's tokens are a line of bits in shared memory, which its thread follows from parent to parent when the CTA starts.  In front of the call's
+//    own tokens nothing is masked, and in the last steps 32 keys are one word of the line.
+//  * The keys of all heads are cut into pieces about as long as one another, whatever the lengths are, on a CTA for each SM (even_pieces).
+//  * Up to 128 rows, which are one tile, are in both, and the tiles take the steps in turns (tree_plan says where); their sums are joined like pieces.
+// Measured: 8 sequences of up to 8192 tokens, 8 heads of 128 features and 244 rows 66 us, 503 TFLOP/s (one piece length for all: 94); 16 sequences of 8192 tokens and 4 heads, 64 rows 66,
+// of 64 features 54 (82 before the look-up ahead and the turns).  A step is 4200 cycles as above, 3000 in turns.
 // Every wait is bounded; one that gives up ends the CTA's others, and the next call on the device reports it.
 #include <math_constants.h>
 

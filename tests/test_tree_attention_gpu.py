@@ -130,6 +130,44 @@ def test_parents_that_cannot_be_count_as_none_and_are_reported(N):
     ma.cached_attention_b200(q, cache, table, *sizes)
 
 
+@pytest.mark.parametrize("N", [8, 60, 130])
+def test_one_tree_for_all_and_results_in_place(N):
+    """Parents with a batch stride of zero; a result in the query's place and beside its rows; a call on a stream of its own."""
+    import monarch_attention_b200 as ma
+    lengths, page = [N, 900, 2000], 32
+    cache, table = filled(3, 70, 2, 64, page, lengths)
+    both = torch.empty(3, N, 2, 4, 64, dtype=BF, device="cuda")   # rows of queries beside those of results
+    q, beside = (both[:, :, i].transpose(1, 2) for i in range(2))
+    q.copy_(queries(3, 4, N, 64, BF, "heads"))
+    one = trees(1, N, "random", 2)
+    sizes, alone = on_gpu(lengths), q.clone()
+    want = ma.cached_attention_b200(alone, cache, table, *sizes, parents=one.repeat(3, 1))
+    check(want, alone, cache, table, lengths, None, page, one.repeat(3, 1))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        assert ma.cached_attention_b200(q, cache, table, *sizes, parents=one.expand(3, N), out=beside) is not None
+        in_place = ma.cached_attention_b200(q, cache, table, *sizes, parents=one.expand(3, N), out=q)
+    torch.cuda.current_stream().wait_stream(side)
+    assert torch.equal(beside, want) and torch.equal(in_place, want)
+
+
+@pytest.mark.parametrize("E,H,Hk,N,D,lengths,counts", [(16, 4, 4, 33, 128, [1400] * 16, None), (20, 4, 4, 50, 64, list(range(50, 2050, 100)), [50, 7] * 10), (40, 8, 8, 64, 64, [2100] * 20 + [70] * 20, None),
+                                                       (16, 8, 4, 64, 128, [5000] * 15 + [64], None), (3, 8, 8, 128, 64, [128, 9000, 300], [128, 0, 100]), (148, 1, 1, 40, 64, list(range(40, 188)), None)])
+def test_many_rows_in_any_shares(E, H, Hk, N, D, lengths, counts):
+    """Even pieces of ragged lengths, tiles of the same rows in turns, more heads than SMs."""
+    import monarch_attention_b200 as ma
+    page, per = 64, max(lengths) // 64 + 20
+    cache, table = filled(E, per, Hk, D, page, lengths, spare=1)
+    q, parents = queries(E, H, N, D, HF, "tokens"), trees(E, N, "random", 4)
+    out = ma.cached_attention_b200(q, cache, table, *on_gpu(lengths, counts), parents=parents)
+    look = [0, E // 2, E - 1]   # (the definition in 64 bits takes a second a sequence)
+    check(out[look], q[look], cache, table[look], [lengths[i] for i in look], None if counts is None else [counts[i] for i in look], page, parents[look])
+    assert torch.isfinite(out).all()
+    again = ma.cached_attention_b200(q, cache, table, *on_gpu(lengths, counts), parents=parents)
+    assert torch.equal(out, again)
+
+
 # --- the append --------------------------------------------------------------------------------------------------------------
 
 @pytest.mark.parametrize("E,H,Hk,N,D,page,dim,pairs,dtype,layout", [
