@@ -23,7 +23,7 @@
 //    own tokens nothing is masked, and in the last steps 32 keys are one word of the line.
 //  * The keys of all heads are cut into pieces about as long as one another, whatever the lengths are, on a CTA for each SM (even_pieces).
 //  * Up to 128 rows, which are one tile, are in both, and the tiles take the steps in turns (tree_plan says where); their sums are joined like pieces.
-// Measured: 8 sequences of up to 8192 tokens, 8 heads of 128 features and 244 rows 66 us, 503 TFLOP/s (one piece length for all: 94); 16 sequences of 8192 tokens and 4 heads, 64 rows 66,
+// Measured: 8 sequences of up to 8192 tokens, 8 heads of 128 features and 244 rows 63 us, 525 TFLOP/s (one piece length for all: 94); 16 sequences of 8192 tokens and 4 heads, 64 rows 66,
 // of 64 features 54 (82 before the look-up ahead and the turns).  A step is 4200 cycles as above, 3000 in turns.
 // Every wait is bounded; one that gives up ends the CTA's others, and the next call on the device reports it.
 #include <math_constants.h>
@@ -42,7 +42,7 @@ constexpr int kKeys = 128, kTileRows = 128, kRows = 2 * kTileRows;
 constexpr int kThreads = 512, kBringers = 128;  // warps 0-3, 4-7: rows; 8-11: keys and values; 12: products; 13: pages and scales (14, 15 make it a warpgroup)
 constexpr int kMostRing = 16, kGroup = 4, kGroups = kMostRing / kGroup;  // steps whose pages and scales are kept; so many are looked up at a time by a warp of their own
 // Pages and scales are looked up by a warp of their own, some ten steps ahead (kAhead), or a step at a time by eight of the threads that bring keys and values.  us, the one / the
-// other: 64 features, 2 x 1024 tokens over 16384 keys 260 / 268 (f16 256 / 272), 8 x 64 tokens over 4096 37 / 44; 128 features 281 / 284 (f16 287 / 280), 46 / 46, 300 tokens 19.5 / 18.6:
+// other: 64 features, 2 x 1024 tokens over 16384 keys 262 / 267 (f16 256 / 272), 8 x 64 tokens over 4096 37 / 44; 128 features 281 / 283 (f16 287 / 280), 46 / 46:
 // there the products and the exponentials bind, and the rows can use the registers.  Trees, which have fewer rows, always.
 template <int D, bool kTree>
 struct Roles {
@@ -63,16 +63,20 @@ struct alignas(16) Blocks {
   int page[2][8];  // of keys and of values; -1: zeros
 };
 
-template <int D>
+template <int D, bool kTree>
 struct Layout {
   static constexpr int kTileBytes = 128 * D * 2;  // 128 rows in f16: panels of 64 features
   static constexpr int kQ = 0, kK = 2 * kTileBytes, kV = kK + 2 * kTileBytes, kBlocks = kV + 2 * kTileBytes;
-  static constexpr int kBarriers = kBlocks + kMostRing * (int)sizeof(Blocks), kFlags = kBarriers + 8 * kBars, kBytes = kFlags + 16;
-  static constexpr int kSmem = kBytes + 1024;  // (tiles start on 1024-byte boundaries)
+  static constexpr int kBarriers = kBlocks + Roles<D, kTree>::kRing * (int)sizeof(Blocks);
+  static constexpr int kFlags = kBarriers + 8 * (Roles<D, kTree>::kAhead ? (int)kBars : (int)kKnown), kBytes = kFlags + 16;
   // of trees: the rows' lines, a bit for each of the call's tokens (word by word, a row next to the other), and their parents
-  static constexpr int kLines = kBytes, kLineWords = kTreeTokens / 32, kParents = kLines + kLineWords * kRows * 4, kTreeSmem = kParents + kTreeTokens * 2 + 1024;
+  static constexpr int kLines = kBytes, kLineWords = kTreeTokens / 32, kParents = kLines + kLineWords * kRows * 4;
+  static constexpr int kSmem = (kTree ? kParents + kTreeTokens * 2 : kBytes) + 1024;  // (tiles start on 1024-byte boundaries)
 };
-static_assert(Layout<128>::kTreeSmem <= 227 * 1024 && kTreeTokens <= kThreads, "a thread brings a parent");
+static_assert(Layout<128, true>::kSmem <= 227 * 1024 && kTreeTokens <= kThreads, "a thread brings a parent");
+// An SM keeps 196 KB for shared memory, or 228, which leaves its L1 32 KB less: with some 100 bytes more than the first (a CTA has 1 KB of its own), 300 tokens over
+// themselves, 8 heads of 128 features, 18.2 -> 19.5 us, 2 x 1024 tokens over 16384 keys 283 -> 285.
+static_assert(Layout<128, false>::kSmem + 1024 <= 196 * 1024, "does not fit beside the larger L1");
 
 struct PromptArgs {
   AttendArgs a;
@@ -298,7 +302,7 @@ __device__ __forceinline__ void put_block(Blocks& b, int block, int page, float 
 // kTree: the call's tokens are a tree (a.parents).
 template <typename T, int D, bool kExpire = false, bool kTree = false>
 __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_constant__ PromptArgs args) {
-  using L = Layout<D>;
+  using L = Layout<D, kTree>;
   using R = Roles<D, kTree>;
   constexpr int kRing = R::kRing;
   constexpr int kPanel = 128 * 128;  // bytes of 128 rows of 64 features
@@ -322,10 +326,10 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
 
   grid_wait();
   // --- the CTA's rows and keys; row blocks with more keys come first
-  int pieces = args.pieces, piece, unit, e, head, block;
-  if (!kTree || pieces > 0) {
-    piece = blockIdx.x % pieces;
-    unit = blockIdx.x / pieces;  // (block from the last on, sequence, head)
+  int own_pieces = args.pieces, piece, unit, e, head, block;
+  if (!kTree || own_pieces > 0) {
+    piece = blockIdx.x % args.pieces;
+    unit = blockIdx.x / args.pieces;  // (block from the last on, sequence, head)
     const int e_head = unit % (a.E * c.heads);
     block = a.row_blocks - 1 - unit / (a.E * c.heads);
     e = e_head / c.heads;
@@ -336,12 +340,13 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
     __syncthreads();
     e = shares[0];
     if (e < 0) return;  // (a CTA too many)
-    pieces = shares[1];
+    own_pieces = shares[1];
     piece = shares[2];
     head = shares[3] / a.row_blocks;
     block = shares[3] - head * a.row_blocks;
     unit = (e * c.heads + head) * a.row_blocks + block;
   }
+  const int& pieces = kTree ? own_pieces : args.pieces;  // (of a call, read where it is used: a register through the loop costs 0.8 %)
   const int row0 = block * kRows;
   int len, count;
   const bool fine = sequence_of(c, e, a.N, &len, &count);
@@ -604,13 +609,17 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
       }
       if ((pieces > 1 || turns) && exists) *reinterpret_cast<float2*>(a.part_ml + 2 * slot) = make_float2(top, sum * unit_of);
     }
-    if ((args.pieces != 1 || turns) && tid == 0 && piece == 0) {
-      int first = kTree && args.pieces == 0 ? blockIdx.x : unit * pieces, last = first + pieces - 1;
-      if (turns) {  // (each tile's rows are a piece)
-        first = 2 * first;
-        last = 2 * last + 1;
+    if constexpr (kTree) {
+      if ((args.pieces != 1 || turns) && tid == 0 && piece == 0) {
+        int first = args.pieces == 0 ? blockIdx.x : unit * pieces, last = first + pieces - 1;
+        if (turns) {  // (each tile's rows are a piece)
+          first = 2 * first;
+          last = 2 * last + 1;
+        }
+        a.split[unit] = make_int4(pieces > 1 || turns ? (e * c.heads + head) * a.row_blocks + block : -1, first, last, 0);
       }
-      a.split[unit] = make_int4(pieces > 1 || turns ? (e * c.heads + head) * a.row_blocks + block : -1, first, last, 0);
+    } else if (args.pieces > 1 && tid == 0 && piece == 0) {
+      a.split[unit] = make_int4((e * c.heads + head) * a.row_blocks + block, unit * args.pieces, (unit + 1) * args.pieces - 1, 0);
     }
   } else if (warp < 12) {
     // =========================== keys and values =====================================================================
@@ -900,7 +909,7 @@ cudaError_t launch_prompt(AttendArgs a, int dtype, int width, void* workspace, l
   if (tree) fn = width == 128 ? (bf ? (const void*)prompt_kernel<__nv_bfloat16, 128, false, true> : (const void*)prompt_kernel<__half, 128, false, true>)
                               : (bf ? (const void*)prompt_kernel<__nv_bfloat16, 64, false, true> : (const void*)prompt_kernel<__half, 64, false, true>);
   if (wait_expiry) fn = width == 128 ? (const void*)prompt_kernel<__nv_bfloat16, 128, true> : (const void*)prompt_kernel<__nv_bfloat16, 64, true>;
-  const size_t smem = width == 128 ? (tree ? Layout<128>::kTreeSmem : Layout<128>::kSmem) : tree ? Layout<64>::kTreeSmem : Layout<64>::kSmem;
+  const size_t smem = width == 128 ? (tree ? Layout<128, true>::kSmem : Layout<128, false>::kSmem) : tree ? Layout<64, true>::kSmem : Layout<64, false>::kSmem;
   // a build whose launch does not cover the roles' registers must not start: setmaxnreg would wait for them without end
   static std::atomic<unsigned long long> checked[10];
   int dev = 0;
