@@ -158,7 +158,7 @@ __global__ void __launch_bounds__(kThreads, 2) append_kernel(const __grid_consta
     const int behind = min(base + last - start, count);  // (a token's ancestors are in front of it)
     for (int i = tid; any && i < behind; i += kThreads) parents[i] = (int16_t)parent_of(a.parents + e * a.parents_se, i, c.status);
     __syncthreads();
-    if (any && tid >= first && tid < last) {
+    if (any && pairs > 0 && tid >= first && tid < last) {
       int depth = -1;
       for (int i = base + tid - start; i >= 0; i = parents[i]) ++depth;
       places[tid] = start + depth;
@@ -246,7 +246,8 @@ __global__ void __launch_bounds__(kThreads, 2) append_kernel(const __grid_consta
 
 // One token of each sequence: a row of 128 features, two to a warp, or of 64, four.  (Six CTAs of an SM, 40 registers: 256 sequences of 8 + 32 heads
 // are one round of them, 4.7 us; with 47 registers and five 6.1.)
-template <typename T, int D>
+// kTree: the token is a tree, whose parent can only be none: the position is that of its place, and another parent is reported.
+template <typename T, int D, bool kTree>
 __global__ void __launch_bounds__(kThreads, 6) append_token_kernel(const __grid_constant__ AppendArgs a) {
   constexpr int kLanes = D / F, kRows = 32 / kLanes;
   __shared__ float2 table[D / 2];
@@ -263,6 +264,9 @@ __global__ void __launch_bounds__(kThreads, 6) append_token_kernel(const __grid_
   }
   int len, count;
   span_of(c, e, 1, threadIdx.x == 0 && blockIdx.y == 0, &len, &count);
+  if constexpr (kTree) {
+    if (count > 0 && threadIdx.x == 0 && blockIdx.y == 0) (void)parent_of(a.parents + e * a.parents_se, 0, c.status);
+  }
   const int position = max(len - 1, 0), first = position & (kScaleBlock - 1), pairs = a.rotary.pairs;
   const int page = count > 0 ? page_of(c, e, position) : -1;
   if (threadIdx.x < pairs) table[threadIdx.x] = rotary_turn(a.rotary, threadIdx.x, position);
@@ -310,16 +314,18 @@ cudaError_t launch_append(const AppendArgs& a, int dtype, int width, cudaStream_
   void* args[] = {(void*)&a};
   const bool bf = dtype == MA_B200_BF16;
   // us, the kernel for single tokens / the other: 8 sequences of 4 heads 3.5 / 9.9, 256 of 8 heads 5.4 / 20.1
-  // (The one token of a tree is at the position of its place.)
   if (a.N == 1) {
     const int rows = kWarps * 32 * F / width;  // of a CTA
-    const void* fn = bf ? (width == 128 ? (const void*)append_token_kernel<__nv_bfloat16, 128> : (const void*)append_token_kernel<__nv_bfloat16, 64>)
-                        : (width == 128 ? (const void*)append_token_kernel<__half, 128> : (const void*)append_token_kernel<__half, 64>);
+    const void* fn = bf ? (width == 128 ? (const void*)append_token_kernel<__nv_bfloat16, 128, false> : (const void*)append_token_kernel<__nv_bfloat16, 64, false>)
+                        : (width == 128 ? (const void*)append_token_kernel<__half, 128, false> : (const void*)append_token_kernel<__half, 64, false>);
+    if (a.parents != nullptr)
+      fn = bf ? (width == 128 ? (const void*)append_token_kernel<__nv_bfloat16, 128, true> : (const void*)append_token_kernel<__nv_bfloat16, 64, true>)
+              : (width == 128 ? (const void*)append_token_kernel<__half, 128, true> : (const void*)append_token_kernel<__half, 64, true>);
     return launch_kernel(fn, dim3(a.E, (2 * a.cache.heads + a.H + rows - 1) / rows), dim3(kThreads), args, 0, stream);
   }
   const void* fn = bf ? (width == 128 ? (const void*)append_kernel<__nv_bfloat16, 128, false> : (const void*)append_kernel<__nv_bfloat16, 64, false>)
                       : (width == 128 ? (const void*)append_kernel<__half, 128, false> : (const void*)append_kernel<__half, 64, false>);
-  if (a.parents != nullptr && a.rotary.pairs > 0)  // (where nothing is rotated a tree's tokens are like any others)
+  if (a.parents != nullptr)  // (also where nothing is rotated: parents that cannot be are reported)
     fn = bf ? (width == 128 ? (const void*)append_kernel<__nv_bfloat16, 128, true> : (const void*)append_kernel<__nv_bfloat16, 64, true>)
             : (width == 128 ? (const void*)append_kernel<__half, 128, true> : (const void*)append_kernel<__half, 64, true>);
   const long long blocks = (long long)a.E * ((a.N + kScaleBlock - 2) / kScaleBlock + 1);
