@@ -113,10 +113,7 @@ __global__ void __launch_bounds__(kThreads, 1) fork_kernel(const __grid_constant
     }
 #pragma unroll
     for (int k = 0; k < kInFlight; ++k)  // (only where a run of pages ends: the rest of a row says the same)
-      if (e[k] >= 0 && page_in(c, now[k]) < 0 && page_in(c, before[k]) >= 0) {
-        atomicMin(&held[e[k]], j[k]);
-        if (now[k] >= 0) report(c.status, kBadPage);
-      }
+      if (e[k] >= 0 && page_in(c, now[k]) < 0 && page_in(c, before[k]) >= 0) atomicMin(&held[e[k]], j[k]);
   }
   for (int e = me; e < E; e += all) {
     const int s = source_of(e);
@@ -201,8 +198,9 @@ __global__ void __launch_bounds__(kThreads, 1) fork_kernel(const __grid_constant
     }
   }
   for (int e = me; e < E; e += all) {  // (a page that is copied is not given out)
-    const int page = __ldcg(&plan[e].w);
+    const int page = __ldcg(&plan[e].w), end = row(e).held;
     if (page >= 0) atomicAdd(&a.uses[page], 1);
+    if (end < P && a.table[e * c.table_se + end] >= 0) report(c.status, kBadPage);  // (what is behind a row's end may be anything)
   }
   cluster.sync();
 
