@@ -121,7 +121,7 @@ class CachedAttention(nn.Module):
     ``forward(query, key, value, cache, page_table, lengths, counts=None, parents=None)`` has query, key and value of one step (a prompt, a piece of
     one, or a token) in the (E, H, N, width) views that :class:`MonarchAttention` takes, key and value with the cache's heads.  With
     ``key`` and ``value`` None nothing is appended and the query is not rotated: attention to an encoder's output that is in the cache already.
-    With ``parents`` the step's tokens are a tree of drafted ones (:func:`accept_drafts_b200` then keeps those that the model confirms).
+    With ``parents`` (``causal`` only) the step's tokens are a tree of drafted ones (:func:`accept_drafts_b200` then keeps those that the model confirms).
     """
 
     def __init__(self, rotary: RotaryPositions | None = None, causal: bool = True, scale: float | None = None, softcap: float = 0.0,
@@ -136,6 +136,8 @@ class CachedAttention(nn.Module):
     def forward(self, query, key, value, cache, page_table, lengths, counts=None, parents=None):
         if (key is None) != (value is None):
             raise ValueError("key and value must be given together")
+        if parents is not None and not self.causal:  # (before the append changes the cache)
+            raise ValueError("parents need causal: a tree's tokens see their ancestors")
         if key is not None:
             rotated = append_kv_b200(cache, key, value, page_table, lengths, counts, query=query if self.rotary is not None else None,
                                      rotary=self.rotary, parents=parents)
