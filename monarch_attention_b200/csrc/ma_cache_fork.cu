@@ -31,7 +31,7 @@ struct ForkLayout {
   long long held, keeper, plan, first, staged, free_list, copies, total;
   __host__ __device__ ForkLayout(long long E, long long P, long long pages) {
     const long long rows = (E + 3) / 4 * 4;
-    long long at = 8 + kMostCtas;  // [0] copies, [1] pages wanted, [8 ..] free pages of each CTA's part
+    long long at = 8 + kMostCtas;  // [0] copies, [8 ..] free pages of each CTA's part
     held = at; at += rows;
     keeper = at; at += rows;
     plan = at; at += 4 * rows;     // length, entries kept, entries wanted in all, page that is copied (-1: none)
@@ -93,7 +93,7 @@ __global__ void __launch_bounds__(kThreads, 1) fork_kernel(const __grid_constant
     keeper[e] = 0x7fffffff;
     if (a.source != nullptr && (a.source[e] < -1 || a.source[e] >= E)) report(c.status, kBadSource);
   }
-  if (me < 2) ws[me] = 0;
+  if (me == 0) ws[0] = 0;
   cluster.sync();
 
   // --- 1

@@ -80,7 +80,7 @@ static_assert(Layout<128, false>::kSmem + 1024 <= 196 * 1024, "does not fit besi
 
 struct PromptArgs {
   AttendArgs a;
-  int pieces;        // that the keys of a CTA's rows are cut into; 0 (trees): as many as make all CTAs' about equal
+  int pieces;        // that the keys of a CTA's rows are cut into; trees: 1, or 0: as many as make all CTAs' about equal
   int turns;         // (trees) 1: both tiles have the same rows, and take the steps in turns
   int* wait_status;  // mapped host word: a wait that gave up
 };
@@ -583,8 +583,8 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
       if (turns && i0 >= steps) works = false;  // (no step was this tile's)
       const float unit_of = ex2(top_log);  // (a piece's reference is one number)
       const float inverse = top > -CUDART_INF_F ? 1.0f / sum : 0.0f;  // (no key, no reference)
-      // (even pieces have a place for each CTA)
-      const size_t slot = (kTree && args.pieces == 0 ? (size_t)blockIdx.x : (size_t)unit * pieces + piece) * kRows + tile * kTileRows + r;
+      // (a place for each CTA, which those of a tree's pieces are in a row)
+      const size_t slot = (kTree ? (size_t)blockIdx.x : (size_t)unit * pieces + piece) * kRows + tile * kTileRows + r;
       T* const dst = reinterpret_cast<T*>(const_cast<void*>(a.out.ptr)) + e * a.out.se + h * a.out.sh + token * a.out.sn;
 #pragma unroll
       for (int q = 0; q < D / 32; ++q) {
@@ -611,7 +611,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
     }
     if constexpr (kTree) {
       if ((args.pieces != 1 || turns) && tid == 0 && piece == 0) {
-        int first = args.pieces == 0 ? blockIdx.x : unit * pieces, last = first + pieces - 1;
+        int first = blockIdx.x, last = first + pieces - 1;
         if (turns) {  // (each tile's rows are a piece)
           first = 2 * first;
           last = 2 * last + 1;
@@ -859,8 +859,7 @@ int prompt_pieces(int E, int N, int H, int kv_heads, long long longest) {
 
 // How a tree's rows and keys are shared out.
 struct TreePlan {
-  bool turns, even;
-  int pieces;      // (not even)
+  bool turns, even;  // (not even: heads stay whole, of which there are more than SMs, or which are short)
   long long units, grid;
 };
 TreePlan tree_plan(int E, int N, int H, int kv_heads, long long longest) {
@@ -869,8 +868,7 @@ TreePlan tree_plan(int E, int N, int H, int kv_heads, long long longest) {
   p.units = units;
   // Even pieces, on a CTA for each SM.  us, even / the same number for all: 8 sequences of up to 8192 tokens, 8 heads of 244 rows, 67.9 / 94.1.
   p.even = units <= sm_count() && sm_count() <= 160 && longest > 4 * kKeys;
-  p.pieces = p.even ? 0 : prompt_pieces(E, N, H, kv_heads, longest);
-  p.grid = p.even ? sm_count() : units * p.pieces;
+  p.grid = p.even ? sm_count() : units;
   // Rows of one tile take the other for every other step, where a CTA has steps enough for what the join of twice the pieces costs, and a head not so many pieces that it is long.  us, in
   // turns / not: 16 sequences of 8192 tokens, 4 heads of 64 rows 67 / 78 (128 rows 76 / 82; 64 features, 64 rows 54 / 63), 24 of 2000 and 48 rows 41 / 44; 32 of 1024 and 8
   // heads of 64 rows 58 / 49, of 4096 128 / 136 (128 rows 150 / 140); one of 131071 tokens and 2 heads 68 / 57.
@@ -881,7 +879,7 @@ TreePlan tree_plan(int E, int N, int H, int kv_heads, long long longest) {
 
 size_t prompt_tree_workspace(int E, int N, int H, int kv_heads, int width, long long longest) {
   const TreePlan p = tree_plan(E, N, H, kv_heads, longest);
-  if (p.pieces == 1 && !p.turns) return 256;
+  if (!p.even && !p.turns) return 256;
   return ((size_t)p.units * sizeof(int4) + 255) / 256 * 256 + (size_t)p.grid * kRows * (width + 2) * sizeof(float);
 }
 
@@ -896,7 +894,7 @@ cudaError_t launch_prompt(AttendArgs a, int dtype, int width, void* workspace, l
   a.row_blocks = (a.group * a.N + kRows - 1) / kRows;
   const long long units = (long long)a.E * a.cache.heads * a.row_blocks;
   const TreePlan p = a.parents != nullptr ? tree_plan(a.E, a.N, a.H, a.cache.heads, longest) : TreePlan{};
-  PromptArgs args{a, a.parents != nullptr ? p.pieces : prompt_pieces(a.E, a.N, a.H, a.cache.heads, longest), p.turns, wait_status};
+  PromptArgs args{a, a.parents != nullptr ? (p.even ? 0 : 1) : prompt_pieces(a.E, a.N, a.H, a.cache.heads, longest), p.turns, wait_status};
   const long long grid = a.parents != nullptr ? p.grid : units * args.pieces;
   char* at = reinterpret_cast<char*>(workspace);
   args.a.split = reinterpret_cast<int4*>(at);
