@@ -334,12 +334,20 @@ cudaError_t launch_append(const AppendArgs& a, int dtype, int width, cudaStream_
   // prompt of 1999 and 4 heads 11.0 / 9.9 / 10.0; two of them 17.6 / 17.6 / 14.1, four 27 / 32 / 27.
   const int per = width == 128 ? 2 : 4;
   const int groups = (a.cache.heads + per - 1) / per;
-  // Trees come by the batch: where their blocks are one to two for each SM, of which it holds two, and of many heads, the heads are spread so that the second round is not
-  // nearly empty.  us, spread / not: 64 sequences of 61 tokens, 8 + 32 heads of 128 features 27 / 29 (without padding 36 / 42), 32 of them 15 / 22, 64 of 25 tokens and 12 + 12 heads of 64 features
-  // 12 / 13; 128 of 20 tokens (384 blocks) 13.8 / 12.6.
-  const long long sms = sm_count();
-  const bool spread = a.parents != nullptr && blocks > sms && 5 * blocks <= 11 * sms && 2 * a.cache.heads + a.H >= 32;
-  const long long ctas = spread ? 3 * sms : (a.N < kScaleBlock ? 4LL : 1LL) * sms, wanted = (ctas + blocks - 1) / blocks;
+  const long long sms = sm_count(), ctas = (a.N < kScaleBlock ? 4LL : 1LL) * sms;
+  long long wanted = (ctas + blocks - 1) / blocks;
+  // Trees come by the batch.  With more blocks than SMs and many heads it counts how many of the blocks have a token (not every sequence's tokens touch all of its blocks): up to one an SM,
+  // two groups of heads keep both of its places busy; up to 1.35, groups smaller than the most there can be even the SMs with two blocks out with those of one; more than both places and up to 2.8, two
+  // groups, so that the second round is not half empty.  (128 features, where a CTA is long: as soon as there are more blocks than places, with or without a token.)
+  // us, one group / so many, tokens x sequences, 8 + 32 heads of 128 features: 61 x 30 22.1 / 16.1 (two), 61 x 38 24.1 / 22.0 (three), 25 x 74 22.3 / 21.1 (three), 61 x 64 40.7 / 35.9 (two), 61 x 80
+  // 46.8 / 41.0, 25 x 147 43.5 / 38.4; 12 + 12 of 64 features: 25 x 64 13.2 / 11.4 (two), 25 x 123 21.7 / 19.6.  Between and behind, where one group is taken, one / two: 61 x 48 25.2 / 27.6, 61 x 59
+  // 26.1 / 29.2, 61 x 100 49.3 / 51.2; 64 features: 25 x 93 13.7 / 15.4, 25 x 117 16.6 / 18.5, 25 x 197 25.9 / 29.3; 24 + 8 heads, 40 x 56 12.7 / 14.8.
+  if (a.parents != nullptr && blocks > sms && 2 * a.cache.heads + a.H >= 32) {
+    const long long full = (long long)a.E * (a.N + kScaleBlock - 1) / kScaleBlock;  // blocks with a token, as a mean over where sequences end
+    if (full <= sms) wanted = 2;
+    else if (20 * full <= 27 * sms) wanted = groups <= 2 ? 1 : groups == 3 ? 2 : 3;
+    else wanted = 20 * (width == 128 ? blocks : full) > 41 * sms && 5 * full <= 14 * sms ? 2 : 1;
+  }
   return launch_kernel(fn, dim3((unsigned)blocks, (unsigned)(wanted < groups ? wanted : groups)), dim3(kThreads), args, 0, stream);
 }
 
