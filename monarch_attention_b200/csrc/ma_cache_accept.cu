@@ -109,16 +109,14 @@ __global__ void __launch_bounds__(kThreads) accept_kernel(const __grid_constant_
       uint8_t* const rows = codes + page * sp + row0 * st;
       float* const scale_at = scales + page * ssp + row0 / kScaleBlock;
       uint4 x[kPasses];
-      float xs[kPasses], amax = 0.0f;
-      unsigned moves = 0;  // a bit a pass: the lane has a token to move (whose scale may be anything: NaN makes NaN of it)
+      float xs[kPasses], amax = 0.0f;  // xs: the tokens' scales, -1 where there is none to move; NaN makes NaN of a token
 #pragma unroll
       for (int p = 0; p < kPasses; ++p) {
         const int i = i0 + p * kRows + lane_row;
         const int2 src = i >= in_place && i < taken ? from[i] : make_int2(-1, 0);
         x[p] = make_uint4(0, 0, 0, 0);
-        xs[p] = 0.0f;
+        xs[p] = -1.0f;
         if (src.x >= 0) {
-          moves |= 1u << p;
           x[p] = *reinterpret_cast<const uint4*>(codes + src.x * sp + src.y * st);
           xs[p] = scales[src.x * ssp + src.y / kScaleBlock];
         }
@@ -126,14 +124,14 @@ __global__ void __launch_bounds__(kThreads) accept_kernel(const __grid_constant_
       const bool older = i0 < in_place;  // tokens stay in the block
       const float before = older ? *scale_at : 0.0f;
 #pragma unroll
-      for (int p = 0; p < kPasses; ++p) amax = fmaxf(amax, largest_code(x[p]) * xs[p]);  // (a NaN asks for no scale)
+      for (int p = 0; p < kPasses; ++p) amax = fmaxf(amax, xs[p] < 0.0f ? 0.0f : largest_code(x[p]) * xs[p]);  // (a NaN asks for no scale)
       const float scale = fmaxf(scale_for(__uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(amax)))), before);
       __syncwarp();  // (all of the block's tokens, and the scales that they come with, have been read)
 #pragma unroll
       for (int p = 0; p < kPasses; ++p) {
         const int slot = p * kRows + lane_row;
         uint4* const at = reinterpret_cast<uint4*>(rows + slot * st);
-        if (moves >> p & 1) *at = moved16(x[p], xs[p] / scale);
+        if (!(xs[p] < 0.0f)) *at = moved16(x[p], xs[p] / scale);
         else if (i0 + slot < in_place && scale != before) *at = moved16(*at, before / scale);
       }
       if (lane == 0) *scale_at = scale;
