@@ -406,7 +406,7 @@ MA_B200_API int ma_b200_cache_attend_tree(const ma_b200_attend* p, const ma_b200
 /* Which tokens of a tree stand, and the caches of all layers (HOST array, one shape and strides) closed up over them.  drafted and answers (E, N; int32, or
  * int64 with ids_i64): the call's tokens, and what the model answered each with.  Token 0 of a sequence stands; another one does if its parent does and its
  * drafted value is the parent's answer (the first of several).  Those that stand move to the slots lengths[e] - counts[e] + 0, 1, ..; a block that
- * tokens move into gets the scale that an append of them would have given it.  Written: new_lengths (E), path (E, N contiguous; the tokens that
+ * tokens move into gets the smallest scale that holds them, or keeps its own where that is larger and older tokens stay in it (rejected tokens may have raised it).  Written: new_lengths (E), path (E, N contiguous; the tokens that
  * stand, -1 behind), answer (E; of the last of them, -1 where there is none).  They must not overlap what is read.  A count above N or the length stands for none. */
 typedef struct ma_b200_accept {
   int32_t abi_version;

@@ -8,8 +8,9 @@
 //
 // A CTA finds the path of its sequence (two reads that depend on each other, a minimum in shared memory for each token's first fitting child, and a
 // walk along it), then its warps take a head's keys or values of a layer each.  All layers are in one launch: the path is the same for them.
-// Bound by latency: a chain of six reads (length, parent, answer, page, row, and the page's other rows) for some hundred bytes of a head.  Measured: one sequence of 7 tokens, 12 layers
-// of 12 heads of 64 features 6.2 us, 64 of 61 tokens, 16 layers of 8 heads of 128 features 14; a call is 10.5 and 12, by the host's checks of all layers.
+// Bound by latency: a chain of six reads (length, parent, answer, page, row, and the page's other rows) for some hundred bytes of a head.  Measured in a
+// graph: one sequence of 7 tokens, 12 layers of 12 heads of 64 features 4.4 us, 64 of up to 61 tokens, 16 layers of 8 heads of 128 features 11.1 (14.6 where passes without a token look for their
+// maximum too); a call from the host is 10.5 and 12, by its checks of all layers.
 #include "ma_cache_codes.cuh"
 
 namespace ma {

@@ -14,8 +14,9 @@
 //   5  the free pages that are wanted, the lowest first, into a list; from there into the rows
 // The pages' contents are copied by a second kernel, all layers at once, a warp taking the keys and values of 16 tokens of a head.  Pages that are read there are not given
 // out in the same call.
-// The first is bound by latency: some 15 reads one after another and six barriers.  Measured: 4 rows of 33 pages 7.8 us, 128 rows of 17 15, 8 rows of 3752 15 (23 with atomics for
-// pages that stay).  The second by memory: 70 half pages of 16 layers, 8 heads of 128 features, 127 MB in 20.5 us, 6.2 TB/s.
+// The first is bound by latency: some 15 reads one after another and six barriers.  Measured in a graph, the first alone / both: 4 rows of 33 pages, 12 layers 9.4 / 11.6 us,
+// 128 rows of 17, 16 layers 14.2 / 36.2, 8 rows of 3752, 2 layers 16.4 / 18.7 (5 more with rows' numbers from global memory in each step and atomics for pages that stay).  Eight SMs do it whatever the
+// table's size: 64 rows of 8192 entries, 524288 pages 68 (exchanged 89, shared anew by four 145).  The second by memory: 70 half pages of 16 layers, 8 heads of 128 features, 127 MB in 20.5 us, 6.2 TB/s.
 #include <cooperative_groups.h>
 
 #include "ma_cache.cuh"
@@ -327,7 +328,8 @@ cudaError_t launch_fork_copies(const ForkArgs& a, int width, cudaStream_t stream
 
 cudaError_t launch_fork(const ForkArgs& a, int width, cudaStream_t stream) {
   void* args[] = {(void*)&a};
-  // (few entries and pages: one CTA, whose barriers are its own)
+  // Few entries and pages: one CTA, whose barriers are its own.  us of the call in a graph, one / eight, each row going on from itself: 4 rows of 36 entries and 200 pages 7.0 / 9.8, 16 x 100 and
+  // 1600 8.6 / 10.4, 32 x 64 and 2000 8.7 / 10.4, 64 x 40 and 2600 11.0 / 11.2, 128 x 17 and 2183 14.0 / 11.3, 32 x 128 and 4000 10.3 / 10.5, 8 x 1000 and 8000 13.5 / 10.1, 256 x 32 and 8000 26 / 11.5.
   const long long work = (long long)a.E * a.cache.table_pages + a.cache.pages;
   const int ctas = work <= 4 * kThreads ? 1 : kMostCtas;
   const cudaError_t err = launch_kernel((const void*)fork_kernel, dim3(ctas), dim3(kThreads), args, 0, stream, ctas);

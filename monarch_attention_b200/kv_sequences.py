@@ -45,8 +45,9 @@ def accept_drafts_b200(caches: PagedKV | Sequence[PagedKV], page_table: Tensor, 
     answers that name the chosen children.
 
     The tokens that stand move to the places right behind what was cached before the step, where their depth has put them in the rotation already.  Values stay what they
-    are: a block that tokens move into has the scale that an append of them would have given it, and codes move by whole exponents, exact but for values that become
-    subnormal (scales that are no powers of two cost a rounding).  As with the append, pages from the call's first token on must stand once in one sequence's row.  ``lengths`` is not changed; the new ones are returned.  The pages behind the new ends stay with their rows
+    are: a block that tokens move into has the smallest scale that holds them, as an append would give it, but where older tokens stay in the block no less than it has, and codes
+    move by whole exponents, exact but for values that become subnormal (scales that are no powers of two cost a rounding).  A rejected token may have raised the scale of a block
+    that it shared with older ones, and that stays: where it was of far larger magnitude, small values of up to 15 tokens that stand have lost bits, or become zero.  As with the append, pages from the call's first token on must stand once in one sequence's row.  ``lengths`` is not changed; the new ones are returned.  The pages behind the new ends stay with their rows
     (:func:`fork_sequences_b200` gives them back).  A count above N or the length is none.
     """
     if _accept is None:
